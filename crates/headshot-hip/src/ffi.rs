@@ -142,6 +142,30 @@ extern "C" {
                                k: *const c_void, v: *const c_void, out: *mut c_void, s: i32,
                                h: i32, t: i32, d: i32) -> HsStatus;
 
+    // sequences that grow: a paged key-value cache and the attention around it
+    // (int32 device arrays are c_void)
+    pub fn hs_kv_append(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
+                        k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64,
+                        qn_w: *const f32, qn_b: *const f32, kn_w: *const f32, kn_b: *const f32,
+                        sin_tab: *const f32, cos_tab: *const f32, table_rows: i32,
+                        positions: *const c_void, offsets: *const c_void,
+                        page_table: *const c_void, lens: *const c_void, q_out: *mut c_void,
+                        k_out: *mut c_void, k_cache: *mut c_void, v_cache: *mut c_void, n: i64,
+                        b: i32, h: i32, h_kv: i32, d: i32, page: i32, n_pages: i32,
+                        max_pages: i32, eps: f32) -> HsStatus;
+    pub fn hs_attention_packed(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
+                               k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64,
+                               q_offsets: *const c_void, k_offsets: *const c_void,
+                               out: *mut c_void, n_q: i64, n_k: i64, b: i32, h: i32, h_kv: i32,
+                               d: i32, causal: i32, scale: f32) -> HsStatus;
+    pub fn hs_attention_paged_workspace(b: i32, h: i32, h_kv: i32, d: i32) -> i64;
+    pub fn hs_attention_paged(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
+                              k_cache: *const c_void, v_cache: *const c_void,
+                              page_table: *const c_void, lens: *const c_void, out: *mut c_void,
+                              workspace: *mut c_void, workspace_bytes: i64, b: i32, h: i32,
+                              h_kv: i32, d: i32, page: i32, n_pages: i32, max_pages: i32,
+                              scale: f32) -> HsStatus;
+
     // host-side RoPE tables
     pub fn hs_rope_periods(out16: *mut f32);
     pub fn hs_rope_tables(periods16: *const f32, h_p: i32, w_p: i32, sin_out: *mut f32,

@@ -159,6 +159,29 @@ fn i32_of(v: usize, what: &str) -> i32 {
 }
 
 /// One device's op surface on one HIP stream.
+/// One layer's paged key-value cache: `k`, `v` (n_pages, heads, page, d) and
+/// int32 device arrays (sequences, max_pages) and (sequences) that the caller
+/// owns and layers share. `lens` counts a call's new tokens already.
+pub struct PagedKv {
+    pub k: HipTensor,
+    pub v: HipTensor,
+    pub page_table: *const i32,
+    pub lens: *const i32,
+    pub sequences: usize,
+    pub max_pages: usize,
+}
+
+impl PagedKv {
+    fn shape(&self) -> [usize; 4] {
+        assert_eq!(self.k.shape, self.v.shape, "cache k and v shapes");
+        assert_eq!(self.k.dtype, self.v.dtype, "cache k and v dtype");
+        let [pages, heads, page, d] = self.k.shape[..] else {
+            panic!("cache wants (n_pages, heads, page, d)")
+        };
+        [pages, heads, page, d]
+    }
+}
+
 pub struct HipContext {
     stream: ffi::HsStream,
 }
@@ -745,6 +768,103 @@ impl HipContext {
                                     n_blocks as i64, rows_per_block as i64,
                                     src.row_bytes() as i64)
         }, "copy_row_blocks");
+    }
+
+    /// Appends new tokens' keys and values to their pages: `q` (n, any heads *
+    /// d) or none, `k`, `v` (n, heads * d); `offsets` (sequences + 1) int32 on
+    /// the device, null for one token per sequence. `rope` = (sin, cos) f32
+    /// (rows, d), by `positions` (n) or, null, the keys' numbers. Returns the
+    /// normalised and rotated (q, k) rows, k only with `k_rows`.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_append(&self, cache: &PagedKv, q: Option<&HipTensor>, k: &HipTensor, v: &HipTensor,
+                     offsets: *const i32, qn: Option<(&HipTensor, &HipTensor)>,
+                     kn: Option<(&HipTensor, &HipTensor)>, rope: Option<(&HipTensor, &HipTensor)>,
+                     positions: *const i32, eps: f32, k_rows: bool)
+                     -> (Option<HipTensor>, Option<HipTensor>) {
+        let [n_pages, h_kv, page, d] = cache.shape();
+        let dt = cache.k.dtype;
+        let (n, width) = k.dims();
+        assert_eq!(width, h_kv * d, "kv_append k width");
+        assert_eq!(v.dims(), (n, width), "kv_append v shape");
+        assert!(k.dtype == dt && v.dtype == dt, "kv_append k/v dtype");
+        let q_width = q.map_or(0, |q| {
+            let (rows, w) = q.dims();
+            assert!(rows == n && w % d == 0 && q.dtype == dt, "kv_append q");
+            w
+        });
+        let norm = |p: Option<(&HipTensor, &HipTensor)>, what: &str| {
+            p.map_or((ptr::null(), ptr::null()),
+                     |(w, b)| (opt_f32(Some(w), d, what), opt_f32(Some(b), d, what)))
+        };
+        let ((qw, qb), (kw, kb)) = (norm(qn, "q-norm"), norm(kn, "k-norm"));
+        let rows = rope.map_or(0, |(sin, _)| sin.len() / d);
+        let (sn, cs) = rope.map_or((ptr::null(), ptr::null()), |(sin, cos)| {
+            (opt_f32(Some(sin), rows * d, "rope sin table"),
+             opt_f32(Some(cos), rows * d, "rope cos table"))
+        });
+        let q_out = q.map(|_| self.empty_typed(&[n, q_width], dt));
+        let k_out = k_rows.then(|| self.empty_typed(&[n, width], dt));
+        let out = |t: &Option<HipTensor>| t.as_ref().map_or(ptr::null_mut(), |t| t.mptr());
+        check(unsafe {
+            ffi::hs_kv_append(self.stream, dt.raw(), q.map_or(ptr::null(), |q| q.cptr()),
+                              q_width as i64, k.cptr(), width as i64, v.cptr(), width as i64,
+                              qw, qb, kw, kb, sn, cs, i32_of(rows, "rows"),
+                              positions as *const c_void, offsets as *const c_void,
+                              cache.page_table as *const c_void, cache.lens as *const c_void,
+                              out(&q_out), out(&k_out), cache.k.mptr(), cache.v.mptr(), n as i64,
+                              i32_of(cache.sequences, "sequences"), i32_of(q_width / d, "h"),
+                              i32_of(h_kv, "h_kv"), i32_of(d, "d"), i32_of(page, "page"),
+                              i32_of(n_pages, "n_pages"), i32_of(cache.max_pages, "max_pages"), eps)
+        }, "kv_append");
+        (q_out, k_out)
+    }
+
+    /// Attention of packed sequences: `q` (n, heads * d), `k`, `v` (m, kv_heads
+    /// * d), `offsets` (sequences + 1) and `k_offsets` (null: the same) int32 on
+    /// the device; `causal` 0 = every key, c = by groups of c tokens.
+    #[allow(clippy::too_many_arguments)]
+    pub fn attention_packed(&self, q: &HipTensor, k: &HipTensor, v: &HipTensor, d: usize,
+                            offsets: *const i32, sequences: usize, k_offsets: *const i32,
+                            causal: usize) -> HipTensor {
+        let ((n, width), (m, kv_width)) = (q.dims(), k.dims());
+        assert_eq!(v.dims(), (m, kv_width), "attention_packed v shape");
+        assert!(k.dtype == q.dtype && v.dtype == q.dtype, "attention_packed dtype");
+        assert!(d > 0 && width % d == 0 && kv_width % d == 0, "attention_packed widths");
+        let out = self.empty_typed(&[n, width], q.dtype);
+        check(unsafe {
+            ffi::hs_attention_packed(self.stream, q.dtype.raw(), q.cptr(), width as i64, k.cptr(),
+                                     kv_width as i64, v.cptr(), kv_width as i64,
+                                     offsets as *const c_void, k_offsets as *const c_void,
+                                     out.mptr(), n as i64, m as i64, i32_of(sequences, "sequences"),
+                                     i32_of(width / d, "h"), i32_of(kv_width / d, "h_kv"),
+                                     i32_of(d, "d"), i32_of(causal, "causal"),
+                                     1.0 / (d as f32).sqrt())
+        }, "attention_packed");
+        out
+    }
+
+    /// Attention of one new token per sequence over its pages: `q` (sequences,
+    /// heads * d).
+    pub fn attention_paged(&self, q: &HipTensor, cache: &PagedKv) -> HipTensor {
+        let [n_pages, h_kv, page, d] = cache.shape();
+        let (b, width) = q.dims();
+        assert_eq!(b, cache.sequences, "attention_paged q rows");
+        assert!(width % d == 0 && q.dtype == cache.k.dtype, "attention_paged q");
+        let (bi, h, kv, di) = (i32_of(b, "b"), i32_of(width / d, "h"), i32_of(h_kv, "h_kv"),
+                               i32_of(d, "d"));
+        let bytes = unsafe { ffi::hs_attention_paged_workspace(bi, h, kv, di) };
+        let ws = self.empty_typed(&[(bytes as usize + 3) / 4], Dtype::F32);
+        let out = self.empty_typed(&[b, width], q.dtype);
+        check(unsafe {
+            ffi::hs_attention_paged(self.stream, q.dtype.raw(), q.cptr(), width as i64,
+                                    cache.k.cptr(), cache.v.cptr(),
+                                    cache.page_table as *const c_void,
+                                    cache.lens as *const c_void, out.mptr(), ws.mptr(), bytes, bi,
+                                    h, kv, di, i32_of(page, "page"), i32_of(n_pages, "n_pages"),
+                                    i32_of(cache.max_pages, "max_pages"),
+                                    1.0 / (d as f32).sqrt())
+        }, "attention_paged");
+        out
     }
 
     /// attention + attn_merge (model/block.rs:148-149) in one pass.

@@ -65,6 +65,14 @@ SIGNATURES = {
     "hs_attention": (_S, [_P, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _I32]),
     "hs_attn_merge": (_S, [_P, _I32, _P, _P, _I32, _I32, _I32, _I32]),
     "hs_attention_merged": (_S, [_P, _I32, _P, _P, _P, _P, _I32, _I32, _I32, _I32]),
+    "hs_kv_append": (_S, [_P, _I32, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I32,
+                          _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32,
+                          _I32, _F]),
+    "hs_attention_packed": (_S, [_P, _I32, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64,
+                                 _I32, _I32, _I32, _I32, _I32, _F]),
+    "hs_attention_paged_workspace": (_I64, [_I32, _I32, _I32, _I32]),
+    "hs_attention_paged": (_S, [_P, _I32, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32,
+                                _I32, _I32, _I32, _I32, _F]),
     "hs_rope_periods": (None, [_P]),
     "hs_rope_tables": (_S, [_P, _I32, _I32, _P, _P]),
 }

@@ -353,3 +353,30 @@ def block_forward_reference(ctx: HipContext, wts: BlockWeights, x, s: int, t: in
     normed2 = ctx.layernorm(x1, *p.ln2, eps=eps)
     mlp = ctx.linear(ctx.gelu(ctx.linear(normed2, wts.fc1_w, p.fc1_b)), wts.fc2_w, p.fc2_b)
     return ctx.residual_ls(x1, mlp, p.ls2)
+
+
+def block_forward_cached(ctx: HipContext, wts: BlockWeights, x, cache, heads: int = HEADS,
+                         offsets=None, rope=None, positions=None, causal: int = 1,
+                         eps: float = 1e-6):
+    """``block_forward`` for sequences that grow, over this block's ``cache``
+    (``PagedKV``, its ``lens`` counting x's tokens already). With ``offsets``
+    x holds whole prompts, sequence after sequence, that fill empty sequences
+    and attend among themselves (``causal`` as ``attention_packed``: 1 by
+    token, T by frames of T tokens); without, one new token per sequence, that
+    sees every key the cache holds. ``rope`` = (sin, cos) with ``positions`` as
+    ``kv_append``, or None. Returns the block output, x's shape."""
+    p = wts.p
+    dim = x.shape[1]
+    d = dim // heads
+    normed = ctx.layernorm(x, *p.ln1, eps=eps)
+    q, k, v = ctx.linear(normed, wts.qkv_w, wts.qkv_b).split(dim, 1)
+    q, k = ctx.kv_append(cache, k, v, offsets, q=q, qn=p.qn, kn=p.kn, rope=rope,
+                         positions=positions, eps=eps, k_rows=offsets is not None)
+    if offsets is None:
+        attn = ctx.attention_paged(q, cache)
+    else:
+        q, k, v = (t.unflatten(1, (heads, d)) for t in (q, k, v))
+        attn = ctx.attention_packed(q, k, v, offsets, causal=causal)
+    x1 = ctx.linear_ls_residual(attn, wts.proj_w, p.ls1, x, p.proj_b)
+    act = ctx.linear_gelu(ctx.layernorm(x1, *p.ln2, eps=eps), wts.fc1_w, p.fc1_b)
+    return ctx.linear_ls_residual(act, wts.fc2_w, p.ls2, x1, p.fc2_b)

@@ -30,6 +30,8 @@ HIP_SOURCES = [
     "hs_elementwise.hip",
     "hs_assemble.hip",
     "hs_attention.hip",
+    "hs_attention_packed.hip",
+    "hs_paged.hip",
     "hs_cache.hip",
     "hs_gemm.hip",
 ]

@@ -73,6 +73,39 @@ def _param(t, n: int, what: str) -> int:
     return _dev(t, what)
 
 
+def _here(t: torch.Tensor, what: str) -> _Ptr:
+    """Address of a tensor of the current device, whose stream the launch goes
+    to; any strides."""
+    assert t.is_cuda, f"{what} must live in device memory"
+    current = torch.cuda.current_device() if _raw_device is None else _raw_device()
+    assert t.device.index == current, f"{what} must live on the current device"
+    p = _Ptr(t.data_ptr())
+    p.tensor = t
+    return p
+
+
+def _rows(t: torch.Tensor, heads: int | None, d: int, dtype, what: str):
+    """Token rows of head vectors, (n, heads, d) or (n, heads * d), possibly
+    columns of wider rows: (address, n, elements between rows)."""
+    assert t.dim() in (2, 3), f"{what} wants (n, heads, d) or (n, heads * d)"
+    assert t.dtype == dtype, f"{what} dtype"
+    width = t.shape[1] * (t.shape[2] if t.dim() == 3 else 1)
+    assert t.dim() == 2 or t.shape[2] == d, f"{what} head dim"
+    assert width == heads * d, f"{what} width {width} != {heads} heads of {d}"
+    n = t.shape[0]
+    if n and width:
+        assert t.stride(-1) == 1, f"{what}: a head vector must be contiguous"
+        assert t.dim() == 2 or t.shape[1] == 1 or t.stride(1) == d, f"{what}: a row's heads must be contiguous"
+        assert n == 1 or t.stride(0) >= width, f"{what}: rows overlap"
+    return _here(t, what), n, t.stride(0) if n > 1 else width
+
+
+def _int_array(t: torch.Tensor, n: int, what: str) -> _Ptr:
+    assert t.dtype == torch.int32, f"{what} must be int32"
+    assert t.is_contiguous() and t.numel() == n, f"{what} must be {n} contiguous values"
+    return _here(t, what)
+
+
 def _opt(t, n: int, what: str):
     return None if t is None else _param(t, n, what)
 
@@ -563,6 +596,138 @@ class HipContext:
         self._launch("attention_merged", self.lib.hs_attention_merged, _dt(q), _dev(q, "q"),
                      _dev(k, "k"), _dev(v, "v"), _dev(out, "out"), s, h, t, d)
         return out
+
+    # ---------------------------------------------- sequences that grow (paged.py)
+
+    def _cache_args(self, cache):
+        """A PagedKV's (k, v, page_table, lens) addresses and shape."""
+        assert cache.k.dim() == 4 and cache.v.shape == cache.k.shape, "cache: k and v (n_pages, heads, page, d)"
+        assert cache.v.dtype == cache.k.dtype, "cache: k and v dtype"
+        assert cache.k.is_contiguous() and cache.v.is_contiguous(), "cache pages must be contiguous"
+        assert cache.page_table.dim() == 2, "page_table wants (sequences, max_pages)"
+        b, max_pages = cache.page_table.shape
+        return (_here(cache.k, "k cache"), _here(cache.v, "v cache"),
+                _int_array(cache.page_table, b * max_pages, "page_table"),
+                _int_array(cache.lens, b, "lens"), b, max_pages)
+
+    def kv_append(self, cache, k, v, offsets=None, q=None, qn=None, kn=None, rope=None,
+                  positions=None, eps: float = 1e-5, k_rows: bool = False, out_q=None, out_k=None):
+        """Appends new tokens' keys and values to their sequences' pages
+        (``PagedKV``), with QK-norm and the position rotation of
+        ``rope_apply`` on the way.
+
+        ``k``, ``v`` (n, heads * d) or (n, heads, d) rows, sequence after
+        sequence, at int32 ``offsets`` (sequences + 1); None is one token per
+        sequence. Columns of a wider product serve as they are.
+        ``cache.lens`` counts the new tokens already: the last of sequence s
+        becomes its key ``lens[s] - 1``. ``q`` (n, any heads * d) goes through
+        the same. ``qn``, ``kn`` = (weight, bias) f32 (d) or None; ``rope`` =
+        (sin, cos) f32 (rows, d), by row ``positions[token]`` (int32) or the
+        key's number; a row outside the tables is not rotated. A token whose
+        page lies outside the table or the pool is not stored, and rows behind
+        ``offsets[-1]`` stay as they are. Returns (q, k) as contiguous
+        rows, None for what was not asked (``q``, ``k_rows``)."""
+        kc, vc, table, lens, b, max_pages = self._cache_args(cache)
+        n_pages, h_kv, page, d = cache.k.shape
+        dtype = cache.k.dtype
+        dt = _dt(cache.k)
+        kp, n, ks = _rows(k, h_kv, d, dtype, "k")
+        vp, nv, vs = _rows(v, h_kv, d, dtype, "v")
+        assert nv == n, "k and v rows"
+        off = None if offsets is None else _int_array(offsets, b + 1, "offsets")
+        assert offsets is not None or n == b, "without offsets, one token per sequence"
+        qp, qs, h, qo, ko = None, 0, 0, None, None
+        if q is not None:
+            h = math.prod(q.shape[1:]) // d
+            qp, nq, qs = _rows(q, h, d, dtype, "q")
+            assert nq == n, "q and k rows"
+            if out_q is None:
+                out_q = self.empty_typed((n, h * d), dtype)
+            assert out_q.dtype == dtype and out_q.numel() == n * h * d and out_q.is_contiguous(), "out_q"
+            qo = _here(out_q, "out_q")
+        assert q is not None or (qn is None and out_q is None), "qn or out_q without q"
+        if k_rows or out_k is not None:
+            if out_k is None:
+                out_k = self.empty_typed((n, h_kv * d), dtype)
+            assert out_k.dtype == dtype and out_k.numel() == n * h_kv * d and out_k.is_contiguous(), "out_k"
+            ko = _here(out_k, "out_k")
+        qw = qb = kw = kb = sn = cs = pos = None
+        rows = 0
+        if qn is not None:
+            qw, qb = _param(qn[0], d, "q-norm weight"), _param(qn[1], d, "q-norm bias")
+        if kn is not None:
+            kw, kb = _param(kn[0], d, "k-norm weight"), _param(kn[1], d, "k-norm bias")
+        if rope is not None:
+            rows = rope[0].shape[0]
+            sn = _param(rope[0], rows * d, "rope sin table")
+            cs = _param(rope[1], rows * d, "rope cos table")
+        if positions is not None:
+            assert rope is not None, "positions without rope"
+            pos = _int_array(positions, n, "positions")
+        self._launch("kv_append", self.lib.hs_kv_append, dt, qp, qs, kp, ks, vp, vs, qw, qb, kw, kb,
+                     sn, cs, rows, pos, off, table, lens, qo, ko, kc, vc, n, b, h, h_kv, d, page,
+                     n_pages, max_pages, eps)
+        return out_q, out_k
+
+    def attention_packed(self, q, k, v, offsets, k_offsets=None, causal: int = 1, scale=None,
+                         out=None) -> torch.Tensor:
+        """Attention of packed sequences of different lengths: ``q`` (n, heads,
+        d), ``k``, ``v`` (m, kv_heads, d) rows at int32 ``offsets`` (and
+        ``k_offsets`` where the keys' differ) -> token-major (n, heads * d), as
+        ``attention_merged``. heads is a multiple of kv_heads. ``causal`` 0:
+        every key of the sequence; c >= 1: a token sees its own group of c
+        tokens and the ones before (1 the causal mask, T frames of T tokens);
+        with more keys than queries the last query stands at the last key.
+        A query that sees nothing gets zeros; rows behind ``offsets[-1]`` are
+        not written. ``scale`` None is 1 / sqrt(d)."""
+        assert q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "attention_packed wants (n, heads, d)"
+        h, d = q.shape[1:]
+        h_kv = k.shape[1]
+        assert offsets.dim() == 1 and offsets.numel() >= 1, "offsets wants (sequences + 1)"
+        b = offsets.numel() - 1
+        dt = _dt(q)
+        qp, n, qs = _rows(q, h, d, q.dtype, "q")
+        kp, m, ks = _rows(k, h_kv, d, q.dtype, "k")
+        vp, mv, vs = _rows(v, h_kv, d, q.dtype, "v")
+        assert mv == m, "k and v rows"
+        assert k_offsets is not None or m == n, "without k_offsets, as many keys as queries"
+        off = _int_array(offsets, b + 1, "offsets")
+        koff = None if k_offsets is None else _int_array(k_offsets, b + 1, "k_offsets")
+        if out is None:
+            out = self.empty_typed((n, h * d), q.dtype)
+        assert out.dtype == q.dtype and out.numel() == n * h * d and out.is_contiguous(), "out shape/dtype"
+        self._launch("attention_packed", self.lib.hs_attention_packed, dt, qp, qs, kp, ks, vp, vs,
+                     off, koff, _here(out, "out"), n, m, b, h, h_kv, d, causal,
+                     1.0 / math.sqrt(d) if scale is None else scale)
+        return out
+
+    def attention_paged(self, q, cache, scale=None, out=None, workspace=None) -> torch.Tensor:
+        """Attention of one new token per sequence over the keys that
+        ``cache`` (``PagedKV``) holds: ``q`` (sequences, heads, d) or
+        (sequences, heads * d) -> (sequences, heads * d), zeros for a sequence
+        without keys. heads is a multiple of the cache's. ``workspace`` (uint8,
+        ``attention_paged_workspace`` bytes) keeps the call from allocating;
+        calls that may run at the same time need one each. ``scale`` None is 1
+        / sqrt(d)."""
+        kc, vc, table, lens, b, max_pages = self._cache_args(cache)
+        n_pages, h_kv, page, d = cache.k.shape
+        h = math.prod(q.shape[1:]) // d if q.dim() > 1 else 0
+        qp, n, qs = _rows(q, h, d, cache.k.dtype, "q")
+        assert n == b, "one query row per sequence"
+        if out is None:
+            out = self.empty_typed((b, h * d), q.dtype)
+        assert out.dtype == q.dtype and out.numel() == b * h * d and out.is_contiguous(), "out shape/dtype"
+        if workspace is None:
+            workspace = self.empty_typed((self.attention_paged_workspace(b, h, h_kv, d),), torch.uint8)
+        assert workspace.dtype == torch.uint8 and workspace.is_contiguous(), "workspace wants uint8"
+        self._launch("attention_paged", self.lib.hs_attention_paged, _dt(q), qp, qs, kc, vc, table,
+                     lens, _here(out, "out"), _here(workspace, "workspace"), workspace.numel(), b, h,
+                     h_kv, d, page, n_pages, max_pages, 1.0 / math.sqrt(d) if scale is None else scale)
+        return out
+
+    def attention_paged_workspace(self, sequences: int, heads: int, kv_heads: int, d: int) -> int:
+        """Bytes of workspace of ``attention_paged``."""
+        return self.lib.hs_attention_paged_workspace(sequences, heads, kv_heads, d)
 
     def bias_gelu(self, x, bias=None, out=None) -> torch.Tensor:
         """fc1 bias epilogue + GELU (model/block.rs:173-174)."""

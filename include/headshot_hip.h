@@ -357,6 +357,92 @@ hs_status hs_attention_merged(hs_stream_t stream, hs_dtype dt, const void* q, co
                               int32_t d);
 
 /* ---------------------------------------------------------------------- */
+/* Sequences that grow: a paged key-value cache and the attention around it  */
+/* (no counterpart in the reference, whose sequences are whole, equally long */
+/* and unmasked)                                                             */
+/*
+ * A cache is k_cache and v_cache (n_pages, Hkv, page, D) in dt, page_table
+ * (b, max_pages) and lens (b), both int32. Sequence s has lens[s] keys; key p
+ * is row p % page of page page_table[s][p / page]. lens counts a call's new
+ * tokens already: a step adds to it once, for every layer's calls.
+ *
+ * Packed tokens are rows, sequence after sequence: sequence s is rows
+ * [offsets[s], offsets[s + 1]) with offsets (b + 1) int32, ascending. A row
+ * holds its heads' vectors one after the other; rows are `stride` elements
+ * apart, so column ranges of a wider product serve as they are. Rows behind
+ * the last sequence are neither read nor written.
+ *
+ * Lengths, offsets and page numbers are device data that no check can see
+ * before the launch: a token whose page lies outside the table or the pool is
+ * not written, such keys are not seen, and offsets are held to the rows given,
+ * so no call reads or writes outside its buffers.
+ *
+ * D is 64 or 128, Hq a multiple of Hkv (query head h reads key head h / (Hq /
+ * Hkv)), page a power of two; buffers are 16-byte aligned and strides whole
+ * 16-byte vectors (HS_EUNSUPPORTED otherwise). int32 arrays are given as const
+ * void*. */
+
+/* Appends the n new tokens' keys and values to their sequences' pages,
+ * normalising and rotating the keys on the way, and the queries beside them.
+ * offsets NULL: one token per sequence, n == b. Token i of the m new ones of
+ * sequence s becomes key lens[s] - m + i.
+ * k (n, Hkv*D) -> [LayerNorm over each head's D with kn_w, kn_b and eps] ->
+ * [rotation] -> its page, and row of k_out (n, Hkv*D) if given; v (n, Hkv*D)
+ * -> its page; q (n, Hq*D), if given, likewise with qn_w, qn_b -> q_out (n,
+ * Hq*D). The rotation is hs_rope_apply's, by row positions[token] of the f32
+ * tables (table_rows, D), or by the key's number where positions is NULL; a
+ * token whose row lies outside the tables is not rotated. Norms (f32, D) and
+ * tables are given or NULL in pairs. Arithmetic is f32, rounded once when
+ * stored. q_out, k_out and the caches overlap nothing else. Two tokens of one
+ * call must not have the same place. */
+hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                       const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                       const float* qn_w, const float* qn_b, const float* kn_w,
+                       const float* kn_b, const float* sin_tab, const float* cos_tab,
+                       int32_t table_rows, const void* positions, const void* offsets,
+                       const void* page_table, const void* lens, void* q_out, void* k_out,
+                       void* k_cache, void* v_cache, int64_t n, int32_t b, int32_t h,
+                       int32_t h_kv, int32_t d, int32_t page, int32_t n_pages,
+                       int32_t max_pages, float eps);
+
+/* Attention of packed sequences: out[i] = softmax(scale q[i] K^T) V over the
+ * keys that token i sees, per head, written token-major (n_q, Hq*D) (as
+ * hs_attention_merged). Sequence s has queries [q_offsets[s], q_offsets[s +
+ * 1]) and keys [k_offsets[s], k_offsets[s + 1]) (k_offsets NULL: the
+ * queries'); its last query stands at its last key. causal 0: every key; c >=
+ * 1: a token sees the keys up to the end of its own group of c tokens (1 the
+ * usual causal mask, T frames of T tokens), groups counted from the first key.
+ * A query that sees no key gets zeros. Keys and values that a query does not
+ * see do not touch it, whatever they hold. Softmax statistics and sums are
+ * f32; in f16 the weights of the product with V are rounded to f16, relative
+ * to the largest. out overlaps no input. */
+hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                              const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                              const void* q_offsets, const void* k_offsets, void* out,
+                              int64_t n_q, int64_t n_k, int32_t b, int32_t h, int32_t h_kv,
+                              int32_t d, int32_t causal, float scale);
+
+/* Bytes of workspace that hs_attention_paged takes for b sequences on the
+ * current device; 0 for shapes that it refuses. */
+int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d);
+
+/* Attention of one new token per sequence over its paged keys: q (b, Hq*D),
+ * rows q_stride apart -> out (b, Hq*D): out[s] = softmax(scale q[s] K_s^T) V_s
+ * over the lens[s] keys of sequence s, zeros where there are none. Long
+ * sequences are split over their keys and joined; the split, and with it the
+ * order of the sums, follows all lengths of the call. workspace (16-byte
+ * aligned, hs_attention_paged_workspace bytes) holds nothing between calls:
+ * calls that may run at the same time need one each. Nothing is read on the
+ * host, so a captured call follows lens and page_table. out overlaps
+ * nothing else. */
+hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                             const void* k_cache, const void* v_cache, const void* page_table,
+                             const void* lens, void* out, void* workspace,
+                             int64_t workspace_bytes, int32_t b, int32_t h, int32_t h_kv,
+                             int32_t d, int32_t page, int32_t n_pages, int32_t max_pages,
+                             float scale);
+
+/* ---------------------------------------------------------------------- */
 /* Host-side RoPE tables (computed once per session, as the reference does) */
 
 /* rope::periods (engine/rope.rs:5-10): out16[i] = 100^(2i/32) in f32. */

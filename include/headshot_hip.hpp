@@ -148,6 +148,16 @@ class HipTensor {
     Dtype dtype_ = Dtype::F32;
 };
 
+// One layer's paged key-value cache (headshot_hip.h): k and v (n_pages, heads,
+// page, d); page_table (sequences, max_pages) and lens (sequences) are int32
+// device arrays that the caller owns and layers share.
+struct PagedKV {
+    HipTensor k, v;
+    const int32_t* page_table;
+    const int32_t* lens;
+    size_t sequences, max_pages;
+};
+
 // RoPE tables + unrotated prefix for one attention call (model/block.rs:42-47).
 struct Rope {
     const HipTensor* sin;
@@ -414,6 +424,91 @@ class HipContext {
         check(hs_attention_merged(stream_, hs_dtype(q.dtype()), q.data(), k.data(), v.data(),
                                   out.data(), i32(sh[0]), i32(sh[1]), i32(sh[2]), i32(sh[3])),
               "attention_merged");
+        return out;
+    }
+
+    // Appends new tokens' keys and values to their pages (hs_kv_append): q (n,
+    // any heads * d) or none, k, v (n, heads * d); offsets (sequences + 1) int32
+    // on the device, null for one token per sequence. Norms as linear_qkv_heads;
+    // sin, cos (rows, d) with positions (n) or the keys' numbers. Returns (q, k)
+    // rows, k empty unless k_rows.
+    std::pair<HipTensor, HipTensor> kv_append(PagedKV& cache, const HipTensor* q, const HipTensor& k,
+                                              const HipTensor& v, const int32_t* offsets,
+                                              const Norm* qn = nullptr, const Norm* kn = nullptr,
+                                              const HipTensor* sin = nullptr, const HipTensor* cos = nullptr,
+                                              const int32_t* positions = nullptr, float eps = 1e-5f,
+                                              bool k_rows = false) const {
+        HS_REQUIRE(cache.k.shape().size() == 4 && cache.v.shape() == cache.k.shape(), "kv_append: cache shape");
+        HS_REQUIRE(cache.v.dtype() == cache.k.dtype(), "kv_append: cache dtype");
+        const auto& c = cache.k.shape();
+        const size_t h_kv = c[1], page = c[2], d = c[3], width = h_kv * d;
+        const Dtype dt = cache.k.dtype();
+        HS_REQUIRE(width > 0 && k.dtype() == dt && v.dtype() == dt && k.last() == width && v.len() == k.len(),
+                   "kv_append: k and v must be (n, heads * d) in the cache's dtype");
+        const size_t n = k.len() / width;
+        size_t qw = 0;
+        if (q) {
+            qw = q->last();
+            HS_REQUIRE(q->dtype() == dt && qw % d == 0 && q->len() == n * qw, "kv_append: q must be (n, heads * d)");
+        }
+        for (const Norm* norm : {qn, kn})
+            if (norm) ln_params(*norm, d);
+        HS_REQUIRE(!sin == !cos, "kv_append: sin and cos go together");
+        if (sin)
+            HS_REQUIRE(sin->dtype() == Dtype::F32 && cos->dtype() == Dtype::F32 && sin->last() == d &&
+                           cos->len() == sin->len(), "kv_append: tables must be f32 (rows, d)");
+        HipTensor q_out = empty_typed({q ? n : 0, qw}, dt), k_out = empty_typed({k_rows ? n : 0, width}, dt);
+        check(hs_kv_append(stream_, hs_dtype(dt), q ? q->data() : nullptr, static_cast<int64_t>(qw), k.data(),
+                           static_cast<int64_t>(width), v.data(), static_cast<int64_t>(width),
+                           qn ? qn->weight->f32() : nullptr, qn ? qn->bias->f32() : nullptr,
+                           kn ? kn->weight->f32() : nullptr, kn ? kn->bias->f32() : nullptr,
+                           sin ? sin->f32() : nullptr, cos ? cos->f32() : nullptr,
+                           sin ? i32(sin->len() / d) : 0, positions, offsets, cache.page_table, cache.lens,
+                           q_out.data(), k_out.data(), cache.k.data(), cache.v.data(), static_cast<int64_t>(n),
+                           i32(cache.sequences), i32(qw / d), i32(h_kv), i32(d), i32(page), i32(c[0]),
+                           i32(cache.max_pages), eps),
+              "kv_append");
+        return {std::move(q_out), std::move(k_out)};
+    }
+
+    // Attention of packed sequences (hs_attention_packed): q (n, heads * d), k,
+    // v (m, kv_heads * d), offsets (sequences + 1) int32 on the device.
+    HipTensor attention_packed(const HipTensor& q, const HipTensor& k, const HipTensor& v, size_t d,
+                               const int32_t* offsets, size_t sequences, const int32_t* k_offsets = nullptr,
+                               int32_t causal = 1) const {
+        HS_REQUIRE(d > 0 && q.last() > 0 && q.last() % d == 0 && k.last() > 0 && k.last() % d == 0,
+                   "attention_packed: widths must be heads * d");
+        HS_REQUIRE(k.dtype() == q.dtype() && v.dtype() == q.dtype(), "attention_packed: dtype");
+        HS_REQUIRE(v.len() == k.len() && v.last() == k.last(), "attention_packed: k and v shapes");
+        const size_t n = q.len() / q.last(), m = k.len() / k.last();
+        HipTensor out = empty_typed({n, q.last()}, q.dtype());
+        check(hs_attention_packed(stream_, hs_dtype(q.dtype()), q.data(), static_cast<int64_t>(q.last()), k.data(),
+                                  static_cast<int64_t>(k.last()), v.data(), static_cast<int64_t>(v.last()), offsets,
+                                  k_offsets, out.data(), static_cast<int64_t>(n), static_cast<int64_t>(m),
+                                  i32(sequences), i32(q.last() / d), i32(k.last() / d), i32(d), causal,
+                                  1.0f / std::sqrt(static_cast<float>(d))),
+              "attention_packed");
+        return out;
+    }
+
+    // Attention of one token per sequence over its pages (hs_attention_paged): q
+    // (sequences, heads * d).
+    HipTensor attention_paged(const HipTensor& q, const PagedKV& cache) const {
+        HS_REQUIRE(cache.k.shape().size() == 4 && cache.v.shape() == cache.k.shape(), "attention_paged: cache shape");
+        HS_REQUIRE(q.dtype() == cache.k.dtype() && cache.v.dtype() == q.dtype(), "attention_paged: dtype");
+        const auto& c = cache.k.shape();
+        const size_t d = c[3];
+        HS_REQUIRE(d > 0 && q.last() % d == 0 && q.len() == cache.sequences * q.last(),
+                   "attention_paged: q must be (sequences, heads * d)");
+        const int32_t b = i32(cache.sequences), h = i32(q.last() / d), h_kv = i32(c[1]);
+        const int64_t bytes = hs_attention_paged_workspace(b, h, h_kv, i32(d));
+        HipTensor out = empty_typed({cache.sequences, q.last()}, q.dtype());
+        HipTensor ws = empty_typed({static_cast<size_t>(bytes + 3) / 4}, Dtype::F32);
+        check(hs_attention_paged(stream_, hs_dtype(q.dtype()), q.data(), static_cast<int64_t>(q.last()),
+                                 cache.k.data(), cache.v.data(), cache.page_table, cache.lens, out.data(), ws.data(),
+                                 bytes, b, h, h_kv, i32(d), i32(c[2]), i32(c[0]), i32(cache.max_pages),
+                                 1.0f / std::sqrt(static_cast<float>(d))),
+              "attention_paged");
         return out;
     }
 

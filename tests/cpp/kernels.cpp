@@ -498,6 +498,50 @@ void layernorm_prologue_equals_sequence(HipContext& ctx) {
     }
 }
 
+// A prompt of two sequences and a step of both: the pages hold what was
+// appended, and a step's attention is the packed attention's next row.
+void paged_step_continues_a_prompt(HipContext& ctx) {
+    const size_t h = 2, d = 64, page = 16, w = h * d;
+    const int32_t offsets[3] = {0, 20, 27}, all[3] = {0, 21, 29}, table[6] = {3, 0, 5, 1, 4, 2}, lens[2] = {20, 7};
+    const int32_t lens1[2] = {21, 8};
+    int32_t* dev = nullptr;
+    hs::hip_check(hipMalloc(&dev, 64 * sizeof(int32_t)), "hipMalloc");
+    const auto up = [&](size_t at, const int32_t* src, size_t n) {
+        hs::hip_check(hipMemcpy(dev + at, src, n * sizeof(int32_t), hipMemcpyHostToDevice), "hipMemcpy");
+        return dev + at;
+    };
+    Rng rng{77};
+    for (Dtype dt : {Dtype::F32, Dtype::F16}) {
+        const auto q = rng.vec(29 * w), k = rng.vec(29 * w), v = rng.vec(29 * w);
+        // rows 0..20 and 21..28 are the sequences' tokens, the last of each the step's
+        const auto rows = [&](const std::vector<float>& x, bool step) {
+            std::vector<float> r;
+            for (size_t t = 0; t < 29; t++)
+                if ((t == 20 || t == 28) == step) r.insert(r.end(), x.begin() + t * w, x.begin() + (t + 1) * w);
+            return r;
+        };
+        hs::PagedKV cache{ctx.empty_typed({6, h, page, d}, dt), ctx.empty_typed({6, h, page, d}, dt), up(0, table, 6),
+                          up(8, lens, 2), 2, 3};
+        const auto tensor = [&](const std::vector<float>& x) { return ctx.tensor_from_f32({x.size() / w, w}, x, dt); };
+        ctx.kv_append(cache, nullptr, tensor(rows(k, false)), tensor(rows(v, false)), up(16, offsets, 3));
+        ctx.sync();
+        up(8, lens1, 2);
+        auto [sq, sk] = [&] {
+            auto tq = tensor(rows(q, true));
+            return ctx.kv_append(cache, &tq, tensor(rows(k, true)), tensor(rows(v, true)), nullptr);
+        }();
+        const auto got = ctx.download(ctx.attention_paged(sq, cache));
+        const auto want = ctx.download(ctx.attention_packed(tensor(q), tensor(k), tensor(v), d, up(24, all, 3), 2));
+        for (size_t s = 0; s < 2; s++)
+            for (size_t c = 0; c < w; c++) {
+                const float a = got[s * w + c], b = want[(s ? 28 : 20) * w + c];
+                // both are off by at most their type's roundings (values below 4)
+                if (!(std::fabs(a - b) <= (dt == Dtype::F32 ? 1e-5f : 1.6e-2f))) throw Failure("paged step differs from the packed row");
+            }
+    }
+    hs::hip_check(hipFree(dev), "hipFree");
+}
+
 void contract_violations_throw(HipContext& ctx) {
     auto x = ctx.tensor_from_slice({4, 8}, std::vector<float>(32, 1.0f));
     auto w = ctx.tensor_from_slice({7}, std::vector<float>(7, 1.0f));
@@ -536,6 +580,7 @@ int main(int argc, char** argv) {
         {"qkv_heads_equal_sequence", qkv_heads_equal_sequence},
         {"qknorm_rope_pair_equals_two_calls", qknorm_rope_pair_equals_two_calls},
         {"layernorm_prologue_equals_sequence", layernorm_prologue_equals_sequence},
+        {"paged_step_continues_a_prompt", paged_step_continues_a_prompt},
         {"contract_violations_throw", contract_violations_throw},
     };
     HipContext ctx;
