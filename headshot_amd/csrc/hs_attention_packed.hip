@@ -1,12 +1,337 @@
 // Attention of packed sequences for gfx950: whole prompts of different lengths
 // in one call, causal by token or by group of tokens, query heads sharing key
 // heads.
-#include <math.h>
+#include <cmath>
 
 #include "hs_packed.hpp"
 
 namespace hs {
 namespace {
+
+typedef f16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+constexpr int kXcds = 8;
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+constexpr int kBM = 32 * kWaves;  // queries per workgroup
+constexpr int kBN = 64;           // keys per tile
+
+__device__ __forceinline__ h8 as_h8(u32x4 v) { return __builtin_bit_cast(h8, v); }
+__device__ __forceinline__ uint32_t pk_f16(float a, float b) {
+    f16x2 h;
+    h.x = static_cast<f16>(a), h.y = static_cast<f16>(b);
+    return h22u(h);
+}
+// v of this lane and of lane ^ 32, in the same order in both.
+__device__ __forceinline__ f32x2 both_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+    return f32x2{u2f(static_cast<uint32_t>(r[0])), u2f(static_cast<uint32_t>(r[1]))};
+}
+__device__ __forceinline__ float halves_max(float v) {
+    const f32x2 r = both_halves(v);
+    return fmaxf(r.x, r.y);
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const f32x2 r = both_halves(v);
+    return r.x + r.y;
+}
+
+struct PackedArgs {
+    const void *q, *k, *v;
+    void* out;
+    int64_t q_stride, k_stride, v_stride;
+    const int *q_off, *k_off;
+    int n_q, n_k, b, h, h_kv, tiles, causal;
+    float scale;
+};
+
+// What a workgroup works on: a tile of one sequence's queries, one head.
+struct PackedTile {
+    int q0, nq;       // first query of the sequence's rows, its queries
+    int k0, nk;       // the keys likewise
+    int first, head;  // first query of the tile, within the sequence
+};
+
+// Keys that query i of a sequence sees.
+__device__ __forceinline__ int keys_seen(int i, int nq, int nk, int causal) {
+    if (causal == 0) return nk;
+    const int at = i + nk - nq;
+    if (at < 0) return 0;
+    const int64_t end = (static_cast<int64_t>(at / causal) + 1) * causal;
+    return end < nk ? static_cast<int>(end) : nk;
+}
+
+// Workgroup b's tile. A sequence's last queries see the most keys and go first.
+// Workgroup b runs on XCD b % 8: where the heads divide by it, an XCD takes
+// h / 8 heads in a row, so that the heads of a key head, and a head's tiles,
+// read their keys through one L2.
+__device__ __forceinline__ bool packed_tile(const PackedArgs& a, PackedTile& t) {
+    const int b = blockIdx.x;
+    int tile;
+    if (a.h % kXcds == 0) {
+        const int slot = b / kXcds;
+        tile = slot % a.tiles;
+        t.head = b % kXcds * (a.h / kXcds) + slot / a.tiles;
+    } else {
+        tile = b / a.h;
+        t.head = b % a.h;
+    }
+    int s, local;
+    if (!find_tile(a.q_off, a.b, a.n_q, kBM, tile, s, local)) return false;
+    const RowRange q = row_range(a.q_off, s, a.n_q), k = row_range(a.k_off, s, a.n_k);
+    t.q0 = q.begin, t.nq = q.end - q.begin, t.k0 = k.begin, t.nk = k.end - k.begin;
+    t.first = ((t.nq + kBM - 1) / kBM - 1 - local) * kBM;
+    return true;
+}
+
+// ---------------------------------------------------------------------------
+// f16
+//
+// Flash attention on v_mfma_f32_32x32x16_f16, scores transposed: a wave takes
+// 32 queries, and S^T = K Q^T puts one query in a lane's column (lanes n and n
+// + 32 share its keys), so its softmax statistics are the lane's own. Keys go
+// through LDS 64 at a time, double-buffered, the next tile's rows in registers
+// while the current one computes; V^T comes through the transposing LDS read
+// and takes P^T from the registers that the scores were in.
+template <int D>
+struct FlashF16 {
+    static constexpr int KS = D / 16;             // 16-dim slices of a score
+    static constexpr int DB = D / 32;             // 32-channel blocks of an output
+    static constexpr int kRowChunks = D / 8;      // 16-byte pieces of a row
+    static constexpr int kPer = kBN * kRowChunks / kThreads;
+    // Row pitches in halves. 16-byte reads of 16 rows at a time start 4 banks
+    // (of 64) apart in K, and the transposing read's 4 rows of 64 bytes take a
+    // quarter of the banks each in V: no conflicts.
+    static constexpr int kKPitch = D + 8, kVPitch = D + 32;
+    struct Smem {
+        f16 k[2][kBN * kKPitch];
+        f16 v[2][kBN * kVPitch];
+        int odd[2];  // the buffer's V tile holds an infinity or NaN
+    };
+};
+
+// A weight's exponent may run this far (log2) above the reference maximum
+// before the reference moves.
+constexpr float kLazyMax = 8.0f;
+// A lane's row sum over a tile beyond which a weight may not fit f16.
+constexpr float kRowSumMax = 32768.0f;
+
+template <int D>
+__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(PackedArgs a) {
+    using F = FlashF16<D>;
+    constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
+    __shared__ __align__(16) typename F::Smem sm;
+    PackedTile t;
+    if (!packed_tile(a, t)) return;  // workgroup-uniform, before any barrier
+    const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
+    const int n = lane & 31, hh = lane >> 5;
+    const int kv = t.head / (a.h / a.h_kv);
+    const f16* kb = static_cast<const f16*>(a.k) + t.k0 * a.k_stride + kv * D;
+    const f16* vb = static_cast<const f16*>(a.v) + t.k0 * a.v_stride + kv * D;
+
+    // The keys seen grow with the query: the tile's last live query has the most
+    const int qi = t.first + 32 * wave + n;
+    const bool live = t.first + 32 * wave < t.nq;  // wave-uniform
+    const int seen = keys_seen(min(qi, t.nq - 1), t.nq, t.nk, a.causal);
+    const int wave_least = keys_seen(min(t.first + 32 * wave, t.nq - 1), t.nq, t.nk, a.causal);
+    const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
+    const int tile_least = keys_seen(t.first, t.nq, t.nk, a.causal);
+    const int most = keys_seen(min(t.first + kBM, t.nq) - 1, t.nq, t.nk, a.causal);
+    const int ntiles = (most + kBN - 1) / kBN;
+
+    // Q^T as the B operand: lane (n, hh) holds dims 16 ks + 8 hh .. + 8. A
+    // negative scale is taken as one of -q.
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    h8 qa[KS];
+    {
+        const f16* qr = static_cast<const f16*>(a.q) + (t.q0 + min(qi, t.nq - 1)) * a.q_stride + t.head * D + 8 * hh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            u32x4 x = ld16(qr + 16 * ks);
+            x ^= flip;
+            qa[ks] = as_h8(x);
+        }
+        // arrived before the loop, whose prefetches it would wait for otherwise
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) asm volatile("" ::"v"(qa[ks]));
+    }
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] = f32x16{};
+    // a finite floor: a tile of masked scores then weighs exp2(-inf) = 0
+    float m = -3.0e38f, l = 0.0f;
+
+    u32x4 pk[kPer], pv[kPer];
+    const int row0 = tid / F::kRowChunks, col0 = tid % F::kRowChunks * 8;
+    constexpr int kRowStep = kThreads / F::kRowChunks;
+    auto load = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int64_t row = min(key0 + row0 + kRowStep * i, t.nk - 1);  // past the end: masked
+            pk[i] = ld16(kb + row * a.k_stride + col0);
+            pv[i] = ld16(vb + row * a.v_stride + col0);
+        }
+    };
+    auto store = [&](int buf, int key0) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            st16(&sm.k[buf][(row0 + kRowStep * i) * F::kKPitch + col0], pk[i]);
+            st16(&sm.v[buf][(row0 + kRowStep * i) * F::kVPitch + col0], pv[i]);
+        }
+        if (key0 + kBN > tile_least) {  // some query does not see all of these values
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    odd |= (pv[i][w] & 0x7C00u) == 0x7C00u || (pv[i][w] & 0x7C000000u) == 0x7C000000u;
+            if (odd) sm.odd[buf] = key0 + 1;
+        }
+    };
+    if (tid < 2) sm.odd[tid] = 0;
+    if (ntiles > 0) load(0);
+    __syncthreads();
+    if (ntiles > 0) store(0, 0);
+    __syncthreads();
+    for (int j = 0; j < ntiles; j++) {
+        const int cur = j & 1, key0 = j * kBN;
+        if (j + 1 < ntiles) load(key0 + kBN);
+        if (key0 < wave_most) {
+            // S^T: s[kb] holds keys 32 kb .. + 32 of the tile, register r of
+            // lane (n, hh) key 8 (r / 4) + 4 hh + r % 4, query n
+            f32x16 s[2];
+            const f32x16 z = {};
+            const f16* ka = sm.k[cur] + n * F::kKPitch + 8 * hh;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(ld16(ka + 32 * i * F::kKPitch + 16 * ks)), qa[ks],
+                                                                  ks ? s[i] : z, 0, 0, 0);
+            const bool partial = key0 + kBN > wave_least;
+            if (partial) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (key0 + 32 * i + 8 * (r / 4) + 4 * hh + r % 4 >= seen) s[i][r] = -INFINITY;
+            }
+            u32x4 p[2][2];
+            // The tile's weights against a reference, rounded to f16 (2^-11 of
+            // each, inside the result's own rounding), and the sum of the
+            // rounded ones over the lane's keys: two packed f16 levels (sums
+            // of four), then f32.
+            auto weights = [&](float ref) {
+                f16x2 w2[16];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r += 2) {
+                        const uint32_t w = pk_f16(__builtin_amdgcn_exp2f(fmaf(s[i][r], c, -ref)),
+                                                  __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], c, -ref)));
+                        p[i][r / 8][r % 8 / 2] = w;
+                        w2[8 * i + r / 2] = u2h2(w);
+                    }
+#pragma unroll
+                for (int i = 0; i < 8; i++) w2[i] = w2[i] + w2[i + 8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) w2[i] = w2[i] + w2[i + 4];
+                const f16x2 one = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2(w2[i], one, sum, false);
+                return sum;
+            };
+            // Past the first tile the weights are taken against the reference
+            // as it is; only a query whose sum says that one may not fit f16
+            // moves its own.
+            bool own = j == 0, move = own;
+            if (!move) {
+                const float sum = weights(m);
+                own = !(halves_max(sum) <= kRowSumMax) || !(sum <= kRowSumMax);
+                move = __any(own);
+                if (!move) l += sum;
+            }
+            if (move) {
+                float mx = s[0][0];
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[i][r]);
+                const float cand = fmaxf(m, halves_max(mx) * c);
+                const float next = own && cand > m + kLazyMax ? cand : m;
+                const float corr = __builtin_amdgcn_exp2f(m - next);
+                l = fmaf(l, corr, weights(next));
+                m = next;
+#pragma unroll
+                for (int i = 0; i < DB; i++) o[i] *= corr;
+            }
+            // O^T += V^T P^T. The transposing read gives lane i of 16 channel
+            // i of 4 keys: two reads make the 8 keys, in the scores' order.
+            const int l16 = n & 15;
+            const f16* va = sm.v[cur] + (4 * hh + l16 / 4) * F::kVPitch + (n & 16) + 4 * (l16 % 4);
+            auto read_v = [&](int g, int db) {
+                const f16* r0 = va + 16 * g * F::kVPitch + 32 * db;
+                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)r0));
+                const u32x2 hi =
+                    __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(r0 + 8 * F::kVPitch)));
+                u32x4 w;
+                w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
+                return w;
+            };
+            if (partial && sm.odd[cur] == key0 + 1) {
+                // Infinities or NaN among values that not every query sees:
+                // key by key, each into the queries that see it.
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll 1
+                    for (int e = 0; e < 16; e++) {
+                        const int el = (e & 3) + 4 * (e >> 3);  // its element in the lanes with hh == e / 4 % 2
+                        const uint32_t keep = hh == (e >> 2 & 1) ? (el & 1 ? 0xFFFF0000u : 0xFFFFu) : 0u;
+                        u32x4 one = {}, w;
+#pragma unroll
+                        for (int x = 0; x < 4; x++) one[x] = x == el / 2 ? p[g / 2][g % 2][x] & keep : 0u;
+#pragma unroll
+                        for (int db = 0; db < DB; db++) {
+                            w = read_v(g, db);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) w[x] = x == el / 2 ? w[x] & keep : 0u;
+                            const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(w), as_h8(one), z, 0, 0, 0);
+                            if (key0 + 16 * g + e < seen) o[db] += add;
+                        }
+                    }
+            } else {
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int db = 0; db < DB; db++)
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(read_v(g, db)), as_h8(p[g / 2][g % 2]), o[db], 0, 0, 0);
+            }
+        }
+        if (j + 1 < ntiles) store(cur ^ 1, key0 + kBN);
+        __syncthreads();
+    }
+
+    if (qi >= t.nq) return;
+    const float inv = 1.0f / halves_sum(l);
+    f16* orow = static_cast<f16*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = seen > 0 ? o[db][4 * r4 + e] * inv : 0.0f;
+            u32x2 w;
+            w[0] = pk_f16(x[0], x[1]), w[1] = pk_f16(x[2], x[3]);
+            *reinterpret_cast<u32x2*>(orow + 32 * db + 8 * r4) = w;
+        }
+}
 
 // One wave per (query row, head), its lanes over the head dim, key by key.
 template <typename T, int D>
@@ -77,6 +402,27 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
         overlaps(out, out_bytes, k, row_bytes(n_k, k_stride, kv_width, dt)) ||
         overlaps(out, out_bytes, v, row_bytes(n_k, v_stride, kv_width, dt)))
         return fail(HS_EINVAL, "%s: out overlaps an input", op);
+    if (!std::isfinite(scale)) return fail(HS_EINVAL, "%s: scale must be finite", op);
+    PackedArgs a;
+    a.q = q, a.k = k, a.v = v, a.out = out;
+    a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
+    a.q_off = static_cast<const int*>(q_offsets);
+    a.k_off = static_cast<const int*>(k_offsets ? k_offsets : q_offsets);
+    a.n_q = static_cast<int>(n_q), a.n_k = static_cast<int>(n_k), a.b = b, a.h = h, a.h_kv = h_kv;
+    a.causal = causal, a.scale = scale;
+    // as many tiles as sequences of these rows can have
+    const int64_t tiles = n_q / kBM + (b < n_q ? b : n_q);
+    if (tiles * h >= (int64_t{1} << 31) / kThreads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
+    a.tiles = static_cast<int>(tiles);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dt == HS_F16) {
+        const dim3 grid(static_cast<uint32_t>(tiles * h));
+        if (d == 64)
+            packed_f16_kernel<64><<<grid, dim3(kThreads), 0, st>>>(a);
+        else
+            packed_f16_kernel<128><<<grid, dim3(kThreads), 0, st>>>(a);
+        return check_launch(op);
+    }
     const auto run = [&](auto zero) {
         using T = decltype(zero);
         const dim3 grid(static_cast<uint32_t>(n_q * h));
@@ -92,9 +438,6 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
         else
             go(attention_packed_kernel<T, 128>);
     };
-    if (dt == HS_F16)
-        run(f16{});
-    else
-        run(float{});
+    run(float{});
     return check_launch(op);
 }

@@ -30,6 +30,46 @@ __device__ __forceinline__ int sequence_of(const int* __restrict__ offsets, int 
     return lo > 0 && row < offsets[lo] ? lo - 1 : -1;
 }
 
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// Sum of v over this lane and the ones before it.
+__device__ __forceinline__ int wave_prefix_sum(int v) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) {
+        const int up = __shfl_up(v, step, 64);
+        if (lane >= step) v += up;
+    }
+    return v;
+}
+
+// Which sequence the tile-th tile of bm rows belongs to, all sequences' tiles
+// counted one after the other, and the tile's number within it; false past the
+// last. The lengths are device data, so a launch has as many workgroups as
+// there can be tiles and each finds its own (64 sequences a step).
+__device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int b, int n, int bm, int tile, int& s,
+                                          int& local) {
+    const int lane = lane_id();
+    int before = 0;
+    for (int base = 0; base < b; base += 64) {
+        int count = 0;
+        if (base + lane < b) {
+            const RowRange r = row_range(offsets, base + lane, n);
+            count = static_cast<int>((static_cast<int64_t>(r.end - r.begin) + bm - 1) / bm);
+        }
+        const int sum = wave_prefix_sum(count);
+        const uint64_t hit = __ballot(before + sum > tile);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            s = base + l;
+            local = tile - before - (lane_value(sum, l) - lane_value(count, l));
+            return true;
+        }
+        before += lane_value(sum, 63);
+    }
+    return false;
+}
+
 // Keys of sequence s that its row of the page table has room for.
 __device__ __forceinline__ int64_t held_length(const int* __restrict__ lens, int s, int max_pages, int page_shift) {
     const int64_t room = static_cast<int64_t>(max_pages) << page_shift;
