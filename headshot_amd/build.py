@@ -55,6 +55,7 @@ HIP_FLAGS = [
 # softmax max (NaN inputs give NaN-polluted output either way).
 SOURCE_FLAGS = {
     "hs_attention_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "hs_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "hs_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
 }
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-Wall",

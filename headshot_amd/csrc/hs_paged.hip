@@ -1,6 +1,6 @@
 // A paged key-value cache for gfx950: appending new tokens (with QK-norm and
 // the position rotation) and the attention of one new token per sequence.
-#include <math.h>
+#include <cmath>
 
 #include "hs_packed.hpp"
 
@@ -154,51 +154,408 @@ void launch_append(hipStream_t st, const AppendArgs<T>& a) {
 }
 
 // ---------------------------------------------------------------------------
-// attention_paged: one wave per (sequence, query head), its lanes over the head
-// dim, key by key.
+// attention_paged
+//
+// Bandwidth: every key and value is read once, by the workgroup of its
+// (sequence, key head, range of keys), for all query heads of that key head (up
+// to 16 a pass) at once. A wave takes kStep keys at a time on its own: scores
+// transposed on the matrix cores, S^T = K Q^T with the query heads as columns,
+// so that lanes n, n + 16, .. share query head n; K straight from memory as the
+// A operand; V through the wave's own slice of LDS, from which V^T takes P^T as
+// the scores' registers hold it. Loads run a step ahead. The four waves' (O, m,
+// l) join in LDS, the ranges of a sequence in a second launch.
+//
+// Ranges: a sequence's keys are cut into pieces of `chunk` units of 4 kStep
+// keys, so that all sequences together make about kItems pieces. Lengths are
+// device data: each workgroup computes chunk and finds its piece from all of
+// them (64 a step).
+
+typedef f16 h8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+__device__ __forceinline__ h8 as_h8(u32x4 v) { return __builtin_bit_cast(h8, v); }
+
+constexpr int kGroup = 16;  // query heads per pass
+constexpr int kPagedWaves = 4;
+constexpr float kNone = -3.0e38f;   // a running maximum that has seen no key
+constexpr float kFloor = -2.9e38f;  // the least of one that has
 
 template <typename T, int D>
-__global__ __launch_bounds__(64) void attention_paged_kernel(
-    const T* __restrict__ q, int64_t q_stride, const T* __restrict__ k_cache, const T* __restrict__ v_cache,
-    const int* __restrict__ page_table, const int* __restrict__ lens, T* __restrict__ out, int h, int h_kv,
-    int page_shift, int n_pages, int max_pages, float scale) {
-    constexpr int E = D / 64;
-    const int s = blockIdx.x / h, head = blockIdx.x % h, kv = head / (h / h_kv);
-    const int lane = lane_id();
-    const int64_t len = held_length(lens, s, max_pages, page_shift);
-    float qv[E], o[E];
+struct Paged {
+    static constexpr bool kHalf = sizeof(T) == 2;
+    static constexpr int kStep = kHalf ? 32 : 16;  // keys per wave and step
+    static constexpr int kUnit = kPagedWaves * kStep;
+    static constexpr int V = Vec<T>::N;
+    static constexpr int kRowLanes = D / V;               // 16-byte pieces of a row
+    static constexpr int kVRows = 64 / kRowLanes;         // rows per load of a wave
+    static constexpr int kVLoads = kStep / kVRows;
+    static constexpr int kKLoads = kStep / 16 * (D * static_cast<int>(sizeof(T)) / 64);
+    // LDS pitch of V's rows in elements. f16: the transposing read takes 8 rows
+    // of 32 bytes at a time, which start 32 bytes apart modulo the 64 banks;
+    // f32: 4 rows of 64 bytes, 4 rows apart.
+    static constexpr int kPitch = kHalf ? D + 16 : D + 4;
+    static constexpr int kOPitch = D + 4;
+    struct Smem {
+        union {
+            T v[kPagedWaves][kStep * kPitch];
+            float o[kPagedWaves][kGroup * kOPitch];
+        };
+        float m[kPagedWaves][kGroup], l[kPagedWaves][kGroup];
+    };
+};
+
+struct PagedArgs {
+    const void *q, *k, *v;
+    void* out;
+    float *ws_o, *ws_ml;  // per (piece, query head): D sums; maximum and weight sum
+    const int *page_table, *lens;
+    int64_t q_stride;
+    int b, h, h_kv, page_shift, n_pages, max_pages, target;
+    int group, passes, width;  // query heads per key head, passes over them, heads per pass
+    float scale;
+};
+
+// The pieces of all sequences, by units of keys.
+struct Cut {
+    int64_t chunk;  // units per piece
+
+    __device__ Cut(const PagedArgs& a, int unit) {
+        int64_t total = 0;
+        for (int s = lane_id(); s < a.b; s += 64) total += (held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit;
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        qv[e] = static_cast<float>(q[s * q_stride + head * D + lane + 64 * e]) * scale, o[e] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    bool any = false;
-    for (int64_t key = 0; key < len; key++) {
-        const int page = page_table[static_cast<int64_t>(s) * max_pages + (key >> page_shift)];
-        if (page < 0 || page >= n_pages) continue;
-        any = true;
-        const int64_t at = (((static_cast<int64_t>(page) * h_kv + kv) << page_shift) + (key & ((1 << page_shift) - 1))) * D + lane;
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) dot = fmaf(qv[e], static_cast<float>(k_cache[at + 64 * e]), dot);
-        const float score = wave_sum(dot);
-        const float m_new = fmaxf(m, score);
-        const float ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float corr = expf(m - ref), p = expf(score - ref);
-        l = l * corr + p;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * corr + p * static_cast<float>(v_cache[at + 64 * e]);
-        m = m_new;
+        for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step, 64);
+        const int64_t per = total * a.h_kv * a.passes;
+        chunk = (per + a.target - 1) / a.target;
+        if (chunk < 1) chunk = 1;
     }
+    __device__ int pieces(const PagedArgs& a, int s, int unit) const {
+        const int64_t units = (held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit;
+        return units <= chunk ? 1 : static_cast<int>((units + chunk - 1) / chunk);
+    }
+};
+
+template <typename T, int D, bool ONE_PAGE>
+__global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(PagedArgs a) {
+    using P = Paged<T, D>;
+    constexpr int V = P::V, kStep = P::kStep;
+    __shared__ __align__(16) typename P::Smem sm;
+    const int lane = lane_id(), wave = wave_in_block();
+    const int n = lane & 15, g = lane >> 4;
+
+    // the piece: sequence s, range `local` of its `count`, key head, pass
+    const int heads = a.h_kv * a.passes;
+    const int piece = static_cast<int>(blockIdx.x) / heads;
+    const int rest = static_cast<int>(blockIdx.x) - piece * heads;
+    const int kv = rest / a.passes, pass = rest - kv * a.passes;
+    const Cut cut(a, P::kUnit);
+    int s = -1, local = 0, count = 0, before = 0;
+    for (int base = 0; base < a.b; base += 64) {
+        const int c = base + lane < a.b ? cut.pieces(a, base + lane, P::kUnit) : 0;
+        const int sum = wave_prefix_sum(c);
+        const uint64_t hit = __ballot(before + sum > piece);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            s = base + l;
+            count = lane_value(c, l);
+            local = piece - before - (lane_value(sum, l) - count);
+            break;
+        }
+        before += lane_value(sum, 63);
+    }
+    if (s < 0) return;  // workgroup-uniform, before any barrier
+    const int len = static_cast<int>(held_length(a.lens, s, a.max_pages, a.page_shift));
+    const int64_t first = local * cut.chunk * P::kUnit, last = first + cut.chunk * P::kUnit;
+    const int begin = static_cast<int>(first < len ? first : len), end = static_cast<int>(last < len ? last : len);
+    const int live_heads = min(a.width, a.group - pass * a.width);
+    const int head0 = kv * a.group + pass * a.width;
+
+    // Q^T as the B operand, column n the query head (a copy of the last beyond
+    // them); a negative scale is taken as one of -q
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
+    const T* qr = static_cast<const T*>(a.q) + s * a.q_stride + (head0 + min(n, live_heads - 1)) * D;
+    constexpr int KS = D * static_cast<int>(sizeof(T)) / 64;  // 16-byte pieces of a row per lane group
+    u32x4 qa[KS];
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        out[(static_cast<int64_t>(s) * h + head) * D + lane + 64 * e] = static_cast<T>(any ? o[e] / l : 0.0f);
+    for (int i = 0; i < KS; i++) {
+        qa[i] = ld16(qr + (4 * i + g) * V);
+        if (a.scale < 0.0f) qa[i] ^= P::kHalf ? 0x80008000u : 0x80000000u;
+    }
+
+    const int* pages = a.page_table + static_cast<int64_t>(s) * a.max_pages;
+    const T* kb = static_cast<const T*>(a.k);
+    const T* vb = static_cast<const T*>(a.v);
+    const int in_page = (1 << a.page_shift) - 1;
+    // Row of key `key` in the pool (all heads' rows), -1 where there is none
+    auto row_of = [&](int page, int key) {
+        return page >= 0 && page < a.n_pages ? ((static_cast<int64_t>(page) * a.h_kv + kv) << a.page_shift) + (key & in_page) : int64_t{-1};
+    };
+    auto page_of = [&](int key) { return pages[min(key, end - 1) >> a.page_shift]; };
+    u32x4 kr[P::kKLoads], vr[P::kVLoads];
+    uint32_t k_ok = 0, v_ok = 0;  // which of the lane's rows there are
+    auto load_k = [&](int key0, int page) {
+        k_ok = 0;
+#pragma unroll
+        for (int i = 0; i < kStep / 16; i++) {
+            const int key = key0 + 16 * i + n;
+            const int64_t row = row_of(ONE_PAGE ? page : page_of(key), key);
+            if (row >= 0 && key < end) k_ok |= 1u << i;
+            const T* p = kb + (row < 0 ? 0 : row) * D + g * V;
+#pragma unroll
+            for (int x = 0; x < KS; x++) kr[i * KS + x] = ld16_nt(p + 4 * x * V);
+        }
+    };
+    auto load_v = [&](int key0, int page) {
+        v_ok = 0;
+#pragma unroll
+        for (int i = 0; i < P::kVLoads; i++) {
+            const int key = key0 + P::kVRows * i + lane / P::kRowLanes;
+            const int64_t row = row_of(ONE_PAGE ? page : page_of(key), key);
+            if (row >= 0 && key < end) v_ok |= 1u << i;
+            vr[i] = ld16_nt(vb + (row < 0 ? 0 : row) * D + lane % P::kRowLanes * V);
+        }
+    };
+
+    constexpr int DB = D / 16;
+    f32x4 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] = f32x4{};
+    float m = kNone, l = 0.0f;  // l: this lane's keys only
+    T* vs = sm.v[wave];
+    const int start = begin + wave * kStep;
+    int page = 0;
+    if (start < end) {
+        if (ONE_PAGE) page = page_of(start);
+        load_v(start, page);
+        load_k(start, page);
+        if (ONE_PAGE) page = page_of(start + P::kUnit);
+    }
+    for (int key0 = start; key0 < end; key0 += P::kUnit) {
+        const bool more = key0 + P::kUnit < end;
+        // rows that are not there count as zeros: their weight is 0, and 0
+        // times what they hold may not be
+        if (__any(v_ok != (1u << P::kVLoads) - 1)) {
+#pragma unroll
+            for (int i = 0; i < P::kVLoads; i++)
+                if (!(v_ok >> i & 1)) vr[i] = u32x4{};
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < P::kVLoads; i++)
+            st16(vs + (P::kVRows * i + lane / P::kRowLanes) * P::kPitch + lane % P::kRowLanes * V, vr[i]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (more) load_v(key0 + P::kUnit, page);
+
+        // S^T: register j of lane (n, g) is key 16 i + 4 g + j, query head n
+        f32x4 sc[kStep / 16];
+#pragma unroll
+        for (int i = 0; i < kStep / 16; i++) {
+            f32x4 acc[2] = {f32x4{}, f32x4{}};
+#pragma unroll
+            for (int x = 0; x < KS; x++) {
+                if constexpr (P::kHalf) {
+                    acc[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(kr[i * KS + x]), as_h8(qa[x]), acc[0], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        acc[e % 2] = __builtin_amdgcn_mfma_f32_16x16x4f32(u2f(kr[i * KS + x][e]), u2f(qa[x][e]), acc[e % 2], 0, 0, 0);
+                }
+            }
+            sc[i] = acc[0] + acc[1];
+        }
+        // which of the lane's scores count: key rows 4 g + j, held by lanes 4 g + j
+        if (__any(k_ok != (1u << kStep / 16) - 1)) {
+#pragma unroll
+            for (int i = 0; i < kStep / 16; i++) {
+                const uint64_t there = __ballot(k_ok >> i & 1);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (!(there >> (4 * g + j) & 1)) sc[i][j] = -INFINITY;
+            }
+        }
+        const bool some = __any(k_ok != 0);
+        if (more) {
+            load_k(key0 + P::kUnit, page);
+            if (ONE_PAGE) page = page_of(key0 + 2 * P::kUnit);
+        }
+
+        float mx = sc[0][0];
+#pragma unroll
+        for (int i = 0; i < kStep / 16; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) mx = fmaxf(mx, sc[i][j]);
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float next = fmaxf(fmaxf(m, mx * c), some ? kFloor : kNone);
+        const float corr = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kStep / 16; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                sc[i][j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], c, -m));
+                sum += sc[i][j];
+            }
+        l = fmaf(l, corr, sum);
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[i] *= corr;
+        // O^T += V^T P^T
+        if constexpr (P::kHalf) {
+            // the weights rounded to f16 (2^-11 of each)
+            u32x4 p;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    f16x2 w;
+                    w.x = static_cast<f16>(sc[i][j]), w.y = static_cast<f16>(sc[i][j + 1]);
+                    p[2 * i + j / 2] = h22u(w);
+                }
+            const T* va = vs + (4 * g + n / 4) * P::kPitch + 4 * (n % 4);
+#pragma unroll
+            for (int i = 0; i < DB; i++) {
+                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + 16 * i)));
+                const u32x2 hi =
+                    __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + 16 * P::kPitch + 16 * i)));
+                u32x4 w;
+                w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), as_h8(p), o[i], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < DB; i++)
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(vs[(4 * g + j) * P::kPitch + 16 * i + n], sc[0][j], o[i], 0, 0, 0);
+        }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+
+    // join the waves
+    __syncthreads();
+    if (n < live_heads) {
+#pragma unroll
+        for (int i = 0; i < DB; i++) *reinterpret_cast<f32x4*>(&sm.o[wave][n * P::kOPitch + 16 * i + 4 * g]) = o[i];
+        if (g == 0) sm.m[wave][n] = m, sm.l[wave][n] = l;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < live_heads * (D / 4); x += 64 * kPagedWaves) {
+        const int head = x / (D / 4), d0 = x % (D / 4) * 4;
+        float top = sm.m[0][head];
+#pragma unroll
+        for (int w = 1; w < kPagedWaves; w++) top = fmaxf(top, sm.m[w][head]);
+        f32x4 sum = {};
+        float weight = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(sm.m[w][head] - top);
+            sum += *reinterpret_cast<const f32x4*>(&sm.o[w][head * P::kOPitch + d0]) * f;
+            weight = fmaf(sm.l[w][head], f, weight);
+        }
+        if (count == 1) {
+            T* orow = static_cast<T*>(a.out) + (static_cast<int64_t>(s) * a.h + head0 + head) * D + d0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(top == kNone ? 0.0f : sum[e] / weight);
+        } else {
+            const int64_t row = static_cast<int64_t>(blockIdx.x) * a.width + head;
+            *reinterpret_cast<f32x4*>(a.ws_o + row * D + d0) = sum;
+            if (d0 == 0) a.ws_ml[2 * row] = top, a.ws_ml[2 * row + 1] = weight;
+        }
+    }
+}
+
+// The pieces of one (sequence, query head) joined, THREADS / (D / 4) at a time.
+template <typename T, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
+    constexpr int kUnit = Paged<T, D>::kUnit, kLanes = D / 4, kRows = THREADS / kLanes;
+    __shared__ __align__(16) f32x4 part[kRows][kLanes];
+    __shared__ float tops[kRows], weights[kRows];
+    const int s = static_cast<int>(blockIdx.x) / a.h, head = static_cast<int>(blockIdx.x) - s * a.h;
+    const Cut cut(a, kUnit);
+    const int count = cut.pieces(a, s, kUnit);
+    if (count == 1) return;  // workgroup-uniform: written by its only piece
+    int64_t before = 0;
+    for (int i = lane_id(); i < s; i += 64) before += cut.pieces(a, i, kUnit);
+#pragma unroll
+    for (int step = 1; step < 64; step *= 2) before += __shfl_xor(before, step, 64);
+    const int kv = head / a.group, in_group = head - kv * a.group;
+    const int pass = in_group / a.width, x = in_group - pass * a.width;
+    const auto row_of = [&](int i) { return (((before + i) * a.h_kv + kv) * a.passes + pass) * a.width + x; };
+    const int row = threadIdx.x / kLanes, col = threadIdx.x % kLanes;
+    float top = kNone, weight = 0.0f;
+    f32x4 sum = {};
+    for (int i = row; i < count; i += kRows) {
+        const int64_t r = row_of(i);
+        const float m = a.ws_ml[2 * r], l = a.ws_ml[2 * r + 1];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + r * D + 4 * col);
+        const float next = fmaxf(top, m);
+        const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
+        sum = sum * old + v * f;
+        weight = fmaf(weight, old, l * f);
+        top = next;
+    }
+    part[row][col] = sum;
+    if (col == 0) tops[row] = top, weights[row] = weight;
+    __syncthreads();
+    if (row != 0) return;
+    const int rows = min(kRows, count);
+    for (int i = 0; i < rows; i++) top = fmaxf(top, tops[i]);
+    sum = f32x4{}, weight = 0.0f;
+    for (int i = 0; i < rows; i++) {
+        const float f = __builtin_amdgcn_exp2f(tops[i] - top);
+        sum += part[i][col] * f;
+        weight = fmaf(weights[i], f, weight);
+    }
+    T* orow = static_cast<T*>(a.out) + (static_cast<int64_t>(s) * a.h + head) * D + 4 * col;
+#pragma unroll
+    for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(top == kNone ? 0.0f : sum[e] / weight);
+}
+
+// How the query heads of a key head are taken, and how many pieces there are
+// at most.
+struct PagedPlan {
+    int group, passes, width, target;
+    int64_t items, rows;
+    PagedPlan(int b, int h, int h_kv) {
+        group = h / h_kv;
+        passes = static_cast<int>(ceil_div(group, kGroup));
+        width = static_cast<int>(ceil_div(group, passes));
+        target = 16 * num_cus();
+        // each sequence's last piece may be short
+        const int64_t heads = static_cast<int64_t>(h_kv) * passes;
+        items = (target / heads + b) * heads;
+        rows = items * width;
+    }
+};
+
+template <typename T, int D>
+hs_status launch_paged(const char* op, hipStream_t st, PagedArgs a, int64_t items) {
+    using P = Paged<T, D>;
+    const dim3 grid(static_cast<uint32_t>(items));
+    if ((1 << a.page_shift) >= P::kStep)
+        attention_paged_kernel<T, D, true><<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
+    else
+        attention_paged_kernel<T, D, false><<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
+    if (hs_status rc = check_launch(op)) return rc;
+    if ((static_cast<int64_t>(a.max_pages) << a.page_shift) <= P::kUnit) return HS_OK;  // no sequence has two pieces
+    const int64_t rows = static_cast<int64_t>(a.b) * a.h;
+    const dim3 joins(static_cast<uint32_t>(rows));
+    // few rows may have a thousand pieces each
+    if (rows <= 64)
+        paged_join_kernel<T, D, 1024><<<joins, dim3(1024), 0, st>>>(a);
+    else
+        paged_join_kernel<T, D, 256><<<joins, dim3(256), 0, st>>>(a);
+    return check_launch(op);
 }
 
 hs_status check_cache(const char* op, const void* k_cache, const void* v_cache, const void* page_table,
                       const void* lens, int32_t page, int32_t n_pages, int32_t max_pages, int32_t h_kv, int32_t d) {
     if (page <= 0 || n_pages < 0 || max_pages < 0) return fail(HS_EINVAL, "%s: page %d, n_pages %d, max_pages %d", op, page, n_pages, max_pages);
     if (exact_log2(page) < 0) return fail(HS_EUNSUPPORTED, "%s: page %d is no power of two", op, page);
-    if (static_cast<int64_t>(max_pages) * page >= (int64_t{1} << 31)) return fail(HS_EINVAL, "%s: max_pages * page must be below 2^31", op);
+    if (static_cast<int64_t>(max_pages) * page >= (int64_t{1} << 30)) return fail(HS_EINVAL, "%s: max_pages * page must be below 2^30", op);
     if (too_large(static_cast<int64_t>(n_pages) * page, static_cast<int64_t>(h_kv) * d))
         return fail(HS_EINVAL, "%s: cache too large", op);
     if (!lens || (max_pages > 0 && !page_table) || (n_pages > 0 && (!k_cache || !v_cache)))
@@ -280,7 +637,9 @@ extern "C" hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q
 
 extern "C" int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d) {
     if (b <= 0 || h <= 0 || h_kv <= 0 || h % h_kv != 0 || (d != 64 && d != 128)) return 0;
-    return 0;
+    using namespace hs;
+    if (b > (1 << 24) / h) return 0;
+    return PagedPlan(b, h, h_kv).rows * (d + 2) * 4;
 }
 
 extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
@@ -309,23 +668,16 @@ extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const v
         return fail(HS_EINVAL, "%s: out overlaps another buffer", op);
     if (overlaps(workspace, need, q, in_bytes) || overlaps(workspace, need, k_cache, cache) || overlaps(workspace, need, v_cache, cache))
         return fail(HS_EINVAL, "%s: workspace overlaps an input", op);
-    const auto run = [&](auto zero) {
-        using T = decltype(zero);
-        const dim3 grid(static_cast<uint32_t>(b * h));
-        const auto go = [&](auto kernel) {
-            kernel<<<grid, dim3(64), 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const T*>(q), q_stride, static_cast<const T*>(k_cache), static_cast<const T*>(v_cache),
-                static_cast<const int*>(page_table), static_cast<const int*>(lens), static_cast<T*>(out), h, h_kv,
-                exact_log2(page), n_pages, max_pages, scale);
-        };
-        if (d == 64)
-            go(attention_paged_kernel<T, 64>);
-        else
-            go(attention_paged_kernel<T, 128>);
-    };
-    if (dt == HS_F16)
-        run(f16{});
-    else
-        run(float{});
-    return check_launch(op);
+    if (!std::isfinite(scale)) return fail(HS_EINVAL, "%s: scale must be finite", op);
+    const PagedPlan plan(b, h, h_kv);
+    PagedArgs a;
+    a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.q_stride = q_stride;
+    a.ws_o = static_cast<float*>(workspace), a.ws_ml = a.ws_o + plan.rows * d;
+    a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens);
+    a.b = b, a.h = h, a.h_kv = h_kv, a.page_shift = exact_log2(page), a.n_pages = n_pages;
+    a.max_pages = n_pages > 0 ? max_pages : 0;  // no page to read: no sequence has keys
+    a.group = plan.group, a.passes = plan.passes, a.width = plan.width, a.target = plan.target, a.scale = scale;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dt == HS_F16) return d == 64 ? launch_paged<f16, 64>(op, st, a, plan.items) : launch_paged<f16, 128>(op, st, a, plan.items);
+    return d == 64 ? launch_paged<float, 64>(op, st, a, plan.items) : launch_paged<float, 128>(op, st, a, plan.items);
 }

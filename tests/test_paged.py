@@ -58,7 +58,7 @@ def test_append_refusals():
     refused(append(vc=at(8)), EINVAL, "outputs overlap")
     refused(append(qo=at(9)), EINVAL, "outputs overlap")
     refused(append(n=1 << 29), EINVAL, "2^31")
-    refused(append(page=1 << 20, max_pages=1 << 11), EINVAL, "2^31")
+    refused(append(page=1 << 20, max_pages=1 << 10), EINVAL, "2^30")
     refused(append(n_pages=1 << 30), EINVAL, "too large")
     assert append(n=0, q=None, k=None, v=None, qo=None, ko=None, kc=None, vc=None, lens=None) == OK
     assert append(n=0, b=0, off=None) == OK
