@@ -32,14 +32,19 @@ __device__ __forceinline__ int sequence_of(const int* __restrict__ offsets, int 
 
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
-// Sum of v over this lane and the ones before it.
+// Sum of v over this lane and the ones before it (DPP: shifts within rows of
+// 16, then the rows' sums).
+template <int CTRL, int ROW_MASK = 0xF>
+__device__ __forceinline__ int dpp_zero(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xF, false);
+}
 __device__ __forceinline__ int wave_prefix_sum(int v) {
-    const int lane = lane_id();
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) {
-        const int up = __shfl_up(v, step, 64);
-        if (lane >= step) v += up;
-    }
+    v += dpp_zero<0x111>(v);  // row_shr 1, 2, 4, 8
+    v += dpp_zero<0x112>(v);
+    v += dpp_zero<0x114>(v);
+    v += dpp_zero<0x118>(v);
+    v += dpp_zero<kRowBcast15, 0xA>(v);
+    v += dpp_zero<kRowBcast31, 0xC>(v);
     return v;
 }
 
@@ -71,10 +76,9 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int b
 }
 
 // Keys of sequence s that its row of the page table has room for.
-__device__ __forceinline__ int64_t held_length(const int* __restrict__ lens, int s, int max_pages, int page_shift) {
-    const int64_t room = static_cast<int64_t>(max_pages) << page_shift;
-    const int64_t len = lens[s];
-    return len < 0 ? 0 : len < room ? len : room;
+// (max_pages * page is below 2^30.)
+__device__ __forceinline__ int held_length(const int* __restrict__ lens, int s, int max_pages, int page_shift) {
+    return min(max(lens[s], 0), max_pages << page_shift);
 }
 
 // Log2 of a power of two, -1 for anything else.

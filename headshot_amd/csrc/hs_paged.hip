@@ -210,33 +210,35 @@ struct PagedArgs {
     const void *q, *k, *v;
     void* out;
     float *ws_o, *ws_ml;  // per (piece, query head): D sums; maximum and weight sum
+    int* ws_cut;          // per sequence: its first piece, its pieces
     const int *page_table, *lens;
     int64_t q_stride;
-    int b, h, h_kv, page_shift, n_pages, max_pages, target;
+    int b, h, h_kv, page_shift, n_pages, max_pages;
+    float per_target;  // 1 / ranges wanted of all sequences together
     int group, passes, width;  // query heads per key head, passes over them, heads per pass
     float scale;
 };
 
-// The pieces of all sequences, by units of keys.
-struct Cut {
-    int64_t chunk;  // units per piece
-
-    __device__ Cut(const PagedArgs& a, int unit) {
-        int64_t total = 0;
-        for (int s = lane_id(); s < a.b; s += 64) total += (held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit;
-#pragma unroll
-        for (int step = 1; step < 64; step *= 2) total += __shfl_xor(total, step, 64);
-        const int64_t per = total * a.h_kv * a.passes;
-        chunk = (per + a.target - 1) / a.target;
-        if (chunk < 1) chunk = 1;
+// Units of keys per piece: total / (pieces wanted), rounded up. The total is
+// summed in f32, whose error (2^-24 a step) the factor covers, so that there
+// are never more pieces than the launch has workgroups for.
+__device__ __forceinline__ int units_per_piece(const PagedArgs& a, int unit) {
+    float total = 0.0f;
+    for (int base = 0; base < a.b; base += 64) {
+        const int s = base + lane_id();
+        total += s < a.b ? static_cast<float>((held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit) : 0.0f;
     }
-    __device__ int pieces(const PagedArgs& a, int s, int unit) const {
-        const int64_t units = (held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit;
-        return units <= chunk ? 1 : static_cast<int>((units + chunk - 1) / chunk);
-    }
-};
+    const float per = wave_sum(total) * a.per_target;
+    return per < 16777216.0f ? max(1, static_cast<int>(ceilf(per))) : 16777216;
+}
+__device__ __forceinline__ int pieces_of(const PagedArgs& a, int s, int unit, int chunk) {
+    const uint32_t units = static_cast<uint32_t>((held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit);
+    return units <= static_cast<uint32_t>(chunk) ? 1 : static_cast<int>((units + chunk - 1) / static_cast<uint32_t>(chunk));
+}
 
-template <typename T, int D, bool ONE_PAGE>
+// WHOLE: pages of at least 16 keys, so that 16 keys from a multiple of 16 lie in
+// one page; else each row looks its own up.
+template <typename T, int D, bool WHOLE>
 __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(PagedArgs a) {
     using P = Paged<T, D>;
     constexpr int V = P::V, kStep = P::kStep;
@@ -249,10 +251,10 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
     const int piece = static_cast<int>(blockIdx.x) / heads;
     const int rest = static_cast<int>(blockIdx.x) - piece * heads;
     const int kv = rest / a.passes, pass = rest - kv * a.passes;
-    const Cut cut(a, P::kUnit);
+    const int chunk = units_per_piece(a, P::kUnit);
     int s = -1, local = 0, count = 0, before = 0;
     for (int base = 0; base < a.b; base += 64) {
-        const int c = base + lane < a.b ? cut.pieces(a, base + lane, P::kUnit) : 0;
+        const int c = base + lane < a.b ? pieces_of(a, base + lane, P::kUnit, chunk) : 0;
         const int sum = wave_prefix_sum(c);
         const uint64_t hit = __ballot(before + sum > piece);
         if (hit) {
@@ -265,9 +267,10 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
         before += lane_value(sum, 63);
     }
     if (s < 0) return;  // workgroup-uniform, before any barrier
-    const int len = static_cast<int>(held_length(a.lens, s, a.max_pages, a.page_shift));
-    const int64_t first = local * cut.chunk * P::kUnit, last = first + cut.chunk * P::kUnit;
+    const int len = held_length(a.lens, s, a.max_pages, a.page_shift);
+    const int64_t first = static_cast<int64_t>(local) * chunk * P::kUnit, last = first + static_cast<int64_t>(chunk) * P::kUnit;
     const int begin = static_cast<int>(first < len ? first : len), end = static_cast<int>(last < len ? last : len);
+    if (local == 0 && rest == 0 && threadIdx.x == 0) a.ws_cut[2 * s] = piece, a.ws_cut[2 * s + 1] = count;
     const int live_heads = min(a.width, a.group - pass * a.width);
     const int head0 = kv * a.group + pass * a.width;
 
@@ -294,24 +297,30 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
     auto page_of = [&](int key) { return pages[min(key, end - 1) >> a.page_shift]; };
     u32x4 kr[P::kKLoads], vr[P::kVLoads];
     uint32_t k_ok = 0, v_ok = 0;  // which of the lane's rows there are
-    auto load_k = [&](int key0, int page) {
+    constexpr int kTiles = kStep / 16;
+    int page[kTiles];  // WHOLE: of the step's 16-key tiles
+    auto find_pages = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < kTiles; i++) page[i] = page_of(key0 + 16 * i);
+    };
+    auto load_k = [&](int key0) {
         k_ok = 0;
 #pragma unroll
-        for (int i = 0; i < kStep / 16; i++) {
+        for (int i = 0; i < kTiles; i++) {
             const int key = key0 + 16 * i + n;
-            const int64_t row = row_of(ONE_PAGE ? page : page_of(key), key);
+            const int64_t row = row_of(WHOLE ? page[i] : page_of(key), key);
             if (row >= 0 && key < end) k_ok |= 1u << i;
             const T* p = kb + (row < 0 ? 0 : row) * D + g * V;
 #pragma unroll
             for (int x = 0; x < KS; x++) kr[i * KS + x] = ld16_nt(p + 4 * x * V);
         }
     };
-    auto load_v = [&](int key0, int page) {
+    auto load_v = [&](int key0) {
         v_ok = 0;
 #pragma unroll
         for (int i = 0; i < P::kVLoads; i++) {
             const int key = key0 + P::kVRows * i + lane / P::kRowLanes;
-            const int64_t row = row_of(ONE_PAGE ? page : page_of(key), key);
+            const int64_t row = row_of(WHOLE ? page[P::kVRows * i / 16] : page_of(key), key);
             if (row >= 0 && key < end) v_ok |= 1u << i;
             vr[i] = ld16_nt(vb + (row < 0 ? 0 : row) * D + lane % P::kRowLanes * V);
         }
@@ -324,12 +333,11 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
     float m = kNone, l = 0.0f;  // l: this lane's keys only
     T* vs = sm.v[wave];
     const int start = begin + wave * kStep;
-    int page = 0;
     if (start < end) {
-        if (ONE_PAGE) page = page_of(start);
-        load_v(start, page);
-        load_k(start, page);
-        if (ONE_PAGE) page = page_of(start + P::kUnit);
+        if (WHOLE) find_pages(start);
+        load_v(start);
+        load_k(start);
+        if (WHOLE) find_pages(start + P::kUnit);
     }
     for (int key0 = start; key0 < end; key0 += P::kUnit) {
         const bool more = key0 + P::kUnit < end;
@@ -345,7 +353,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
         for (int i = 0; i < P::kVLoads; i++)
             st16(vs + (P::kVRows * i + lane / P::kRowLanes) * P::kPitch + lane % P::kRowLanes * V, vr[i]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (more) load_v(key0 + P::kUnit, page);
+        if (more) load_v(key0 + P::kUnit);
 
         // S^T: register j of lane (n, g) is key 16 i + 4 g + j, query head n
         f32x4 sc[kStep / 16];
@@ -376,8 +384,8 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
         }
         const bool some = __any(k_ok != 0);
         if (more) {
-            load_k(key0 + P::kUnit, page);
-            if (ONE_PAGE) page = page_of(key0 + 2 * P::kUnit);
+            load_k(key0 + P::kUnit);
+            if (WHOLE) find_pages(key0 + 2 * P::kUnit);
         }
 
         float mx = sc[0][0];
@@ -470,17 +478,13 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
 // The pieces of one (sequence, query head) joined, THREADS / (D / 4) at a time.
 template <typename T, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
-    constexpr int kUnit = Paged<T, D>::kUnit, kLanes = D / 4, kRows = THREADS / kLanes;
+    constexpr int kLanes = D / 4, kRows = THREADS / kLanes;
     __shared__ __align__(16) f32x4 part[kRows][kLanes];
     __shared__ float tops[kRows], weights[kRows];
     const int s = static_cast<int>(blockIdx.x) / a.h, head = static_cast<int>(blockIdx.x) - s * a.h;
-    const Cut cut(a, kUnit);
-    const int count = cut.pieces(a, s, kUnit);
+    const int64_t before = a.ws_cut[2 * s];
+    const int count = a.ws_cut[2 * s + 1];
     if (count == 1) return;  // workgroup-uniform: written by its only piece
-    int64_t before = 0;
-    for (int i = lane_id(); i < s; i += 64) before += cut.pieces(a, i, kUnit);
-#pragma unroll
-    for (int step = 1; step < 64; step *= 2) before += __shfl_xor(before, step, 64);
     const int kv = head / a.group, in_group = head - kv * a.group;
     const int pass = in_group / a.width, x = in_group - pass * a.width;
     const auto row_of = [&](int i) { return (((before + i) * a.h_kv + kv) * a.passes + pass) * a.width + x; };
@@ -517,30 +521,32 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
 // How the query heads of a key head are taken, and how many pieces there are
 // at most.
 struct PagedPlan {
-    int group, passes, width, target;
-    int64_t items, rows;
+    int group, passes, width;
+    int64_t heads, ranges, items, rows;
     PagedPlan(int b, int h, int h_kv) {
         group = h / h_kv;
         passes = static_cast<int>(ceil_div(group, kGroup));
         width = static_cast<int>(ceil_div(group, passes));
-        target = 16 * num_cus();
-        // each sequence's last piece may be short
-        const int64_t heads = static_cast<int64_t>(h_kv) * passes;
-        items = (target / heads + b) * heads;
+        heads = static_cast<int64_t>(h_kv) * passes;
+        ranges = ceil_div(16 * num_cus(), heads);
+        items = (ranges + b) * heads;  // each sequence's last piece may be short
         rows = items * width;
     }
 };
 
 template <typename T, int D>
-hs_status launch_paged(const char* op, hipStream_t st, PagedArgs a, int64_t items) {
+hs_status launch_paged(const char* op, hipStream_t st, PagedArgs a, const PagedPlan& plan) {
     using P = Paged<T, D>;
-    const dim3 grid(static_cast<uint32_t>(items));
-    if ((1 << a.page_shift) >= P::kStep)
+    // no more pieces than a table's width of keys has units, either
+    const int64_t most = ceil_div(static_cast<int64_t>(a.max_pages) << a.page_shift, int64_t{P::kUnit});
+    const int64_t items = a.b * plan.heads * (most > 1 ? most : 1);
+    const dim3 grid(static_cast<uint32_t>(items < plan.items ? items : plan.items));
+    if (a.page_shift >= 4)
         attention_paged_kernel<T, D, true><<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
     else
         attention_paged_kernel<T, D, false><<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
     if (hs_status rc = check_launch(op)) return rc;
-    if ((static_cast<int64_t>(a.max_pages) << a.page_shift) <= P::kUnit) return HS_OK;  // no sequence has two pieces
+    if (most <= 1) return HS_OK;  // no sequence has two pieces
     const int64_t rows = static_cast<int64_t>(a.b) * a.h;
     const dim3 joins(static_cast<uint32_t>(rows));
     // few rows may have a thousand pieces each
@@ -639,7 +645,7 @@ extern "C" int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_
     if (b <= 0 || h <= 0 || h_kv <= 0 || h % h_kv != 0 || (d != 64 && d != 128)) return 0;
     using namespace hs;
     if (b > (1 << 24) / h) return 0;
-    return PagedPlan(b, h, h_kv).rows * (d + 2) * 4;
+    return PagedPlan(b, h, h_kv).rows * (d + 2) * 4 + static_cast<int64_t>(b) * 8;
 }
 
 extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
@@ -676,8 +682,10 @@ extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const v
     a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens);
     a.b = b, a.h = h, a.h_kv = h_kv, a.page_shift = exact_log2(page), a.n_pages = n_pages;
     a.max_pages = n_pages > 0 ? max_pages : 0;  // no page to read: no sequence has keys
-    a.group = plan.group, a.passes = plan.passes, a.width = plan.width, a.target = plan.target, a.scale = scale;
+    a.group = plan.group, a.passes = plan.passes, a.width = plan.width, a.scale = scale;
+    a.ws_cut = reinterpret_cast<int*>(a.ws_ml + 2 * plan.rows);
+    a.per_target = 1.00002f / static_cast<float>(plan.ranges);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dt == HS_F16) return d == 64 ? launch_paged<f16, 64>(op, st, a, plan.items) : launch_paged<f16, 128>(op, st, a, plan.items);
-    return d == 64 ? launch_paged<float, 64>(op, st, a, plan.items) : launch_paged<float, 128>(op, st, a, plan.items);
+    if (dt == HS_F16) return d == 64 ? launch_paged<f16, 64>(op, st, a, plan) : launch_paged<f16, 128>(op, st, a, plan);
+    return d == 64 ? launch_paged<float, 64>(op, st, a, plan) : launch_paged<float, 128>(op, st, a, plan);
 }
