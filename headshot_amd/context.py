@@ -73,37 +73,40 @@ def _param(t, n: int, what: str) -> int:
     return _dev(t, what)
 
 
-def _here(t: torch.Tensor, what: str) -> _Ptr:
-    """Address of a tensor of the current device, whose stream the launch goes
-    to; any strides."""
-    assert t.is_cuda, f"{what} must live in device memory"
-    current = torch.cuda.current_device() if _raw_device is None else _raw_device()
-    assert t.device.index == current, f"{what} must live on the current device"
-    p = _Ptr(t.data_ptr())
-    p.tensor = t
-    return p
+# The device that launches go to. The ops over growing sequences check every
+# tensor against it: such a call is a few microseconds on the device, so its
+# checks are written for the fewest calls into torch.
+_device = _raw_device or torch.cuda.current_device
 
 
-def _rows(t: torch.Tensor, heads: int | None, d: int, dtype, what: str):
+def _here(t: torch.Tensor, dev: int, what: str) -> int:
+    """Address of a tensor of device ``dev``; any strides."""
+    if t.get_device() != dev:
+        raise AssertionError(f"{what} must live in memory of the current device")
+    return t.data_ptr()
+
+
+def _dense(t: torch.Tensor, n: int, dtype, dev: int, what: str) -> int:
+    """Address of ``n`` contiguous values."""
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise AssertionError(f"{what} must be {n} contiguous values of {dtype}")
+    return _here(t, dev, what)
+
+
+def _rows(t: torch.Tensor, heads: int, d: int, dtype, dev: int, what: str):
     """Token rows of head vectors, (n, heads, d) or (n, heads * d), possibly
     columns of wider rows: (address, n, elements between rows)."""
-    assert t.dim() in (2, 3), f"{what} wants (n, heads, d) or (n, heads * d)"
-    assert t.dtype == dtype, f"{what} dtype"
-    width = t.shape[1] * (t.shape[2] if t.dim() == 3 else 1)
-    assert t.dim() == 2 or t.shape[2] == d, f"{what} head dim"
-    assert width == heads * d, f"{what} width {width} != {heads} heads of {d}"
-    n = t.shape[0]
-    if n and width:
-        assert t.stride(-1) == 1, f"{what}: a head vector must be contiguous"
-        assert t.dim() == 2 or t.shape[1] == 1 or t.stride(1) == d, f"{what}: a row's heads must be contiguous"
-        assert n == 1 or t.stride(0) >= width, f"{what}: rows overlap"
-    return _here(t, what), n, t.stride(0) if n > 1 else width
-
-
-def _int_array(t: torch.Tensor, n: int, what: str) -> _Ptr:
-    assert t.dtype == torch.int32, f"{what} must be int32"
-    assert t.is_contiguous() and t.numel() == n, f"{what} must be {n} contiguous values"
-    return _here(t, what)
+    shape, stride, width = t.shape, t.stride(), heads * d
+    if len(shape) == 2:
+        ok = shape[1] == width and (stride[1] == 1 or width <= 1)
+    else:
+        ok = (len(shape) == 3 and shape[1] == heads and shape[2] == d and stride[2] == 1
+              and (stride[1] == d or heads <= 1))
+    n = shape[0]
+    if t.dtype != dtype or not (ok or n == 0) or (n > 1 and stride[0] < width):
+        raise AssertionError(f"{what} wants rows of {heads} contiguous head vectors of {d} in {dtype}, "
+                             f"got {tuple(shape)} {t.dtype} with strides {stride}")
+    return _here(t, dev, what), n, stride[0] if n > 1 else width
 
 
 def _opt(t, n: int, what: str):
@@ -599,16 +602,26 @@ class HipContext:
 
     # ---------------------------------------------- sequences that grow (paged.py)
 
-    def _cache_args(self, cache):
-        """A PagedKV's (k, v, page_table, lens) addresses and shape."""
-        assert cache.k.dim() == 4 and cache.v.shape == cache.k.shape, "cache: k and v (n_pages, heads, page, d)"
-        assert cache.v.dtype == cache.k.dtype, "cache: k and v dtype"
-        assert cache.k.is_contiguous() and cache.v.is_contiguous(), "cache pages must be contiguous"
-        assert cache.page_table.dim() == 2, "page_table wants (sequences, max_pages)"
-        b, max_pages = cache.page_table.shape
-        return (_here(cache.k, "k cache"), _here(cache.v, "v cache"),
-                _int_array(cache.page_table, b * max_pages, "page_table"),
-                _int_array(cache.lens, b, "lens"), b, max_pages)
+    def _launch_held(self, name: str, fn, held, *args) -> None:
+        """``_launch`` of addresses whose tensors are ``held``."""
+        def call():
+            status = fn(_stream(), *args)
+            if status:
+                _lib.check(status, name)
+
+        call.held = held
+        call()
+        self.last_launch = call
+
+    @staticmethod
+    def _cache_shape(cache):
+        """A PagedKV's (n_pages, heads, page, d, sequences, max_pages)."""
+        k, v, table = cache.k, cache.v, cache.page_table
+        shape = k.shape
+        assert len(shape) == 4 and v.shape == shape and v.dtype == k.dtype, "cache: k and v (n_pages, heads, page, d)"
+        assert k.is_contiguous() and v.is_contiguous(), "cache pages must be contiguous"
+        assert table.dim() == 2, "page_table wants (sequences, max_pages)"
+        return (*shape, *table.shape)
 
     def kv_append(self, cache, k, v, offsets=None, q=None, qn=None, kn=None, rope=None,
                   positions=None, eps: float = 1e-5, k_rows: bool = False, out_q=None, out_k=None):
@@ -627,46 +640,49 @@ class HipContext:
         page lies outside the table or the pool is not stored, and rows behind
         ``offsets[-1]`` stay as they are. Returns (q, k) as contiguous
         rows, None for what was not asked (``q``, ``k_rows``)."""
-        kc, vc, table, lens, b, max_pages = self._cache_args(cache)
-        n_pages, h_kv, page, d = cache.k.shape
-        dtype = cache.k.dtype
+        n_pages, h_kv, page, d, b, max_pages = self._cache_shape(cache)
+        dtype, dev = cache.k.dtype, _device()
         dt = _dt(cache.k)
-        kp, n, ks = _rows(k, h_kv, d, dtype, "k")
-        vp, nv, vs = _rows(v, h_kv, d, dtype, "v")
+        kp, n, ks = _rows(k, h_kv, d, dtype, dev, "k")
+        vp, nv, vs = _rows(v, h_kv, d, dtype, dev, "v")
         assert nv == n, "k and v rows"
-        off = None if offsets is None else _int_array(offsets, b + 1, "offsets")
         assert offsets is not None or n == b, "without offsets, one token per sequence"
-        qp, qs, h, qo, ko = None, 0, 0, None, None
+        off = None if offsets is None else _dense(offsets, b + 1, torch.int32, dev, "offsets")
+        table = _dense(cache.page_table, b * max_pages, torch.int32, dev, "page_table")
+        lens = _dense(cache.lens, b, torch.int32, dev, "lens")
+        qp = qo = ko = qw = qb = kw = kb = sn = cs = pos = None
+        qs = h = rows = 0
         if q is not None:
             h = math.prod(q.shape[1:]) // d
-            qp, nq, qs = _rows(q, h, d, dtype, "q")
+            qp, nq, qs = _rows(q, h, d, dtype, dev, "q")
             assert nq == n, "q and k rows"
             if out_q is None:
                 out_q = self.empty_typed((n, h * d), dtype)
-            assert out_q.dtype == dtype and out_q.numel() == n * h * d and out_q.is_contiguous(), "out_q"
-            qo = _here(out_q, "out_q")
-        assert q is not None or (qn is None and out_q is None), "qn or out_q without q"
+            qo = _dense(out_q, n * h * d, dtype, dev, "out_q")
+            if qn is not None:
+                qw = _dense(qn[0], d, F32, dev, "q-norm weight")
+                qb = _dense(qn[1], d, F32, dev, "q-norm bias")
+        else:
+            assert qn is None and out_q is None, "qn or out_q without q"
         if k_rows or out_k is not None:
             if out_k is None:
                 out_k = self.empty_typed((n, h_kv * d), dtype)
-            assert out_k.dtype == dtype and out_k.numel() == n * h_kv * d and out_k.is_contiguous(), "out_k"
-            ko = _here(out_k, "out_k")
-        qw = qb = kw = kb = sn = cs = pos = None
-        rows = 0
-        if qn is not None:
-            qw, qb = _param(qn[0], d, "q-norm weight"), _param(qn[1], d, "q-norm bias")
+            ko = _dense(out_k, n * h_kv * d, dtype, dev, "out_k")
         if kn is not None:
-            kw, kb = _param(kn[0], d, "k-norm weight"), _param(kn[1], d, "k-norm bias")
+            kw = _dense(kn[0], d, F32, dev, "k-norm weight")
+            kb = _dense(kn[1], d, F32, dev, "k-norm bias")
         if rope is not None:
             rows = rope[0].shape[0]
-            sn = _param(rope[0], rows * d, "rope sin table")
-            cs = _param(rope[1], rows * d, "rope cos table")
+            sn = _dense(rope[0], rows * d, F32, dev, "rope sin table")
+            cs = _dense(rope[1], rows * d, F32, dev, "rope cos table")
         if positions is not None:
             assert rope is not None, "positions without rope"
-            pos = _int_array(positions, n, "positions")
-        self._launch("kv_append", self.lib.hs_kv_append, dt, qp, qs, kp, ks, vp, vs, qw, qb, kw, kb,
-                     sn, cs, rows, pos, off, table, lens, qo, ko, kc, vc, n, b, h, h_kv, d, page,
-                     n_pages, max_pages, eps)
+            pos = _dense(positions, n, torch.int32, dev, "positions")
+        self._launch_held("kv_append", self.lib.hs_kv_append,
+                          (cache, k, v, offsets, q, qn, kn, rope, positions, out_q, out_k), dt, qp, qs, kp,
+                          ks, vp, vs, qw, qb, kw, kb, sn, cs, rows, pos, off, table, lens, qo, ko,
+                          _here(cache.k, dev, "k cache"), _here(cache.v, dev, "v cache"), n, b, h, h_kv, d,
+                          page, n_pages, max_pages, eps)
         return out_q, out_k
 
     def attention_packed(self, q, k, v, offsets, k_offsets=None, causal: int = 1, scale=None,
@@ -681,24 +697,23 @@ class HipContext:
         A query that sees nothing gets zeros; rows behind ``offsets[-1]`` are
         not written. ``scale`` None is 1 / sqrt(d)."""
         assert q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "attention_packed wants (n, heads, d)"
-        h, d = q.shape[1:]
-        h_kv = k.shape[1]
-        assert offsets.dim() == 1 and offsets.numel() >= 1, "offsets wants (sequences + 1)"
+        _, h, d = q.shape
+        h_kv, dtype, dev = k.shape[1], q.dtype, _device()
         b = offsets.numel() - 1
+        assert b >= 0, "offsets wants (sequences + 1)"
         dt = _dt(q)
-        qp, n, qs = _rows(q, h, d, q.dtype, "q")
-        kp, m, ks = _rows(k, h_kv, d, q.dtype, "k")
-        vp, mv, vs = _rows(v, h_kv, d, q.dtype, "v")
+        qp, n, qs = _rows(q, h, d, dtype, dev, "q")
+        kp, m, ks = _rows(k, h_kv, d, dtype, dev, "k")
+        vp, mv, vs = _rows(v, h_kv, d, dtype, dev, "v")
         assert mv == m, "k and v rows"
         assert k_offsets is not None or m == n, "without k_offsets, as many keys as queries"
-        off = _int_array(offsets, b + 1, "offsets")
-        koff = None if k_offsets is None else _int_array(k_offsets, b + 1, "k_offsets")
+        off = _dense(offsets, b + 1, torch.int32, dev, "offsets")
+        koff = None if k_offsets is None else _dense(k_offsets, b + 1, torch.int32, dev, "k_offsets")
         if out is None:
-            out = self.empty_typed((n, h * d), q.dtype)
-        assert out.dtype == q.dtype and out.numel() == n * h * d and out.is_contiguous(), "out shape/dtype"
-        self._launch("attention_packed", self.lib.hs_attention_packed, dt, qp, qs, kp, ks, vp, vs,
-                     off, koff, _here(out, "out"), n, m, b, h, h_kv, d, causal,
-                     1.0 / math.sqrt(d) if scale is None else scale)
+            out = self.empty_typed((n, h * d), dtype)
+        self._launch_held("attention_packed", self.lib.hs_attention_packed, (q, k, v, offsets, k_offsets, out),
+                          dt, qp, qs, kp, ks, vp, vs, off, koff, _dense(out, n * h * d, dtype, dev, "out"),
+                          n, m, b, h, h_kv, d, causal, 1.0 / math.sqrt(d) if scale is None else scale)
         return out
 
     def attention_paged(self, q, cache, scale=None, out=None, workspace=None) -> torch.Tensor:
@@ -709,24 +724,27 @@ class HipContext:
         ``attention_paged_workspace`` bytes) keeps the call from allocating;
         calls that may run at the same time need one each. ``scale`` None is 1
         / sqrt(d)."""
-        kc, vc, table, lens, b, max_pages = self._cache_args(cache)
-        n_pages, h_kv, page, d = cache.k.shape
-        h = math.prod(q.shape[1:]) // d if q.dim() > 1 else 0
-        qp, n, qs = _rows(q, h, d, cache.k.dtype, "q")
+        n_pages, h_kv, page, d, b, max_pages = self._cache_shape(cache)
+        dtype, dev = cache.k.dtype, _device()
+        h = math.prod(q.shape[1:]) // d
+        qp, n, qs = _rows(q, h, d, dtype, dev, "q")
         assert n == b, "one query row per sequence"
+        table = _dense(cache.page_table, b * max_pages, torch.int32, dev, "page_table")
+        lens = _dense(cache.lens, b, torch.int32, dev, "lens")
         if out is None:
-            out = self.empty_typed((b, h * d), q.dtype)
-        assert out.dtype == q.dtype and out.numel() == b * h * d and out.is_contiguous(), "out shape/dtype"
+            out = self.empty_typed((b, h * d), dtype)
         if workspace is None:
-            workspace = self.empty_typed((self.attention_paged_workspace(b, h, h_kv, d),), torch.uint8)
-        assert workspace.dtype == torch.uint8 and workspace.is_contiguous(), "workspace wants uint8"
-        self._launch("attention_paged", self.lib.hs_attention_paged, _dt(q), qp, qs, kc, vc, table,
-                     lens, _here(out, "out"), _here(workspace, "workspace"), workspace.numel(), b, h,
-                     h_kv, d, page, n_pages, max_pages, 1.0 / math.sqrt(d) if scale is None else scale)
+            workspace = self.empty_typed((self.lib.hs_attention_paged_workspace(b, h, h_kv, d),), torch.uint8)
+        size = workspace.numel()
+        self._launch_held("attention_paged", self.lib.hs_attention_paged, (q, cache, out, workspace), _dt(cache.k),
+                          qp, qs, _here(cache.k, dev, "k cache"), _here(cache.v, dev, "v cache"), table, lens,
+                          _dense(out, b * h * d, dtype, dev, "out"),
+                          _dense(workspace, size, torch.uint8, dev, "workspace"), size, b, h, h_kv, d, page,
+                          n_pages, max_pages, 1.0 / math.sqrt(d) if scale is None else scale)
         return out
 
     def attention_paged_workspace(self, sequences: int, heads: int, kv_heads: int, d: int) -> int:
-        """Bytes of workspace of ``attention_paged``."""
+        """Bytes of workspace of ``attention_paged`` on the current device."""
         return self.lib.hs_attention_paged_workspace(sequences, heads, kv_heads, d)
 
     def bias_gelu(self, x, bias=None, out=None) -> torch.Tensor:

@@ -68,7 +68,7 @@ __device__ __forceinline__ int keys_seen(int i, int nq, int nk, int causal) {
 // Workgroup b runs on XCD b % 8: where the heads divide by it, an XCD takes
 // h / 8 heads in a row, so that the heads of a key head, and a head's tiles,
 // read their keys through one L2.
-__device__ __forceinline__ bool packed_tile(const PackedArgs& a, PackedTile& t) {
+__device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedTile& t) {
     const int b = blockIdx.x;
     int tile;
     if (a.h % kXcds == 0) {
@@ -80,10 +80,10 @@ __device__ __forceinline__ bool packed_tile(const PackedArgs& a, PackedTile& t) 
         t.head = b % a.h;
     }
     int s, local;
-    if (!find_tile(a.q_off, a.b, a.n_q, kBM, tile, s, local)) return false;
+    if (!find_tile(a.q_off, a.b, a.n_q, bm, tile, s, local)) return false;
     const RowRange q = row_range(a.q_off, s, a.n_q), k = row_range(a.k_off, s, a.n_k);
     t.q0 = q.begin, t.nq = q.end - q.begin, t.k0 = k.begin, t.nk = k.end - k.begin;
-    t.first = ((t.nq + kBM - 1) / kBM - 1 - local) * kBM;
+    t.first = ((t.nq + bm - 1) / bm - 1 - local) * bm;
     return true;
 }
 
@@ -125,7 +125,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
     constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
     __shared__ __align__(16) typename F::Smem sm;
     PackedTile t;
-    if (!packed_tile(a, t)) return;  // workgroup-uniform, before any barrier
+    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int n = lane & 31, hh = lane >> 5;
     const int kv = t.head / (a.h / a.h_kv);
@@ -333,45 +333,329 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
         }
 }
 
-// One wave per (query row, head), its lanes over the head dim, key by key.
-template <typename T, int D>
-__global__ __launch_bounds__(64) void attention_packed_kernel(
-    const T* __restrict__ q, int64_t q_stride, const T* __restrict__ k, int64_t k_stride, const T* __restrict__ v,
-    int64_t v_stride, const int* __restrict__ q_off, const int* __restrict__ k_off, T* __restrict__ out, int n_q,
-    int n_k, int b, int h, int h_kv, int causal, float scale) {
-    constexpr int E = D / 64;
-    const int row = blockIdx.x / h, head = blockIdx.x % h, kv = head / (h / h_kv);
-    const int lane = lane_id();
-    const int s = sequence_of(q_off, b, row);
-    if (s < 0) return;
-    const RowRange qr = row_range(q_off, s, n_q), kr = row_range(k_off, s, n_k);
-    const int nk = kr.end - kr.begin;
-    const int at = row - qr.begin + nk - (qr.end - qr.begin);
-    int seen = nk;
-    if (causal > 0) seen = at < 0 ? 0 : static_cast<int>(min<int64_t>(nk, (static_cast<int64_t>(at / causal) + 1) * causal));
-    float qv[E], o[E];
+// ---------------------------------------------------------------------------
+// f32
+//
+// The same transposed scheme on v_mfma_f32_32x32x2_f32: register j of a
+// 4-element piece is a product's two dims (8 g + j and 8 g + 4 + j, by lane
+// half), and score register r, the key 8 (r / 4) + 4 hh + r % 4, multiplies that
+// key's row of V as it lies. One tile in LDS, the next in registers.
+template <int D>
+struct FlashF32 {
+    static constexpr int DB = D / 32;
+    static constexpr int kRowChunks = D / 4;
+    static constexpr int kPer = kBN * kRowChunks / kThreads;
+    // floats per row: 16-byte reads of 16 rows 4 banks apart in K; in V the two
+    // halves read rows 4 apart, half the banks each
+    static constexpr int kKPitch = D + 4, kVPitch = D + 8;
+    struct Smem {
+        float k[kBN * kKPitch];
+        float v[kBN * kVPitch];
+        int odd;
+    };
+};
+
+__device__ __forceinline__ bool odd_f32(uint32_t bits) { return (bits & 0x7F800000u) == 0x7F800000u; }
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
+    using F = FlashF32<D>;
+    constexpr int DB = F::DB, kPer = F::kPer;
+    __shared__ __align__(16) typename F::Smem sm;
+    PackedTile t;
+    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
+    const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
+    const int n = lane & 31, hh = lane >> 5;
+    const int kv = t.head / (a.h / a.h_kv);
+    const float* kb = static_cast<const float*>(a.k) + t.k0 * a.k_stride + kv * D;
+    const float* vb = static_cast<const float*>(a.v) + t.k0 * a.v_stride + kv * D;
+
+    const int qi = t.first + 32 * wave + n;
+    const bool live = t.first + 32 * wave < t.nq;
+    const int seen = keys_seen(min(qi, t.nq - 1), t.nq, t.nk, a.causal);
+    const int wave_least = keys_seen(min(t.first + 32 * wave, t.nq - 1), t.nq, t.nk, a.causal);
+    const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
+    const int tile_least = keys_seen(t.first, t.nq, t.nk, a.causal);
+    const int most = keys_seen(min(t.first + kBM, t.nq) - 1, t.nq, t.nk, a.causal);
+
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
+    const uint32_t flip = a.scale < 0.0f ? 0x80000000u : 0u;
+    u32x4 qv[D / 8];
+    {
+        const float* qr = static_cast<const float*>(a.q) + (t.q0 + min(qi, t.nq - 1)) * a.q_stride + t.head * D + 4 * hh;
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        qv[e] = static_cast<float>(q[row * q_stride + head * D + lane + 64 * e]) * scale, o[e] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    for (int key = 0; key < seen; key++) {
-        const T* kp = k + (kr.begin + key) * k_stride + kv * D + lane;
-        const T* vp = v + (kr.begin + key) * v_stride + kv * D + lane;
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) dot = fmaf(qv[e], static_cast<float>(kp[64 * e]), dot);
-        const float score = wave_sum(dot);
-        const float m_new = fmaxf(m, score);
-        const float ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float corr = expf(m - ref), p = expf(score - ref);
-        l = l * corr + p;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * corr + p * static_cast<float>(vp[64 * e]);
-        m = m_new;
+        for (int i = 0; i < D / 8; i++) qv[i] = ld16(qr + 8 * i) ^ flip;
     }
+    f32x16 o[DB];
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        out[(static_cast<int64_t>(row) * h + head) * D + lane + 64 * e] = static_cast<T>(seen > 0 ? o[e] / l : 0.0f);
+    for (int i = 0; i < DB; i++) o[i] = f32x16{};
+    float m = -3.0e38f, l = 0.0f;
+
+    u32x4 pk[kPer], pv[kPer];
+    const int row0 = tid / F::kRowChunks, col0 = tid % F::kRowChunks * 4;
+    constexpr int kRowStep = kThreads / F::kRowChunks;
+    auto load = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int64_t row = min(key0 + row0 + kRowStep * i, t.nk - 1);  // past the end: masked
+            pk[i] = ld16(kb + row * a.k_stride + col0);
+            pv[i] = ld16(vb + row * a.v_stride + col0);
+        }
+    };
+    if (tid == 0) sm.odd = 0;
+    if (most > 0) load(0);
+#pragma unroll 1
+    for (int key0 = 0; key0 < most; key0 += kBN) {
+        __syncthreads();  // the previous tile has been read
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            st16(&sm.k[(row0 + kRowStep * i) * F::kKPitch + col0], pk[i]);
+            st16(&sm.v[(row0 + kRowStep * i) * F::kVPitch + col0], pv[i]);
+            if (key0 + kBN > tile_least)  // some query does not see all of these values
+#pragma unroll
+                for (int w = 0; w < 4; w++) odd |= odd_f32(pv[i][w]);
+        }
+        if (odd) sm.odd = key0 + 1;
+        __syncthreads();
+        if (key0 + kBN < most) load(key0 + kBN);
+        if (key0 >= wave_most) continue;
+
+        f32x16 s[2] = {f32x16{}, f32x16{}};
+        const float* ka = sm.k + n * F::kKPitch + 4 * hh;
+#pragma unroll
+        for (int g = 0; g < D / 8; g++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const u32x4 x = ld16(ka + 32 * i * F::kKPitch + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(x[e]), u2f(qv[g][e]), s[i], 0, 0, 0);
+            }
+        const bool partial = key0 + kBN > wave_least;
+        if (partial) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (key0 + 32 * i + 8 * (r / 4) + 4 * hh + r % 4 >= seen) s[i][r] = -INFINITY;
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[i][r]);
+        const float next = fmaxf(m, halves_max(mx) * c);
+        const float corr = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -m));
+                sum += s[i][r];
+            }
+        l = fmaf(l, corr, sum);
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[i] *= corr;
+        const float* va = sm.v + 4 * hh * F::kVPitch + n;
+        if (partial && sm.odd == key0 + 1) {
+            // Infinities or NaN among values that not every query sees: key by
+            // key, each into the queries that see it.
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int key = 32 * i + 8 * (r / 4) + r % 4;
+#pragma unroll 1
+                    for (int half = 0; half < 2; half++)
+#pragma unroll
+                        for (int db = 0; db < DB; db++) {
+                            const float x = hh == half ? va[key * F::kVPitch + 32 * db] : 0.0f;
+                            const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x2f32(x, hh == half ? s[i][r] : 0.0f, f32x16{}, 0, 0, 0);
+                            if (key0 + key + 4 * half < seen) o[db] += add;
+                        }
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+#pragma unroll
+                    for (int db = 0; db < DB; db++)
+                        o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(va[(32 * i + 8 * (r / 4) + r % 4) * F::kVPitch + 32 * db], s[i][r],
+                                                                     o[db], 0, 0, 0);
+        }
+    }
+
+    if (qi >= t.nq) return;
+    const float lsum = halves_sum(l);
+    float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = f2u(seen > 0 ? o[db][4 * r4 + e] / lsum : 0.0f);
+            st16(orow + 32 * db + 8 * r4, w);
+        }
+}
+
+// f32, short sequences: a serial chain per query, so it is cut as finely as the
+// matrix instructions allow. A workgroup takes 16 queries and its four waves
+// share their keys, 16 at a time in turn, on v_mfma_f32_16x16x4_f32: K as the A
+// operand straight from memory, V through the wave's own slice of LDS; the four
+// (O, m, l) join in LDS.
+template <int D>
+struct FewF32 {
+    static constexpr int kQueries = 16;
+    static constexpr int kRowLanes = D / 4, kVRows = 64 / kRowLanes, kVLoads = 16 / kVRows;
+    static constexpr int kPitch = D + 4;
+    struct Smem {
+        union {
+            float v[kWaves][16 * kPitch];
+            float o[kWaves][kQueries * kPitch];
+        };
+        float m[kWaves][kQueries], l[kWaves][kQueries];
+    };
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void packed_few_f32_kernel(PackedArgs a) {
+    using F = FewF32<D>;
+    constexpr int KS = D / 16, DB = D / 16;
+    __shared__ __align__(16) typename F::Smem sm;
+    PackedTile t;
+    if (!packed_tile(a, F::kQueries, t)) return;  // workgroup-uniform, before any barrier
+    const int lane = lane_id(), wave = wave_in_block();
+    const int n = lane & 15, g = lane >> 4;
+    const int kv = t.head / (a.h / a.h_kv);
+    const float* kb = static_cast<const float*>(a.k) + t.k0 * a.k_stride + kv * D;
+    const float* vb = static_cast<const float*>(a.v) + t.k0 * a.v_stride + kv * D;
+    const int qi = t.first + n;
+    const int seen = keys_seen(min(qi, t.nq - 1), t.nq, t.nk, a.causal);
+    const int least = keys_seen(t.first, t.nq, t.nk, a.causal);
+    const int most = keys_seen(min(t.first + F::kQueries, t.nq) - 1, t.nq, t.nk, a.causal);
+
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
+    const uint32_t flip = a.scale < 0.0f ? 0x80000000u : 0u;
+    const float* qr = static_cast<const float*>(a.q) + (t.q0 + min(qi, t.nq - 1)) * a.q_stride + t.head * D + 4 * g;
+    u32x4 qv[KS];
+#pragma unroll
+    for (int i = 0; i < KS; i++) qv[i] = ld16(qr + 16 * i) ^ flip;
+    f32x4 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] = f32x4{};
+    float m = -3.0e38f, l = 0.0f;  // l: this lane's keys only
+    float* vs = sm.v[wave];
+    u32x4 kr[KS], vr[F::kVLoads];
+    auto load_v = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < F::kVLoads; i++) {
+            const int64_t row = min(key0 + F::kVRows * i + lane / F::kRowLanes, t.nk - 1);
+            vr[i] = ld16(vb + row * a.v_stride + lane % F::kRowLanes * 4);
+        }
+    };
+    auto load_k = [&](int key0) {
+        const float* kp = kb + static_cast<int64_t>(min(key0 + n, t.nk - 1)) * a.k_stride + 4 * g;
+#pragma unroll
+        for (int i = 0; i < KS; i++) kr[i] = ld16(kp + 16 * i);
+    };
+    constexpr int kTurn = 16 * kWaves;
+    if (16 * wave < most) load_v(16 * wave), load_k(16 * wave);
+#pragma unroll 1
+    for (int key0 = 16 * wave; key0 < most; key0 += kTurn) {
+        const bool partial = key0 + 16 > least;  // some query does not see all of these keys
+        bool odd = false;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < F::kVLoads; i++) {
+            st16(vs + (F::kVRows * i + lane / F::kRowLanes) * F::kPitch + lane % F::kRowLanes * 4, vr[i]);
+            if (partial)
+#pragma unroll
+                for (int w = 0; w < 4; w++) odd |= odd_f32(vr[i][w]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (key0 + kTurn < most) load_v(key0 + kTurn);
+        f32x4 acc[4] = {f32x4{}, f32x4{}, f32x4{}, f32x4{}};
+#pragma unroll
+        for (int i = 0; i < KS; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(u2f(kr[i][e]), u2f(qv[i][e]), acc[e], 0, 0, 0);
+        f32x4 s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+        if (key0 + kTurn < most) load_k(key0 + kTurn);
+        if (partial)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (key0 + 4 * g + j >= seen) s[j] = -INFINITY;
+        float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
+        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+        const float next = fmaxf(m, mx * c);
+        const float corr = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -m));
+            sum += s[j];
+        }
+        l = fmaf(l, corr, sum);
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[i] *= corr;
+        const float* va = vs + 4 * g * F::kPitch + n;
+        if (partial && __any(odd)) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll 1
+                for (int x = 0; x < 4; x++)
+#pragma unroll
+                    for (int i = 0; i < DB; i++) {
+                        const f32x4 add = __builtin_amdgcn_mfma_f32_16x16x4f32(g == x ? va[j * F::kPitch + 16 * i] : 0.0f,
+                                                                               g == x ? s[j] : 0.0f, f32x4{}, 0, 0, 0);
+                        if (key0 + 4 * x + j < seen) o[i] += add;
+                    }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int i = 0; i < DB; i++)
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[j * F::kPitch + 16 * i], s[j], o[i], 0, 0, 0);
+        }
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < DB; i++) *reinterpret_cast<f32x4*>(&sm.o[wave][n * F::kPitch + 16 * i + 4 * g]) = o[i];
+    if (g == 0) sm.m[wave][n] = m, sm.l[wave][n] = l;
+    __syncthreads();
+    for (int x = threadIdx.x; x < F::kQueries * (D / 4); x += kThreads) {
+        const int q = x / (D / 4), d0 = x % (D / 4) * 4;
+        if (t.first + q >= t.nq) break;
+        const int keys = keys_seen(t.first + q, t.nq, t.nk, a.causal);
+        float top = sm.m[0][q];
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) top = fmaxf(top, sm.m[w][q]);
+        f32x4 sum = {};
+        float weight = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(sm.m[w][q] - top);
+            sum += *reinterpret_cast<const f32x4*>(&sm.o[w][q * F::kPitch + d0]) * f;
+            weight = fmaf(sm.l[w][q], f, weight);
+        }
+        float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + t.first + q) * a.h + t.head) * D + d0;
+        u32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = f2u(keys > 0 ? sum[e] / weight : 0.0f);
+        st16(orow, w);
+    }
 }
 
 }  // namespace
@@ -410,34 +694,18 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     a.k_off = static_cast<const int*>(k_offsets ? k_offsets : q_offsets);
     a.n_q = static_cast<int>(n_q), a.n_k = static_cast<int>(n_k), a.b = b, a.h = h, a.h_kv = h_kv;
     a.causal = causal, a.scale = scale;
-    // as many tiles as sequences of these rows can have
-    const int64_t tiles = n_q / kBM + (b < n_q ? b : n_q);
-    if (tiles * h >= (int64_t{1} << 31) / kThreads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
-    a.tiles = static_cast<int>(tiles);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dt == HS_F16) {
-        const dim3 grid(static_cast<uint32_t>(tiles * h));
-        if (d == 64)
-            packed_f16_kernel<64><<<grid, dim3(kThreads), 0, st>>>(a);
-        else
-            packed_f16_kernel<128><<<grid, dim3(kThreads), 0, st>>>(a);
+    // as many tiles as sequences of these rows can have
+    const auto go = [&](auto kernel, int bm) {
+        const int64_t tiles = n_q / bm + (b < n_q ? b : n_q);
+        if (tiles * h >= (int64_t{1} << 31) / kThreads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
+        a.tiles = static_cast<int>(tiles);
+        kernel<<<dim3(static_cast<uint32_t>(tiles * h)), dim3(kThreads), 0, st>>>(a);
         return check_launch(op);
-    }
-    const auto run = [&](auto zero) {
-        using T = decltype(zero);
-        const dim3 grid(static_cast<uint32_t>(n_q * h));
-        const auto go = [&](auto kernel) {
-            kernel<<<grid, dim3(64), 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const T*>(q), q_stride, static_cast<const T*>(k), k_stride, static_cast<const T*>(v),
-                v_stride, static_cast<const int*>(q_offsets),
-                static_cast<const int*>(k_offsets ? k_offsets : q_offsets), static_cast<T*>(out),
-                static_cast<int>(n_q), static_cast<int>(n_k), b, h, h_kv, causal, scale);
-        };
-        if (d == 64)
-            go(attention_packed_kernel<T, 64>);
-        else
-            go(attention_packed_kernel<T, 128>);
     };
-    run(float{});
-    return check_launch(op);
+    if (dt == HS_F16) return d == 64 ? go(packed_f16_kernel<64>, kBM) : go(packed_f16_kernel<128>, kBM);
+    // Tiles of 32 queries a wave where they fill the chip's SIMDs, else 16 by
+    // four waves
+    if ((n_q / 32 + b) * h >= 4 * num_cus()) return d == 64 ? go(packed_f32_kernel<64>, kBM) : go(packed_f32_kernel<128>, kBM);
+    return d == 64 ? go(packed_few_f32_kernel<64>, 16) : go(packed_few_f32_kernel<128>, 16);
 }

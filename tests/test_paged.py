@@ -129,11 +129,10 @@ def test_workspace_of_refused_shapes():
 def surface(monkeypatch):
     """A HipContext whose launches are recorded: CPU tensors stand in."""
     calls = []
-    monkeypatch.setattr(context, "_here", lambda t, what: context._Ptr(t.data_ptr() or 16))
-    monkeypatch.setattr(context, "_dev", lambda t, what: context._Ptr(t.data_ptr() or 16))
+    monkeypatch.setattr(context, "_device", lambda: -1)  # what get_device() says of a CPU tensor
     ctx = context.HipContext.__new__(context.HipContext)
     ctx.lib, ctx.device, ctx.last_launch = L, torch.device("cpu"), None
-    ctx._launch = lambda name, fn, *args: calls.append((name, args))
+    ctx._launch_held = lambda name, fn, held, *args: calls.append((name, args))
     return ctx, calls
 
 
@@ -205,13 +204,16 @@ def test_python_attention(surface):
 def test_tensors_of_another_device():
     """The launch goes to the current device's stream: a tensor elsewhere is
     refused before it."""
-    with pytest.raises(AssertionError, match="device memory"):
-        context._here(torch.zeros(3), "k")
+    with pytest.raises(AssertionError, match="current device"):
+        context._here(torch.zeros(3), 0, "k")
 
     class Elsewhere:
-        is_cuda, device = True, torch.device("cuda", 1)
+        def get_device(self):
+            return 1
 
-    with pytest.MonkeyPatch.context() as m:
-        m.setattr(context, "_raw_device", lambda: 0)
-        with pytest.raises(AssertionError, match="current device"):
-            context._here(Elsewhere(), "k")
+        def data_ptr(self):
+            return 16
+
+    assert context._here(Elsewhere(), 1, "k") == 16
+    with pytest.raises(AssertionError, match="current device"):
+        context._here(Elsewhere(), 0, "k")
