@@ -64,17 +64,18 @@ __device__ __forceinline__ int keys_seen(int i, int nq, int nk, int causal) {
     return end < nk ? static_cast<int>(end) : nk;
 }
 
-// Workgroup b's tile. A sequence's last queries see the most keys and go first.
-// Workgroup b runs on XCD b % 8: where the heads divide by it, an XCD takes
-// h / 8 heads in a row, so that the heads of a key head, and a head's tiles,
-// read their keys through one L2.
+// Workgroup b's tile. A sequence's last queries see the most keys and go first,
+// tile by tile over the heads, so that the first workgroups, two and more to a
+// CU, are not all a head's longest. Workgroup b runs on XCD b % 8: where the
+// heads divide by it, an XCD takes h / 8 heads in a row, so that the heads of a
+// key head, and a head's tiles, read their keys through one L2.
 __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedTile& t) {
     const int b = blockIdx.x;
     int tile;
     if (a.h % kXcds == 0) {
-        const int slot = b / kXcds;
-        tile = slot % a.tiles;
-        t.head = b % kXcds * (a.h / kXcds) + slot / a.tiles;
+        const int slot = b / kXcds, heads = a.h / kXcds;
+        tile = slot / heads;
+        t.head = b % kXcds * heads + slot % heads;
     } else {
         tile = b / a.h;
         t.head = b % a.h;
@@ -87,6 +88,28 @@ __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedT
     return true;
 }
 
+// An infinity or NaN among a tile's values, where some queries see them and
+// others do not, must not meet the others' weights, which are 0: such values go
+// into LDS as zeros, and a workgroup that has met any adds them here to the sums
+// of the queries that do see them. A weight is positive, so what they make of a
+// sum is what they sum to. First: the first key that some query of the workgroup
+// does not see; o as the kernels hold it, channel 32 db + 8 (r / 4) + 4 hh + r %
+// 4 in register r.
+template <typename T, int DB>
+__device__ __forceinline__ void add_odd(f32x16 (&o)[DB], const PackedArgs& a, const PackedTile& t, int kv, int first,
+                                        int seen, int hh) {
+    for (int key = first / kBN * kBN; key < seen; key++) {
+        const T* row = static_cast<const T*>(a.v) + (t.k0 + key) * a.v_stride + kv * 32 * DB + 4 * hh;
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float x = static_cast<float>(row[32 * db + 8 * (r / 4) + r % 4]);
+                if ((f2u(x) & 0x7F800000u) == 0x7F800000u) o[db][r] += x;
+            }
+    }
+}
+
 // ---------------------------------------------------------------------------
 // f16
 //
@@ -96,26 +119,36 @@ __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedT
 // through LDS 64 at a time, double-buffered, the next tile's rows in registers
 // while the current one computes; V^T comes through the transposing LDS read
 // and takes P^T from the registers that the scores were in.
+//
+// LDS rows are not padded, so that four workgroups (head dim 64) or two (128)
+// fit a CU; a row's 16-byte pieces are permuted instead: 16 rows' reads of K at
+// one column, and the transposing read's 4 rows of 64 bytes, touch every bank
+// once.
 template <int D>
 struct FlashF16 {
     static constexpr int KS = D / 16;             // 16-dim slices of a score
     static constexpr int DB = D / 32;             // 32-channel blocks of an output
-    static constexpr int kRowChunks = D / 8;      // 16-byte pieces of a row
-    static constexpr int kPer = kBN * kRowChunks / kThreads;
-    // Row pitches in halves. 16-byte reads of 16 rows at a time start 4 banks
-    // (of 64) apart in K, and the transposing read's 4 rows of 64 bytes take a
-    // quarter of the banks each in V: no conflicts.
-    static constexpr int kKPitch = D + 8, kVPitch = D + 32;
+    static constexpr int kPieces = D / 8;         // 16-byte pieces of a row
+    static constexpr int kPer = kBN * kPieces / kThreads;
+    static constexpr int kRowStep = kThreads / kPieces;  // rows per load of the workgroup
     struct Smem {
-        f16 k[2][kBN * kKPitch];
-        f16 v[2][kBN * kVPitch];
-        int odd[2];  // the buffer's V tile holds an infinity or NaN
+        f16 k[2][kBN * D];
+        f16 v[2][kBN * D];
+        int odd;  // a tile whose values not every query sees holds an infinity or NaN
     };
+    // What piece numbers are xored with in a row; the same in rows 16 apart.
+    static __device__ __forceinline__ int k_swap(int row) { return D == 64 ? row >> 1 & 7 : row & 15; }
+    static __device__ __forceinline__ int v_swap(int row) { return D == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
 };
 
 // A weight's exponent may run this far (log2) above the reference maximum
 // before the reference moves.
 constexpr float kLazyMax = 8.0f;
+// A running maximum before any score. It is finite, so that a masked score
+// weighs exp2(-inf - kFloor) = 0 against it.
+constexpr float kFloor = -3.0e38f;
+// A maximum (log2) beyond which its rounding, 2^-24 of it, shows in a weight.
+constexpr float kFar = 65536.0f;
 // A lane's row sum over a tile beyond which a weight may not fit f16.
 constexpr float kRowSumMax = 32768.0f;
 
@@ -129,8 +162,6 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int n = lane & 31, hh = lane >> 5;
     const int kv = t.head / (a.h / a.h_kv);
-    const f16* kb = static_cast<const f16*>(a.k) + t.k0 * a.k_stride + kv * D;
-    const f16* vb = static_cast<const f16*>(a.v) + t.k0 * a.v_stride + kv * D;
 
     // The keys seen grow with the query: the tile's last live query has the most
     const int qi = t.first + 32 * wave + n;
@@ -163,40 +194,61 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
-    // a finite floor: a tile of masked scores then weighs exp2(-inf) = 0
-    float m = -3.0e38f, l = 0.0f;
+    float m = kFloor, l = 0.0f;
 
+    // Staging: load i of the thread is row row0 + kRowStep i, piece `piece`. The
+    // tile's address is the scalar part of the load's, the thread's the other.
+    const int row0 = tid / F::kPieces, piece = tid % F::kPieces;
+    const uint32_t k_off = (row0 * static_cast<uint32_t>(a.k_stride) + piece * 8) * 2;
+    const uint32_t v_off = (row0 * static_cast<uint32_t>(a.v_stride) + piece * 8) * 2;
+    const char* kb = reinterpret_cast<const char*>(static_cast<const f16*>(a.k) + t.k0 * a.k_stride + kv * D);
+    const char* vb = reinterpret_cast<const char*>(static_cast<const f16*>(a.v) + t.k0 * a.v_stride + kv * D);
     u32x4 pk[kPer], pv[kPer];
-    const int row0 = tid / F::kRowChunks, col0 = tid % F::kRowChunks * 8;
-    constexpr int kRowStep = kThreads / F::kRowChunks;
     auto load = [&](int key0) {
+        const char* kt = kb + static_cast<int64_t>(key0) * a.k_stride * 2;
+        const char* vt = vb + static_cast<int64_t>(key0) * a.v_stride * 2;
+        if (key0 + kBN <= t.nk) {
 #pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            const int64_t row = min(key0 + row0 + kRowStep * i, t.nk - 1);  // past the end: masked
-            pk[i] = ld16(kb + row * a.k_stride + col0);
-            pv[i] = ld16(vb + row * a.v_stride + col0);
+            for (int i = 0; i < kPer; i++) {
+                pk[i] = ld16(kt + static_cast<int64_t>(i * F::kRowStep) * a.k_stride * 2 + k_off);
+                pv[i] = ld16(vt + static_cast<int64_t>(i * F::kRowStep) * a.v_stride * 2 + v_off);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; i++) {
+                const uint32_t row = min(row0 + i * F::kRowStep, t.nk - 1 - key0);  // past the end: masked
+                pk[i] = ld16(kt + (row * static_cast<uint32_t>(a.k_stride) + piece * 8) * 2);
+                pv[i] = ld16(vt + (row * static_cast<uint32_t>(a.v_stride) + piece * 8) * 2);
+            }
         }
     };
+    const int k_at = row0 * D + (piece ^ F::k_swap(row0)) * 8, v_at = row0 * D + (piece ^ F::v_swap(row0)) * 8;
     auto store = [&](int buf, int key0) {
-#pragma unroll
-        for (int i = 0; i < kPer; i++) {
-            st16(&sm.k[buf][(row0 + kRowStep * i) * F::kKPitch + col0], pk[i]);
-            st16(&sm.v[buf][(row0 + kRowStep * i) * F::kVPitch + col0], pv[i]);
-        }
         if (key0 + kBN > tile_least) {  // some query does not see all of these values
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < kPer; i++)
 #pragma unroll
-                for (int w = 0; w < 4; w++)
-                    odd |= (pv[i][w] & 0x7C00u) == 0x7C00u || (pv[i][w] & 0x7C000000u) == 0x7C000000u;
-            if (odd) sm.odd[buf] = key0 + 1;
+                for (int w = 0; w < 4; w++) {
+                    const uint32_t x = pv[i][w];
+                    const uint32_t keep = ((x & 0x7C00u) == 0x7C00u ? 0u : 0xFFFFu) | ((x & 0x7C000000u) == 0x7C000000u ? 0u : 0xFFFF0000u);
+                    odd |= keep != 0xFFFFFFFFu;
+                    pv[i][w] = x & keep;
+                }
+            if (odd) sm.odd = 1;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            st16(&sm.k[buf][k_at + i * F::kRowStep * D], pk[i]);
+            st16(&sm.v[buf][v_at + i * F::kRowStep * D], pv[i]);
         }
     };
-    if (tid < 2) sm.odd[tid] = 0;
-    if (ntiles > 0) load(0);
+    if (tid == 0) sm.odd = 0;
     __syncthreads();
-    if (ntiles > 0) store(0, 0);
+    if (ntiles > 0) {
+        load(0);
+        store(0, 0);
+    }
     __syncthreads();
     for (int j = 0; j < ntiles; j++) {
         const int cur = j & 1, key0 = j * kBN;
@@ -206,15 +258,15 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
             // lane (n, hh) key 8 (r / 4) + 4 hh + r % 4, query n
             f32x16 s[2];
             const f32x16 z = {};
-            const f16* ka = sm.k[cur] + n * F::kKPitch + 8 * hh;
+            const f16* ka = sm.k[cur] + n * D;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++)
+            for (int ks = 0; ks < KS; ks++) {
+                const int at = ((2 * ks + hh) ^ F::k_swap(n)) * 8;
 #pragma unroll
                 for (int i = 0; i < 2; i++)
-                    s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(ld16(ka + 32 * i * F::kKPitch + 16 * ks)), qa[ks],
-                                                                  ks ? s[i] : z, 0, 0, 0);
-            const bool partial = key0 + kBN > wave_least;
-            if (partial) {
+                    s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(ld16(ka + 32 * i * D + at)), qa[ks], ks ? s[i] : z, 0, 0, 0);
+            }
+            if (key0 + kBN > wave_least) {
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -226,14 +278,14 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
             // each, inside the result's own rounding), and the sum of the
             // rounded ones over the lane's keys: two packed f16 levels (sums
             // of four), then f32.
-            auto weights = [&](float ref) {
+            auto weights = [&](float mul, float ref) {
                 f16x2 w2[16];
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int r = 0; r < 16; r += 2) {
-                        const uint32_t w = pk_f16(__builtin_amdgcn_exp2f(fmaf(s[i][r], c, -ref)),
-                                                  __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], c, -ref)));
+                        const uint32_t w = pk_f16(__builtin_amdgcn_exp2f(fmaf(s[i][r], mul, -ref)),
+                                                  __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], mul, -ref)));
                         p[i][r / 8][r % 8 / 2] = w;
                         w2[8 * i + r / 2] = u2h2(w);
                     }
@@ -250,9 +302,9 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
             // Past the first tile the weights are taken against the reference
             // as it is; only a query whose sum says that one may not fit f16
             // moves its own.
-            bool own = j == 0, move = own;
+            bool own = j == 0 || fabsf(m) > kFar, move = __any(own);
             if (!move) {
-                const float sum = weights(m);
+                const float sum = weights(c, m);
                 own = !(halves_max(sum) <= kRowSumMax) || !(sum <= kRowSumMax);
                 move = __any(own);
                 if (!move) l += sum;
@@ -266,58 +318,44 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
                 const float cand = fmaxf(m, halves_max(mx) * c);
                 const float next = own && cand > m + kLazyMax ? cand : m;
                 const float corr = __builtin_amdgcn_exp2f(m - next);
-                l = fmaf(l, corr, weights(next));
+                // The multiply-add leaves the rounding of s c in the exponent:
+                // where that is not small, the product is rounded first, as
+                // the reference's was.
+                const bool far = __any(fabsf(next) > kFar);
+                if (far) {
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) s[i][r] = as_f32(s[i][r] * c) - next;
+                }
+                l = fmaf(l, corr, weights(far ? 1.0f : c, far ? 0.0f : next));
                 m = next;
 #pragma unroll
                 for (int i = 0; i < DB; i++) o[i] *= corr;
             }
             // O^T += V^T P^T. The transposing read gives lane i of 16 channel
             // i of 4 keys: two reads make the 8 keys, in the scores' order.
-            const int l16 = n & 15;
-            const f16* va = sm.v[cur] + (4 * hh + l16 / 4) * F::kVPitch + (n & 16) + 4 * (l16 % 4);
+            const int vrow = 4 * hh + (n & 15) / 4;
+            const f16* va = sm.v[cur] + vrow * D + (n & 16) + 4 * (n & 3);
             auto read_v = [&](int g, int db) {
-                const f16* r0 = va + 16 * g * F::kVPitch + 32 * db;
+                const f16* r0 = va + 16 * g * D + ((4 * db) ^ F::v_swap(vrow)) * 8;
                 const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)r0));
-                const u32x2 hi =
-                    __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(r0 + 8 * F::kVPitch)));
+                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(r0 + 8 * D)));
                 u32x4 w;
                 w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
                 return w;
             };
-            if (partial && sm.odd[cur] == key0 + 1) {
-                // Infinities or NaN among values that not every query sees:
-                // key by key, each into the queries that see it.
 #pragma unroll
-                for (int g = 0; g < 4; g++)
-#pragma unroll 1
-                    for (int e = 0; e < 16; e++) {
-                        const int el = (e & 3) + 4 * (e >> 3);  // its element in the lanes with hh == e / 4 % 2
-                        const uint32_t keep = hh == (e >> 2 & 1) ? (el & 1 ? 0xFFFF0000u : 0xFFFFu) : 0u;
-                        u32x4 one = {}, w;
+            for (int g = 0; g < 4; g++)
 #pragma unroll
-                        for (int x = 0; x < 4; x++) one[x] = x == el / 2 ? p[g / 2][g % 2][x] & keep : 0u;
-#pragma unroll
-                        for (int db = 0; db < DB; db++) {
-                            w = read_v(g, db);
-#pragma unroll
-                            for (int x = 0; x < 4; x++) w[x] = x == el / 2 ? w[x] & keep : 0u;
-                            const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(w), as_h8(one), z, 0, 0, 0);
-                            if (key0 + 16 * g + e < seen) o[db] += add;
-                        }
-                    }
-            } else {
-#pragma unroll
-                for (int g = 0; g < 4; g++)
-#pragma unroll
-                    for (int db = 0; db < DB; db++)
-                        o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(read_v(g, db)), as_h8(p[g / 2][g % 2]), o[db], 0, 0, 0);
-            }
+                for (int db = 0; db < DB; db++)
+                    o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(read_v(g, db)), as_h8(p[g / 2][g % 2]), o[db], 0, 0, 0);
         }
         if (j + 1 < ntiles) store(cur ^ 1, key0 + kBN);
         __syncthreads();
     }
-
     if (qi >= t.nq) return;
+    if (ntiles > 0 && sm.odd) add_odd<f16, DB>(o, a, t, kv, tile_least, seen, hh);
     const float inv = 1.0f / halves_sum(l);
     f16* orow = static_cast<f16*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
 #pragma unroll
@@ -357,13 +395,12 @@ struct FlashF32 {
 
 __device__ __forceinline__ bool odd_f32(uint32_t bits) { return (bits & 0x7F800000u) == 0x7F800000u; }
 
+// The tile's queries, those of lanes with `mine` stored; every wave of the
+// workgroup calls it (barriers inside).
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
+__device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const PackedTile& t, typename FlashF32<D>::Smem& sm, bool mine) {
     using F = FlashF32<D>;
     constexpr int DB = F::DB, kPer = F::kPer;
-    __shared__ __align__(16) typename F::Smem sm;
-    PackedTile t;
-    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int n = lane & 31, hh = lane >> 5;
     const int kv = t.head / (a.h / a.h_kv);
@@ -389,7 +426,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
     f32x16 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
-    float m = -3.0e38f, l = 0.0f;
+    float m = kFloor, l = 0.0f;
 
     u32x4 pk[kPer], pv[kPer];
     const int row0 = tid / F::kRowChunks, col0 = tid % F::kRowChunks * 4;
@@ -402,21 +439,26 @@ __global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
             pv[i] = ld16(vb + row * a.v_stride + col0);
         }
     };
+    __syncthreads();
     if (tid == 0) sm.odd = 0;
     if (most > 0) load(0);
 #pragma unroll 1
     for (int key0 = 0; key0 < most; key0 += kBN) {
         __syncthreads();  // the previous tile has been read
-        bool odd = false;
+        if (key0 + kBN > tile_least) {  // some query does not see all of these values
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < kPer; i++)
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    if (odd_f32(pv[i][w])) odd = true, pv[i][w] = 0;
+            if (odd) sm.odd = 1;
+        }
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             st16(&sm.k[(row0 + kRowStep * i) * F::kKPitch + col0], pk[i]);
             st16(&sm.v[(row0 + kRowStep * i) * F::kVPitch + col0], pv[i]);
-            if (key0 + kBN > tile_least)  // some query does not see all of these values
-#pragma unroll
-                for (int w = 0; w < 4; w++) odd |= odd_f32(pv[i][w]);
         }
-        if (odd) sm.odd = key0 + 1;
         __syncthreads();
         if (key0 + kBN < most) load(key0 + kBN);
         if (key0 >= wave_most) continue;
@@ -432,20 +474,23 @@ __global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
                 for (int e = 0; e < 4; e++)
                     s[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(u2f(x[e]), u2f(qv[g][e]), s[i], 0, 0, 0);
             }
-        const bool partial = key0 + kBN > wave_least;
-        if (partial) {
+        if (key0 + kBN > wave_least) {
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int r = 0; r < 16; r++)
                     if (key0 + 32 * i + 8 * (r / 4) + 4 * hh + r % 4 >= seen) s[i][r] = -INFINITY;
         }
-        float mx = s[0][0];
+        // rounded before the maximum is taken off: that one then weighs 1
+        float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[i][r]);
-        const float next = fmaxf(m, halves_max(mx) * c);
+            for (int r = 0; r < 16; r++) {
+                s[i][r] = as_f32(s[i][r] * c);
+                mx = fmaxf(mx, s[i][r]);
+            }
+        const float next = fmaxf(m, halves_max(mx));
         const float corr = __builtin_amdgcn_exp2f(m - next);
         m = next;
         float sum = 0.0f;
@@ -453,31 +498,13 @@ __global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
         for (int i = 0; i < 2; i++)
 #pragma unroll
             for (int r = 0; r < 16; r++) {
-                s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], c, -m));
+                s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - m);
                 sum += s[i][r];
             }
         l = fmaf(l, corr, sum);
 #pragma unroll
         for (int i = 0; i < DB; i++) o[i] *= corr;
         const float* va = sm.v + 4 * hh * F::kVPitch + n;
-        if (partial && sm.odd == key0 + 1) {
-            // Infinities or NaN among values that not every query sees: key by
-            // key, each into the queries that see it.
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int r = 0; r < 16; r++) {
-                    const int key = 32 * i + 8 * (r / 4) + r % 4;
-#pragma unroll 1
-                    for (int half = 0; half < 2; half++)
-#pragma unroll
-                        for (int db = 0; db < DB; db++) {
-                            const float x = hh == half ? va[key * F::kVPitch + 32 * db] : 0.0f;
-                            const f32x16 add = __builtin_amdgcn_mfma_f32_32x32x2f32(x, hh == half ? s[i][r] : 0.0f, f32x16{}, 0, 0, 0);
-                            if (key0 + key + 4 * half < seen) o[db] += add;
-                        }
-                }
-        } else {
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -486,10 +513,10 @@ __global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
                     for (int db = 0; db < DB; db++)
                         o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(va[(32 * i + 8 * (r / 4) + r % 4) * F::kVPitch + 32 * db], s[i][r],
                                                                      o[db], 0, 0, 0);
-        }
     }
-
-    if (qi >= t.nq) return;
+    __syncthreads();
+    if (qi >= t.nq || !mine) return;
+    if (sm.odd) add_odd<float, DB>(o, a, t, kv, tile_least, seen, hh);
     const float lsum = halves_sum(l);
     float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
 #pragma unroll
@@ -501,6 +528,291 @@ __global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
             for (int e = 0; e < 4; e++) w[e] = f2u(seen > 0 ? o[db][4 * r4 + e] / lsum : 0.0f);
             st16(orow + 32 * db + 8 * r4, w);
         }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
+    __shared__ __align__(16) typename FlashF32<D>::Smem sm;
+    PackedTile t;
+    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
+    packed_f32_tile<D>(a, t, sm, true);
+}
+
+// f32, head dim 64, on the bf16 matrix instructions, sixteen times the f32
+// ones' rate: each value is three bf16 (split3) and a product six of theirs
+// with f32 accumulators, to 2^-24 of it as one f32 rounding. Queries are split
+// once, K and V as their tiles are staged, the weights where the f16 kernel
+// rounds them. The small products are summed ahead of the large one in the
+// scores and in accumulators of their own in the output, so that they add no
+// rounding of full size; a weight carries a factor 2^23, so that it keeps its 24
+// bits down to 2^-126 of the largest. One tile in LDS (two workgroups per CU:
+// one stages while the other multiplies), the next in registers.
+//
+// A query above 2^50 in magnitude, and every query of a tile that stages such a
+// key or value, an infinity or NaN, or a nonzero value below 2^-100 (where
+// bf16's last part ends), is computed again on the f32 instructions.
+typedef bf16x8 b8;
+constexpr int kSD = 64, kSKPitch = kSD + 8, kSVPitch = kSD + 32;
+constexpr uint32_t kSplitMaxBits = 0x58800000u;  // 2^50
+constexpr float kSplitScale = 0x1p23f;
+
+struct SplitSmem {
+    uint16_t k[3][kBN * kSKPitch];
+    uint16_t v[3][kBN * kSVPitch];
+};
+
+__device__ __forceinline__ b8 as_b8(u32x4 v) { return __builtin_bit_cast(b8, v); }
+
+// 8 floats as h, m and l pieces.
+__device__ __forceinline__ void split_piece(const u32x4 (&f)[2], u32x4 (&part)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t h, m, l;
+        split3(u2f(f[i / 2][2 * (i % 2)]), u2f(f[i / 2][2 * (i % 2) + 1]), h, m, l);
+        part[0][i] = h, part[1][i] = m, part[2][i] = l;
+    }
+}
+__device__ __forceinline__ uint32_t largest(uint32_t most, const u32x4 (&f)[2]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) most = max(most, f[i / 4][i % 4] & 0x7FFFFFFFu);
+    return most;
+}
+
+__global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a) {
+    union Smem {
+        SplitSmem split;
+        FlashF32<kSD>::Smem f32;
+    };
+    __shared__ __align__(16) Smem smem;
+    __shared__ int again;  // bit 0: every query of the tile, bit 1: some
+    SplitSmem& sm = smem.split;
+    PackedTile t;
+    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
+    const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
+    const int n = lane & 31, hh = lane >> 5;
+    const int kv = t.head / (a.h / a.h_kv);
+    const float* kb = static_cast<const float*>(a.k) + t.k0 * a.k_stride + kv * kSD;
+    const float* vb = static_cast<const float*>(a.v) + t.k0 * a.v_stride + kv * kSD;
+    const int qi = t.first + 32 * wave + n;
+    const bool live = t.first + 32 * wave < t.nq;
+    const int seen = keys_seen(min(qi, t.nq - 1), t.nq, t.nk, a.causal);
+    const int wave_least = keys_seen(min(t.first + 32 * wave, t.nq - 1), t.nq, t.nk, a.causal);
+    const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
+    const int most = keys_seen(min(t.first + kBM, t.nq) - 1, t.nq, t.nk, a.causal);
+    const float c = a.scale * 1.4426950408889634f;  // goes into the queries
+    if (tid == 0) again = 0;
+
+    // staging: piece i of the thread is row 32 i + tid / 8, dims 8 (tid % 8) .. + 8
+    const int prow = tid / 8, pd = 8 * (tid % 8);
+    u32x4 kr[2][2], vr[2][2];
+    auto load = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int64_t row = min(key0 + 32 * i + prow, t.nk - 1);  // past the end: masked
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                kr[i][e] = ld16(kb + row * a.k_stride + pd + 4 * e);
+                vr[i][e] = ld16(vb + row * a.v_stride + pd + 4 * e);
+            }
+        }
+    };
+    uint32_t big = 0;  // of K and V
+    SplitSmall small;  // of V
+    auto stage = [&]() {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int row = 32 * i + prow;
+            u32x4 part[3];
+            split_piece(kr[i], part);
+#pragma unroll
+            for (int p = 0; p < 3; p++) st16(&sm.k[p][row * kSKPitch + pd], part[p]);
+            split_piece(vr[i], part);
+#pragma unroll
+            for (int p = 0; p < 3; p++) st16(&sm.v[p][row * kSVPitch + pd], part[p]);
+            big = largest(largest(big, kr[i]), vr[i]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) small.note(u2f(vr[i][e / 2][2 * (e % 2)]), u2f(vr[i][e / 2][2 * (e % 2) + 1]));
+        }
+    };
+    if (most > 0) load(0);
+
+    u32x4 qp[3][4];
+    bool bad_q;
+    {
+        const float* qr = static_cast<const float*>(a.q) + (t.q0 + min(qi, t.nq - 1)) * a.q_stride + t.head * kSD + 8 * hh;
+        uint32_t qbig = 0;
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            u32x4 f[2] = {ld16(qr + 16 * ks), ld16(qr + 16 * ks + 4)};
+#pragma unroll
+            for (int e = 0; e < 8; e++) f[e / 4][e % 4] = f2u(u2f(f[e / 4][e % 4]) * c);
+            u32x4 part[3];
+            split_piece(f, part);
+            qp[0][ks] = part[0], qp[1][ks] = part[1], qp[2][ks] = part[2];
+            qbig = largest(qbig, f);
+        }
+        const auto both = __builtin_amdgcn_permlane32_swap(qbig, qbig, false, false);
+        bad_q = max(static_cast<uint32_t>(both[0]), static_cast<uint32_t>(both[1])) > kSplitMaxBits;
+    }
+
+    f32x16 o[2] = {f32x16{}, f32x16{}}, ol[2] = {f32x16{}, f32x16{}};
+    float m = kFloor, l = 0.0f;
+#pragma unroll 1
+    for (int key0 = 0; key0 < most; key0 += kBN) {
+        __syncthreads();  // the previous tile has been read
+        stage();
+        __syncthreads();
+        const bool more = key0 + kBN < most;
+        if (key0 >= wave_most) {
+            if (more) load(key0 + kBN);
+            continue;
+        }
+        f32x16 s[2];
+        const f32x16 z = {};
+        const int koff = n * kSKPitch + 8 * hh;
+        auto read_k = [&](u32x4(&dst)[2], int part, int ks) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) dst[i] = ld16(sm.k[part] + koff + 32 * i * kSKPitch + 16 * ks);
+        };
+        auto score = [&](const u32x4(&kk)[2], const u32x4& qq, bool first) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+                s[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_b8(kk[i]), as_b8(qq), first ? z : s[i], 0, 0, 0);
+        };
+        // the small products slice by slice (h read a slice ahead, m and l
+        // under the products before theirs), then h h
+        u32x4 kh[2][2], km[2], kl[2];
+        read_k(kh[0], 0, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // LDS reads
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            read_k(km, 1, ks);
+            read_k(kl, 2, ks);
+            read_k(kh[(ks + 1) & 1], 0, (ks + 1) & 3);
+            score(kh[ks & 1], qp[1][ks], ks == 0);
+            score(kh[ks & 1], qp[2][ks], false);
+            score(km, qp[1][ks], false);
+            score(km, qp[0][ks], false);
+            score(kl, qp[0][ks], false);
+            __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 10, 0);  // MFMAs
+        }
+#pragma unroll
+        for (int ks = 0; ks < 4; ks++) {
+            if (ks < 3) read_k(kh[(ks + 1) & 1], 0, ks + 1);
+            score(kh[ks & 1], qp[0][ks], false);
+            if (ks < 3) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+        }
+        if (key0 + kBN > wave_least) {
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (key0 + 32 * i + 8 * (r / 4) + 4 * hh + r % 4 >= seen) s[i][r] = -INFINITY;
+        }
+        // the next rows once the scores' operands have left the registers (at
+        // the top of the tile they spilled: 286 us for 220)
+        if (more) load(key0 + kBN);
+        u32x4 wp[3][2][2];
+        auto weights = [&](float ref) {
+            float ps[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int w = 0; w < 8; w++) {
+                    float p[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        p[e] = kSplitScale * __builtin_amdgcn_exp2f(s[i][2 * w + e] - ref);
+                        ps[e] += p[e];
+                    }
+                    uint32_t h, md, lo;
+                    split3(p[0], p[1], h, md, lo);
+                    wp[0][i][w / 4][w % 4] = h, wp[1][i][w / 4][w % 4] = md, wp[2][i][w / 4][w % 4] = lo;
+                }
+            return ps[0] + ps[1];
+        };
+        // as in f16: the reference moves on the first tile and where a weight
+        // might pass 2^15 times the largest at it, for the query's own sums only
+        bool own = key0 == 0, move = own;
+        if (!move) {
+            const float ps = weights(m);
+            own = !(halves_max(ps) <= kRowSumMax * kSplitScale);
+            move = __any(own);
+            if (!move) l += ps;
+        }
+        if (move) {
+            float mx = s[0][0];
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[i][r]);
+            const float cand = fmaxf(m, halves_max(mx));
+            const float next = own && cand > m + kLazyMax ? cand : m;
+            const float corr = __builtin_amdgcn_exp2f(m - next);
+            l = fmaf(l, corr, weights(next));
+            m = next;
+#pragma unroll
+            for (int i = 0; i < 2; i++) o[i] *= corr, ol[i] *= corr;
+        }
+        const int l16 = n & 15;
+        const int voff = (4 * hh + l16 / 4) * kSVPitch + (n & 16) + 4 * (l16 % 4);
+        auto read_v = [&](u32x4(&dst)[2], int part, int g) {
+#pragma unroll
+            for (int db = 0; db < 2; db++) {
+                const uint16_t* r0 = sm.v[part] + voff + 16 * g * kSVPitch + 32 * db;
+                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)r0));
+                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(r0 + 8 * kSVPitch)));
+                dst[db][0] = lo[0], dst[db][1] = lo[1], dst[db][2] = hi[0], dst[db][3] = hi[1];
+            }
+        };
+        auto add = [&](f32x16(&acc)[2], const u32x4(&vv)[2], const u32x4& w) {
+#pragma unroll
+            for (int db = 0; db < 2; db++)
+                acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_b8(vv[db]), as_b8(w), acc[db], 0, 0, 0);
+        };
+        u32x4 vh[2][2], vm[2], vl[2];
+        read_v(vh[0], 0, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            read_v(vm, 1, g);
+            read_v(vl, 2, g);
+            if (g < 3) read_v(vh[(g + 1) & 1], 0, g + 1);
+            const u32x4 wh = wp[0][g / 2][g % 2], wm = wp[1][g / 2][g % 2], wl = wp[2][g / 2][g % 2];
+            add(o, vh[g & 1], wh);
+            add(ol, vh[g & 1], wm);
+            add(ol, vh[g & 1], wl);
+            add(ol, vm, wm);
+            add(ol, vm, wh);
+            add(ol, vl, wh);
+            if (g < 3)
+                __builtin_amdgcn_sched_group_barrier(0x100, 12, 0);
+            else
+                __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 12, 0);
+        }
+    }
+    const bool bad_kv = big > kSplitMaxBits || small.seen();
+    if (bad_kv || bad_q) atomicOr(&again, (bad_kv ? 1 : 0) | (bad_q ? 2 : 0));
+    __syncthreads();
+    const int redo = again;
+    const bool mine = (redo & 1) != 0 || bad_q;
+    if (qi < t.nq && !mine) {
+        const float lsum = halves_sum(l);
+        float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * kSD + 4 * hh;
+#pragma unroll
+        for (int db = 0; db < 2; db++)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; r4++) {
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = f2u(seen > 0 ? (o[db][4 * r4 + e] + ol[db][4 * r4 + e]) / lsum : 0.0f);
+                st16(orow + 32 * db + 8 * r4, w);
+            }
+    }
+    if (redo) packed_f32_tile<kSD>(a, t, smem.f32, mine);  // workgroup-uniform
 }
 
 // f32, short sequences: a serial chain per query, so it is cut as finely as the
@@ -519,6 +831,7 @@ struct FewF32 {
             float o[kWaves][kQueries * kPitch];
         };
         float m[kWaves][kQueries], l[kWaves][kQueries];
+        int odd;  // as in the kernels above
     };
 };
 
@@ -550,7 +863,9 @@ __global__ __launch_bounds__(kThreads, 2) void packed_few_f32_kernel(PackedArgs 
     f32x4 o[DB];
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x4{};
-    float m = -3.0e38f, l = 0.0f;  // l: this lane's keys only
+    float m = kFloor, l = 0.0f;  // l: this lane's keys only
+    if (threadIdx.x == 0) sm.odd = 0;
+    __syncthreads();
     float* vs = sm.v[wave];
     u32x4 kr[KS], vr[F::kVLoads];
     auto load_v = [&](int key0) {
@@ -570,14 +885,17 @@ __global__ __launch_bounds__(kThreads, 2) void packed_few_f32_kernel(PackedArgs 
 #pragma unroll 1
     for (int key0 = 16 * wave; key0 < most; key0 += kTurn) {
         const bool partial = key0 + 16 > least;  // some query does not see all of these keys
-        bool odd = false;
+        if (partial) {
+#pragma unroll
+            for (int i = 0; i < F::kVLoads; i++)
+#pragma unroll
+                for (int w = 0; w < 4; w++)
+                    if (odd_f32(vr[i][w])) sm.odd = 1, vr[i][w] = 0;
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int i = 0; i < F::kVLoads; i++) {
             st16(vs + (F::kVRows * i + lane / F::kRowLanes) * F::kPitch + lane % F::kRowLanes * 4, vr[i]);
-            if (partial)
-#pragma unroll
-                for (int w = 0; w < 4; w++) odd |= odd_f32(vr[i][w]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (key0 + kTurn < most) load_v(key0 + kTurn);
@@ -588,6 +906,9 @@ __global__ __launch_bounds__(kThreads, 2) void packed_few_f32_kernel(PackedArgs 
             for (int e = 0; e < 4; e++)
                 acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(u2f(kr[i][e]), u2f(qv[i][e]), acc[e], 0, 0, 0);
         f32x4 s = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+        // rounded before the maximum is taken off: that one then weighs 1
+#pragma unroll
+        for (int j = 0; j < 4; j++) s[j] = as_f32(s[j] * c);
         if (key0 + kTurn < most) load_k(key0 + kTurn);
         if (partial)
 #pragma unroll
@@ -596,37 +917,24 @@ __global__ __launch_bounds__(kThreads, 2) void packed_few_f32_kernel(PackedArgs 
         float mx = fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3]));
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float next = fmaxf(m, mx * c);
+        const float next = fmaxf(m, mx);
         const float corr = __builtin_amdgcn_exp2f(m - next);
         m = next;
         float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            s[j] = __builtin_amdgcn_exp2f(fmaf(s[j], c, -m));
+            s[j] = __builtin_amdgcn_exp2f(s[j] - m);
             sum += s[j];
         }
         l = fmaf(l, corr, sum);
 #pragma unroll
         for (int i = 0; i < DB; i++) o[i] *= corr;
         const float* va = vs + 4 * g * F::kPitch + n;
-        if (partial && __any(odd)) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll 1
-                for (int x = 0; x < 4; x++)
-#pragma unroll
-                    for (int i = 0; i < DB; i++) {
-                        const f32x4 add = __builtin_amdgcn_mfma_f32_16x16x4f32(g == x ? va[j * F::kPitch + 16 * i] : 0.0f,
-                                                                               g == x ? s[j] : 0.0f, f32x4{}, 0, 0, 0);
-                        if (key0 + 4 * x + j < seen) o[i] += add;
-                    }
-        } else {
 #pragma unroll
             for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int i = 0; i < DB; i++)
                     o[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(va[j * F::kPitch + 16 * i], s[j], o[i], 0, 0, 0);
-        }
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
@@ -650,6 +958,13 @@ __global__ __launch_bounds__(kThreads, 2) void packed_few_f32_kernel(PackedArgs 
             sum += *reinterpret_cast<const f32x4*>(&sm.o[w][q * F::kPitch + d0]) * f;
             weight = fmaf(sm.l[w][q], f, weight);
         }
+        if (sm.odd)
+            for (int key = least / 16 * 16; key < keys; key++) {
+                const u32x4 v = ld16(vb + key * a.v_stride + d0);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (odd_f32(v[e])) sum[e] += u2f(v[e]);
+            }
         float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + t.first + q) * a.h + t.head) * D + d0;
         u32x4 w;
 #pragma unroll
@@ -706,6 +1021,6 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     if (dt == HS_F16) return d == 64 ? go(packed_f16_kernel<64>, kBM) : go(packed_f16_kernel<128>, kBM);
     // Tiles of 32 queries a wave where they fill the chip's SIMDs, else 16 by
     // four waves
-    if ((n_q / 32 + b) * h >= 4 * num_cus()) return d == 64 ? go(packed_f32_kernel<64>, kBM) : go(packed_f32_kernel<128>, kBM);
+    if ((n_q / 32 + b) * h >= 4 * num_cus()) return d == 64 ? go(packed_split_kernel, kBM) : go(packed_f32_kernel<128>, kBM);
     return d == 64 ? go(packed_few_f32_kernel<64>, 16) : go(packed_few_f32_kernel<128>, 16);
 }

@@ -106,6 +106,7 @@ inline hs_status check_rows(const char* op, const char* what, const void* p, int
     if (n == 0 || width == 0) return HS_OK;
     if (!p) return fail(HS_EINVAL, "%s: null %s", op, what);
     if (stride < width) return fail(HS_EINVAL, "%s: %s rows overlap", op, what);
+    if (stride >= (1 << 22)) return fail(HS_EINVAL, "%s: %s rows of 2^22 elements or more apart", op, what);
     if (too_large(n, stride)) return fail(HS_EINVAL, "%s: %s too large", op, what);
     if (!aligned16(p) || stride * dtype_size(dt) % 16 != 0)
         return fail(HS_EUNSUPPORTED, "%s: %s rows must be 16-byte aligned", op, what);

@@ -388,14 +388,18 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
             if (WHOLE) find_pages(key0 + 2 * P::kUnit);
         }
 
-        float mx = sc[0][0];
+        // rounded before the maximum is taken off: that one then weighs 1
+        float mx = -INFINITY;
 #pragma unroll
         for (int i = 0; i < kStep / 16; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) mx = fmaxf(mx, sc[i][j]);
+            for (int j = 0; j < 4; j++) {
+                sc[i][j] = as_f32(sc[i][j] * c);
+                mx = fmaxf(mx, sc[i][j]);
+            }
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float next = fmaxf(fmaxf(m, mx * c), some ? kFloor : kNone);
+        const float next = fmaxf(fmaxf(m, mx), some ? kFloor : kNone);
         const float corr = __builtin_amdgcn_exp2f(m - next);
         m = next;
         float sum = 0.0f;
@@ -403,7 +407,7 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
         for (int i = 0; i < kStep / 16; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                sc[i][j] = __builtin_amdgcn_exp2f(fmaf(sc[i][j], c, -m));
+                sc[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - m);
                 sum += sc[i][j];
             }
         l = fmaf(l, corr, sum);

@@ -224,7 +224,7 @@ def test_packed_other_keys(ctx, dtype, causal):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_packed_scales(ctx, dtype):
     """Peaked weights, a scale of the caller's, negative and zero ones."""
-    for scale, std in [(1.0, 1.0), (0.05, 3.0), (-0.125, 1.0), (0.0, 1.0)]:
+    for scale, std in [(1.0, 1.0), (0.05, 3.0), (-0.125, 1.0), (0.0, 1.0), (0.125, 400.0)]:
         run_packed(ctx, 420, dtype, 64, 2, 1, [90, 140], [90, 140], 1, scale=scale, std=std)
 
 
@@ -287,6 +287,65 @@ def test_packed_longer(ctx, dtype):
             bound = R.attention_bound(ref, mag, *(x[a:a + m].cpu() for x in (q, k, v)),
                                       R.seen_keys(m, m, causal), 1 / math.sqrt(d), dtype)
             R.assert_within(got[a:a + m], ref, bound, f"d={d} length {m}")
+
+
+def gpu_reference(q, k, v, seen, scale):
+    """(result, sum(p |v|)) of one sequence in f64 on the GPU; values that a
+    query does not see count as zeros."""
+    h, h_kv = q.shape[1], k.shape[1]
+    qs, ks, vs = (x.double().transpose(0, 1) for x in (q, k, v))
+    ks, vs = ks.repeat_interleave(h // h_kv, 0), vs.repeat_interleave(h // h_kv, 0)
+    hidden = torch.arange(k.shape[0], device=DEV) >= seen.to(DEV)[:, None]
+    out, mag = torch.empty_like(qs), torch.empty_like(qs)
+    for i in range(h):
+        s = (qs[i] @ ks[i].T * scale).masked_fill(hidden, -math.inf)
+        p = torch.softmax(s, -1)
+        odd = ~vs[i].isfinite()
+        plain = torch.where(odd, 0.0, vs[i])
+        out[i], mag[i] = p @ plain, p @ plain.abs()
+        for j in odd.any(1).nonzero().flatten().tolist():
+            at = ~hidden[:, j]
+            out[i, at] += torch.where(odd[j], p[at, j, None] * vs[i, j], 0.0)
+    return out.transpose(0, 1).cpu(), mag.transpose(0, 1).cpu()
+
+
+@pytest.mark.parametrize("what", ["plain", "inf", "nan", "huge", "huge q", "tiny"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_f32_tiles(ctx, d, what):
+    """f32 over enough queries for the tiles of 32 a wave, with values that the
+    three bf16 parts do not hold among them."""
+    lens, h, h_kv = [1301, 900, 130], 16, 8
+    gen = torch.Generator().manual_seed(d)
+    q, k, v = (normal(gen, (sum(lens), x, d), F32) for x in (h, h_kv, h_kv))
+    if what in ("inf", "nan"):
+        x = math.inf if what == "inf" else math.nan
+        v[700, 3, 7], v[1310, :, 1], v[2331 - 40, 5] = x, -x, x
+    elif what == "huge":
+        v[700] *= 2.0 ** 60
+        k[1500, 2] *= 2.0 ** 55
+    elif what == "huge q":
+        q[800:803] *= 2.0 ** 52
+        q[2000, 5] *= 2.0 ** 70
+    elif what == "tiny":
+        v[:1301] *= 2.0 ** -110
+        k[1400:1500] *= 2.0 ** -115
+        q[1600:1700] *= 2.0 ** -115
+    for causal in (1, 0, 137):
+        print(f"[packed f32 tiles d={d} {what} causal={causal}]", flush=True)
+        got = ctx.attention_packed(*(x.to(DEV) for x in (q, k, v)), i32(offsets_of(lens)), causal=causal)
+        got = got.unflatten(1, (h, d)).cpu()
+        for s, (a, n) in enumerate(zip(offsets_of(lens), lens)):
+            qs, ks, vs = (x[a:a + n] for x in (q, k, v))
+            seen = R.seen_keys(n, n, causal)
+            ref, mag = gpu_reference(*(x.to(DEV) for x in (qs, ks, vs)), seen, 1 / math.sqrt(d))
+            fin = [torch.nan_to_num(x, 0.0, 0.0, 0.0) for x in (qs, ks, vs)]
+            bound = R.attention_bound(ref.nan_to_num(0.0, 0.0, 0.0), mag, *fin, seen, 1 / math.sqrt(d), F32)
+            g = got[a:a + n]
+            odd = ~ref.isfinite()
+            nans = g.isnan(), ref.isnan()
+            assert torch.equal(*nans), f"sequence {s}: NaN places"
+            assert torch.equal(g[odd].nan_to_num(0.0), ref[odd].float().nan_to_num(0.0)), f"sequence {s}: infinities"
+            R.assert_within(g[~odd], ref[~odd], bound[~odd], f"sequence {s}")
 
 
 # -------------------------------------------------------------- attention_paged
@@ -360,7 +419,7 @@ def test_paged_long(ctx, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_scales(ctx, dtype):
-    for scale, std in [(1.0, 1.0), (0.3, 3.0), (-0.125, 1.0), (0.0, 1.0)]:
+    for scale, std in [(1.0, 1.0), (0.3, 3.0), (-0.125, 1.0), (0.0, 1.0), (40.0, 100.0)]:
         run_paged(ctx, 530, dtype, 64, 4, 2, 16, [500, 90], scale=scale, std=std)
 
 
