@@ -120,25 +120,29 @@ __device__ __forceinline__ void add_odd(f32x16 (&o)[DB], const PackedArgs& a, co
 // while the current one computes; V^T comes through the transposing LDS read
 // and takes P^T from the registers that the scores were in.
 //
-// LDS rows are not padded, so that four workgroups (head dim 64) or two (128)
-// fit a CU; a row's 16-byte pieces are permuted instead: 16 rows' reads of K at
-// one column, and the transposing read's 4 rows of 64 bytes, touch every bank
-// once.
-template <int D>
+// LDS rows are padded so that 16 rows' reads of K at one column, and the
+// transposing read's 4 rows of 64 bytes, touch every bank once; every read is
+// then one register and a constant. (Unpadded rows with permuted pieces let a
+// third more waves of four-wave workgroups in, but the addresses cost more
+// registers than there are.)
+//
+// Eight waves share a tile's keys and their staging (two workgroups per CU at
+// head dim 64, one at 128), four where the grid is small.
+template <int D, int W>
 struct FlashF16 {
+    static constexpr int kThr = 64 * W;
+    static constexpr int kQueries = 32 * W;
     static constexpr int KS = D / 16;             // 16-dim slices of a score
     static constexpr int DB = D / 32;             // 32-channel blocks of an output
     static constexpr int kPieces = D / 8;         // 16-byte pieces of a row
-    static constexpr int kPer = kBN * kPieces / kThreads;
-    static constexpr int kRowStep = kThreads / kPieces;  // rows per load of the workgroup
+    static constexpr int kPer = kBN * kPieces / kThr;
+    static constexpr int kRowStep = kThr / kPieces;          // rows per load of the workgroup
+    static constexpr int kKPitch = D + 8, kVPitch = D + 32;  // halves
     struct Smem {
-        f16 k[2][kBN * D];
-        f16 v[2][kBN * D];
+        f16 k[2][kBN * kKPitch];
+        f16 v[2][kBN * kVPitch];
         int odd;  // a tile whose values not every query sees holds an infinity or NaN
     };
-    // What piece numbers are xored with in a row; the same in rows 16 apart.
-    static __device__ __forceinline__ int k_swap(int row) { return D == 64 ? row >> 1 & 7 : row & 15; }
-    static __device__ __forceinline__ int v_swap(int row) { return D == 64 ? (row >> 1 & 1) << 2 : (row & 3) << 2; }
 };
 
 // A weight's exponent may run this far (log2) above the reference maximum
@@ -152,13 +156,13 @@ constexpr float kFar = 65536.0f;
 // A lane's row sum over a tile beyond which a weight may not fit f16.
 constexpr float kRowSumMax = 32768.0f;
 
-template <int D>
-__global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(PackedArgs a) {
-    using F = FlashF16<D>;
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed_f16_kernel(PackedArgs a) {
+    using F = FlashF16<D, W>;
     constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
     __shared__ __align__(16) typename F::Smem sm;
     PackedTile t;
-    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
+    if (!packed_tile(a, F::kQueries, t)) return;  // workgroup-uniform, before any barrier
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int n = lane & 31, hh = lane >> 5;
     const int kv = t.head / (a.h / a.h_kv);
@@ -170,7 +174,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
     const int wave_least = keys_seen(min(t.first + 32 * wave, t.nq - 1), t.nq, t.nk, a.causal);
     const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
     const int tile_least = keys_seen(t.first, t.nq, t.nk, a.causal);
-    const int most = keys_seen(min(t.first + kBM, t.nq) - 1, t.nq, t.nk, a.causal);
+    const int most = keys_seen(min(t.first + F::kQueries, t.nq) - 1, t.nq, t.nk, a.causal);
     const int ntiles = (most + kBN - 1) / kBN;
 
     // Q^T as the B operand: lane (n, hh) holds dims 16 ks + 8 hh .. + 8. A
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
             }
         }
     };
-    const int k_at = row0 * D + (piece ^ F::k_swap(row0)) * 8, v_at = row0 * D + (piece ^ F::v_swap(row0)) * 8;
+    const int k_at = row0 * F::kKPitch + piece * 8, v_at = row0 * F::kVPitch + piece * 8;
     auto store = [&](int buf, int key0) {
         if (key0 + kBN > tile_least) {  // some query does not see all of these values
             bool odd = false;
@@ -239,8 +243,8 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
         }
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            st16(&sm.k[buf][k_at + i * F::kRowStep * D], pk[i]);
-            st16(&sm.v[buf][v_at + i * F::kRowStep * D], pv[i]);
+            st16(&sm.k[buf][k_at + i * F::kRowStep * F::kKPitch], pk[i]);
+            st16(&sm.v[buf][v_at + i * F::kRowStep * F::kVPitch], pv[i]);
         }
     };
     if (tid == 0) sm.odd = 0;
@@ -258,14 +262,13 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
             // lane (n, hh) key 8 (r / 4) + 4 hh + r % 4, query n
             f32x16 s[2];
             const f32x16 z = {};
-            const f16* ka = sm.k[cur] + n * D;
+            const f16* ka = sm.k[cur] + n * F::kKPitch + 8 * hh;
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                const int at = ((2 * ks + hh) ^ F::k_swap(n)) * 8;
+            for (int ks = 0; ks < KS; ks++)
 #pragma unroll
                 for (int i = 0; i < 2; i++)
-                    s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(ld16(ka + 32 * i * D + at)), qa[ks], ks ? s[i] : z, 0, 0, 0);
-            }
+                    s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(ld16(ka + 32 * i * F::kKPitch + 16 * ks)), qa[ks],
+                                                                  ks ? s[i] : z, 0, 0, 0);
             if (key0 + kBN > wave_least) {
 #pragma unroll
                 for (int i = 0; i < 2; i++)
@@ -336,11 +339,11 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 3 : 2) void packed_f16_kernel(P
             // O^T += V^T P^T. The transposing read gives lane i of 16 channel
             // i of 4 keys: two reads make the 8 keys, in the scores' order.
             const int vrow = 4 * hh + (n & 15) / 4;
-            const f16* va = sm.v[cur] + vrow * D + (n & 16) + 4 * (n & 3);
+            const f16* va = sm.v[cur] + vrow * F::kVPitch + (n & 16) + 4 * (n & 3);
             auto read_v = [&](int g, int db) {
-                const f16* r0 = va + 16 * g * D + ((4 * db) ^ F::v_swap(vrow)) * 8;
+                const f16* r0 = va + 16 * g * F::kVPitch + 32 * db;
                 const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)r0));
-                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(r0 + 8 * D)));
+                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(r0 + 8 * F::kVPitch)));
                 u32x4 w;
                 w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
                 return w;
@@ -1011,16 +1014,25 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     a.causal = causal, a.scale = scale;
     hipStream_t st = static_cast<hipStream_t>(stream);
     // as many tiles as sequences of these rows can have
-    const auto go = [&](auto kernel, int bm) {
+    const auto go = [&](auto kernel, int bm, int threads) {
         const int64_t tiles = n_q / bm + (b < n_q ? b : n_q);
-        if (tiles * h >= (int64_t{1} << 31) / kThreads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
+        if (tiles * h >= (int64_t{1} << 31) / threads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
         a.tiles = static_cast<int>(tiles);
-        kernel<<<dim3(static_cast<uint32_t>(tiles * h)), dim3(kThreads), 0, st>>>(a);
+        kernel<<<dim3(static_cast<uint32_t>(tiles * h)), dim3(threads), 0, st>>>(a);
         return check_launch(op);
     };
-    if (dt == HS_F16) return d == 64 ? go(packed_f16_kernel<64>, kBM) : go(packed_f16_kernel<128>, kBM);
+    if (dt == HS_F16) {
+        // Tiles of 256 queries for long sequences that make enough of them, 128
+        // else (us with 128 and 256; 16 heads of 64: one sequence of 12000
+        // tokens 704, 643, of 6000 185, 199, eight of 1374, causal, 59, 66; 32
+        // heads of 128 over 8: 12000 2520, 2332, 2748 161, 178, twenty of 300
+        // 67, 81): more reuse against more masked keys and longer tails.
+        if ((n_q / 256 + b) * h * 2 >= 5 * num_cus() && n_q >= int64_t{2048} * b)
+            return d == 64 ? go(packed_f16_kernel<64, 8>, 256, 512) : go(packed_f16_kernel<128, 8>, 256, 512);
+        return d == 64 ? go(packed_f16_kernel<64, 4>, 128, 256) : go(packed_f16_kernel<128, 4>, 128, 256);
+    }
     // Tiles of 32 queries a wave where they fill the chip's SIMDs, else 16 by
     // four waves
-    if ((n_q / 32 + b) * h >= 4 * num_cus()) return d == 64 ? go(packed_split_kernel, kBM) : go(packed_f32_kernel<128>, kBM);
-    return d == 64 ? go(packed_few_f32_kernel<64>, 16) : go(packed_few_f32_kernel<128>, 16);
+    if ((n_q / 32 + b) * h >= 4 * num_cus()) return d == 64 ? go(packed_split_kernel, kBM, kThreads) : go(packed_f32_kernel<128>, kBM, kThreads);
+    return d == 64 ? go(packed_few_f32_kernel<64>, 16, kThreads) : go(packed_few_f32_kernel<128>, 16, kThreads);
 }

@@ -166,9 +166,12 @@ void launch_append(hipStream_t st, const AppendArgs<T>& a) {
 // l) join in LDS, the ranges of a sequence in a second launch.
 //
 // Ranges: a sequence's keys are cut into pieces of `chunk` units of 4 kStep
-// keys, so that all sequences together make about kItems pieces. Lengths are
-// device data: each workgroup computes chunk and finds its piece from all of
-// them (64 a step).
+// keys, the same for all sequences of the call. A piece costs some 5 us before
+// its first product (lengths, pages, keys: one load behind the other) and a
+// unit 1 us, so pieces are as many as the chip holds at once while that leaves
+// them up to four units, and then four times as many, which evens their ends
+// out. Lengths are device data: each workgroup computes chunk and finds its
+// piece from all of them (64 a step).
 
 typedef f16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -178,6 +181,7 @@ typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 __device__ __forceinline__ h8 as_h8(u32x4 v) { return __builtin_bit_cast(h8, v); }
 
 constexpr int kGroup = 16;  // query heads per pass
+constexpr int kRounds = 4;  // rounds of workgroups that a long call makes
 constexpr int kPagedWaves = 4;
 constexpr float kNone = -3.0e38f;   // a running maximum that has seen no key
 constexpr float kFloor = -2.9e38f;  // the least of one that has
@@ -197,6 +201,7 @@ struct Paged {
     // f32: 4 rows of 64 bytes, 4 rows apart.
     static constexpr int kPitch = kHalf ? D + 16 : D + 4;
     static constexpr int kOPitch = D + 4;
+    static constexpr int kPerCu = D == 64 ? 4 : kHalf ? 3 : 2;  // workgroups, by their registers
     struct Smem {
         union {
             T v[kPagedWaves][kStep * kPitch];
@@ -214,12 +219,12 @@ struct PagedArgs {
     const int *page_table, *lens;
     int64_t q_stride;
     int b, h, h_kv, page_shift, n_pages, max_pages;
-    float per_target;  // 1 / ranges wanted of all sequences together
+    float per_round;  // 1 / ranges that the chip holds at once
     int group, passes, width;  // query heads per key head, passes over them, heads per pass
     float scale;
 };
 
-// Units of keys per piece: total / (pieces wanted), rounded up. The total is
+// Units of keys per piece. The total is
 // summed in f32, whose error (2^-24 a step) the factor covers, so that there
 // are never more pieces than the launch has workgroups for.
 __device__ __forceinline__ int units_per_piece(const PagedArgs& a, int unit) {
@@ -228,8 +233,8 @@ __device__ __forceinline__ int units_per_piece(const PagedArgs& a, int unit) {
         const int s = base + lane_id();
         total += s < a.b ? static_cast<float>((held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit) : 0.0f;
     }
-    const float per = wave_sum(total) * a.per_target;
-    return per < 16777216.0f ? max(1, static_cast<int>(ceilf(per))) : 16777216;
+    const float per = wave_sum(total) * a.per_round;
+    return static_cast<int>(fminf(fmaxf(fmaxf(ceilf(per * (1.0f / kRounds)), fminf(ceilf(per), 4.0f)), 1.0f), 16777216.0f));
 }
 __device__ __forceinline__ int pieces_of(const PagedArgs& a, int s, int unit, int chunk) {
     const uint32_t units = static_cast<uint32_t>((held_length(a.lens, s, a.max_pages, a.page_shift) + unit - 1) / unit);
@@ -527,20 +532,25 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
 struct PagedPlan {
     int group, passes, width;
     int64_t heads, ranges, items, rows;
-    PagedPlan(int b, int h, int h_kv) {
+    PagedPlan(int b, int h, int h_kv, int per_cu) {
         group = h / h_kv;
         passes = static_cast<int>(ceil_div(group, kGroup));
         width = static_cast<int>(ceil_div(group, passes));
         heads = static_cast<int64_t>(h_kv) * passes;
-        ranges = ceil_div(16 * num_cus(), heads);
-        items = (ranges + b) * heads;  // each sequence's last piece may be short
+        ranges = ceil_div(per_cu * num_cus(), heads);
+        items = (ranges * kRounds + b) * heads;  // each sequence's last piece may be short
         rows = items * width;
     }
 };
 
 template <typename T, int D>
-hs_status launch_paged(const char* op, hipStream_t st, PagedArgs a, const PagedPlan& plan) {
+hs_status launch_paged(const char* op, hipStream_t st, PagedArgs a) {
     using P = Paged<T, D>;
+    const PagedPlan plan(a.b, a.h, a.h_kv, P::kPerCu);
+    a.ws_ml = a.ws_o + plan.rows * D;
+    a.ws_cut = reinterpret_cast<int*>(a.ws_ml + 2 * plan.rows);
+    a.group = plan.group, a.passes = plan.passes, a.width = plan.width;
+    a.per_round = 1.00002f / static_cast<float>(plan.ranges);
     // no more pieces than a table's width of keys has units, either
     const int64_t most = ceil_div(static_cast<int64_t>(a.max_pages) << a.page_shift, int64_t{P::kUnit});
     const int64_t items = a.b * plan.heads * (most > 1 ? most : 1);
@@ -649,7 +659,8 @@ extern "C" int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_
     if (b <= 0 || h <= 0 || h_kv <= 0 || h % h_kv != 0 || (d != 64 && d != 128)) return 0;
     using namespace hs;
     if (b > (1 << 24) / h) return 0;
-    return PagedPlan(b, h, h_kv).rows * (d + 2) * 4 + static_cast<int64_t>(b) * 8;
+    // (of the type that takes the most workgroups)
+    return PagedPlan(b, h, h_kv, d == 64 ? Paged<f16, 64>::kPerCu : Paged<f16, 128>::kPerCu).rows * (d + 2) * 4 + static_cast<int64_t>(b) * 8;
 }
 
 extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
@@ -679,17 +690,14 @@ extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const v
     if (overlaps(workspace, need, q, in_bytes) || overlaps(workspace, need, k_cache, cache) || overlaps(workspace, need, v_cache, cache))
         return fail(HS_EINVAL, "%s: workspace overlaps an input", op);
     if (!std::isfinite(scale)) return fail(HS_EINVAL, "%s: scale must be finite", op);
-    const PagedPlan plan(b, h, h_kv);
     PagedArgs a;
     a.q = q, a.k = k_cache, a.v = v_cache, a.out = out, a.q_stride = q_stride;
-    a.ws_o = static_cast<float*>(workspace), a.ws_ml = a.ws_o + plan.rows * d;
+    a.ws_o = static_cast<float*>(workspace);
     a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens);
     a.b = b, a.h = h, a.h_kv = h_kv, a.page_shift = exact_log2(page), a.n_pages = n_pages;
     a.max_pages = n_pages > 0 ? max_pages : 0;  // no page to read: no sequence has keys
-    a.group = plan.group, a.passes = plan.passes, a.width = plan.width, a.scale = scale;
-    a.ws_cut = reinterpret_cast<int*>(a.ws_ml + 2 * plan.rows);
-    a.per_target = 1.00002f / static_cast<float>(plan.ranges);
+    a.scale = scale;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (dt == HS_F16) return d == 64 ? launch_paged<f16, 64>(op, st, a, plan) : launch_paged<f16, 128>(op, st, a, plan);
-    return d == 64 ? launch_paged<float, 64>(op, st, a, plan) : launch_paged<float, 128>(op, st, a, plan);
+    if (dt == HS_F16) return d == 64 ? launch_paged<f16, 64>(op, st, a) : launch_paged<f16, 128>(op, st, a);
+    return d == 64 ? launch_paged<float, 64>(op, st, a) : launch_paged<float, 128>(op, st, a);
 }
