@@ -182,6 +182,7 @@ __device__ __forceinline__ h8 as_h8(u32x4 v) { return __builtin_bit_cast(h8, v);
 
 constexpr int kGroup = 16;  // query heads per pass
 constexpr int kRounds = 4;  // rounds of workgroups that a long call makes
+constexpr int kMostPerCu = 4;  // workgroups of any of the kernels
 constexpr int kPagedWaves = 4;
 constexpr float kNone = -3.0e38f;   // a running maximum that has seen no key
 constexpr float kFloor = -2.9e38f;  // the least of one that has
@@ -201,7 +202,7 @@ struct Paged {
     // f32: 4 rows of 64 bytes, 4 rows apart.
     static constexpr int kPitch = kHalf ? D + 16 : D + 4;
     static constexpr int kOPitch = D + 4;
-    static constexpr int kPerCu = D == 64 ? 4 : kHalf ? 3 : 2;  // workgroups, by their registers
+    static constexpr int kPerCu = D == 64 ? 4 : 3;  // workgroups, by their registers
     struct Smem {
         union {
             T v[kPagedWaves][kStep * kPitch];
@@ -241,6 +242,52 @@ __device__ __forceinline__ int pieces_of(const PagedArgs& a, int s, int unit, in
     return units <= static_cast<uint32_t>(chunk) ? 1 : static_cast<int>((units + chunk - 1) / static_cast<uint32_t>(chunk));
 }
 
+// A workgroup's piece: keys [begin, end) of sequence s, the local-th of its
+// count pieces, key head kv, pass `pass` over its query heads.
+struct Piece {
+    int s, begin, end, count, kv, pass;
+};
+__device__ __forceinline__ bool find_piece(const PagedArgs& a, int unit, Piece& t) {
+    const int lane = lane_id();
+    const int heads = a.h_kv * a.passes;
+    const int piece = static_cast<int>(blockIdx.x) / heads;
+    const int rest = static_cast<int>(blockIdx.x) - piece * heads;
+    t.kv = rest / a.passes, t.pass = rest - t.kv * a.passes;
+    const int chunk = units_per_piece(a, unit);
+    int local = 0, before = 0;
+    t.s = -1;
+    for (int base = 0; base < a.b; base += 64) {
+        const int c = base + lane < a.b ? pieces_of(a, base + lane, unit, chunk) : 0;
+        const int sum = wave_prefix_sum(c);
+        const uint64_t hit = __ballot(before + sum > piece);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            t.s = base + l;
+            t.count = lane_value(c, l);
+            local = piece - before - (lane_value(sum, l) - t.count);
+            break;
+        }
+        before += lane_value(sum, 63);
+    }
+    if (t.s < 0) return false;
+    const int len = held_length(a.lens, t.s, a.max_pages, a.page_shift);
+    const int64_t first = static_cast<int64_t>(local) * chunk * unit, last = first + static_cast<int64_t>(chunk) * unit;
+    t.begin = static_cast<int>(first < len ? first : len), t.end = static_cast<int>(last < len ? last : len);
+    if (local == 0 && rest == 0 && threadIdx.x == 0) a.ws_cut[2 * t.s] = piece, a.ws_cut[2 * t.s + 1] = t.count;
+    return true;
+}
+
+// Where key `key`'s row lies in the pool (in rows), page 0's where its page is
+// none of the pool's.
+struct Tile16 {
+    int64_t row;
+    bool there;
+};
+__device__ __forceinline__ Tile16 tile_of(const PagedArgs& a, int page, int kv, int key) {
+    const bool there = page >= 0 && page < a.n_pages;
+    return {((static_cast<int64_t>(there ? page : 0) * a.h_kv + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1)), there};
+}
+
 // WHOLE: pages of at least 16 keys, so that 16 keys from a multiple of 16 lie in
 // one page; else each row looks its own up.
 template <typename T, int D, bool WHOLE>
@@ -251,31 +298,9 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
     const int lane = lane_id(), wave = wave_in_block();
     const int n = lane & 15, g = lane >> 4;
 
-    // the piece: sequence s, range `local` of its `count`, key head, pass
-    const int heads = a.h_kv * a.passes;
-    const int piece = static_cast<int>(blockIdx.x) / heads;
-    const int rest = static_cast<int>(blockIdx.x) - piece * heads;
-    const int kv = rest / a.passes, pass = rest - kv * a.passes;
-    const int chunk = units_per_piece(a, P::kUnit);
-    int s = -1, local = 0, count = 0, before = 0;
-    for (int base = 0; base < a.b; base += 64) {
-        const int c = base + lane < a.b ? pieces_of(a, base + lane, P::kUnit, chunk) : 0;
-        const int sum = wave_prefix_sum(c);
-        const uint64_t hit = __ballot(before + sum > piece);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            s = base + l;
-            count = lane_value(c, l);
-            local = piece - before - (lane_value(sum, l) - count);
-            break;
-        }
-        before += lane_value(sum, 63);
-    }
-    if (s < 0) return;  // workgroup-uniform, before any barrier
-    const int len = held_length(a.lens, s, a.max_pages, a.page_shift);
-    const int64_t first = static_cast<int64_t>(local) * chunk * P::kUnit, last = first + static_cast<int64_t>(chunk) * P::kUnit;
-    const int begin = static_cast<int>(first < len ? first : len), end = static_cast<int>(last < len ? last : len);
-    if (local == 0 && rest == 0 && threadIdx.x == 0) a.ws_cut[2 * s] = piece, a.ws_cut[2 * s + 1] = count;
+    Piece t;
+    if (!find_piece(a, P::kUnit, t)) return;  // workgroup-uniform, before any barrier
+    const int s = t.s, begin = t.begin, end = t.end, count = t.count, kv = t.kv, pass = t.pass;
     const int live_heads = min(a.width, a.group - pass * a.width);
     const int head0 = kv * a.group + pass * a.width;
 
@@ -294,16 +319,14 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
     const int* pages = a.page_table + static_cast<int64_t>(s) * a.max_pages;
     const T* kb = static_cast<const T*>(a.k);
     const T* vb = static_cast<const T*>(a.v);
-    const int in_page = (1 << a.page_shift) - 1;
-    // Row of key `key` in the pool (all heads' rows), -1 where there is none
-    auto row_of = [&](int page, int key) {
-        return page >= 0 && page < a.n_pages ? ((static_cast<int64_t>(page) * a.h_kv + kv) << a.page_shift) + (key & in_page) : int64_t{-1};
-    };
     auto page_of = [&](int key) { return pages[min(key, end - 1) >> a.page_shift]; };
     u32x4 kr[P::kKLoads], vr[P::kVLoads];
-    uint32_t k_ok = 0, v_ok = 0;  // which of the lane's rows there are
     constexpr int kTiles = kStep / 16;
-    int page[kTiles];  // WHOLE: of the step's 16-key tiles
+    // WHOLE: of the step's 16-key tiles, their pages, and the keys up to which
+    // those loaded are there; else by row of the lane
+    int page[kTiles], k_end[kTiles], v_end[kTiles];
+    uint32_t k_ok = 0, v_ok = 0;
+    const uint32_t k_lane = n * D + g * V, v_lane = lane / P::kRowLanes * D + lane % P::kRowLanes * V;
     auto find_pages = [&](int key0) {
 #pragma unroll
         for (int i = 0; i < kTiles; i++) page[i] = page_of(key0 + 16 * i);
@@ -312,22 +335,35 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
         k_ok = 0;
 #pragma unroll
         for (int i = 0; i < kTiles; i++) {
-            const int key = key0 + 16 * i + n;
-            const int64_t row = row_of(WHOLE ? page[i] : page_of(key), key);
-            if (row >= 0 && key < end) k_ok |= 1u << i;
-            const T* p = kb + (row < 0 ? 0 : row) * D + g * V;
+            const int key = key0 + 16 * i + (WHOLE ? 0 : n);
+            const Tile16 tile = tile_of(a, WHOLE ? page[i] : page_of(key), kv, key);
+            const T* p = kb + tile.row * D + (WHOLE ? k_lane : g * V);
 #pragma unroll
             for (int x = 0; x < KS; x++) kr[i * KS + x] = ld16_nt(p + 4 * x * V);
+            k_end[i] = tile.there ? end : 0;
+            if (!WHOLE && tile.there && key < end) k_ok |= 1u << i;
         }
     };
     auto load_v = [&](int key0) {
         v_ok = 0;
+        if constexpr (WHOLE) {
 #pragma unroll
-        for (int i = 0; i < P::kVLoads; i++) {
-            const int key = key0 + P::kVRows * i + lane / P::kRowLanes;
-            const int64_t row = row_of(WHOLE ? page[P::kVRows * i / 16] : page_of(key), key);
-            if (row >= 0 && key < end) v_ok |= 1u << i;
-            vr[i] = ld16_nt(vb + (row < 0 ? 0 : row) * D + lane % P::kRowLanes * V);
+            for (int i = 0; i < kTiles; i++) {
+                const Tile16 tile = tile_of(a, page[i], kv, key0 + 16 * i);
+                const T* p = vb + tile.row * D;
+#pragma unroll
+                for (int x = 0; x < P::kVLoads / kTiles; x++)
+                    vr[i * (P::kVLoads / kTiles) + x] = ld16_nt(p + v_lane + P::kVRows * x * D);
+                v_end[i] = tile.there ? end : 0;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < P::kVLoads; i++) {
+                const int key = key0 + P::kVRows * i + lane / P::kRowLanes;
+                const Tile16 tile = tile_of(a, page_of(key), kv, key);
+                if (tile.there && key < end) v_ok |= 1u << i;
+                vr[i] = ld16_nt(vb + tile.row * D + lane % P::kRowLanes * V);
+            }
         }
     };
 
@@ -348,10 +384,15 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
         const bool more = key0 + P::kUnit < end;
         // rows that are not there count as zeros: their weight is 0, and 0
         // times what they hold may not be
-        if (__any(v_ok != (1u << P::kVLoads) - 1)) {
+        bool gaps = !WHOLE && __any(v_ok != (1u << P::kVLoads) - 1);
 #pragma unroll
-            for (int i = 0; i < P::kVLoads; i++)
-                if (!(v_ok >> i & 1)) vr[i] = u32x4{};
+        for (int i = 0; i < kTiles; i++) gaps |= WHOLE && key0 + 16 * i + 16 > v_end[i];
+        if (gaps) {
+#pragma unroll
+            for (int i = 0; i < P::kVLoads; i++) {
+                const int row = P::kVRows * i + lane / P::kRowLanes;
+                if (WHOLE ? key0 + row >= v_end[P::kVRows * i / 16] : !(v_ok >> i & 1)) vr[i] = u32x4{};
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
@@ -377,17 +418,27 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
             }
             sc[i] = acc[0] + acc[1];
         }
-        // which of the lane's scores count: key rows 4 g + j, held by lanes 4 g + j
-        if (__any(k_ok != (1u << kStep / 16) - 1)) {
+        // scores of keys that are not there; the lane's are rows 4 g + j, which
+        // lanes 4 g + j have looked up
+        bool some = false;
 #pragma unroll
-            for (int i = 0; i < kStep / 16; i++) {
+        for (int i = 0; i < kTiles; i++) {
+            if constexpr (WHOLE) {
+                if (key0 + 16 * i + 16 > k_end[i]) {
+                    const int left = k_end[i] - key0 - 16 * i - 4 * g;
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        if (j >= left) sc[i][j] = -INFINITY;
+                }
+                some |= key0 + 16 * i < k_end[i];
+            } else {
                 const uint64_t there = __ballot(k_ok >> i & 1);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     if (!(there >> (4 * g + j) & 1)) sc[i][j] = -INFINITY;
+                some |= there != 0;
             }
         }
-        const bool some = __any(k_ok != 0);
         if (more) {
             load_k(key0 + P::kUnit);
             if (WHOLE) find_pages(key0 + 2 * P::kUnit);
@@ -484,6 +535,172 @@ __global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(Paged
     }
 }
 
+// f32, a key head of one query head (no sharing): the matrix instructions would
+// take 2048 cycles for 16 keys of 128 dims, fifteen sixteenths of them for
+// columns that are not there, and the vector ones take some 500. Lanes r, r +
+// 16, .. hold key row r between them (K) and sum its product by halves and
+// quarters; V's rows lie a few to a load, each lane summing its four channels.
+// (16 waves to a workgroup, so that 1024 keys need no second launch, are slower:
+// a CU draws some 50 GB/s, and the longest sequence waits for its one.)
+template <int D>
+struct PagedSingle {
+    static constexpr int W = kPagedWaves;
+    static constexpr int kUnit = 16 * W;
+    static constexpr int kPerCu = 4;
+    struct Smem {
+        float q[D];  // (registers hold K and V)
+        float o[W][D];
+        float m[W], l[W];
+    };
+};
+
+template <int D, bool WHOLE>
+__global__ __launch_bounds__(64 * kPagedWaves, 4) void paged_single_kernel(PagedArgs a) {
+    using P = PagedSingle<D>;
+    constexpr int W = P::W;
+    constexpr int KS = D / 16, kRowLanes = D / 4, kVRows = 64 / kRowLanes, kVLoads = 16 / kVRows;
+    __shared__ __align__(16) typename P::Smem sm;
+    Piece t;
+    if (!find_piece(a, P::kUnit, t)) return;  // workgroup-uniform, before any barrier
+    const int lane = lane_id(), wave = wave_in_block();
+    const int n = lane & 15, g = lane >> 4;
+    const float c = a.scale * 1.4426950408889634f;
+    if (threadIdx.x < D) sm.q[threadIdx.x] = static_cast<const float*>(a.q)[t.s * a.q_stride + t.kv * D + threadIdx.x];
+    const int* pages = a.page_table + static_cast<int64_t>(t.s) * a.max_pages;
+    const float* kb = static_cast<const float*>(a.k);
+    const float* vb = static_cast<const float*>(a.v);
+    auto page_of = [&](int key) { return pages[min(key, t.end - 1) >> a.page_shift]; };
+    u32x4 kr[KS], vr[kVLoads];
+    bool k_ok = false;
+    uint32_t v_ok = 0;  // by load
+    int v_end = 0;      // WHOLE: the keys below it are there
+    int page = 0;       // WHOLE: of the step's 16 keys
+    const uint32_t v_lane = lane / kRowLanes * D + lane % kRowLanes * 4;
+    auto load_k = [&](int key0) {
+        if constexpr (WHOLE) {
+            const Tile16 tile = tile_of(a, page, t.kv, key0);
+            k_ok = tile.there && key0 + n < t.end;
+            const float* p = kb + tile.row * D;
+#pragma unroll
+            for (int i = 0; i < KS; i++) kr[i] = ld16_nt(p + (n * D + 4 * g) + 16 * i);
+        } else {
+            const Tile16 tile = tile_of(a, page_of(key0 + n), t.kv, key0 + n);
+            k_ok = tile.there && key0 + n < t.end;
+            const float* p = kb + tile.row * D + 4 * g;
+#pragma unroll
+            for (int i = 0; i < KS; i++) kr[i] = ld16_nt(p + 16 * i);
+        }
+    };
+    auto load_v = [&](int key0) {
+        if constexpr (WHOLE) {
+            const Tile16 tile = tile_of(a, page, t.kv, key0);
+            const float* p = vb + tile.row * D;
+#pragma unroll
+            for (int i = 0; i < kVLoads; i++) vr[i] = ld16_nt(p + v_lane + kVRows * i * D);
+            v_end = tile.there ? t.end : 0;
+        } else {
+            v_ok = 0;
+#pragma unroll
+            for (int i = 0; i < kVLoads; i++) {
+                const int key = key0 + kVRows * i + lane / kRowLanes;
+                const Tile16 tile = tile_of(a, page_of(key), t.kv, key);
+                if (tile.there && key < t.end) v_ok |= 1u << i;
+                vr[i] = ld16_nt(vb + tile.row * D + lane % kRowLanes * 4);
+            }
+        }
+    };
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float m = kNone, l = 0.0f;  // l: the lane's key row only
+    const int start = t.begin + 16 * wave;
+    if (start < t.end) {
+        if (WHOLE) page = page_of(start);
+        load_k(start);
+        load_v(start);
+        if (WHOLE) page = page_of(start + P::kUnit);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int key0 = start; key0 < t.end; key0 += P::kUnit) {
+        const bool more = key0 + P::kUnit < t.end;
+        float dot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < KS; i++) {
+            const float4 q = ld_f32x4(&sm.q[16 * i + 4 * g]);
+            dot[0] = fmaf(u2f(kr[i][0]), q.x, dot[0]);
+            dot[1] = fmaf(u2f(kr[i][1]), q.y, dot[1]);
+            dot[2] = fmaf(u2f(kr[i][2]), q.z, dot[2]);
+            dot[3] = fmaf(u2f(kr[i][3]), q.w, dot[3]);
+        }
+        float s = (dot[0] + dot[1]) + (dot[2] + dot[3]);
+        s += __shfl_xor(s, 16, 64);
+        s += __shfl_xor(s, 32, 64);
+        // rounded before the maximum is taken off: that one then weighs 1
+        s = k_ok ? as_f32(s * c) : -INFINITY;
+        const bool some = __any(k_ok);
+        if (more) load_k(key0 + P::kUnit);
+        float mx = s;
+        mx = fmaxf(mx, dpp<kQuadXor1>(mx));
+        mx = fmaxf(mx, dpp<kQuadXor2>(mx));
+        mx = fmaxf(mx, dpp<kRowHalfMirror>(mx));
+        mx = fmaxf(mx, dpp<kRowMirror>(mx));
+        const float next = fmaxf(fmaxf(m, mx), some ? kFloor : kNone);
+        const float corr = __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        const float p = __builtin_amdgcn_exp2f(s - m);
+        l = fmaf(l, corr, p);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] *= corr;
+        // a row that is not there weighs 0, and 0 times what it holds may not be 0
+        if (WHOLE ? key0 + 16 > v_end : __any(v_ok != (1u << kVLoads) - 1)) {
+#pragma unroll
+            for (int i = 0; i < kVLoads; i++)
+                if (WHOLE ? key0 + kVRows * i + lane / kRowLanes >= v_end : !(v_ok >> i & 1)) vr[i] = u32x4{};
+        }
+#pragma unroll
+        for (int i = 0; i < kVLoads; i++) {
+            const float w = __shfl(p, kVRows * i + lane / kRowLanes, 64);
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = fmaf(w, u2f(vr[i][e]), o[e]);
+        }
+        if (more) {
+            load_v(key0 + P::kUnit);
+            if (WHOLE) page = page_of(key0 + 2 * P::kUnit);
+        }
+    }
+    l = sum16(l);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        if constexpr (D == 64) o[e] += __shfl_xor(o[e], 16, 64);
+        o[e] += __shfl_xor(o[e], 32, 64);
+    }
+    if (lane < kRowLanes) *reinterpret_cast<f32x4*>(&sm.o[wave][4 * lane]) = f32x4{o[0], o[1], o[2], o[3]};
+    if (lane == 0) sm.m[wave] = m, sm.l[wave] = l;
+    __syncthreads();
+    if (threadIdx.x >= D / 4) return;
+    float top = sm.m[0];
+#pragma unroll
+    for (int w = 1; w < W; w++) top = fmaxf(top, sm.m[w]);
+    f32x4 sum = {};
+    float weight = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        const float f = __builtin_amdgcn_exp2f(sm.m[w] - top);
+        sum += *reinterpret_cast<const f32x4*>(&sm.o[w][4 * threadIdx.x]) * f;
+        weight = fmaf(sm.l[w], f, weight);
+    }
+    const int d0 = 4 * threadIdx.x;
+    if (t.count == 1) {
+        f32x4 x;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = top == kNone ? 0.0f : sum[e] / weight;
+        *reinterpret_cast<f32x4*>(static_cast<float*>(a.out) + (static_cast<int64_t>(t.s) * a.h + t.kv) * D + d0) = x;
+    } else {
+        const int64_t row = blockIdx.x;
+        *reinterpret_cast<f32x4*>(a.ws_o + row * D + d0) = sum;
+        if (d0 == 0) a.ws_ml[2 * row] = top, a.ws_ml[2 * row + 1] = weight;
+    }
+}
+
 // The pieces of one (sequence, query head) joined, THREADS / (D / 4) at a time.
 template <typename T, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
@@ -543,32 +760,40 @@ struct PagedPlan {
     }
 };
 
-template <typename T, int D>
-hs_status launch_paged(const char* op, hipStream_t st, PagedArgs a) {
-    using P = Paged<T, D>;
-    const PagedPlan plan(a.b, a.h, a.h_kv, P::kPerCu);
+template <typename T, int D, typename K>
+hs_status launch_pieces(const char* op, hipStream_t st, PagedArgs a, K whole, K rows, int unit, int per_cu) {
+    const PagedPlan plan(a.b, a.h, a.h_kv, per_cu);
     a.ws_ml = a.ws_o + plan.rows * D;
     a.ws_cut = reinterpret_cast<int*>(a.ws_ml + 2 * plan.rows);
     a.group = plan.group, a.passes = plan.passes, a.width = plan.width;
     a.per_round = 1.00002f / static_cast<float>(plan.ranges);
-    // no more pieces than a table's width of keys has units, either
-    const int64_t most = ceil_div(static_cast<int64_t>(a.max_pages) << a.page_shift, int64_t{P::kUnit});
+    // no more pieces than a table's width of keys has, either
+    const int64_t most = ceil_div(static_cast<int64_t>(a.max_pages) << a.page_shift, int64_t{unit});
     const int64_t items = a.b * plan.heads * (most > 1 ? most : 1);
     const dim3 grid(static_cast<uint32_t>(items < plan.items ? items : plan.items));
-    if (a.page_shift >= 4)
-        attention_paged_kernel<T, D, true><<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
-    else
-        attention_paged_kernel<T, D, false><<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
+    (a.page_shift >= 4 ? whole : rows)<<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
     if (hs_status rc = check_launch(op)) return rc;
     if (most <= 1) return HS_OK;  // no sequence has two pieces
-    const int64_t rows = static_cast<int64_t>(a.b) * a.h;
-    const dim3 joins(static_cast<uint32_t>(rows));
+    const int64_t joined = static_cast<int64_t>(a.b) * a.h;
+    const dim3 joins(static_cast<uint32_t>(joined));
     // few rows may have a thousand pieces each
-    if (rows <= 64)
+    if (joined <= 64)
         paged_join_kernel<T, D, 1024><<<joins, dim3(1024), 0, st>>>(a);
     else
         paged_join_kernel<T, D, 256><<<joins, dim3(256), 0, st>>>(a);
     return check_launch(op);
+}
+
+template <typename T, int D>
+hs_status launch_paged(const char* op, hipStream_t st, const PagedArgs& a) {
+    if constexpr (sizeof(T) == 4) {
+        if (a.h == a.h_kv) {
+            using P = PagedSingle<D>;
+            return launch_pieces<T, D>(op, st, a, paged_single_kernel<D, true>, paged_single_kernel<D, false>, P::kUnit, P::kPerCu);
+        }
+    }
+    using P = Paged<T, D>;
+    return launch_pieces<T, D>(op, st, a, attention_paged_kernel<T, D, true>, attention_paged_kernel<T, D, false>, P::kUnit, P::kPerCu);
 }
 
 hs_status check_cache(const char* op, const void* k_cache, const void* v_cache, const void* page_table,
@@ -659,8 +884,7 @@ extern "C" int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_
     if (b <= 0 || h <= 0 || h_kv <= 0 || h % h_kv != 0 || (d != 64 && d != 128)) return 0;
     using namespace hs;
     if (b > (1 << 24) / h) return 0;
-    // (of the type that takes the most workgroups)
-    return PagedPlan(b, h, h_kv, d == 64 ? Paged<f16, 64>::kPerCu : Paged<f16, 128>::kPerCu).rows * (d + 2) * 4 + static_cast<int64_t>(b) * 8;
+    return PagedPlan(b, h, h_kv, kMostPerCu).rows * (d + 2) * 4 + static_cast<int64_t>(b) * 8;
 }
 
 extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
