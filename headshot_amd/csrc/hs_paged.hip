@@ -10,11 +10,15 @@ namespace {
 // ---------------------------------------------------------------------------
 // kv_append
 //
-// A head vector is spread over G = D / 2V lanes (V elements per 16-byte load),
-// each holding the two chunks [c, c + V) and [D/2 + c, .. + V): a rotation's
-// pair sits in one lane and a norm is one G-lane sum of both. A wave takes one
-// token and walks its heads, q | k | v one after the other, 64 / G at a time,
-// so the token's table rows are read into registers once for all of them.
+// Bandwidth: one pass over the rows. A wave takes one token and up to two loads
+// of its heads, q | k | v one after the other, so there are many waves with a
+// few loads each (6 a token at 48 heads of 128 f16: 77 us for 82 with one wave
+// a token). A head vector is spread over G lanes. Two chunks each, [c, c + V)
+// and [D/2 + c, .. + V) with V elements per 16-byte load, put a rotation's pair
+// into one lane and make a norm one G-lane sum of both. f16 vectors of 64 are a
+// 128-byte line, which two such loads would touch by halves: there a lane takes
+// one chunk, the upper half's in reverse, so that a pair sits in mirror lanes,
+// and two heads instead.
 
 template <int G>
 __device__ __forceinline__ float lanes_sum(float v) {
@@ -38,7 +42,8 @@ struct AppendArgs {
 
 template <typename T, int D, bool NORM, bool ROPE>
 __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs<T> a) {
-    constexpr int V = Vec<T>::N, G = D / (2 * V), HPW = 64 / G;
+    constexpr bool kLine = sizeof(T) == 2 && D == 64;  // one chunk per lane and head
+    constexpr int V = Vec<T>::N, G = kLine ? D / V : D / (2 * V), HPW = 64 / G * (kLine ? 2 : 1);
     const int unit = static_cast<int>(blockIdx.x) * 4 + wave_in_block();
     const int token = unit / a.parts;
     if (token >= a.n) return;  // wave-uniform; no barriers
@@ -57,83 +62,115 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs<T> a) {
     const bool placed = page >= 0 && page < a.n_pages;
     const int64_t slot = pos & ((1 << a.page_shift) - 1);
 
-    const int lane = lane_id();
-    const int c = (lane % G) * V;
+    const int lane = lane_id(), piece = lane % G;
+    const int c = kLine && piece >= G / 2 ? D / 2 + (G - 1 - piece) * V : piece * V;
+    const int c2 = kLine ? c : D / 2 + c;  // the second chunk's channels
     float cl[V], ch[V], sl[V], sh[V];
     bool rot = false;
     if constexpr (ROPE) {
         const int row = a.positions ? a.positions[token] : pos;
         rot = row >= 0 && row < a.table_rows;
         if (rot) {
-            const float* cr = a.cos_tab + static_cast<int64_t>(row) * D + c;
-            const float* sr = a.sin_tab + static_cast<int64_t>(row) * D + c;
+            const float* cr = a.cos_tab + static_cast<int64_t>(row) * D;
+            const float* sr = a.sin_tab + static_cast<int64_t>(row) * D;
+            const float sign = kLine && piece < G / 2 ? -1.0f : 1.0f;
 #pragma unroll
-            for (int e = 0; e < V; e++) cl[e] = cr[e], ch[e] = cr[D / 2 + e], sl[e] = sr[e], sh[e] = sr[D / 2 + e];
+            for (int e = 0; e < V; e++) cl[e] = cr[c + e], sl[e] = sign * sr[c + e];
+            if constexpr (!kLine) {
+#pragma unroll
+                for (int e = 0; e < V; e++) ch[e] = cr[c2 + e], sh[e] = sr[c2 + e];
+            }
         }
     }
     const int part = unit - token * a.parts;
     const int heads = a.h + 2 * a.h_kv;
-    for (int j = part * HPW + lane / G; j < heads; j += a.parts * HPW) {
-        const bool is_q = j < a.h, is_v = j >= a.h + a.h_kv;
-        const int head = is_q ? j : is_v ? j - a.h - a.h_kv : j - a.h;
-        const T* src = is_q   ? a.q + static_cast<int64_t>(token) * a.q_stride
-                       : is_v ? a.v + static_cast<int64_t>(token) * a.v_stride
-                              : a.k + static_cast<int64_t>(token) * a.k_stride;
-        src += head * D + c;
-        u32x4 lo = ld_stream(src), hi = ld_stream(src + D / 2);
-        if ((NORM || ROPE) && !is_v) {
-            float x[V], y[V];
-            unpack(lo, x, T{});
-            unpack(hi, y, T{});
-            if constexpr (NORM) {
-                const float* w = is_q ? a.qn_w : a.kn_w;
-                const float* b = is_q ? a.qn_b : a.kn_b;
-                if (w) {
-                    float sum = 0.0f;
+    const auto source = [&](int j) {
+        return j < a.h            ? a.q + static_cast<int64_t>(token) * a.q_stride + j * D
+               : j < a.h + a.h_kv ? a.k + static_cast<int64_t>(token) * a.k_stride + (j - a.h) * D
+                                  : a.v + static_cast<int64_t>(token) * a.v_stride + (j - a.h - a.h_kv) * D;
+    };
+    // head j's chunk of channels ch0 to where it goes
+    const auto put = [&](int j, int ch0, u32x4 x) {
+        if (j < a.h) {
+            st_stream(a.q_out + (static_cast<int64_t>(token) * a.h + j) * D + ch0, x);
+            return;
+        }
+        const bool is_v = j >= a.h + a.h_kv;
+        const int head = is_v ? j - a.h - a.h_kv : j - a.h;
+        if (placed)
+            st_stream((is_v ? a.v_cache : a.k_cache) + ((((static_cast<int64_t>(page) * a.h_kv + head) << a.page_shift) + slot) * D + ch0), x);
+        if (!is_v && a.k_out) st_stream(a.k_out + (static_cast<int64_t>(token) * a.h_kv + head) * D + ch0, x);
+    };
+    const auto normalise = [&](float (&x)[V], const float* w, const float* b, int ch0, float mean, float inv) {
+#pragma unroll
+        for (int e = 0; e < V; e++) x[e] = fmaf((x[e] - mean) * inv, w[ch0 + e], b[ch0 + e]);
+    };
+    for (int j0 = part * HPW; j0 < heads; j0 += a.parts * HPW) {
+        if constexpr (kLine) {
+            const int j[2] = {j0 + lane / G, j0 + 64 / G + lane / G};
+            u32x4 raw[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+                if (j[u] < heads) raw[u] = ld_stream(source(j[u]) + c);
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                if (j[u] >= heads) continue;
+                if ((NORM || rot) && j[u] < a.h + a.h_kv) {
+                    float x[V];
+                    unpack(raw[u], x, T{});
+                    const float* w = j[u] < a.h ? a.qn_w : a.kn_w;
+                    if (NORM && w) {
+                        float sum = 0.0f, sq = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < V; e++) sum += x[e];
+                        const float mean = lanes_sum<G>(sum) * (1.0f / D);
+#pragma unroll
+                        for (int e = 0; e < V; e++) sq = fmaf(x[e] - mean, x[e] - mean, sq);
+                        normalise(x, w, j[u] < a.h ? a.qn_b : a.kn_b, c, mean, rsqrtf(lanes_sum<G>(sq) * (1.0f / D) + a.eps));
+                    }
+                    if (rot) {
+#pragma unroll
+                        for (int e = 0; e < V; e++) x[e] = fmaf(x[e], cl[e], dpp<kRowHalfMirror>(x[e]) * sl[e]);
+                    }
+                    raw[u] = pack(x, T{});
+                }
+                put(j[u], c, raw[u]);
+            }
+        } else {
+            const int j = j0 + lane / G;
+            if (j >= heads) continue;
+            const T* src = source(j);
+            u32x4 lo = ld_stream(src + c), hi = ld_stream(src + c2);
+            if ((NORM || rot) && j < a.h + a.h_kv) {
+                float x[V], y[V];
+                unpack(lo, x, T{});
+                unpack(hi, y, T{});
+                const float* w = j < a.h ? a.qn_w : a.kn_w;
+                if (NORM && w) {
+                    float sum = 0.0f, sq = 0.0f;
 #pragma unroll
                     for (int e = 0; e < V; e++) sum += x[e] + y[e];
                     const float mean = lanes_sum<G>(sum) * (1.0f / D);
-                    float sq = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < V; e++) {
-                        x[e] -= mean, y[e] -= mean;
-                        sq = fmaf(x[e], x[e], fmaf(y[e], y[e], sq));
-                    }
+                    for (int e = 0; e < V; e++) sq = fmaf(x[e] - mean, x[e] - mean, fmaf(y[e] - mean, y[e] - mean, sq));
                     const float inv = rsqrtf(lanes_sum<G>(sq) * (1.0f / D) + a.eps);
+                    const float* b = j < a.h ? a.qn_b : a.kn_b;
+                    normalise(x, w, b, c, mean, inv);
+                    normalise(y, w, b, c2, mean, inv);
+                }
+                if (rot) {
 #pragma unroll
                     for (int e = 0; e < V; e++) {
-                        x[e] = fmaf(x[e] * inv, w[c + e], b[c + e]);
-                        y[e] = fmaf(y[e] * inv, w[D / 2 + c + e], b[D / 2 + c + e]);
+                        const float u = x[e], v = y[e];
+                        x[e] = fmaf(u, cl[e], -(v * sl[e]));
+                        y[e] = fmaf(v, ch[e], u * sh[e]);
                     }
                 }
+                lo = pack(x, T{});
+                hi = pack(y, T{});
             }
-            if (rot) {
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const float u = x[e], w = y[e];
-                    x[e] = fmaf(u, cl[e], -(w * sl[e]));
-                    y[e] = fmaf(w, ch[e], u * sh[e]);
-                }
-            }
-            lo = pack(x, T{});
-            hi = pack(y, T{});
-        }
-        if (is_q) {
-            T* dst = a.q_out + (static_cast<int64_t>(token) * a.h + head) * D + c;
-            st_stream(dst, lo);
-            st_stream(dst + D / 2, hi);
-            continue;
-        }
-        if (placed) {
-            T* dst = (is_v ? a.v_cache : a.k_cache) +
-                     ((((static_cast<int64_t>(page) * a.h_kv + head) << a.page_shift) + slot) * D + c);
-            st_stream(dst, lo);
-            st_stream(dst + D / 2, hi);
-        }
-        if (!is_v && a.k_out) {
-            T* dst = a.k_out + (static_cast<int64_t>(token) * a.h_kv + head) * D + c;
-            st_stream(dst, lo);
-            st_stream(dst + D / 2, hi);
+            put(j, c, lo);
+            put(j, c2, hi);
         }
     }
 }
@@ -867,7 +904,9 @@ extern "C" hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q
         a.k_cache = static_cast<T*>(k_cache), a.v_cache = static_cast<T*>(v_cache);
         a.n = static_cast<int>(n), a.b = b, a.h = h, a.h_kv = h_kv, a.table_rows = table_rows;
         a.page_shift = exact_log2(page), a.n_pages = n_pages, a.max_pages = max_pages, a.eps = eps;
-        a.parts = 1;
+        // heads of one pass of a wave
+        const int per_wave = dt == HS_F16 ? 1024 / d : 512 / d;
+        a.parts = static_cast<int>(ceil_div(heads, per_wave));
         if (d == 64)
             launch_append<T, 64>(static_cast<hipStream_t>(stream), a);
         else
