@@ -657,8 +657,10 @@ class HipContext:
             qp, nq, qs = _rows(q, h, d, dtype, dev, "q")
             assert nq == n, "q and k rows"
             if out_q is None:
-                out_q = self.empty_typed((n, h * d), dtype)
-            qo = _dense(out_q, n * h * d, dtype, dev, "out_q")
+                out_q = torch.empty((n, h * d), dtype=dtype, device=q.device)
+                qo = out_q.data_ptr()
+            else:
+                qo = _dense(out_q, n * h * d, dtype, dev, "out_q")
             if qn is not None:
                 qw = _dense(qn[0], d, F32, dev, "q-norm weight")
                 qb = _dense(qn[1], d, F32, dev, "q-norm bias")
@@ -666,8 +668,10 @@ class HipContext:
             assert qn is None and out_q is None, "qn or out_q without q"
         if k_rows or out_k is not None:
             if out_k is None:
-                out_k = self.empty_typed((n, h_kv * d), dtype)
-            ko = _dense(out_k, n * h_kv * d, dtype, dev, "out_k")
+                out_k = torch.empty((n, h_kv * d), dtype=dtype, device=k.device)
+                ko = out_k.data_ptr()
+            else:
+                ko = _dense(out_k, n * h_kv * d, dtype, dev, "out_k")
         if kn is not None:
             kw = _dense(kn[0], d, F32, dev, "k-norm weight")
             kb = _dense(kn[1], d, F32, dev, "k-norm bias")
@@ -710,7 +714,7 @@ class HipContext:
         off = _dense(offsets, b + 1, torch.int32, dev, "offsets")
         koff = None if k_offsets is None else _dense(k_offsets, b + 1, torch.int32, dev, "k_offsets")
         if out is None:
-            out = self.empty_typed((n, h * d), dtype)
+            out = torch.empty((n, h * d), dtype=dtype, device=q.device)
         self._launch_held("attention_packed", self.lib.hs_attention_packed, (q, k, v, offsets, k_offsets, out),
                           dt, qp, qs, kp, ks, vp, vs, off, koff, _dense(out, n * h * d, dtype, dev, "out"),
                           n, m, b, h, h_kv, d, causal, 1.0 / math.sqrt(d) if scale is None else scale)
@@ -732,9 +736,10 @@ class HipContext:
         table = _dense(cache.page_table, b * max_pages, torch.int32, dev, "page_table")
         lens = _dense(cache.lens, b, torch.int32, dev, "lens")
         if out is None:
-            out = self.empty_typed((b, h * d), dtype)
+            out = torch.empty((b, h * d), dtype=dtype, device=q.device)
         if workspace is None:
-            workspace = self.empty_typed((self.lib.hs_attention_paged_workspace(b, h, h_kv, d),), torch.uint8)
+            workspace = torch.empty(self.lib.hs_attention_paged_workspace(b, h, h_kv, d), dtype=torch.uint8,
+                                    device=q.device)
         size = workspace.numel()
         self._launch_held("attention_paged", self.lib.hs_attention_paged, (q, cache, out, workspace), _dt(cache.k),
                           qp, qs, _here(cache.k, dev, "k cache"), _here(cache.v, dev, "v cache"), table, lens,

@@ -60,6 +60,7 @@ __device__ __forceinline__ int keys_seen(int i, int nq, int nk, int causal) {
     if (causal == 0) return nk;
     const int at = i + nk - nq;
     if (at < 0) return 0;
+    if (causal == 1) return at + 1;
     const int64_t end = (static_cast<int64_t>(at / causal) + 1) * causal;
     return end < nk ? static_cast<int>(end) : nk;
 }
@@ -604,6 +605,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
     const int most = keys_seen(min(t.first + kBM, t.nq) - 1, t.nq, t.nk, a.causal);
     const float c = a.scale * 1.4426950408889634f;  // goes into the queries
     if (tid == 0) again = 0;
+    __syncthreads();
 
     // staging: piece i of the thread is row 32 i + tid / 8, dims 8 (tid % 8) .. + 8
     const int prow = tid / 8, pd = 8 * (tid % 8);
@@ -991,8 +993,8 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     if (causal < 0) return fail(HS_EINVAL, "%s: causal %d", op, causal);
     if (!k_offsets && n_q != n_k) return fail(HS_EINVAL, "%s: without k_offsets, as many keys as queries", op);
     if (n_q == 0 || b == 0 || h == 0) return HS_OK;
-    if (n_k >= (int64_t{1} << 31) || n_q >= (int64_t{1} << 31) / h)
-        return fail(HS_EINVAL, "%s: n_q * Hq and n_k must be below 2^31", op);
+    if (n_k >= (int64_t{1} << 30) || n_q >= (int64_t{1} << 30) / h)
+        return fail(HS_EINVAL, "%s: n_q * Hq and n_k must be below 2^30", op);
     const int64_t width = static_cast<int64_t>(h) * d, kv_width = static_cast<int64_t>(h_kv) * d;
     if (hs_status rc = check_rows(op, "q", q, n_q, q_stride, width, dt)) return rc;
     if (hs_status rc = check_rows(op, "k", k, n_k, k_stride, kv_width, dt)) return rc;

@@ -262,9 +262,9 @@ struct PagedArgs {
     float scale;
 };
 
-// Units of keys per piece. The total is
-// summed in f32, whose error (2^-24 a step) the factor covers, so that there
-// are never more pieces than the launch has workgroups for.
+// Units of keys per piece. The total is summed in f32, whose error (2^-24 a
+// step) per_round covers, so that there are never more pieces than the launch
+// has workgroups for.
 __device__ __forceinline__ int units_per_piece(const PagedArgs& a, int unit) {
     float total = 0.0f;
     for (int base = 0; base < a.b; base += 64) {
@@ -803,7 +803,8 @@ hs_status launch_pieces(const char* op, hipStream_t st, PagedArgs a, K whole, K 
     a.ws_ml = a.ws_o + plan.rows * D;
     a.ws_cut = reinterpret_cast<int*>(a.ws_ml + 2 * plan.rows);
     a.group = plan.group, a.passes = plan.passes, a.width = plan.width;
-    a.per_round = 1.00002f / static_cast<float>(plan.ranges);
+    // (rounded up by twice the error of the kernels' sum over the lengths)
+    a.per_round = static_cast<float>((1.0 + (a.b / 64 + 64) * 0x1p-23) / static_cast<double>(plan.ranges));
     // no more pieces than a table's width of keys has, either
     const int64_t most = ceil_div(static_cast<int64_t>(a.max_pages) << a.page_shift, int64_t{unit});
     const int64_t items = a.b * plan.heads * (most > 1 ? most : 1);
@@ -868,7 +869,7 @@ extern "C" hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q
     if ((qn_w || kn_w) && !(eps > 0.0f)) return fail(HS_EINVAL, "%s: eps must be positive", op);
     if (!q) h = 0;
     const int64_t heads = static_cast<int64_t>(h) + 2 * h_kv;
-    if (n >= (int64_t{1} << 31) / heads) return fail(HS_EINVAL, "%s: n * (Hq + 2 Hkv) must be below 2^31", op);
+    if (n >= (int64_t{1} << 30) / heads) return fail(HS_EINVAL, "%s: n * (Hq + 2 Hkv) must be below 2^30", op);
     if (too_large(table_rows, d)) return fail(HS_EINVAL, "%s: tables too large", op);
     if (n == 0 || b == 0) return HS_OK;
     if (hs_status rc = check_rows(op, "q", q, h ? n : 0, q_stride, static_cast<int64_t>(h) * d, dt)) return rc;
@@ -892,6 +893,9 @@ extern "C" hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q
         for (int j = 0; j < i; j++)
             if (overlaps(outs[i].p, outs[i].bytes, outs[j].p, outs[j].bytes)) return fail(HS_EINVAL, "%s: outputs overlap", op);
     }
+    // waves per token: as many heads each as two loads hold
+    const int parts = static_cast<int>(ceil_div(heads, dt == HS_F16 ? 1024 / d : 512 / d));
+    if (n * parts >= (int64_t{1} << 26)) return fail(HS_EINVAL, "%s: too many tokens", op);
     const auto run = [&](auto zero) {
         using T = decltype(zero);
         AppendArgs<T> a;
@@ -904,9 +908,7 @@ extern "C" hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q
         a.k_cache = static_cast<T*>(k_cache), a.v_cache = static_cast<T*>(v_cache);
         a.n = static_cast<int>(n), a.b = b, a.h = h, a.h_kv = h_kv, a.table_rows = table_rows;
         a.page_shift = exact_log2(page), a.n_pages = n_pages, a.max_pages = max_pages, a.eps = eps;
-        // heads of one pass of a wave
-        const int per_wave = dt == HS_F16 ? 1024 / d : 512 / d;
-        a.parts = static_cast<int>(ceil_div(heads, per_wave));
+        a.parts = parts;
         if (d == 64)
             launch_append<T, 64>(static_cast<hipStream_t>(stream), a);
         else
@@ -922,7 +924,7 @@ extern "C" hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q
 extern "C" int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d) {
     if (b <= 0 || h <= 0 || h_kv <= 0 || h % h_kv != 0 || (d != 64 && d != 128)) return 0;
     using namespace hs;
-    if (b > (1 << 24) / h) return 0;
+    if (static_cast<int64_t>(b) * h >= (int64_t{1} << 23)) return 0;
     return PagedPlan(b, h, h_kv, kMostPerCu).rows * (d + 2) * 4 + static_cast<int64_t>(b) * 8;
 }
 
@@ -936,7 +938,7 @@ extern "C" hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const v
     if (hs_status rc = check_heads(op, dt, h, h_kv, d)) return rc;
     if (b < 0) return fail(HS_EINVAL, "%s: negative count", op);
     if (b == 0 || h == 0) return HS_OK;
-    if (static_cast<int64_t>(b) * h >= (int64_t{1} << 24)) return fail(HS_EINVAL, "%s: b * Hq must be below 2^24", op);
+    if (static_cast<int64_t>(b) * h >= (int64_t{1} << 23)) return fail(HS_EINVAL, "%s: b * Hq must be below 2^23", op);
     const int64_t width = static_cast<int64_t>(h) * d;
     if (hs_status rc = check_rows(op, "q", q, b, q_stride, width, dt)) return rc;
     if (!out) return fail(HS_EINVAL, "%s: null out", op);

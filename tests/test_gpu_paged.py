@@ -348,6 +348,93 @@ def test_packed_f32_tiles(ctx, d, what):
             R.assert_within(g[~odd], ref[~odd], bound[~odd], f"sequence {s}")
 
 
+@pytest.mark.parametrize("what", ["plain", "odd", "growing"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_f16_long(ctx, d, what):
+    """f16 over enough long sequences for tiles of eight waves."""
+    lens, h, h_kv = [5203, 130], 32, 8
+    gen = torch.Generator().manual_seed(d + 1)
+    q, k, v = (normal(gen, (sum(lens), x, d), F16) for x in (h, h_kv, h_kv))
+    if what == "odd":
+        v[700, 3, 7], v[1310, :, 1], v[5100, 5], v[5210, 2, 2] = math.inf, -math.inf, math.nan, math.inf
+    elif what == "growing":
+        k.mul_(0.1)
+        q.copy_(torch.ones_like(q) * 0.5)
+        k.add_(((torch.arange(k.shape[0]) * 7919 % 61)[:, None, None] / d ** 0.5).half())
+    for causal in (1, 1374, 0):
+        print(f"[packed f16 long d={d} {what} causal={causal}]", flush=True)
+        got = ctx.attention_packed(*(x.to(DEV) for x in (q, k, v)), i32(offsets_of(lens)), causal=causal)
+        got = got.unflatten(1, (h, d)).cpu()
+        for s, (a, n) in enumerate(zip(offsets_of(lens), lens)):
+            qs, ks, vs = (x[a:a + n, :1 + i] for x, i in ((q, 7), (k, 1), (v, 1)))  # two key heads of the eight
+            seen = R.seen_keys(n, n, causal)
+            ref, mag = gpu_reference(*(x.to(DEV) for x in (qs, ks, vs)), seen, 1 / math.sqrt(d))
+            fin = [torch.nan_to_num(x, 0.0, 0.0, 0.0) for x in (qs, ks, vs)]
+            bound = R.attention_bound(ref.nan_to_num(0.0, 0.0, 0.0), mag, *fin, seen, 1 / math.sqrt(d), F16)
+            g = got[a:a + n, :8]
+            odd = ~ref.isfinite()
+            nans = g.isnan(), ref.isnan()
+            assert torch.equal(*nans), f"sequence {s}: NaN places"
+            assert torch.equal(g[odd].nan_to_num(0.0), ref[odd].half().nan_to_num(0.0)), f"sequence {s}: infinities"
+            R.assert_within(g[~odd], ref[~odd], bound[~odd], f"sequence {s}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_many_sequences(ctx, dtype):
+    """More sequences than a wave has lanes, empty ones among them."""
+    lens = [(i * 37) % 23 for i in range(200)]
+    run_packed(ctx, 450, dtype, 64, 2, 1, lens, lens, 1, behind=2)
+    run_packed(ctx, 451, dtype, 128, 8, 8, lens, [n + i % 3 for i, n in enumerate(lens)], 3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_no_keys(ctx, dtype):
+    """Queries of sequences without keys get zeros, also large ones."""
+    q = torch.full((700, 32, 64), 1e30 if dtype == F32 else 6e4, dtype=dtype, device=DEV)
+    k = torch.empty((0, 32, 64), dtype=dtype, device=DEV)
+    got = ctx.attention_packed(q, k, k, i32([0, 400, 700]), i32([0, 0, 0]))
+    assert (got == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_graph(ctx, dtype):
+    """A captured prompt follows its offsets."""
+    gen = torch.Generator().manual_seed(12)
+    q, k, v = (normal(gen, (300, h, 64), dtype).to(DEV) for h in (4, 2, 2))
+    off = i32([0, 100, 300])
+    ctx.attention_packed(q, k, v, off)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ctx.attention_packed(q, k, v, off)
+    for cut in (100, 0, 299, 300, 17):
+        off.copy_(i32([0, cut, 300]))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = captured.clone()
+        assert torch.equal(got, ctx.attention_packed(q, k, v, off)), f"cut {cut}"
+
+
+def test_two_streams(ctx):
+    """Calls on two streams at once, a workspace each, give what they give alone."""
+    gen = torch.Generator().manual_seed(13)
+    sides = []
+    for i in range(2):
+        cpu, gpu = make_cache(gen, [3000 + i, 40, 900], 4, 16, 64, F16)
+        q = normal(gen, (3, 8, 64), F16).to(DEV)
+        ws = torch.empty(ctx.attention_paged_workspace(3, 8, 4, 64), dtype=torch.uint8, device=DEV)
+        sides.append((torch.cuda.Stream(), q, gpu, ws, ctx.attention_paged(q, gpu)))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (stream, q, gpu, ws, _alone) in enumerate(sides):
+            with torch.cuda.stream(stream):
+                got[i].append(ctx.attention_paged(q, gpu, workspace=ws))
+    torch.cuda.synchronize()
+    for i, side in enumerate(sides):
+        assert all(torch.equal(x, side[4]) for x in got[i])
+
+
 # -------------------------------------------------------------- attention_paged
 
 

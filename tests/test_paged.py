@@ -57,7 +57,7 @@ def test_append_refusals():
     refused(append(kc=at(2)), EINVAL, "overlaps an input")
     refused(append(vc=at(8)), EINVAL, "outputs overlap")
     refused(append(qo=at(9)), EINVAL, "outputs overlap")
-    refused(append(n=1 << 29), EINVAL, "2^31")
+    refused(append(n=1 << 29), EINVAL, "2^30")
     refused(append(page=1 << 20, max_pages=1 << 10), EINVAL, "2^30")
     refused(append(n_pages=1 << 30), EINVAL, "too large")
     assert append(n=0, q=None, k=None, v=None, qo=None, ko=None, kc=None, vc=None, lens=None) == OK
@@ -80,11 +80,14 @@ def test_packed_refusals():
     refused(packed(out=None), EINVAL, "null")
     refused(packed(q=None), EINVAL, "null q")
     refused(packed(qs=248), EINVAL, "overlap")
+    refused(packed(ks=1 << 22), EINVAL, "2^22")
+    refused(packed(scale=float("inf")), EINVAL, "finite")
+    refused(packed(scale=float("nan")), EINVAL, "finite")
     refused(packed(qs=260), EUNSUPPORTED, "16-byte")
     refused(packed(v=ctypes.c_void_p(0x30000004)), EUNSUPPORTED, "16-byte")
     refused(packed(out=ctypes.c_void_p(0x60000008)), EUNSUPPORTED, "16-byte")
     refused(packed(out=at(2)), EINVAL, "overlaps")
-    refused(packed(n=1 << 30), EINVAL, "2^31")
+    refused(packed(n=1 << 29), EINVAL, "2^30")
     assert packed(n=0, koff=at(4)) == OK
     assert packed(b=0) == OK
 
@@ -106,9 +109,10 @@ def test_paged_refusals():
     refused(paged(lens=None), EINVAL, "null")
     refused(paged(table=None), EINVAL, "null")
     refused(paged(qs=200), EINVAL, "overlap")
+    refused(paged(scale=float("nan")), EINVAL, "finite")
     refused(paged(qs=260), EUNSUPPORTED, "16-byte")
     refused(paged(out=at(0)), EINVAL, "overlaps")
-    refused(paged(b=1 << 23, qs=256), EINVAL, "2^24")
+    refused(paged(b=1 << 21, qs=256), EINVAL, "2^23")
     if L.hs_attention_paged_workspace(2, 4, 2, 64) > 0:
         refused(paged(nbytes=0), EINVAL, "workspace")
         refused(paged(ws=None), EINVAL, "workspace")
