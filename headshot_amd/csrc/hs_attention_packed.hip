@@ -97,9 +97,9 @@ __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedT
 // does not see; o as the kernels hold it, channel 32 db + 8 (r / 4) + 4 hh + r %
 // 4 in register r.
 template <typename T, int DB>
-__device__ __forceinline__ void add_odd(f32x16 (&o)[DB], const PackedArgs& a, const PackedTile& t, int kv, int first,
-                                        int seen, int hh) {
-    for (int key = first / kBN * kBN; key < seen; key++) {
+__device__ __forceinline__ void add_odd(f32x16 (&o)[DB], const PackedArgs& a, const PackedTile& t, int kv, int tile,
+                                        int first, int seen, int hh) {
+    for (int key = first / tile * tile; key < seen; key++) {
         const T* row = static_cast<const T*>(a.v) + (t.k0 + key) * a.v_stride + kv * 32 * DB + 4 * hh;
 #pragma unroll
         for (int db = 0; db < DB; db++)
@@ -127,21 +127,26 @@ __device__ __forceinline__ void add_odd(f32x16 (&o)[DB], const PackedArgs& a, co
 // third more waves of four-wave workgroups in, but the addresses cost more
 // registers than there are.)
 //
-// Eight waves share a tile's keys and their staging (two workgroups per CU at
-// head dim 64, one at 128), four where the grid is small.
-template <int D, int W>
+// Eight waves share the keys and their staging (two workgroups per CU at head
+// dim 64, one at 128), four where the grid is small. SUB tiles lie between two
+// barriers: with one workgroup on a CU the waves drift apart in between, one's
+// softmax beside another's products (prompts of 32 heads of 128: 528 us with two
+// tiles, 551 with one; at head dim 64 two tiles leave one workgroup: 224 for
+// 213).
+template <int D, int W, int SUB>
 struct FlashF16 {
+    static constexpr int kKeys = SUB * kBN;       // keys between barriers
     static constexpr int kThr = 64 * W;
     static constexpr int kQueries = 32 * W;
     static constexpr int KS = D / 16;             // 16-dim slices of a score
     static constexpr int DB = D / 32;             // 32-channel blocks of an output
     static constexpr int kPieces = D / 8;         // 16-byte pieces of a row
-    static constexpr int kPer = kBN * kPieces / kThr;
+    static constexpr int kPer = kKeys * kPieces / kThr;
     static constexpr int kRowStep = kThr / kPieces;          // rows per load of the workgroup
     static constexpr int kKPitch = D + 8, kVPitch = D + 32;  // halves
     struct Smem {
-        f16 k[2][kBN * kKPitch];
-        f16 v[2][kBN * kVPitch];
+        f16 k[2][kKeys * kKPitch];
+        f16 v[2][kKeys * kVPitch];
         int odd;  // a tile whose values not every query sees holds an infinity or NaN
     };
 };
@@ -157,9 +162,9 @@ constexpr float kFar = 65536.0f;
 // A lane's row sum over a tile beyond which a weight may not fit f16.
 constexpr float kRowSumMax = 32768.0f;
 
-template <int D, int W>
+template <int D, int W, int SUB>
 __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed_f16_kernel(PackedArgs a) {
-    using F = FlashF16<D, W>;
+    using F = FlashF16<D, W, SUB>;
     constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
     __shared__ __align__(16) typename F::Smem sm;
     PackedTile t;
@@ -176,7 +181,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
     const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
     const int tile_least = keys_seen(t.first, t.nq, t.nk, a.causal);
     const int most = keys_seen(min(t.first + F::kQueries, t.nq) - 1, t.nq, t.nk, a.causal);
-    const int ntiles = (most + kBN - 1) / kBN;
+    const int ntiles = (most + F::kKeys - 1) / F::kKeys;
 
     // Q^T as the B operand: lane (n, hh) holds dims 16 ks + 8 hh .. + 8. A
     // negative scale is taken as one of -q.
@@ -212,7 +217,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
     auto load = [&](int key0) {
         const char* kt = kb + static_cast<int64_t>(key0) * a.k_stride * 2;
         const char* vt = vb + static_cast<int64_t>(key0) * a.v_stride * 2;
-        if (key0 + kBN <= t.nk) {
+        if (key0 + F::kKeys <= t.nk) {
 #pragma unroll
             for (int i = 0; i < kPer; i++) {
                 pk[i] = ld16(kt + static_cast<int64_t>(i * F::kRowStep) * a.k_stride * 2 + k_off);
@@ -229,7 +234,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
     };
     const int k_at = row0 * F::kKPitch + piece * 8, v_at = row0 * F::kVPitch + piece * 8;
     auto store = [&](int buf, int key0) {
-        if (key0 + kBN > tile_least) {  // some query does not see all of these values
+        if (key0 + F::kKeys > tile_least) {  // some query does not see all of these values
             bool odd = false;
 #pragma unroll
             for (int i = 0; i < kPer; i++)
@@ -256,14 +261,17 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
     }
     __syncthreads();
     for (int j = 0; j < ntiles; j++) {
-        const int cur = j & 1, key0 = j * kBN;
-        if (j + 1 < ntiles) load(key0 + kBN);
-        if (key0 < wave_most) {
+        const int cur = j & 1;
+        if (j + 1 < ntiles) load((j + 1) * F::kKeys);
+#pragma unroll
+        for (int sub = 0; sub < SUB; sub++) {
+            const int key0 = j * F::kKeys + sub * kBN;
+            if (key0 >= wave_most) continue;
             // S^T: s[kb] holds keys 32 kb .. + 32 of the tile, register r of
             // lane (n, hh) key 8 (r / 4) + 4 hh + r % 4, query n
             f32x16 s[2];
             const f32x16 z = {};
-            const f16* ka = sm.k[cur] + n * F::kKPitch + 8 * hh;
+            const f16* ka = sm.k[cur] + (sub * kBN + n) * F::kKPitch + 8 * hh;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -306,7 +314,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
             // Past the first tile the weights are taken against the reference
             // as it is; only a query whose sum says that one may not fit f16
             // moves its own.
-            bool own = j == 0 || fabsf(m) > kFar, move = __any(own);
+            bool own = key0 == 0 || fabsf(m) > kFar, move = __any(own);
             if (!move) {
                 const float sum = weights(c, m);
                 own = !(halves_max(sum) <= kRowSumMax) || !(sum <= kRowSumMax);
@@ -340,7 +348,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
             // O^T += V^T P^T. The transposing read gives lane i of 16 channel
             // i of 4 keys: two reads make the 8 keys, in the scores' order.
             const int vrow = 4 * hh + (n & 15) / 4;
-            const f16* va = sm.v[cur] + vrow * F::kVPitch + (n & 16) + 4 * (n & 3);
+            const f16* va = sm.v[cur] + (sub * kBN + vrow) * F::kVPitch + (n & 16) + 4 * (n & 3);
             auto read_v = [&](int g, int db) {
                 const f16* r0 = va + 16 * g * F::kVPitch + 32 * db;
                 const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)r0));
@@ -355,11 +363,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
                 for (int db = 0; db < DB; db++)
                     o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(read_v(g, db)), as_h8(p[g / 2][g % 2]), o[db], 0, 0, 0);
         }
-        if (j + 1 < ntiles) store(cur ^ 1, key0 + kBN);
+        if (j + 1 < ntiles) store(cur ^ 1, (j + 1) * F::kKeys);
         __syncthreads();
     }
     if (qi >= t.nq) return;
-    if (ntiles > 0 && sm.odd) add_odd<f16, DB>(o, a, t, kv, tile_least, seen, hh);
+    if (ntiles > 0 && sm.odd) add_odd<f16, DB>(o, a, t, kv, F::kKeys, tile_least, seen, hh);
     const float inv = 1.0f / halves_sum(l);
     f16* orow = static_cast<f16*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
 #pragma unroll
@@ -520,7 +528,7 @@ __device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const Packe
     }
     __syncthreads();
     if (qi >= t.nq || !mine) return;
-    if (sm.odd) add_odd<float, DB>(o, a, t, kv, tile_least, seen, hh);
+    if (sm.odd) add_odd<float, DB>(o, a, t, kv, kBN, tile_least, seen, hh);
     const float lsum = halves_sum(l);
     float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
 #pragma unroll
@@ -1030,8 +1038,8 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
         // heads of 128 over 8: 12000 2520, 2332, 2748 161, 178, twenty of 300
         // 67, 81): more reuse against more masked keys and longer tails.
         if ((n_q / 256 + b) * h * 2 >= 5 * num_cus() && n_q >= int64_t{2048} * b)
-            return d == 64 ? go(packed_f16_kernel<64, 8>, 256, 512) : go(packed_f16_kernel<128, 8>, 256, 512);
-        return d == 64 ? go(packed_f16_kernel<64, 4>, 128, 256) : go(packed_f16_kernel<128, 4>, 128, 256);
+            return d == 64 ? go(packed_f16_kernel<64, 8, 1>, 256, 512) : go(packed_f16_kernel<128, 8, 2>, 256, 512);
+        return d == 64 ? go(packed_f16_kernel<64, 4, 1>, 128, 256) : go(packed_f16_kernel<128, 4, 1>, 128, 256);
     }
     // Tiles of 32 queries a wave where they fill the chip's SIMDs, else 16 by
     // four waves
