@@ -43,7 +43,7 @@ struct PackedArgs {
     const void *q, *k, *v;
     void* out;
     int64_t q_stride, k_stride, v_stride;
-    const int *q_off, *k_off;
+    const int *q_off, *k_off;  // k_off null: the queries'
     int n_q, n_k, b, h, h_kv, tiles, causal;
     float scale;
 };
@@ -82,8 +82,9 @@ __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedT
         t.head = b % a.h;
     }
     int s, local;
-    if (!find_tile(a.q_off, a.b, a.n_q, bm, tile, s, local)) return false;
-    const RowRange q = row_range(a.q_off, s, a.n_q), k = row_range(a.k_off, s, a.n_k);
+    RowRange q;
+    if (!find_tile(a.q_off, a.b, a.n_q, bm, tile, s, q, local)) return false;
+    const RowRange k = a.k_off ? row_range(a.k_off, s, a.n_k) : q;
     t.q0 = q.begin, t.nq = q.end - q.begin, t.k0 = k.begin, t.nk = k.end - k.begin;
     t.first = ((t.nq + bm - 1) / bm - 1 - local) * bm;
     return true;
@@ -851,7 +852,7 @@ struct FewF32 {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 template <int D>
-__global__ __launch_bounds__(kThreads, 2) void packed_few_f32_kernel(PackedArgs a) {
+__global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kernel(PackedArgs a) {
     using F = FewF32<D>;
     constexpr int KS = D / 16, DB = D / 16;
     __shared__ __align__(16) typename F::Smem sm;
@@ -1019,7 +1020,7 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     a.q = q, a.k = k, a.v = v, a.out = out;
     a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
     a.q_off = static_cast<const int*>(q_offsets);
-    a.k_off = static_cast<const int*>(k_offsets ? k_offsets : q_offsets);
+    a.k_off = static_cast<const int*>(k_offsets);
     a.n_q = static_cast<int>(n_q), a.n_k = static_cast<int>(n_k), a.b = b, a.h = h, a.h_kv = h_kv;
     a.causal = causal, a.scale = scale;
     hipStream_t st = static_cast<hipStream_t>(stream);

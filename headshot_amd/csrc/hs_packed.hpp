@@ -49,17 +49,18 @@ __device__ __forceinline__ int wave_prefix_sum(int v) {
 }
 
 // Which sequence the tile-th tile of bm rows belongs to, all sequences' tiles
-// counted one after the other, and the tile's number within it; false past the
-// last. The lengths are device data, so a launch has as many workgroups as
+// counted one after the other, its rows, and the tile's number within it; false
+// past the last. The lengths are device data, so a launch has as many workgroups as
 // there can be tiles and each finds its own (64 sequences a step).
 __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int b, int n, int bm, int tile, int& s,
-                                          int& local) {
+                                          RowRange& rows, int& local) {
     const int lane = lane_id();
     int before = 0;
     for (int base = 0; base < b; base += 64) {
         int count = 0;
+        RowRange r = {};
         if (base + lane < b) {
-            const RowRange r = row_range(offsets, base + lane, n);
+            r = row_range(offsets, base + lane, n);
             count = static_cast<int>((static_cast<int64_t>(r.end - r.begin) + bm - 1) / bm);
         }
         const int sum = wave_prefix_sum(count);
@@ -67,6 +68,7 @@ __device__ __forceinline__ bool find_tile(const int* __restrict__ offsets, int b
         if (hit) {
             const int l = __builtin_ctzll(hit);
             s = base + l;
+            rows = {lane_value(r.begin, l), lane_value(r.end, l)};
             local = tile - before - (lane_value(sum, l) - lane_value(count, l));
             return true;
         }

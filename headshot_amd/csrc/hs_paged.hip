@@ -328,7 +328,7 @@ __device__ __forceinline__ Tile16 tile_of(const PagedArgs& a, int page, int kv, 
 // WHOLE: pages of at least 16 keys, so that 16 keys from a multiple of 16 lie in
 // one page; else each row looks its own up.
 template <typename T, int D, bool WHOLE>
-__global__ __launch_bounds__(64 * kPagedWaves) void attention_paged_kernel(PagedArgs a) {
+__global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_paged_kernel(PagedArgs a) {
     using P = Paged<T, D>;
     constexpr int V = P::V, kStep = P::kStep;
     __shared__ __align__(16) typename P::Smem sm;
