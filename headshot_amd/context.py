@@ -26,6 +26,7 @@ from . import _lib
 
 F32 = torch.float32
 F16 = torch.float16
+_DT = {F32: _lib.HS_F32, F16: _lib.HS_F16}
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -97,12 +98,12 @@ def _rows(t: torch.Tensor, heads: int, d: int, dtype, dev: int, what: str):
     """Token rows of head vectors, (n, heads, d) or (n, heads * d), possibly
     columns of wider rows: (address, n, elements between rows)."""
     shape, stride, width = t.shape, t.stride(), heads * d
+    n = shape[0]
     if len(shape) == 2:
         ok = shape[1] == width and (stride[1] == 1 or width <= 1)
     else:
         ok = (len(shape) == 3 and shape[1] == heads and shape[2] == d and stride[2] == 1
               and (stride[1] == d or heads <= 1))
-    n = shape[0]
     if t.dtype != dtype or not (ok or n == 0) or (n > 1 and stride[0] < width):
         raise AssertionError(f"{what} wants rows of {heads} contiguous head vectors of {d} in {dtype}, "
                              f"got {tuple(shape)} {t.dtype} with strides {stride}")
@@ -613,16 +614,6 @@ class HipContext:
         call()
         self.last_launch = call
 
-    @staticmethod
-    def _cache_shape(cache):
-        """A PagedKV's (n_pages, heads, page, d, sequences, max_pages)."""
-        k, v, table = cache.k, cache.v, cache.page_table
-        shape = k.shape
-        assert len(shape) == 4 and v.shape == shape and v.dtype == k.dtype, "cache: k and v (n_pages, heads, page, d)"
-        assert k.is_contiguous() and v.is_contiguous(), "cache pages must be contiguous"
-        assert table.dim() == 2, "page_table wants (sequences, max_pages)"
-        return (*shape, *table.shape)
-
     def kv_append(self, cache, k, v, offsets=None, q=None, qn=None, kn=None, rope=None,
                   positions=None, eps: float = 1e-5, k_rows: bool = False, out_q=None, out_k=None):
         """Appends new tokens' keys and values to their sequences' pages
@@ -640,16 +631,15 @@ class HipContext:
         page lies outside the table or the pool is not stored, and rows behind
         ``offsets[-1]`` stay as they are. Returns (q, k) as contiguous
         rows, None for what was not asked (``q``, ``k_rows``)."""
-        n_pages, h_kv, page, d, b, max_pages = self._cache_shape(cache)
-        dtype, dev = cache.k.dtype, _device()
-        dt = _dt(cache.k)
+        n_pages, h_kv, page, d, b, max_pages = cache.shape
+        dtype, dev = cache.dtype, _device()
+        if cache.device_index != dev:
+            raise AssertionError("the cache must live in memory of the current device")
         kp, n, ks = _rows(k, h_kv, d, dtype, dev, "k")
         vp, nv, vs = _rows(v, h_kv, d, dtype, dev, "v")
         assert nv == n, "k and v rows"
         assert offsets is not None or n == b, "without offsets, one token per sequence"
         off = None if offsets is None else _dense(offsets, b + 1, torch.int32, dev, "offsets")
-        table = _dense(cache.page_table, b * max_pages, torch.int32, dev, "page_table")
-        lens = _dense(cache.lens, b, torch.int32, dev, "lens")
         qp = qo = ko = qw = qb = kw = kb = sn = cs = pos = None
         qs = h = rows = 0
         if q is not None:
@@ -657,7 +647,7 @@ class HipContext:
             qp, nq, qs = _rows(q, h, d, dtype, dev, "q")
             assert nq == n, "q and k rows"
             if out_q is None:
-                out_q = torch.empty((n, h * d), dtype=dtype, device=q.device)
+                out_q = q.new_empty((n, h * d))
                 qo = out_q.data_ptr()
             else:
                 qo = _dense(out_q, n * h * d, dtype, dev, "out_q")
@@ -668,7 +658,7 @@ class HipContext:
             assert qn is None and out_q is None, "qn or out_q without q"
         if k_rows or out_k is not None:
             if out_k is None:
-                out_k = torch.empty((n, h_kv * d), dtype=dtype, device=k.device)
+                out_k = k.new_empty((n, h_kv * d))
                 ko = out_k.data_ptr()
             else:
                 ko = _dense(out_k, n * h_kv * d, dtype, dev, "out_k")
@@ -683,10 +673,10 @@ class HipContext:
             assert rope is not None, "positions without rope"
             pos = _dense(positions, n, torch.int32, dev, "positions")
         self._launch_held("kv_append", self.lib.hs_kv_append,
-                          (cache, k, v, offsets, q, qn, kn, rope, positions, out_q, out_k), dt, qp, qs, kp,
-                          ks, vp, vs, qw, qb, kw, kb, sn, cs, rows, pos, off, table, lens, qo, ko,
-                          _here(cache.k, dev, "k cache"), _here(cache.v, dev, "v cache"), n, b, h, h_kv, d,
-                          page, n_pages, max_pages, eps)
+                          (cache.k, cache.v, cache.page_table, cache.lens, k, v, offsets, q, qn, kn, rope, positions,
+                           out_q, out_k), _DT[dtype], qp, qs, kp, ks, vp, vs, qw, qb, kw, kb, sn, cs, rows, pos, off,
+                          cache.page_table.data_ptr(), cache.lens.data_ptr(), qo, ko, cache.k.data_ptr(),
+                          cache.v.data_ptr(), n, b, h, h_kv, d, page, n_pages, max_pages, eps)
         return out_q, out_k
 
     def attention_packed(self, q, k, v, offsets, k_offsets=None, causal: int = 1, scale=None,
@@ -714,7 +704,7 @@ class HipContext:
         off = _dense(offsets, b + 1, torch.int32, dev, "offsets")
         koff = None if k_offsets is None else _dense(k_offsets, b + 1, torch.int32, dev, "k_offsets")
         if out is None:
-            out = torch.empty((n, h * d), dtype=dtype, device=q.device)
+            out = q.new_empty((n, h * d))
         self._launch_held("attention_packed", self.lib.hs_attention_packed, (q, k, v, offsets, k_offsets, out),
                           dt, qp, qs, kp, ks, vp, vs, off, koff, _dense(out, n * h * d, dtype, dev, "out"),
                           n, m, b, h, h_kv, d, causal, 1.0 / math.sqrt(d) if scale is None else scale)
@@ -728,24 +718,30 @@ class HipContext:
         ``attention_paged_workspace`` bytes) keeps the call from allocating;
         calls that may run at the same time need one each. ``scale`` None is 1
         / sqrt(d)."""
-        n_pages, h_kv, page, d, b, max_pages = self._cache_shape(cache)
-        dtype, dev = cache.k.dtype, _device()
+        n_pages, h_kv, page, d, b, max_pages = cache.shape
+        dtype, dev = cache.dtype, _device()
+        if cache.device_index != dev:
+            raise AssertionError("the cache must live in memory of the current device")
         h = math.prod(q.shape[1:]) // d
         qp, n, qs = _rows(q, h, d, dtype, dev, "q")
         assert n == b, "one query row per sequence"
-        table = _dense(cache.page_table, b * max_pages, torch.int32, dev, "page_table")
-        lens = _dense(cache.lens, b, torch.int32, dev, "lens")
         if out is None:
-            out = torch.empty((b, h * d), dtype=dtype, device=q.device)
+            out = q.new_empty((b, h * d))
+            op = out.data_ptr()
+        else:
+            op = _dense(out, b * h * d, dtype, dev, "out")
         if workspace is None:
-            workspace = torch.empty(self.lib.hs_attention_paged_workspace(b, h, h_kv, d), dtype=torch.uint8,
-                                    device=q.device)
-        size = workspace.numel()
-        self._launch_held("attention_paged", self.lib.hs_attention_paged, (q, cache, out, workspace), _dt(cache.k),
-                          qp, qs, _here(cache.k, dev, "k cache"), _here(cache.v, dev, "v cache"), table, lens,
-                          _dense(out, b * h * d, dtype, dev, "out"),
-                          _dense(workspace, size, torch.uint8, dev, "workspace"), size, b, h, h_kv, d, page,
-                          n_pages, max_pages, 1.0 / math.sqrt(d) if scale is None else scale)
+            size = self.lib.hs_attention_paged_workspace(b, h, h_kv, d)
+            workspace = q.new_empty(size, dtype=torch.uint8)
+            wp = workspace.data_ptr()
+        else:
+            size = workspace.numel()
+            wp = _dense(workspace, size, torch.uint8, dev, "workspace")
+        self._launch_held("attention_paged", self.lib.hs_attention_paged,
+                          (q, cache.k, cache.v, cache.page_table, cache.lens, out, workspace), _DT[dtype], qp, qs,
+                          cache.k.data_ptr(), cache.v.data_ptr(), cache.page_table.data_ptr(), cache.lens.data_ptr(),
+                          op, wp, size, b, h, h_kv, d, page, n_pages, max_pages,
+                          1.0 / math.sqrt(d) if scale is None else scale)
         return out
 
     def attention_paged_workspace(self, sequences: int, heads: int, kv_heads: int, d: int) -> int:

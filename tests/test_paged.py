@@ -199,10 +199,31 @@ def test_python_attention(surface):
         lambda: ctx.attention_paged(q, cache()),
         lambda: ctx.attention_paged(q[:2].float(), cache()),
         lambda: ctx.attention_paged(q[:2], cache(), workspace=torch.zeros(4)),
+        lambda: ctx.attention_paged(q[:2], cache(), out=torch.zeros(2, 128, dtype=f16)),
     ]):
         with pytest.raises(AssertionError):
             f()
             pytest.fail(f"call {i} was taken")
+
+
+def test_python_cache():
+    """A cache is checked when it is made and when a tensor of it is replaced."""
+    c = cache()
+    assert (c.heads, c.page, c.head_dim) == (2, 16, 64) and c.shape == (4, 2, 16, 64, 2, 3)
+    c.lens += 1  # in place
+    assert c.lens.tolist() == [1, 1]
+    c.lens = torch.tensor([5, 6], dtype=torch.int32)
+    c.page_table = torch.zeros((2, 9), dtype=torch.int32)
+    assert c.shape[5] == 9
+    kept = c.lens
+    for name, t in [("lens", torch.zeros(3, dtype=torch.int32)), ("lens", torch.zeros(2, dtype=torch.int64)),
+                    ("page_table", torch.zeros(6, dtype=torch.int32)), ("k", c.k[:3]), ("v", c.v.float()),
+                    ("k", c.k.transpose(1, 2).contiguous().transpose(1, 2)), ("v", c.v[0])]:
+        with pytest.raises(AssertionError):
+            setattr(c, name, t)
+    assert c.lens is kept and c.k.shape == c.v.shape
+    with pytest.raises(AssertionError):
+        PagedKV(c.k.double(), c.v.double(), c.page_table, c.lens)
 
 
 def test_tensors_of_another_device():
@@ -221,3 +242,12 @@ def test_tensors_of_another_device():
     assert context._here(Elsewhere(), 1, "k") == 16
     with pytest.raises(AssertionError, match="current device"):
         context._here(Elsewhere(), 0, "k")
+
+
+def test_cache_of_another_device(surface, monkeypatch):
+    ctx, _ = surface
+    c, rows = cache(), torch.zeros((2, 128), dtype=torch.float16)
+    monkeypatch.setattr(context, "_device", lambda: 1)
+    for f in (lambda: ctx.kv_append(c, rows, rows), lambda: ctx.attention_paged(rows, c)):
+        with pytest.raises(AssertionError, match="current device"):
+            f()
