@@ -1,6 +1,21 @@
 // Attention of packed sequences for gfx950: whole prompts of different lengths
 // in one call, causal by token or by group of tokens, query heads sharing key
-// heads.
+// heads: O_i = sum_j w_ij v_j / sum_j w_ij, w_ij = exp(scale q_i k_j - m_i) over
+// the keys j that query i sees, in one pass over the keys with a running m_i.
+//
+// A workgroup takes a tile of one sequence's queries and one head, and finds
+// both on the device: lengths are device data, and the launch has a workgroup
+// for every tile that there can be. Keys past the tile's last query's are not
+// read, a wave whose queries see none of a tile sits it out, and only tiles that
+// some query sees in part are masked.
+//
+// Bounds: matrix and vector issue. f16: by frames, 10992 tokens of 16 heads of
+// 64, 204 us (795 TFLOP/s, matrix cores busy 45% of the time); prompts of 12926
+// tokens, 32 heads of 128 over 8, 517 us (937 TFLOP/s, 45%); a plain product of
+// 8192^3 reaches 1246. f32, head dim 64: 4122 tokens by frames 215 us (144
+// TFLOP/s; 363 on the f32 matrix instructions, whose plain product reaches 154).
+// Short calls are a chain of loads, find a tile, read it, multiply, of 6 us and
+// more: eight f32 sequences of up to 200 tokens, 16 heads of 128, 20 us.
 #include <cmath>
 
 #include "hs_packed.hpp"
@@ -1034,16 +1049,19 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     };
     if (dt == HS_F16) {
         // Tiles of 256 queries for long sequences that make enough of them, 128
-        // else (us with 128 and 256; 16 heads of 64: one sequence of 12000
-        // tokens 704, 643, of 6000 185, 199, eight of 1374, causal, 59, 66; 32
-        // heads of 128 over 8: 12000 2520, 2332, 2748 161, 178, twenty of 300
-        // 67, 81): more reuse against more masked keys and longer tails.
-        if ((n_q / 256 + b) * h * 2 >= 5 * num_cus() && n_q >= int64_t{2048} * b)
+        // else: more reuse against more masked keys and longer tails (us with
+        // 128 and 256; 16 heads of 64: one sequence of 12000 tokens 694, 630, of
+        // 6000 182, 195, eight of 1374, causal, 58, 66; 32 heads of 128 over 8:
+        // 12000 2486, 2236, 4122 362, 345, 2748 160, 171, twenty of 300 68, 81).
+        if ((n_q / 256 + b) * h >= 2 * num_cus() && n_q >= int64_t{2048} * b)
             return d == 64 ? go(packed_f16_kernel<64, 8, 1>, 256, 512) : go(packed_f16_kernel<128, 8, 2>, 256, 512);
         return d == 64 ? go(packed_f16_kernel<64, 4, 1>, 128, 256) : go(packed_f16_kernel<128, 4, 1>, 128, 256);
     }
-    // Tiles of 32 queries a wave where they fill the chip's SIMDs, else 16 by
-    // four waves
-    if ((n_q / 32 + b) * h >= 4 * num_cus()) return d == 64 ? go(packed_split_kernel, kBM, kThreads) : go(packed_f32_kernel<128>, kBM, kThreads);
+    // Tiles of 32 queries a wave where they fill the chip's SIMDs and themselves,
+    // else 16 by four waves (us with these and with tiles, 16 heads of 64 and of
+    // 128: one sequence of 200 tokens 10, 21 and 13, 42; of 1000 49, 65 and 106,
+    // 143; eight of 200 27, 24 and 51, 46; a hundred of 50 41, 46 and 78, 87).
+    if ((n_q / 32 + b) * h >= 4 * num_cus() && n_q >= int64_t{128} * b)
+        return d == 64 ? go(packed_split_kernel, kBM, kThreads) : go(packed_f32_kernel<128>, kBM, kThreads);
     return d == 64 ? go(packed_few_f32_kernel<64>, 16, kThreads) : go(packed_few_f32_kernel<128>, 16, kThreads);
 }

@@ -12,13 +12,15 @@ namespace {
 //
 // Bandwidth: one pass over the rows. A wave takes one token and up to two loads
 // of its heads, q | k | v one after the other, so there are many waves with a
-// few loads each (6 a token at 48 heads of 128 f16: 77 us for 82 with one wave
-// a token). A head vector is spread over G lanes. Two chunks each, [c, c + V)
-// and [D/2 + c, .. + V) with V elements per 16-byte load, put a rotation's pair
-// into one lane and make a norm one G-lane sum of both. f16 vectors of 64 are a
-// 128-byte line, which two such loads would touch by halves: there a lane takes
-// one chunk, the upper half's in reverse, so that a pair sits in mirror lanes,
-// and two heads instead.
+// few loads each (6 a token: 16381 tokens of 48 heads of 128 f16, rotated, 76
+// us, 5.8 TB/s; 82 with one wave a token). A head vector is spread over G lanes.
+// Two chunks each, [c, c + V) and [D/2 + c, .. + V) with V elements per 16-byte
+// load, put a rotation's pair into one lane and make a norm one G-lane sum of
+// both. f16 vectors of 64 are a 128-byte line, which two such loads would touch
+// by halves: there a lane takes one chunk, the upper half's in reverse, so that a
+// pair sits in mirror lanes, and two heads instead (10992 tokens of 48 heads,
+// QK-norm: 32 us, 5.0 TB/s; 42 by halves). A step's few tokens take 3-5 us, a
+// chain of four loads.
 
 template <int G>
 __device__ __forceinline__ float lanes_sum(float v) {
@@ -201,6 +203,10 @@ void launch_append(hipStream_t st, const AppendArgs<T>& a) {
 // A operand; V through the wave's own slice of LDS, from which V^T takes P^T as
 // the scores' registers hold it. Loads run a step ahead. The four waves' (O, m,
 // l) join in LDS, the ranges of a sequence in a second launch.
+//
+// 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 177 us, 5.8
+// TB/s; one token over 130531 keys of 16 heads of 64 89 us, 6.0 TB/s. 19
+// sequences of up to 3001 keys, 28 heads of 64 over 4, 13 us.
 //
 // Ranges: a sequence's keys are cut into pieces of `chunk` units of 4 kStep
 // keys, the same for all sequences of the call. A piece costs some 5 us before
@@ -577,6 +583,9 @@ __global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_p
 // columns that are not there, and the vector ones take some 500. Lanes r, r +
 // 16, .. hold key row r between them (K) and sum its product by halves and
 // quarters; V's rows lie a few to a load, each lane summing its four channels.
+// 16 heads of 128, us here and on the matrix instructions: 8 sequences of 400
+// keys 15.7, 17.2, of 800 24.5, 28.8, one of 8000 27.6, 30.8 (4.8 TB/s). With
+// two query heads to a key head the matrix instructions take 17.3 for 800.
 // (16 waves to a workgroup, so that 1024 keys need no second launch, are slower:
 // a CU draws some 50 GB/s, and the longest sequence waits for its one.)
 template <int D>

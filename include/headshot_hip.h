@@ -379,8 +379,11 @@ hs_status hs_attention_merged(hs_stream_t stream, hs_dtype dt, const void* q, co
  *
  * D is 64 or 128, Hq a multiple of Hkv (query head h reads key head h / (Hq /
  * Hkv)), page a power of two; buffers are 16-byte aligned and strides whole
- * 16-byte vectors (HS_EUNSUPPORTED otherwise). int32 arrays are given as const
- * void*. */
+ * 16-byte vectors (HS_EUNSUPPORTED otherwise). HS_EINVAL at the limits: rows
+ * 2^22 elements apart, more than 4096 heads, 2^30 for n_q * Hq, n_k and max_pages
+ * * page, 2^23 for b * Hq of hs_attention_paged, 2^27 or more (what one launch
+ * holds) for n * (Hq + 2 Hkv) of hs_kv_append; scale is finite. int32 arrays are
+ * given as const void*. */
 
 /* Appends the n new tokens' keys and values to their sequences' pages,
  * normalising and rotating the keys on the way, and the queries beside them.
@@ -413,8 +416,8 @@ hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q
  * 1: a token sees the keys up to the end of its own group of c tokens (1 the
  * usual causal mask, T frames of T tokens), groups counted from the first key.
  * A query that sees no key gets zeros. Keys and values that a query does not
- * see do not touch it, whatever they hold. Softmax statistics and sums are
- * f32; in f16 the weights of the product with V are rounded to f16, relative
+ * see do not enter its result, whatever they hold. Softmax statistics and sums
+ * are f32; in f16 the weights of the product with V are rounded to f16, relative
  * to the largest. out overlaps no input. */
 hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                               const void* k, int64_t k_stride, const void* v, int64_t v_stride,

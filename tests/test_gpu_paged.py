@@ -267,6 +267,22 @@ def test_packed_masked_values(ctx, dtype, d, value):
     assert torch.equal(got[:40], clean[:40])
 
 
+def test_block_by_frames(ctx):
+    """A prompt of frames through a block, masked by frames: the first frame is
+    the plain block's over it alone."""
+    from headshot_amd.aggregator import block_forward
+
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    w = BlockWeights.random(256, 512, 64, F16, DEV, gen, ls_init=0.1)
+    t, frames = 37, 3
+    x = torch.randn((t * frames, 256), generator=gen, device=DEV).half()
+    _, cache = make_cache(torch.Generator().manual_seed(4), [t * frames], 4, 16, 64, F16)
+    got = block_forward_cached(ctx, w, x, cache, 4, offsets=i32([0, t * frames]), causal=t)
+    alone = block_forward(ctx, w, x[:t], 1, t, 4)
+    # both within the bound that test_prompt_then_steps derives for a block
+    R.assert_within(got[:t], alone.cpu().double(), 2 * 2.0 ** -11 * 4 * (2 + 8 * 0.5), "first frame")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_packed_longer(ctx, dtype):
     """Several query tiles and many key tiles: against f64 on the GPU."""
@@ -604,21 +620,26 @@ def test_paged_far_pages(ctx):
 # --------------------------------------------------------------------- together
 
 
-def block_reference(w, x, heads, seen, eps):
-    """The block over one sequence in f64 on the CPU."""
+def block_reference(w, x, heads, seen, eps, tables=None):
+    """The block over one sequence in f64 on the CPU, rotated by position."""
     p, d = w.p, x.shape[1] // heads
     f = lambda t: t.cpu().double()  # noqa: E731
     ln = lambda t, n: torch.nn.functional.layer_norm(t, t.shape[-1:], f(n[0]), f(n[1]), eps)  # noqa: E731
     qkv = ln(x, p.ln1) @ f(w.qkv_w).T + f(w.qkv_b)
     q, k, v = (t.unflatten(1, (heads, d)) for t in qkv.chunk(3, 1))
-    att, _ = R.attention(ln(q, p.qn), ln(k, p.kn), v, seen, 1 / math.sqrt(d))
+    q, k = ln(q, p.qn), ln(k, p.kn)
+    if tables is not None:
+        q, k = (torch.stack([torch.stack([R.norm_rope(t[i, h], None, tables, i, eps) for h in range(heads)])
+                             for i in range(len(t))]) for t in (q, k))
+    att, _ = R.attention(q, k, v, seen, 1 / math.sqrt(d))
     x = x + f(p.ls1) * (att.flatten(1) @ f(w.proj_w).T + f(p.proj_b))
     h = torch.nn.functional.gelu(ln(x, p.ln2) @ f(w.fc1_w).T + f(p.fc1_b))
     return x + f(p.ls2) * (h @ f(w.fc2_w).T + f(p.fc2_b))
 
 
+@pytest.mark.parametrize("rope", [False, True])
 @pytest.mark.parametrize("dtype,dim,heads", [(F32, 256, 2), (F16, 256, 4)])
-def test_prompt_then_steps(ctx, dtype, dim, heads):
+def test_prompt_then_steps(ctx, dtype, dim, heads, rope):
     """Prompts of different lengths, then single tokens, through a block: each
     row is the one of the whole sequence in 64 bits."""
     gen = torch.Generator(device=DEV).manual_seed(3)
@@ -628,12 +649,17 @@ def test_prompt_then_steps(ctx, dtype, dim, heads):
     x = [torch.randn((n, dim), generator=gen, device=DEV).to(dtype) for n in total]
     _, cache = make_cache(torch.Generator().manual_seed(4), total, heads, 16, dim // heads, dtype)
     cache.lens.copy_(i32(lens))
+    tables = rope_tables(max(total), dim // heads) if rope else None
+    up = tuple(t.to(DEV) for t in tables) if rope else None
+    # the prompt's positions given, the steps' from the cache
+    positions = i32([i for n in lens for i in range(n)]) if rope else None
     got = block_forward_cached(ctx, w, torch.cat([a[:n] for a, n in zip(x, lens)]), cache, heads,
-                               offsets=i32(offsets_of(lens)), eps=eps)
+                               offsets=i32(offsets_of(lens)), rope=up, positions=positions, eps=eps)
     rows = [list(t) for t in got.split(lens)]
     for i in range(steps):
         cache.lens += 1
-        y = block_forward_cached(ctx, w, torch.stack([a[n + i] for a, n in zip(x, lens)]), cache, heads, eps=eps)
+        y = block_forward_cached(ctx, w, torch.stack([a[n + i] for a, n in zip(x, lens)]), cache, heads,
+                                 rope=up, eps=eps)
         for r, t in zip(rows, y):
             r.append(t)
     # The f32 block's sums are of up to 512 terms; in f16 each of the eight
@@ -641,5 +667,5 @@ def test_prompt_then_steps(ctx, dtype, dim, heads):
     # factors of 0.1 (LayerScale) for all but the last two.
     tol = 512 * R.U32 * 8 if dtype == F32 else 2.0 ** -11 * 4 * (2 + 8 * 0.5)
     for a, n, r in zip(x, total, rows):
-        ref = block_reference(w, a.cpu().double(), heads, R.seen_keys(n, n, 1), eps)
+        ref = block_reference(w, a.cpu().double(), heads, R.seen_keys(n, n, 1), eps, tables)
         R.assert_within(torch.stack(r), ref, torch.full_like(ref, tol), f"length {n}")
