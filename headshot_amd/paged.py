@@ -32,6 +32,9 @@ class PagedKV:
                 object.__setattr__(self, name, old)
                 raise
 
+    def __reduce__(self):  # copies and pickles
+        return PagedKV, (self.k, self.v, self.page_table, self.lens)
+
     def _check(self) -> None:
         k, v, table, lens = self.k, self.v, self.page_table, self.lens
         assert k.dim() == 4 and v.shape == k.shape, "cache: k and v (n_pages, heads, page, d)"

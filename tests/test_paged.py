@@ -1,5 +1,6 @@
 """The paged-cache operators' refusals on the CPU: the C ABI with addresses that
 are never dereferenced, and the Python surface. Nothing here launches a kernel."""
+import copy
 import ctypes
 
 import pytest
@@ -224,6 +225,15 @@ def test_python_cache():
     assert c.lens is kept and c.k.shape == c.v.shape
     with pytest.raises(AssertionError):
         PagedKV(c.k.double(), c.v.double(), c.page_table, c.lens)
+
+
+def test_python_cache_copies():
+    """A shallow copy shares the pages, a deep one has its own."""
+    c = cache()
+    near, far = copy.copy(c), copy.deepcopy(c)
+    assert near.shape == far.shape == c.shape and near.k is c.k and near.lens is c.lens
+    far.lens += 1
+    assert far.k is not c.k and c.lens.tolist() == [0, 0]
 
 
 def test_tensors_of_another_device():
