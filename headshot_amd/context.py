@@ -695,6 +695,7 @@ class HipContext:
         h_kv, dtype, dev = k.shape[1], q.dtype, _device()
         b = offsets.numel() - 1
         assert b >= 0, "offsets wants (sequences + 1)"
+        assert 0 <= causal < 2 ** 31, f"causal {causal}"
         dt = _dt(q)
         qp, n, qs = _rows(q, h, d, dtype, dev, "q")
         kp, m, ks = _rows(k, h_kv, d, dtype, dev, "k")

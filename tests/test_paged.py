@@ -197,6 +197,8 @@ def test_python_attention(surface):
         lambda: ctx.attention_packed(q, k, k, off.long()),
         lambda: ctx.attention_packed(q, k, k, off, off[:2]),
         lambda: ctx.attention_packed(q, k, k, off, out=torch.zeros(5, 256)),
+        lambda: ctx.attention_packed(q, k, k, off, causal=-1),
+        lambda: ctx.attention_packed(q, k, k, off, causal=2 ** 32 + 1),  # 1 in 32 bits
         lambda: ctx.attention_paged(q, cache()),
         lambda: ctx.attention_paged(q[:2].float(), cache()),
         lambda: ctx.attention_paged(q[:2], cache(), workspace=torch.zeros(4)),
