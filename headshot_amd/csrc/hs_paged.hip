@@ -931,7 +931,7 @@ extern "C" hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q
 }
 
 extern "C" int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d) {
-    if (b <= 0 || h <= 0 || h_kv <= 0 || h % h_kv != 0 || (d != 64 && d != 128)) return 0;
+    if (b <= 0 || h <= 0 || h > 4096 || h_kv <= 0 || h % h_kv != 0 || (d != 64 && d != 128)) return 0;
     using namespace hs;
     if (static_cast<int64_t>(b) * h >= (int64_t{1} << 23)) return 0;
     return PagedPlan(b, h, h_kv, kMostPerCu).rows * (d + 2) * 4 + static_cast<int64_t>(b) * 8;

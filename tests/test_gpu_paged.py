@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import paged_reference as R
-from headshot_amd.aggregator import BlockWeights, block_forward_cached
+from headshot_amd.aggregator import BlockWeights, block_forward, block_forward_cached
 from headshot_amd.paged import PagedKV
 
 pytestmark = pytest.mark.gpu
@@ -267,22 +267,6 @@ def test_packed_masked_values(ctx, dtype, d, value):
     assert torch.equal(got[:40], clean[:40])
 
 
-def test_block_by_frames(ctx):
-    """A prompt of frames through a block, masked by frames: the first frame is
-    the plain block's over it alone."""
-    from headshot_amd.aggregator import block_forward
-
-    gen = torch.Generator(device=DEV).manual_seed(21)
-    w = BlockWeights.random(256, 512, 64, F16, DEV, gen, ls_init=0.1)
-    t, frames = 37, 3
-    x = torch.randn((t * frames, 256), generator=gen, device=DEV).half()
-    _, cache = make_cache(torch.Generator().manual_seed(4), [t * frames], 4, 16, 64, F16)
-    got = block_forward_cached(ctx, w, x, cache, 4, offsets=i32([0, t * frames]), causal=t)
-    alone = block_forward(ctx, w, x[:t], 1, t, 4)
-    # both within the bound that test_prompt_then_steps derives for a block
-    R.assert_within(got[:t], alone.cpu().double(), 2 * 2.0 ** -11 * 4 * (2 + 8 * 0.5), "first frame")
-
-
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_packed_longer(ctx, dtype):
     """Several query tiles and many key tiles: against f64 on the GPU."""
@@ -521,6 +505,18 @@ def test_paged_long(ctx, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+def test_paged_shared_pages(ctx, dtype):
+    """Sequences with a common prefix read the same pages, and a table may name
+    a page twice."""
+    def share(c):
+        c.page_table[1, :2] = c.page_table[0, :2]
+        c.page_table[2, :3] = c.page_table[0, :1]
+
+    for h, h_kv in [(3, 3), (8, 2)]:
+        run_paged(ctx, 535, dtype, 64, h, h_kv, 16, [100, 61, 48], spoil=share)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_scales(ctx, dtype):
     for scale, std in [(1.0, 1.0), (0.3, 3.0), (-0.125, 1.0), (0.0, 1.0), (40.0, 100.0)]:
         run_paged(ctx, 530, dtype, 64, 4, 2, 16, [500, 90], scale=scale, std=std)
@@ -669,3 +665,17 @@ def test_prompt_then_steps(ctx, dtype, dim, heads, rope):
     for a, n, r in zip(x, total, rows):
         ref = block_reference(w, a.cpu().double(), heads, R.seen_keys(n, n, 1), eps, tables)
         R.assert_within(torch.stack(r), ref, torch.full_like(ref, tol), f"length {n}")
+
+
+def test_block_by_frames(ctx):
+    """A prompt of frames through a block, masked by frames: the first frame is
+    the plain block's over it alone."""
+    gen = torch.Generator(device=DEV).manual_seed(21)
+    w = BlockWeights.random(256, 512, 64, F16, DEV, gen, ls_init=0.1)
+    t, frames = 37, 3
+    x = torch.randn((t * frames, 256), generator=gen, device=DEV).half()
+    _, cache = make_cache(torch.Generator().manual_seed(4), [t * frames], 4, 16, 64, F16)
+    got = block_forward_cached(ctx, w, x, cache, 4, offsets=i32([0, t * frames]), causal=t)
+    alone = block_forward(ctx, w, x[:t], 1, t, 4)
+    # both within the bound that test_prompt_then_steps derives for a block
+    R.assert_within(got[:t], alone.cpu().double(), 2 * 2.0 ** -11 * 4 * (2 + 8 * 0.5), "first frame")

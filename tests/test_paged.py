@@ -125,6 +125,8 @@ def test_paged_refusals():
 def test_workspace_of_refused_shapes():
     f = L.hs_attention_paged_workspace
     assert f(0, 4, 2, 64) == 0 and f(2, 5, 2, 64) == 0 and f(2, 4, 0, 64) == 0 and f(2, 4, 2, 80) == 0
+    assert f(2, 8192, 2, 64) == 0
+    refused(paged(h=8192, qs=8192 * 64), EINVAL, "4096")
 
 
 # ------------------------------------------------------------ the Python surface
