@@ -156,8 +156,11 @@ extern "C" {
     pub fn hs_attention_packed(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
                                k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64,
                                q_offsets: *const c_void, k_offsets: *const c_void,
-                               out: *mut c_void, n_q: i64, n_k: i64, b: i32, h: i32, h_kv: i32,
-                               d: i32, causal: i32, scale: f32) -> HsStatus;
+                               out: *mut c_void, workspace: *mut c_void, workspace_bytes: i64,
+                               n_q: i64, n_k: i64, b: i32, h: i32, h_kv: i32, d: i32, causal: i32,
+                               scale: f32) -> HsStatus;
+    pub fn hs_attention_packed_workspace(dt: HsDtype, n_q: i64, n_k: i64, b: i32, h: i32,
+                                         h_kv: i32, d: i32, causal: i32) -> i64;
     pub fn hs_attention_paged_workspace(b: i32, h: i32, h_kv: i32, d: i32) -> i64;
     pub fn hs_attention_paged(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
                               k_cache: *const c_void, v_cache: *const c_void,

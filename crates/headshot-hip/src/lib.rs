@@ -830,15 +830,20 @@ impl HipContext {
         assert_eq!(v.dims(), (m, kv_width), "attention_packed v shape");
         assert!(k.dtype == q.dtype && v.dtype == q.dtype, "attention_packed dtype");
         assert!(d > 0 && width % d == 0 && kv_width % d == 0, "attention_packed widths");
+        let (b, h, h_kv) = (i32_of(sequences, "sequences"), i32_of(width / d, "h"),
+                            i32_of(kv_width / d, "h_kv"));
+        let (di, c) = (i32_of(d, "d"), i32_of(causal, "causal"));
+        let bytes = unsafe {
+            ffi::hs_attention_packed_workspace(q.dtype.raw(), n as i64, m as i64, b, h, h_kv, di, c)
+        };
+        let ws = self.empty_typed(&[(bytes as usize + 3) / 4], Dtype::F32);
         let out = self.empty_typed(&[n, width], q.dtype);
         check(unsafe {
             ffi::hs_attention_packed(self.stream, q.dtype.raw(), q.cptr(), width as i64, k.cptr(),
                                      kv_width as i64, v.cptr(), kv_width as i64,
                                      offsets as *const c_void, k_offsets as *const c_void,
-                                     out.mptr(), n as i64, m as i64, i32_of(sequences, "sequences"),
-                                     i32_of(width / d, "h"), i32_of(kv_width / d, "h_kv"),
-                                     i32_of(d, "d"), i32_of(causal, "causal"),
-                                     1.0 / (d as f32).sqrt())
+                                     out.mptr(), ws.mptr(), bytes, n as i64, m as i64, b, h, h_kv,
+                                     di, c, 1.0 / (d as f32).sqrt())
         }, "attention_packed");
         out
     }

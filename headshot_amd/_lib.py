@@ -68,8 +68,9 @@ SIGNATURES = {
     "hs_kv_append": (_S, [_P, _I32, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I32,
                           _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32,
                           _I32, _F]),
-    "hs_attention_packed": (_S, [_P, _I32, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _I64, _I64,
-                                 _I32, _I32, _I32, _I32, _I32, _F]),
+    "hs_attention_packed": (_S, [_P, _I32, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I64,
+                                 _I64, _I64, _I32, _I32, _I32, _I32, _I32, _F]),
+    "hs_attention_packed_workspace": (_I64, [_I32, _I64, _I64, _I32, _I32, _I32, _I32, _I32]),
     "hs_attention_paged_workspace": (_I64, [_I32, _I32, _I32, _I32]),
     "hs_attention_paged": (_S, [_P, _I32, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32,
                                 _I32, _I32, _I32, _I32, _F]),

@@ -680,7 +680,7 @@ class HipContext:
         return out_q, out_k
 
     def attention_packed(self, q, k, v, offsets, k_offsets=None, causal: int = 1, scale=None,
-                         out=None) -> torch.Tensor:
+                         out=None, workspace=None) -> torch.Tensor:
         """Attention of packed sequences of different lengths: ``q`` (n, heads,
         d), ``k``, ``v`` (m, kv_heads, d) rows at int32 ``offsets`` (and
         ``k_offsets`` where the keys' differ) -> token-major (n, heads * d), as
@@ -689,7 +689,10 @@ class HipContext:
         tokens and the ones before (1 the causal mask, T frames of T tokens);
         with more keys than queries the last query stands at the last key.
         A query that sees nothing gets zeros; rows behind ``offsets[-1]`` are
-        not written. ``scale`` None is 1 / sqrt(d)."""
+        not written. ``scale`` None is 1 / sqrt(d). Few queries over many keys
+        are split over the keys: ``workspace`` (uint8,
+        ``attention_packed_workspace`` bytes) keeps such a call from
+        allocating; calls that may run at the same time need one each."""
         assert q.dim() == 3 and k.dim() == 3 and v.dim() == 3, "attention_packed wants (n, heads, d)"
         _, h, d = q.shape
         h_kv, dtype, dev = k.shape[1], q.dtype, _device()
@@ -706,9 +709,19 @@ class HipContext:
         koff = None if k_offsets is None else _dense(k_offsets, b + 1, torch.int32, dev, "k_offsets")
         if out is None:
             out = q.new_empty((n, h * d))
-        self._launch_held("attention_packed", self.lib.hs_attention_packed, (q, k, v, offsets, k_offsets, out),
+        wp, size = None, 0
+        if workspace is not None:
+            size = workspace.numel()
+            wp = _dense(workspace, size, torch.uint8, dev, "workspace")
+        else:
+            size = self.lib.hs_attention_packed_workspace(dt, n, m, b, h, h_kv, d, causal)
+            if size:
+                workspace = q.new_empty(size, dtype=torch.uint8)
+                wp = workspace.data_ptr()
+        self._launch_held("attention_packed", self.lib.hs_attention_packed,
+                          (q, k, v, offsets, k_offsets, out, workspace),
                           dt, qp, qs, kp, ks, vp, vs, off, koff, _dense(out, n * h * d, dtype, dev, "out"),
-                          n, m, b, h, h_kv, d, causal, 1.0 / math.sqrt(d) if scale is None else scale)
+                          wp, size, n, m, b, h, h_kv, d, causal, 1.0 / math.sqrt(d) if scale is None else scale)
         return out
 
     def attention_paged(self, q, cache, scale=None, out=None, workspace=None) -> torch.Tensor:
@@ -744,6 +757,12 @@ class HipContext:
                           op, wp, size, b, h, h_kv, d, page, n_pages, max_pages,
                           1.0 / math.sqrt(d) if scale is None else scale)
         return out
+
+    def attention_packed_workspace(self, dtype, n_q: int, n_k: int, sequences: int, heads: int,
+                                   kv_heads: int, d: int, causal: int = 1) -> int:
+        """Bytes of workspace of ``attention_packed`` on the current device; 0
+        where the keys are not split."""
+        return self.lib.hs_attention_packed_workspace(_DT[dtype], n_q, n_k, sequences, heads, kv_heads, d, causal)
 
     def attention_paged_workspace(self, sequences: int, heads: int, kv_heads: int, d: int) -> int:
         """Bytes of workspace of ``attention_paged`` on the current device."""

@@ -7,15 +7,17 @@
 // both on the device: lengths are device data, and the launch has a workgroup
 // for every tile that there can be. Keys past the tile's last query's are not
 // read, a wave whose queries see none of a tile sits it out, and only tiles that
-// some query sees in part are masked.
+// some query sees in part are masked. Few queries over many keys are split over
+// the keys, too (PackedPlan).
 //
 // Bounds: matrix and vector issue. f16: by frames, 10992 tokens of 16 heads of
-// 64, 204 us (795 TFLOP/s, matrix cores busy 45% of the time); prompts of 12926
-// tokens, 32 heads of 128 over 8, 517 us (937 TFLOP/s, 45%); a plain product of
-// 8192^3 reaches 1246. f32, head dim 64: 4122 tokens by frames 215 us (144
-// TFLOP/s; 363 on the f32 matrix instructions, whose plain product reaches 154).
-// Short calls are a chain of loads, find a tile, read it, multiply, of 6 us and
-// more: eight f32 sequences of up to 200 tokens, 16 heads of 128, 20 us.
+// 64, 204-214 us (760-795 TFLOP/s, matrix cores busy 45% of the time); prompts of
+// 12926 tokens, 32 heads of 128 over 8, 517-545 us (890-937 TFLOP/s, 45%); a plain
+// product of 8192^3 reaches 1246. f32, head dim 64: 4122 tokens by frames 215-226
+// us (137-144 TFLOP/s; some 360 on the f32 matrix instructions, whose plain
+// product reaches 154). Short calls are a chain of loads, find a tile, read it,
+// multiply, of 6 us and more: eight f32 sequences of up to 200 tokens, 16 heads
+// of 128, 20 us.
 #include <cmath>
 
 #include "hs_packed.hpp"
@@ -59,15 +61,22 @@ struct PackedArgs {
     void* out;
     int64_t q_stride, k_stride, v_stride;
     const int *q_off, *k_off;  // k_off null: the queries'
-    int n_q, n_k, b, h, h_kv, tiles, causal;
+    int n_q, n_k, b, h, h_kv, causal;
+    int share;  // log2 of the query heads that a workgroup takes
     float scale;
+    // split keys only
+    float *ws_o, *ws_ml;  // per (item, head, row of the tile): D sums; maximum and weight sum
+    float per_piece;      // 1 / pieces wanted of a head
+    int items, pitch;     // items of a head that the launch has, rows of each
 };
 
 // What a workgroup works on: a tile of one sequence's queries, one head.
 struct PackedTile {
     int q0, nq;       // first query of the sequence's rows, its queries
     int k0, nk;       // the keys likewise
-    int first, head;  // first query of the tile, within the sequence
+    int first, head;  // first query of the tile, within the sequence, and head
+    // split keys: those of this piece, of how many the tile has, and its place
+    int begin, end, count, item;
 };
 
 // Keys that query i of a sequence sees.
@@ -80,21 +89,104 @@ __device__ __forceinline__ int keys_seen(int i, int nq, int nk, int causal) {
     return end < nk ? static_cast<int>(end) : nk;
 }
 
+// Split keys: where the tiles of a call are few, its keys are cut into pieces of
+// `chunk` units of 64, and an item is a piece of a tile; a second launch joins
+// them. chunk makes them as many as wanted and, lengths being device data, every
+// workgroup computes it from all of them (64 a step). A piece has kLeastUnits
+// units at least: it costs some 5 us before its first product and a unit 0.7 us.
+// (16 queries over 131072 keys, 32 heads of 128 over 8, f16: 118 us, 4.6 TB/s;
+// whole, 2.8 ms. 1374 tokens, 16 heads of 64, over 30000 keys: 264 us, 440.)
+constexpr int kLeastUnits = 4;
+
+struct PackedCut {
+    RowRange q, k;
+    int tiles;  // of the sequence
+    int local;  // the tile among them
+    int piece, pieces, chunk;
+    int item;   // piece 0's
+};
+__device__ __forceinline__ int units_of(const RowRange& k) { return (k.end - k.begin + kBN - 1) / kBN; }
+
+// The tile numbered `index` of a call (BY_TILE) or the item. chunk is at least
+// half the total of tiles times units over the pieces wanted (the f32 sum's error
+// is covered by per_piece), so a sequence's items pass neither twice those and
+// its tiles nor 31 bits whatever the offsets hold.
+template <bool BY_TILE>
+__device__ __forceinline__ bool find_cut(const PackedArgs& a, int bm, int index, PackedCut& t) {
+    const int lane = lane_id();
+    const auto ranges = [&](int s, RowRange& q, RowRange& k) {
+        q = row_range(a.q_off, s, a.n_q);
+        k = a.k_off ? row_range(a.k_off, s, a.n_k) : q;
+    };
+    float total = 0.0f;
+    for (int base = 0; base < a.b; base += 64) {
+        RowRange q = {}, k = {};
+        if (base + lane < a.b) ranges(base + lane, q, k);
+        const int masked = a.causal ? min(q.end - q.begin, k.end - k.begin) : 0;  // up to half of the keys, on average
+        total += static_cast<float>((q.end - q.begin + bm - 1) / bm) *
+                 (static_cast<float>(units_of(k)) - static_cast<float>(masked) * (0.5f / kBN));
+    }
+    t.chunk = static_cast<int>(fminf(fmaxf(ceilf(wave_sum(total) * a.per_piece), static_cast<float>(kLeastUnits)), 16777216.0f));
+    int tiles_before = 0, items_before = 0;
+    for (int base = 0; base < a.b; base += 64) {
+        RowRange q = {}, k = {};
+        if (base + lane < a.b) ranges(base + lane, q, k);
+        const int tiles = (q.end - q.begin + bm - 1) / bm;
+        const int pieces = max((units_of(k) + t.chunk - 1) / t.chunk, 1);
+        const int tile_sum = wave_prefix_sum(tiles), item_sum = wave_prefix_sum(tiles * pieces);
+        const uint64_t hit = __ballot((BY_TILE ? tiles_before + tile_sum : items_before + item_sum) > index);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            t.q = {lane_value(q.begin, l), lane_value(q.end, l)};
+            t.k = {lane_value(k.begin, l), lane_value(k.end, l)};
+            t.tiles = lane_value(tiles, l), t.pieces = lane_value(pieces, l);
+            const int before = items_before + lane_value(item_sum, l) - t.tiles * t.pieces;
+            t.local = BY_TILE ? index - tiles_before - (lane_value(tile_sum, l) - t.tiles) : (index - before) / t.pieces;
+            t.item = before + t.local * t.pieces;
+            // in another order from tile to tile: the last pieces, which an early
+            // tile's queries do not see, are not one XCD's
+            t.piece = BY_TILE ? 0 : (index - t.item + t.local) % t.pieces;
+            return true;
+        }
+        tiles_before += lane_value(tile_sum, 63), items_before += lane_value(item_sum, 63);
+    }
+    return false;
+}
+// Pieces of a tile whose last query sees `most` keys: the ones that see any.
+__device__ __forceinline__ int pieces_seen(int most, int chunk) {
+    return max((most + kBN * chunk - 1) / (kBN * chunk), 1);
+}
+
 // Workgroup b's tile. A sequence's last queries see the most keys and go first,
 // tile by tile over the heads, so that the first workgroups, two and more to a
 // CU, are not all a head's longest. Workgroup b runs on XCD b % 8: where the
 // heads divide by it, an XCD takes h / 8 heads in a row, so that the heads of a
 // key head, and a head's tiles, read their keys through one L2.
+template <bool SPLIT>
 __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedTile& t) {
     const int b = blockIdx.x;
+    const int all = a.h >> a.share;
     int tile;
-    if (a.h % kXcds == 0) {
-        const int slot = b / kXcds, heads = a.h / kXcds;
+    if (all % kXcds == 0) {
+        const int slot = b / kXcds, heads = all / kXcds;
         tile = slot / heads;
         t.head = b % kXcds * heads + slot % heads;
     } else {
-        tile = b / a.h;
-        t.head = b % a.h;
+        tile = b / all;
+        t.head = b % all;
+    }
+    t.head <<= a.share;
+    if constexpr (SPLIT) {
+        PackedCut c;
+        if (!find_cut<false>(a, bm, tile, c)) return false;
+        t.q0 = c.q.begin, t.nq = c.q.end - c.q.begin, t.k0 = c.k.begin, t.nk = c.k.end - c.k.begin;
+        t.first = (c.tiles - 1 - c.local) * bm;
+        const int most = keys_seen(min(t.first + bm, t.nq) - 1, t.nq, t.nk, a.causal);
+        t.count = pieces_seen(most, c.chunk), t.item = c.item + c.piece;
+        if (c.piece >= t.count) return false;
+        t.begin = c.piece * c.chunk * kBN;
+        t.end = c.piece + 1 < t.count ? t.begin + c.chunk * kBN : most;
+        return true;
     }
     int s, local;
     RowRange q;
@@ -102,7 +194,30 @@ __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedT
     const RowRange k = a.k_off ? row_range(a.k_off, s, a.n_k) : q;
     t.q0 = q.begin, t.nq = q.end - q.begin, t.k0 = k.begin, t.nk = k.end - k.begin;
     t.first = ((t.nq + bm - 1) / bm - 1 - local) * bm;
+    t.begin = 0, t.end = keys_seen(min(t.first + bm, t.nq) - 1, t.nq, t.nk, a.causal), t.count = 1;
     return true;
+}
+
+// Row `row` of the tile's place in the workspace.
+__device__ __forceinline__ int64_t partial_row(const PackedArgs& a, const PackedTile& t, int row) {
+    return (static_cast<int64_t>(t.item) * a.h + t.head) * a.pitch + row;
+}
+// A piece's sums of a query, in the layout of the 32 x 32 products.
+template <int DB>
+__device__ __forceinline__ void put_partial(const PackedArgs& a, const PackedTile& t, int row, int hh, const f32x16 (&o)[DB],
+                                            float m, float l, float factor) {
+    const int64_t at = partial_row(a, t, row);
+    float* p = a.ws_o + at * 32 * DB + 4 * hh;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = f2u(o[db][4 * r4 + e] * factor);
+            st16(p + 32 * db + 8 * r4, w);
+        }
+    if (hh == 0) a.ws_ml[2 * at] = m, a.ws_ml[2 * at + 1] = l * factor;
 }
 
 // An infinity or NaN among a tile's values, where some queries see them and
@@ -110,12 +225,12 @@ __device__ __forceinline__ bool packed_tile(const PackedArgs& a, int bm, PackedT
 // into LDS as zeros, and a workgroup that has met any adds them here to the sums
 // of the queries that do see them. A weight is positive, so what they make of a
 // sum is what they sum to. First: the first key that some query of the workgroup
-// does not see; o as the kernels hold it, channel 32 db + 8 (r / 4) + 4 hh + r %
+// does not see, seen: the end of the query's own; o as the kernels hold it, channel 32 db + 8 (r / 4) + 4 hh + r %
 // 4 in register r.
 template <typename T, int DB>
 __device__ __forceinline__ void add_odd(f32x16 (&o)[DB], const PackedArgs& a, const PackedTile& t, int kv, int tile,
                                         int first, int seen, int hh) {
-    for (int key = first / tile * tile; key < seen; key++) {
+    for (int key = max(first / tile * tile, t.begin); key < min(seen, t.end); key++) {
         const T* row = static_cast<const T*>(a.v) + (t.k0 + key) * a.v_stride + kv * 32 * DB + 4 * hh;
 #pragma unroll
         for (int db = 0; db < DB; db++)
@@ -178,26 +293,28 @@ constexpr float kFar = 65536.0f;
 // A lane's row sum over a tile beyond which a weight may not fit f16.
 constexpr float kRowSumMax = 32768.0f;
 
-template <int D, int W, int SUB>
+template <int D, int W, int SUB, bool SPLIT>
 __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed_f16_kernel(PackedArgs a) {
     using F = FlashF16<D, W, SUB>;
     constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
     __shared__ __align__(16) typename F::Smem sm;
     PackedTile t;
-    if (!packed_tile(a, F::kQueries, t)) return;  // workgroup-uniform, before any barrier
+    const int share = W == 4 ? a.share : 0, rows = F::kQueries >> share;
+    if (!packed_tile<SPLIT>(a, rows, t)) return;  // workgroup-uniform, before any barrier
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int n = lane & 31, hh = lane >> 5;
     const int kv = t.head / (a.h / a.h_kv);
+    const int block = 32 * (wave & ((W >> share) - 1));  // the wave's queries
+    t.head += wave * 32 / rows;
 
     // The keys seen grow with the query: the tile's last live query has the most
-    const int qi = t.first + 32 * wave + n;
-    const bool live = t.first + 32 * wave < t.nq;  // wave-uniform
+    const int qi = t.first + block + n;
+    const bool live = t.first + block < t.nq;  // wave-uniform
     const int seen = keys_seen(min(qi, t.nq - 1), t.nq, t.nk, a.causal);
-    const int wave_least = keys_seen(min(t.first + 32 * wave, t.nq - 1), t.nq, t.nk, a.causal);
-    const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
+    const int wave_least = keys_seen(min(t.first + block, t.nq - 1), t.nq, t.nk, a.causal);
+    const int wave_most = live ? keys_seen(min(t.first + block + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
     const int tile_least = keys_seen(t.first, t.nq, t.nk, a.causal);
-    const int most = keys_seen(min(t.first + F::kQueries, t.nq) - 1, t.nq, t.nk, a.causal);
-    const int ntiles = (most + F::kKeys - 1) / F::kKeys;
+    const int tile0 = SPLIT ? t.begin / F::kKeys : 0, ntiles = (t.end + F::kKeys - 1) / F::kKeys;
 
     // Q^T as the B operand: lane (n, hh) holds dims 16 ks + 8 hh .. + 8. A
     // negative scale is taken as one of -q.
@@ -271,12 +388,12 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
     };
     if (tid == 0) sm.odd = 0;
     __syncthreads();
-    if (ntiles > 0) {
-        load(0);
-        store(0, 0);
+    if (tile0 < ntiles) {
+        load(tile0 * F::kKeys);
+        store(tile0 & 1, tile0 * F::kKeys);
     }
     __syncthreads();
-    for (int j = 0; j < ntiles; j++) {
+    for (int j = tile0; j < ntiles; j++) {
         const int cur = j & 1;
         if (j + 1 < ntiles) load((j + 1) * F::kKeys);
 #pragma unroll
@@ -330,7 +447,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
             // Past the first tile the weights are taken against the reference
             // as it is; only a query whose sum says that one may not fit f16
             // moves its own.
-            bool own = key0 == 0 || fabsf(m) > kFar, move = __any(own);
+            bool own = key0 == (SPLIT ? t.begin : 0) || fabsf(m) > kFar, move = __any(own);
             if (!move) {
                 const float sum = weights(c, m);
                 own = !(halves_max(sum) <= kRowSumMax) || !(sum <= kRowSumMax);
@@ -383,7 +500,11 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
         __syncthreads();
     }
     if (qi >= t.nq) return;
-    if (ntiles > 0 && sm.odd) add_odd<f16, DB>(o, a, t, kv, F::kKeys, tile_least, seen, hh);
+    if (tile0 < ntiles && sm.odd) add_odd<f16, DB>(o, a, t, kv, F::kKeys, tile_least, seen, hh);
+    if (SPLIT && t.count > 1) {
+        put_partial<DB>(a, t, block + n, hh, o, m, halves_sum(l), 1.0f);
+        return;
+    }
     const float inv = 1.0f / halves_sum(l);
     f16* orow = static_cast<f16*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
 #pragma unroll
@@ -425,7 +546,7 @@ __device__ __forceinline__ bool odd_f32(uint32_t bits) { return (bits & 0x7F8000
 
 // The tile's queries, those of lanes with `mine` stored; every wave of the
 // workgroup calls it (barriers inside).
-template <int D>
+template <int D, bool SPLIT>
 __device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const PackedTile& t, typename FlashF32<D>::Smem& sm, bool mine) {
     using F = FlashF32<D>;
     constexpr int DB = F::DB, kPer = F::kPer;
@@ -441,7 +562,7 @@ __device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const Packe
     const int wave_least = keys_seen(min(t.first + 32 * wave, t.nq - 1), t.nq, t.nk, a.causal);
     const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
     const int tile_least = keys_seen(t.first, t.nq, t.nk, a.causal);
-    const int most = keys_seen(min(t.first + kBM, t.nq) - 1, t.nq, t.nk, a.causal);
+    const int begin = SPLIT ? t.begin : 0;
 
     const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
     const uint32_t flip = a.scale < 0.0f ? 0x80000000u : 0u;
@@ -469,9 +590,9 @@ __device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const Packe
     };
     __syncthreads();
     if (tid == 0) sm.odd = 0;
-    if (most > 0) load(0);
+    if (begin < t.end) load(begin);
 #pragma unroll 1
-    for (int key0 = 0; key0 < most; key0 += kBN) {
+    for (int key0 = begin; key0 < t.end; key0 += kBN) {
         __syncthreads();  // the previous tile has been read
         if (key0 + kBN > tile_least) {  // some query does not see all of these values
             bool odd = false;
@@ -488,7 +609,7 @@ __device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const Packe
             st16(&sm.v[(row0 + kRowStep * i) * F::kVPitch + col0], pv[i]);
         }
         __syncthreads();
-        if (key0 + kBN < most) load(key0 + kBN);
+        if (key0 + kBN < t.end) load(key0 + kBN);
         if (key0 >= wave_most) continue;
 
         f32x16 s[2] = {f32x16{}, f32x16{}};
@@ -545,6 +666,10 @@ __device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const Packe
     __syncthreads();
     if (qi >= t.nq || !mine) return;
     if (sm.odd) add_odd<float, DB>(o, a, t, kv, kBN, tile_least, seen, hh);
+    if (SPLIT && t.count > 1) {
+        put_partial<DB>(a, t, 32 * wave + n, hh, o, m, halves_sum(l), 1.0f);
+        return;
+    }
     const float lsum = halves_sum(l);
     float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * D + 4 * hh;
 #pragma unroll
@@ -558,12 +683,12 @@ __device__ __forceinline__ void packed_f32_tile(const PackedArgs& a, const Packe
         }
 }
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void packed_f32_kernel(PackedArgs a) {
     __shared__ __align__(16) typename FlashF32<D>::Smem sm;
     PackedTile t;
-    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
-    packed_f32_tile<D>(a, t, sm, true);
+    if (!packed_tile<SPLIT>(a, kBM, t)) return;  // workgroup-uniform, before any barrier
+    packed_f32_tile<D, SPLIT>(a, t, sm, true);
 }
 
 // f32, head dim 64, on the bf16 matrix instructions, sixteen times the f32
@@ -606,6 +731,7 @@ __device__ __forceinline__ uint32_t largest(uint32_t most, const u32x4 (&f)[2]) 
     return most;
 }
 
+template <bool SPLIT>
 __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a) {
     union Smem {
         SplitSmem split;
@@ -615,7 +741,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
     __shared__ int again;  // bit 0: every query of the tile, bit 1: some
     SplitSmem& sm = smem.split;
     PackedTile t;
-    if (!packed_tile(a, kBM, t)) return;  // workgroup-uniform, before any barrier
+    if (!packed_tile<SPLIT>(a, kBM, t)) return;  // workgroup-uniform, before any barrier
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int n = lane & 31, hh = lane >> 5;
     const int kv = t.head / (a.h / a.h_kv);
@@ -626,7 +752,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
     const int seen = keys_seen(min(qi, t.nq - 1), t.nq, t.nk, a.causal);
     const int wave_least = keys_seen(min(t.first + 32 * wave, t.nq - 1), t.nq, t.nk, a.causal);
     const int wave_most = live ? keys_seen(min(t.first + 32 * wave + 31, t.nq - 1), t.nq, t.nk, a.causal) : 0;
-    const int most = keys_seen(min(t.first + kBM, t.nq) - 1, t.nq, t.nk, a.causal);
+    const int begin = SPLIT ? t.begin : 0;
     const float c = a.scale * 1.4426950408889634f;  // goes into the queries
     if (tid == 0) again = 0;
     __syncthreads();
@@ -663,7 +789,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
             for (int e = 0; e < 4; e++) small.note(u2f(vr[i][e / 2][2 * (e % 2)]), u2f(vr[i][e / 2][2 * (e % 2) + 1]));
         }
     };
-    if (most > 0) load(0);
+    if (begin < t.end) load(begin);
 
     u32x4 qp[3][4];
     bool bad_q;
@@ -687,11 +813,11 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
     f32x16 o[2] = {f32x16{}, f32x16{}}, ol[2] = {f32x16{}, f32x16{}};
     float m = kFloor, l = 0.0f;
 #pragma unroll 1
-    for (int key0 = 0; key0 < most; key0 += kBN) {
+    for (int key0 = begin; key0 < t.end; key0 += kBN) {
         __syncthreads();  // the previous tile has been read
         stage();
         __syncthreads();
-        const bool more = key0 + kBN < most;
+        const bool more = key0 + kBN < t.end;
         if (key0 >= wave_most) {
             if (more) load(key0 + kBN);
             continue;
@@ -764,7 +890,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
         };
         // as in f16: the reference moves on the first tile and where a weight
         // might pass 2^15 times the largest at it, for the query's own sums only
-        bool own = key0 == 0, move = own;
+        bool own = key0 == begin, move = own;
         if (!move) {
             const float ps = weights(m);
             own = !(halves_max(ps) <= kRowSumMax * kSplitScale);
@@ -828,7 +954,13 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
     __syncthreads();
     const int redo = again;
     const bool mine = (redo & 1) != 0 || bad_q;
-    if (qi < t.nq && !mine) {
+    if (SPLIT && t.count > 1) {
+        if (qi < t.nq && !mine) {
+#pragma unroll
+            for (int db = 0; db < 2; db++) o[db] += ol[db];
+            put_partial<2>(a, t, 32 * wave + n, hh, o, m, halves_sum(l), 1.0f / kSplitScale);
+        }
+    } else if (qi < t.nq && !mine) {
         const float lsum = halves_sum(l);
         float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + qi) * a.h + t.head) * kSD + 4 * hh;
 #pragma unroll
@@ -841,7 +973,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
                 st16(orow + 32 * db + 8 * r4, w);
             }
     }
-    if (redo) packed_f32_tile<kSD>(a, t, smem.f32, mine);  // workgroup-uniform
+    if (redo) packed_f32_tile<kSD, SPLIT>(a, t, smem.f32, mine);  // workgroup-uniform
 }
 
 // f32, short sequences: a serial chain per query, so it is cut as finely as the
@@ -866,13 +998,13 @@ struct FewF32 {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kernel(PackedArgs a) {
     using F = FewF32<D>;
     constexpr int KS = D / 16, DB = D / 16;
     __shared__ __align__(16) typename F::Smem sm;
     PackedTile t;
-    if (!packed_tile(a, F::kQueries, t)) return;  // workgroup-uniform, before any barrier
+    if (!packed_tile<SPLIT>(a, F::kQueries, t)) return;  // workgroup-uniform, before any barrier
     const int lane = lane_id(), wave = wave_in_block();
     const int n = lane & 15, g = lane >> 4;
     const int kv = t.head / (a.h / a.h_kv);
@@ -881,7 +1013,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kern
     const int qi = t.first + n;
     const int seen = keys_seen(min(qi, t.nq - 1), t.nq, t.nk, a.causal);
     const int least = keys_seen(t.first, t.nq, t.nk, a.causal);
-    const int most = keys_seen(min(t.first + F::kQueries, t.nq) - 1, t.nq, t.nk, a.causal);
+    const int begin = (SPLIT ? t.begin : 0) + 16 * wave;
 
     const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
     const uint32_t flip = a.scale < 0.0f ? 0x80000000u : 0u;
@@ -910,9 +1042,9 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kern
         for (int i = 0; i < KS; i++) kr[i] = ld16(kp + 16 * i);
     };
     constexpr int kTurn = 16 * kWaves;
-    if (16 * wave < most) load_v(16 * wave), load_k(16 * wave);
+    if (begin < t.end) load_v(begin), load_k(begin);
 #pragma unroll 1
-    for (int key0 = 16 * wave; key0 < most; key0 += kTurn) {
+    for (int key0 = begin; key0 < t.end; key0 += kTurn) {
         const bool partial = key0 + 16 > least;  // some query does not see all of these keys
         if (partial) {
 #pragma unroll
@@ -927,7 +1059,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kern
             st16(vs + (F::kVRows * i + lane / F::kRowLanes) * F::kPitch + lane % F::kRowLanes * 4, vr[i]);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (key0 + kTurn < most) load_v(key0 + kTurn);
+        if (key0 + kTurn < t.end) load_v(key0 + kTurn);
         f32x4 acc[4] = {f32x4{}, f32x4{}, f32x4{}, f32x4{}};
 #pragma unroll
         for (int i = 0; i < KS; i++)
@@ -938,7 +1070,7 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kern
         // rounded before the maximum is taken off: that one then weighs 1
 #pragma unroll
         for (int j = 0; j < 4; j++) s[j] = as_f32(s[j] * c);
-        if (key0 + kTurn < most) load_k(key0 + kTurn);
+        if (key0 + kTurn < t.end) load_k(key0 + kTurn);
         if (partial)
 #pragma unroll
             for (int j = 0; j < 4; j++)
@@ -988,12 +1120,18 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kern
             weight = fmaf(sm.l[w][q], f, weight);
         }
         if (sm.odd)
-            for (int key = least / 16 * 16; key < keys; key++) {
+            for (int key = max(least / 16 * 16, t.begin); key < min(keys, t.end); key++) {
                 const u32x4 v = ld16(vb + key * a.v_stride + d0);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     if (odd_f32(v[e])) sum[e] += u2f(v[e]);
             }
+        if (SPLIT && t.count > 1) {
+            const int64_t at = partial_row(a, t, q);
+            *reinterpret_cast<f32x4*>(a.ws_o + at * D + d0) = sum;
+            if (d0 == 0) a.ws_ml[2 * at] = top, a.ws_ml[2 * at + 1] = weight;
+            continue;
+        }
         float* orow = static_cast<float*>(a.out) + (static_cast<int64_t>(t.q0 + t.first + q) * a.h + t.head) * D + d0;
         u32x4 w;
 #pragma unroll
@@ -1002,14 +1140,135 @@ __global__ __launch_bounds__(kThreads, D == 64 ? 2 : 3) void packed_few_f32_kern
     }
 }
 
+// Sums of two pieces joined. An infinity of values stays one where the other
+// piece's maximum leaves it a weight of 0.
+__device__ __forceinline__ void join_sums(f32x4& sum, float& weight, float& top, f32x4 v, float l, float m) {
+    const float next = fmaxf(top, m);
+    const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float x = sum[e] * old, y = v[e] * f;
+        sum[e] = (x != x ? sum[e] : x) + (y != y ? v[e] : y);
+    }
+    weight = fmaf(weight, old, l * f);
+    top = next;
+}
+
+// The pieces of a tile's queries joined: a workgroup takes one (query, head), its
+// threads the pieces (SHARE), or kRows of them, each its pieces in turn.
+template <typename T, int D, bool SHARE>
+__global__ __launch_bounds__(kThreads) void packed_join_kernel(PackedArgs a, int bm) {
+    constexpr int kLanes = D / 4, kRows = kThreads / kLanes;
+    __shared__ __align__(16) f32x4 part[kRows][kLanes];
+    __shared__ float tops[kRows], weights[kRows];
+    const int group = threadIdx.x / kLanes, col = threadIdx.x % kLanes;
+    const int per_tile = SHARE ? a.pitch : (a.pitch + kRows - 1) / kRows;
+    const int tile_head = static_cast<int>(blockIdx.x) / per_tile;
+    const int tile = tile_head / a.h, head = tile_head - tile * a.h;
+    PackedCut c;
+    if (!find_cut<true>(a, bm, tile, c)) return;  // workgroup-uniform, as what follows
+    const int nq = c.q.end - c.q.begin, nk = c.k.end - c.k.begin;
+    const int first = (c.tiles - 1 - c.local) * bm, rows = min(bm, nq - first);
+    const int count = pieces_seen(keys_seen(first + rows - 1, nq, nk, a.causal), c.chunk);
+    if (count == 1) return;                // written by its only piece
+    if (c.item + count > a.items) return;  // offsets that do not ascend
+    const int row0 = static_cast<int>(blockIdx.x) - tile_head * per_tile;
+    const int row = SHARE ? row0 : row0 * kRows + group;
+    float top = kFloor, weight = 0.0f;
+    f32x4 sum = {};
+    if (row < rows) {
+        PackedTile t;
+        t.head = head;
+        for (int i = SHARE ? group : 0; i < count; i += SHARE ? kRows : 1) {
+            t.item = c.item + i;
+            const int64_t at = partial_row(a, t, row);
+            const float m = a.ws_ml[2 * at], l = a.ws_ml[2 * at + 1];
+            const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + at * D + 4 * col);
+            join_sums(sum, weight, top, v, l, m);
+        }
+    }
+    if constexpr (SHARE) {
+        part[group][col] = sum;
+        if (col == 0) tops[group] = top, weights[group] = weight;
+        __syncthreads();
+        if (group != 0) return;
+        for (int i = 1; i < min(kRows, count); i++) join_sums(sum, weight, top, part[i][col], weights[i], tops[i]);
+    }
+    if (row >= rows) return;
+    const bool sees = keys_seen(first + row, nq, nk, a.causal) > 0;
+    T* orow = static_cast<T*>(a.out) + (static_cast<int64_t>(c.q.begin + first + row) * a.h + head) * D + 4 * col;
+#pragma unroll
+    for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(sees ? sum[e] / weight : 0.0f);
+}
+
+// How a call is cut into tiles and whether its keys are split.
+struct PackedPlan {
+    enum Kernel { kWide, kFour, kTile, kFew } kernel;
+    int bm, share;          // queries of a tile; log2 of the heads that a workgroup takes
+    int64_t tiles;          // of a head, as many as sequences of these rows can have
+    int64_t pieces, items;  // of a head: wanted, and what they can come to; 0: whole keys
+    int64_t pitch;
+    PackedPlan(hs_dtype dt, int64_t n_q, int64_t n_k, int64_t b, int64_t h, int64_t h_kv, int d, int causal) {
+        const int64_t cus = num_cus(), group = h / h_kv;
+        const bool half = dt == HS_F16;
+        // Enough keys for a second launch to pay (us split and whole, f16, one
+        // causal sequence: 4 heads of 128 over 2, 2000 tokens 26, 49, 1200 28, 33;
+        // 8 heads of 64, 2000 tokens 27, 35; 4 of 64, 1500 27, 28)
+        const bool long_keys = n_k >= (d == 64 ? 1536 : 1024) && n_k >= 256 * b;
+        // f16, few queries a sequence: two or four query heads of a key head share
+        // a workgroup and its keys, which leaves no wave idle (32 heads of 128
+        // over 8, split: 16 queries over 131072 keys 118 us, 221 by head; four
+        // times 64 over 30000 205, 285)
+        share = 0;
+        if (half && n_q <= 64 * b && group % 2 == 0) share = n_q <= 32 * b && group % 4 == 0 ? 2 : 1;
+        const int64_t all = h >> share;
+        const auto cut = [&](Kernel k, int rows) { kernel = k, bm = rows, tiles = n_q / rows + (b < n_q ? b : n_q); };
+        // f16: tiles of 256 queries for long sequences that make enough of them,
+        // 128 else: more reuse against more masked keys and longer tails (us with
+        // 128 and 256; 16 heads of 64: one sequence of 12000 tokens 694, 630, of
+        // 6000 182, 195, eight of 1374, causal, 58, 66; 32 heads of 128 over 8:
+        // 12000 2486, 2236, 4122 362, 345, 2748 160, 171, twenty of 300 68, 81).
+        // f32: tiles of 32 queries a wave where they fill the chip's SIMDs and
+        // themselves, else 16 by four waves (us with these and with tiles, 16
+        // heads of 64 and of 128: one sequence of 200 tokens 10, 21 and 13, 42; of
+        // 1000 49, 65 and 106, 143; eight of 200 27, 24 and 51, 46; a hundred of
+        // 50 41, 46 and 78, 87); at head dim 64 tiles split over many keys, too
+        // (one head of 7000 tokens 71, 117 with 16, causal; 98, 159 not).
+        if (half)
+            (n_q / 256 + b) * h >= 2 * cus && n_q >= 2048 * b ? cut(kWide, 256) : cut(kFour, 128 >> share);
+        else
+            ((n_q / 32 + b) * h >= 4 * cus || (d == 64 && long_keys)) && n_q >= 128 * b ? cut(kTile, kBM) : cut(kFew, 16);
+        pieces = items = pitch = 0;
+        // Keys are split where the tiles fill less than half of the chip: into as
+        // many pieces as it holds at once, or twice that where a tile would have
+        // but two or three (1374 tokens over 30000, 16 heads of 64, f32: 1082 us,
+        // 1204). The causal mask empties up to half of the items, beyond those.
+        const int64_t slots = cus * (kernel == kFew || (half && d == 64) ? 3 : 2);
+        if (kernel == kWide || 2 * tiles * all > slots || !long_keys) return;
+        pieces = (4 * tiles * all > slots && kernel != kFew ? 2 : 1) * slots / all - tiles;
+        if (pieces < 1) pieces = 1;
+        items = (causal ? 2 : 1) * pieces + tiles;
+        pitch = n_q < bm ? n_q : bm;
+    }
+    int64_t workspace(int64_t h, int d) const { return items * h * pitch * (d + 2) * 4; }
+};
+
 }  // namespace
 }  // namespace hs
 
+extern "C" int64_t hs_attention_packed_workspace(hs_dtype dt, int64_t n_q, int64_t n_k, int32_t b, int32_t h,
+                                                 int32_t h_kv, int32_t d, int32_t causal) {
+    using namespace hs;
+    if (n_q <= 0 || n_k <= 0 || b <= 0 || h <= 0 || causal < 0 || n_k >= (int64_t{1} << 30) || n_q >= (int64_t{1} << 30) / h) return 0;
+    if (check_heads("attention_packed_workspace", dt, h, h_kv, d)) return 0;
+    return PackedPlan(dt, n_q, n_k, b, h, h_kv, d, causal).workspace(h, d);
+}
+
 extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                                          const void* k, int64_t k_stride, const void* v, int64_t v_stride,
-                                         const void* q_offsets, const void* k_offsets, void* out, int64_t n_q,
-                                         int64_t n_k, int32_t b, int32_t h, int32_t h_kv, int32_t d, int32_t causal,
-                                         float scale) {
+                                         const void* q_offsets, const void* k_offsets, void* out, void* workspace,
+                                         int64_t workspace_bytes, int64_t n_q, int64_t n_k, int32_t b, int32_t h,
+                                         int32_t h_kv, int32_t d, int32_t causal, float scale) {
     using namespace hs;
     const char* op = "attention_packed";
     if (hs_status rc = check_heads(op, dt, h, h_kv, d)) return rc;
@@ -1024,12 +1283,19 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     if (hs_status rc = check_rows(op, "k", k, n_k, k_stride, kv_width, dt)) return rc;
     if (hs_status rc = check_rows(op, "v", v, n_k, v_stride, kv_width, dt)) return rc;
     if (!out || !q_offsets) return fail(HS_EINVAL, "%s: null out or q_offsets", op);
-    if (!aligned16(out)) return fail(HS_EUNSUPPORTED, "%s: out must be 16-byte aligned", op);
+    if (!aligned16(out) || !aligned16(workspace)) return fail(HS_EUNSUPPORTED, "%s: out and workspace must be 16-byte aligned", op);
+    const PackedPlan plan(dt, n_q, n_k, b, h, h_kv, d, causal);
+    const int64_t need = plan.workspace(h, d);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(HS_EINVAL, "%s: workspace of %lld bytes, %lld needed", op, static_cast<long long>(workspace_bytes), static_cast<long long>(need));
     const int64_t out_bytes = n_q * width * dtype_size(dt);
-    if (overlaps(out, out_bytes, q, row_bytes(n_q, q_stride, width, dt)) ||
-        overlaps(out, out_bytes, k, row_bytes(n_k, k_stride, kv_width, dt)) ||
-        overlaps(out, out_bytes, v, row_bytes(n_k, v_stride, kv_width, dt)))
+    const int64_t q_bytes = row_bytes(n_q, q_stride, width, dt), k_bytes = row_bytes(n_k, k_stride, kv_width, dt);
+    const int64_t v_bytes = row_bytes(n_k, v_stride, kv_width, dt);
+    if (overlaps(out, out_bytes, q, q_bytes) || overlaps(out, out_bytes, k, k_bytes) || overlaps(out, out_bytes, v, v_bytes))
         return fail(HS_EINVAL, "%s: out overlaps an input", op);
+    if (overlaps(workspace, need, q, q_bytes) || overlaps(workspace, need, k, k_bytes) || overlaps(workspace, need, v, v_bytes) ||
+        overlaps(workspace, need, out, out_bytes))
+        return fail(HS_EINVAL, "%s: workspace overlaps another buffer", op);
     if (!std::isfinite(scale)) return fail(HS_EINVAL, "%s: scale must be finite", op);
     PackedArgs a;
     a.q = q, a.k = k, a.v = v, a.out = out;
@@ -1037,31 +1303,46 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     a.q_off = static_cast<const int*>(q_offsets);
     a.k_off = static_cast<const int*>(k_offsets);
     a.n_q = static_cast<int>(n_q), a.n_k = static_cast<int>(n_k), a.b = b, a.h = h, a.h_kv = h_kv;
-    a.causal = causal, a.scale = scale;
+    a.causal = causal, a.scale = scale, a.share = plan.share;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    // as many tiles as sequences of these rows can have
-    const auto go = [&](auto kernel, int bm, int threads) {
-        const int64_t tiles = n_q / bm + (b < n_q ? b : n_q);
-        if (tiles * h >= (int64_t{1} << 31) / threads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
-        a.tiles = static_cast<int>(tiles);
-        kernel<<<dim3(static_cast<uint32_t>(tiles * h)), dim3(threads), 0, st>>>(a);
+    const int threads = plan.kernel == PackedPlan::kWide ? 512 : kThreads;
+    const int64_t per_head = plan.items ? plan.items : plan.tiles;
+    const int64_t groups = per_head * (h >> plan.share);
+    if (groups >= (int64_t{1} << 31) / threads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
+    const auto go = [&](auto kernel) {
+        kernel<<<dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, st>>>(a);
+        return check_launch(op);
+    };
+    if (plan.kernel == PackedPlan::kWide) return d == 64 ? go(packed_f16_kernel<64, 8, 1, false>) : go(packed_f16_kernel<128, 8, 2, false>);
+    if (!plan.items) {
+        if (plan.kernel == PackedPlan::kFour) return d == 64 ? go(packed_f16_kernel<64, 4, 1, false>) : go(packed_f16_kernel<128, 4, 1, false>);
+        if (plan.kernel == PackedPlan::kTile) return d == 64 ? go(packed_split_kernel<false>) : go(packed_f32_kernel<128, false>);
+        return d == 64 ? go(packed_few_f32_kernel<64, false>) : go(packed_few_f32_kernel<128, false>);
+    }
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_ml = a.ws_o + plan.items * h * plan.pitch * d;
+    // (rounded up by twice the error of the kernels' sum over the sequences)
+    a.per_piece = static_cast<float>((1.0 + (b / 64 + 64) * 0x1p-23) / static_cast<double>(plan.pieces));
+    a.items = static_cast<int>(plan.items), a.pitch = static_cast<int>(plan.pitch);
+    hs_status rc;
+    if (plan.kernel == PackedPlan::kFour)
+        rc = d == 64 ? go(packed_f16_kernel<64, 4, 1, true>) : go(packed_f16_kernel<128, 4, 1, true>);
+    else if (plan.kernel == PackedPlan::kTile)
+        rc = d == 64 ? go(packed_split_kernel<true>) : go(packed_f32_kernel<128, true>);
+    else
+        rc = d == 64 ? go(packed_few_f32_kernel<64, true>) : go(packed_few_f32_kernel<128, true>);
+    if (rc) return rc;
+    // many pieces to a query: a workgroup each
+    const bool share = plan.items >= 16 * plan.tiles;
+    const int64_t rows = share ? plan.pitch : ceil_div(plan.pitch, int64_t{kThreads / (d / 4)});
+    const auto join = [&](auto kernel) {
+        kernel<<<dim3(static_cast<uint32_t>(plan.tiles * h * rows)), dim3(kThreads), 0, st>>>(a, plan.bm);
         return check_launch(op);
     };
     if (dt == HS_F16) {
-        // Tiles of 256 queries for long sequences that make enough of them, 128
-        // else: more reuse against more masked keys and longer tails (us with
-        // 128 and 256; 16 heads of 64: one sequence of 12000 tokens 694, 630, of
-        // 6000 182, 195, eight of 1374, causal, 58, 66; 32 heads of 128 over 8:
-        // 12000 2486, 2236, 4122 362, 345, 2748 160, 171, twenty of 300 68, 81).
-        if ((n_q / 256 + b) * h >= 2 * num_cus() && n_q >= int64_t{2048} * b)
-            return d == 64 ? go(packed_f16_kernel<64, 8, 1>, 256, 512) : go(packed_f16_kernel<128, 8, 2>, 256, 512);
-        return d == 64 ? go(packed_f16_kernel<64, 4, 1>, 128, 256) : go(packed_f16_kernel<128, 4, 1>, 128, 256);
+        if (d == 64) return share ? join(packed_join_kernel<f16, 64, true>) : join(packed_join_kernel<f16, 64, false>);
+        return share ? join(packed_join_kernel<f16, 128, true>) : join(packed_join_kernel<f16, 128, false>);
     }
-    // Tiles of 32 queries a wave where they fill the chip's SIMDs and themselves,
-    // else 16 by four waves (us with these and with tiles, 16 heads of 64 and of
-    // 128: one sequence of 200 tokens 10, 21 and 13, 42; of 1000 49, 65 and 106,
-    // 143; eight of 200 27, 24 and 51, 46; a hundred of 50 41, 46 and 78, 87).
-    if ((n_q / 32 + b) * h >= 4 * num_cus() && n_q >= int64_t{128} * b)
-        return d == 64 ? go(packed_split_kernel, kBM, kThreads) : go(packed_f32_kernel<128>, kBM, kThreads);
-    return d == 64 ? go(packed_few_f32_kernel<64>, 16, kThreads) : go(packed_few_f32_kernel<128>, 16, kThreads);
+    if (d == 64) return share ? join(packed_join_kernel<float, 64, true>) : join(packed_join_kernel<float, 64, false>);
+    return share ? join(packed_join_kernel<float, 128, true>) : join(packed_join_kernel<float, 128, false>);
 }

@@ -418,12 +418,22 @@ hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q
  * A query that sees no key gets zeros. Keys and values that a query does not
  * see do not enter its result, whatever they hold. Softmax statistics and sums
  * are f32; in f16 the weights of the product with V are rounded to f16, relative
- * to the largest. out overlaps no input. */
+ * to the largest. Few queries over many keys are split over the keys and joined,
+ * by the counts given and all lengths of the call; such calls take
+ * hs_attention_packed_workspace bytes (16-byte aligned, else NULL), which hold
+ * nothing between calls: calls that may run at the same time need their own. out
+ * overlaps nothing else. */
 hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                               const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                               const void* q_offsets, const void* k_offsets, void* out,
-                              int64_t n_q, int64_t n_k, int32_t b, int32_t h, int32_t h_kv,
-                              int32_t d, int32_t causal, float scale);
+                              void* workspace, int64_t workspace_bytes, int64_t n_q, int64_t n_k,
+                              int32_t b, int32_t h, int32_t h_kv, int32_t d, int32_t causal,
+                              float scale);
+
+/* Bytes of workspace that hs_attention_packed takes on the current device; 0 for
+ * most shapes, whose keys are not split, and for those that it refuses. */
+int64_t hs_attention_packed_workspace(hs_dtype dt, int64_t n_q, int64_t n_k, int32_t b, int32_t h,
+                                      int32_t h_kv, int32_t d, int32_t causal);
 
 /* Bytes of workspace that hs_attention_paged takes for b sequences on the
  * current device; 0 for shapes that it refuses. */

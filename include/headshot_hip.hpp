@@ -481,11 +481,15 @@ class HipContext {
         HS_REQUIRE(k.dtype() == q.dtype() && v.dtype() == q.dtype(), "attention_packed: dtype");
         HS_REQUIRE(v.len() == k.len() && v.last() == k.last(), "attention_packed: k and v shapes");
         const size_t n = q.len() / q.last(), m = k.len() / k.last();
+        const int32_t b = i32(sequences), h = i32(q.last() / d), h_kv = i32(k.last() / d);
+        const int64_t bytes = hs_attention_packed_workspace(hs_dtype(q.dtype()), static_cast<int64_t>(n),
+                                                            static_cast<int64_t>(m), b, h, h_kv, i32(d), causal);
         HipTensor out = empty_typed({n, q.last()}, q.dtype());
+        HipTensor ws = empty_typed({static_cast<size_t>(bytes + 3) / 4}, Dtype::F32);
         check(hs_attention_packed(stream_, hs_dtype(q.dtype()), q.data(), static_cast<int64_t>(q.last()), k.data(),
                                   static_cast<int64_t>(k.last()), v.data(), static_cast<int64_t>(v.last()), offsets,
-                                  k_offsets, out.data(), static_cast<int64_t>(n), static_cast<int64_t>(m),
-                                  i32(sequences), i32(q.last() / d), i32(k.last() / d), i32(d), causal,
+                                  k_offsets, out.data(), ws.data(), bytes, static_cast<int64_t>(n),
+                                  static_cast<int64_t>(m), b, h, h_kv, i32(d), causal,
                                   1.0f / std::sqrt(static_cast<float>(d))),
               "attention_packed");
         return out;

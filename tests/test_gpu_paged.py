@@ -221,6 +221,112 @@ def test_packed_other_keys(ctx, dtype, causal):
     run_packed(ctx, 411, dtype, 128, 2, 1, [130, 1, 66], [64, 300, 1], causal)
 
 
+@pytest.mark.parametrize("causal", [0, 1, 12])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_short_shared_heads(ctx, dtype, d, causal):
+    """Short sequences whose query heads share key heads, by two, four and more."""
+    for i, (h, h_kv, nq, nk) in enumerate([
+        (8, 2, [5, 32, 1, 0, 7], [5, 32, 1, 0, 7]),
+        (12, 1, [33, 20], [33, 320]),
+        (6, 1, [60, 64], [60, 64]),
+        (32, 8, [1, 2, 3], [65, 64, 0]),
+        (64, 4, [9], [130]),
+    ]):
+        print(f"[packed shared {dtype} d={d} causal={causal} case {i}]", flush=True)
+        run_packed(ctx, 445 + i, dtype, d, h, h_kv, nq, nk, causal, wide=i % 2 == 0, behind=i)
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan, "lowest"])
+def test_packed_short_masked_values(ctx, value):
+    x = torch.finfo(F16).min if value == "lowest" else value
+
+    def poison(q, k, v):
+        k[20], v[15, :, 3], v[33] = x, x, x
+
+    run_packed(ctx, 446, F16, 64, 8, 2, [30, 6], [30, 6], 1, poison=poison)
+
+
+def split(ctx, dtype, d, h, h_kv, nq, nk, causal):
+    """Whether a call's keys are split."""
+    return ctx.attention_packed_workspace(dtype, sum(nq), sum(nk), len(nq), h, h_kv, d, causal) > 0
+
+
+@pytest.mark.parametrize("causal", [0, 1, 7, 1000])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_split_keys(ctx, dtype, d, causal):
+    """Few queries over many keys, of sequences long and short; rows that see
+    nothing, no key or no query; wide rows; tiles of both kinds."""
+    for i, (h, h_kv, nq, nk) in enumerate([
+        (2, 1, [1], [2048]),
+        (3, 3, [1, 16, 17], [2500, 1, 900]),
+        (8, 2, [3, 0, 40, 2], [700, 900, 20, 3000]),
+        (2, 2, [1, 1, 1, 1], [0, 2100, 64, 65]),
+        (2, 1, [200, 130], [3001, 1500]),
+        (1, 1, [2200], [2200]),
+    ]):
+        print(f"[packed split {dtype} d={d} causal={causal} case {i}]", flush=True)
+        assert split(ctx, dtype, d, h, h_kv, nq, nk, causal)
+        run_packed(ctx, 450 + i, dtype, d, h, h_kv, nq, nk, causal, wide=i % 2 == 1, behind=i)
+
+
+@pytest.mark.parametrize("nq", [5, 150])
+@pytest.mark.parametrize("value", [math.inf, math.nan, "lowest"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_split_odd_values(ctx, dtype, value, nq):
+    """Infinities and NaN in seen and in masked places of a split call, and
+    scores that move the maximum from piece to piece."""
+    x = torch.finfo(dtype).min if value == "lowest" else value
+
+    def poison(q, k, v):
+        n = k.shape[0]
+        k[: n // 2] *= 1.5
+        v[n // 3, :, 3], v[n - 2, :, 5], k[n - 1, :, 0] = x, x, x
+
+    for causal in (1, 10):
+        assert split(ctx, dtype, 64, 2, 1, [nq], [2700], causal)
+        run_packed(ctx, 460, dtype, 64, 2, 1, [nq], [2700], causal, poison=poison)
+
+
+def test_packed_split_f32_sizes(ctx):
+    """f32 values that the bf16 parts do not hold, in one piece's keys, in the
+    values, in some queries: those are computed another way, the rest is not."""
+    def at(where, x):
+        def poison(q, k, v):
+            {"q": q, "k": k, "v": v}[where][17, :, 5] = x
+        return poison
+
+    for where, x in [("q", 2.0 ** 60), ("k", 2.0 ** 55), ("v", 2.0 ** 70), ("v", 2.0 ** -120), ("k", 2.0 ** -130)]:
+        assert split(ctx, F32, 64, 2, 2, [300], [2500], 1)
+        run_packed(ctx, 470, F32, 64, 2, 2, [300], [2500], 1, poison=at(where, x))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_split_graph(ctx, dtype):
+    """A captured split call follows its offsets, the caller's workspace holding
+    anything; the call's own workspace gives the same."""
+    gen = torch.Generator().manual_seed(14)
+    q, k, v = (normal(gen, (n, h, 64), dtype).to(DEV) for n, h in ((60, 4), (4000, 2), (4000, 2)))
+    off, koff = i32([0, 30, 60]), i32([0, 2000, 4000])
+    size = ctx.attention_packed_workspace(dtype, 60, 4000, 2, 4, 2, 64, 1)
+    assert size > 0
+    ws = torch.full((size,), 0xFF, dtype=torch.uint8, device=DEV)
+    ctx.attention_packed(q, k, v, off, koff, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = ctx.attention_packed(q, k, v, off, koff, workspace=ws)
+    for i, (cut, kcut) in enumerate([(30, 2000), (0, 0), (60, 4000), (1, 3999), (59, 10), (17, 2048)]):
+        off.copy_(i32([0, cut, 60]))
+        koff.copy_(i32([0, kcut, 4000]))
+        ws.fill_(255 if i % 2 else 0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = captured.clone()
+        assert torch.equal(got, ctx.attention_packed(q, k, v, off, koff)), f"cut {cut} {kcut}"
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_packed_scales(ctx, dtype):
     """Peaked weights, a scale of the caller's, negative and zero ones."""

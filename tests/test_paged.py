@@ -65,9 +65,10 @@ def test_append_refusals():
     assert append(n=0, b=0, off=None) == OK
 
 
-def packed(dt=F16, q=at(0), qs=256, k=at(1), ks=128, v=at(2), vs=128, off=at(3), koff=at(4), out=at(5), n=10,
-           m=12, b=2, h=4, h_kv=2, d=64, causal=1, scale=0.125):
-    return L.hs_attention_packed(None, dt, q, qs, k, ks, v, vs, off, koff, out, n, m, b, h, h_kv, d, causal, scale)
+def packed(dt=F16, q=at(0), qs=256, k=at(1), ks=128, v=at(2), vs=128, off=at(3), koff=at(4), out=at(5), ws=at(6),
+           nbytes=1 << 27, n=10, m=12, b=2, h=4, h_kv=2, d=64, causal=1, scale=0.125):
+    return L.hs_attention_packed(None, dt, q, qs, k, ks, v, vs, off, koff, out, ws, nbytes, n, m, b, h, h_kv, d,
+                                 causal, scale)
 
 
 def test_packed_refusals():
@@ -89,6 +90,12 @@ def test_packed_refusals():
     refused(packed(out=ctypes.c_void_p(0x60000008)), EUNSUPPORTED, "16-byte")
     refused(packed(out=at(2)), EINVAL, "overlaps")
     refused(packed(n=1 << 29), EINVAL, "2^30")
+    refused(packed(ws=ctypes.c_void_p(0x70000008)), EUNSUPPORTED, "16-byte")
+    if L.hs_attention_packed_workspace(F16, 10, 5000, 2, 4, 2, 64, 1) > 0:
+        refused(packed(m=5000, nbytes=0), EINVAL, "workspace")
+        refused(packed(m=5000, ws=None), EINVAL, "workspace")
+        refused(packed(m=5000, ws=at(1)), EINVAL, "workspace overlaps")
+        refused(packed(m=5000, ws=at(5)), EINVAL, "workspace overlaps")
     assert packed(n=0, koff=at(4)) == OK
     assert packed(b=0) == OK
 
@@ -126,6 +133,11 @@ def test_workspace_of_refused_shapes():
     f = L.hs_attention_paged_workspace
     assert f(0, 4, 2, 64) == 0 and f(2, 5, 2, 64) == 0 and f(2, 4, 0, 64) == 0 and f(2, 4, 2, 80) == 0
     assert f(2, 8192, 2, 64) == 0
+    g = L.hs_attention_packed_workspace
+    assert g(F16, 0, 5000, 2, 4, 2, 64, 1) == 0 and g(F16, 10, -1, 2, 4, 2, 64, 1) == 0
+    assert g(F16, 10, 5000, 0, 4, 2, 64, 1) == 0 and g(F16, 10, 5000, 2, 5, 2, 64, 1) == 0
+    assert g(F16, 10, 5000, 2, 4, 2, 80, 1) == 0 and g(7, 10, 5000, 2, 4, 2, 64, 1) == 0
+    assert g(F32, 10, 5000, 2, 4, 2, 64, -1) == 0 and g(F32, 1 << 29, 5000, 2, 4, 2, 64, 1) == 0
     refused(paged(h=8192, qs=8192 * 64), EINVAL, "4096")
 
 
@@ -199,6 +211,7 @@ def test_python_attention(surface):
         lambda: ctx.attention_packed(q, k, k, off.long()),
         lambda: ctx.attention_packed(q, k, k, off, off[:2]),
         lambda: ctx.attention_packed(q, k, k, off, out=torch.zeros(5, 256)),
+        lambda: ctx.attention_packed(q, k, k, off, workspace=torch.zeros(64)),
         lambda: ctx.attention_packed(q, k, k, off, causal=-1),
         lambda: ctx.attention_packed(q, k, k, off, causal=2 ** 32 + 1),  # 1 in 32 bits
         lambda: ctx.attention_paged(q, cache()),
