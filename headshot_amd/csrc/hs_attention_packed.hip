@@ -1212,7 +1212,7 @@ struct PackedPlan {
         const int64_t cus = num_cus(), group = h / h_kv;
         const bool half = dt == HS_F16;
         // Enough keys for a second launch to pay (us split and whole, f16, one
-        // causal sequence: 4 heads of 128 over 2, 2000 tokens 26, 49, 1200 28, 33;
+        // causal sequence: 4 heads of 128 over 2, 2000 tokens 27, 49, 1200 22, 33;
         // 8 heads of 64, 2000 tokens 27, 35; 4 of 64, 1500 27, 28)
         const bool long_keys = n_k >= (d == 64 ? 1536 : 1024) && n_k >= 256 * b;
         // f16, few queries a sequence: two or four query heads of a key head share
@@ -1233,7 +1233,7 @@ struct PackedPlan {
         // heads of 64 and of 128: one sequence of 200 tokens 10, 21 and 13, 42; of
         // 1000 49, 65 and 106, 143; eight of 200 27, 24 and 51, 46; a hundred of
         // 50 41, 46 and 78, 87); at head dim 64 tiles split over many keys, too
-        // (one head of 7000 tokens 71, 117 with 16, causal; 98, 159 not).
+        // (one head of 7000 tokens 63, 117 with 16, causal; 94, 159 not).
         if (half)
             (n_q / 256 + b) * h >= 2 * cus && n_q >= 2048 * b ? cut(kWide, 256) : cut(kFour, 128 >> share);
         else
@@ -1332,9 +1332,10 @@ extern "C" hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const 
     else
         rc = d == 64 ? go(packed_few_f32_kernel<64, true>) : go(packed_few_f32_kernel<128, true>);
     if (rc) return rc;
-    // many pieces to a query: a workgroup each
-    const bool share = plan.items >= 16 * plan.tiles;
-    const int64_t rows = share ? plan.pitch : ceil_div(plan.pitch, int64_t{kThreads / (d / 4)});
+    // few queries: a workgroup each (7000 of one head of 64: 19 us so, 11 by 16)
+    const int64_t together = kThreads / (d / 4);
+    const bool share = plan.tiles * h * plan.pitch < together * num_cus();
+    const int64_t rows = share ? plan.pitch : ceil_div(plan.pitch, together);
     const auto join = [&](auto kernel) {
         kernel<<<dim3(static_cast<uint32_t>(plan.tiles * h * rows)), dim3(kThreads), 0, st>>>(a, plan.bm);
         return check_launch(op);
