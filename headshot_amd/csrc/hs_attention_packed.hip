@@ -1239,12 +1239,19 @@ struct PackedPlan {
         else
             ((n_q / 32 + b) * h >= 4 * cus || (d == 64 && long_keys)) && n_q >= 128 * b ? cut(kTile, kBM) : cut(kFew, 16);
         pieces = items = pitch = 0;
-        // Keys are split where the tiles fill less than half of the chip: into as
-        // many pieces as it holds at once, or twice that where a tile would have
-        // but two or three (1374 tokens over 30000, 16 heads of 64, f32: 1082 us,
-        // 1204). The causal mask empties up to half of the items, beyond those.
+        // Keys are split where the tiles fill less than half of the chip, or less
+        // than all of it under a causal mask, whose last tile would hold the call
+        // up: in f32, and in f16 where sequences are long enough for the pieces'
+        // traffic (us split and whole; f32, 16 heads of 64, 3000 tokens 162, 195,
+        // 8 of 128 over 2, 6000 794, 1011; f16, 5 heads of 64, 7000 and 5000
+        // tokens 95, 108, 8 of 128 over 2, 6000 134, 146, but 16 over 4, 3000 86,
+        // 76). Into as many pieces as the chip holds at once, or twice that where
+        // a tile would have but two or three (1374 tokens over 30000, 16 heads of
+        // 64, f32: 1082 us, 1204). The causal mask empties up to half of the
+        // items, beyond those.
         const int64_t slots = cus * (kernel == kFew || (half && d == 64) ? 3 : 2);
-        if (kernel == kWide || 2 * tiles * all > slots || !long_keys) return;
+        const bool uneven = causal && (!half || n_k >= 5120 * b);
+        if (kernel == kWide || (uneven ? 1 : 2) * tiles * all > slots || !long_keys) return;
         pieces = (4 * tiles * all > slots && kernel != kFew ? 2 : 1) * slots / all - tiles;
         if (pieces < 1) pieces = 1;
         items = (causal ? 2 : 1) * pieces + tiles;
