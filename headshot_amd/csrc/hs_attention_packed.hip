@@ -146,7 +146,7 @@ __device__ __forceinline__ bool find_cut(const PackedArgs& a, int bm, int index,
             // in another order from tile to tile: the last pieces, which an early
             // tile's queries do not see, are not one XCD's
             t.piece = BY_TILE ? 0 : (index - t.item + t.local) % t.pieces;
-            return true;
+            return t.item + t.pieces <= a.items;  // more than that: offsets that do not ascend
         }
         tiles_before += lane_value(tile_sum, 63), items_before += lane_value(item_sum, 63);
     }
@@ -1170,8 +1170,7 @@ __global__ __launch_bounds__(kThreads) void packed_join_kernel(PackedArgs a, int
     const int nq = c.q.end - c.q.begin, nk = c.k.end - c.k.begin;
     const int first = (c.tiles - 1 - c.local) * bm, rows = min(bm, nq - first);
     const int count = pieces_seen(keys_seen(first + rows - 1, nq, nk, a.causal), c.chunk);
-    if (count == 1) return;                // written by its only piece
-    if (c.item + count > a.items) return;  // offsets that do not ascend
+    if (count == 1) return;  // written by its only piece
     const int row0 = static_cast<int>(blockIdx.x) - tile_head * per_tile;
     const int row = SHARE ? row0 : row0 * kRows + group;
     float top = kFloor, weight = 0.0f;

@@ -420,9 +420,9 @@ hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q
  * are f32; in f16 the weights of the product with V are rounded to f16, relative
  * to the largest. Few queries over many keys are split over the keys and joined,
  * by the counts given and all lengths of the call; such calls take
- * hs_attention_packed_workspace bytes (16-byte aligned, else NULL), which hold
- * nothing between calls: calls that may run at the same time need their own. out
- * overlaps nothing else. */
+ * hs_attention_packed_workspace bytes (16-byte aligned; NULL serves the others),
+ * which hold nothing between calls: calls that may run at the same time need
+ * their own. out overlaps nothing else. */
 hs_status hs_attention_packed(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                               const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                               const void* q_offsets, const void* k_offsets, void* out,

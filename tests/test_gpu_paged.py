@@ -541,6 +541,50 @@ def test_two_streams(ctx):
         assert all(torch.equal(x, side[4]) for x in got[i])
 
 
+@pytest.mark.parametrize("n,m", [(300, 300), (40, 4000), (400, 2500)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_packed_bad_offsets(ctx, dtype, n, m):
+    """Offsets that do not ascend or leave the rows: no write outside the
+    buffers, whole keys and split ones."""
+    gen = torch.Generator().manual_seed(16)
+    q, k, v = (normal(gen, (rows, h, 64), dtype).to(DEV) for rows, h in ((n, 2), (m, 1), (m, 1)))
+    size = ctx.attention_packed_workspace(dtype, n, m, 4, 2, 1, 64, 1)
+    assert (size > 0) == (m >= 1536)
+    guard = 1 << 16
+    ws = torch.full((size + 2 * guard,), 0xA5, dtype=torch.uint8, device=DEV)
+    out = torch.full((n + 64, 128), 7.0, dtype=dtype, device=DEV)
+    big = 2 ** 31 - 1
+    for off, koff in [([0, n, 0, n, 0], [0, m, 0, m, 0]), ([-5, 3, big, 2, n], [big, -big, m, 1, m + 9]),
+                      ([0, 5, 9, 20, n], [m, m // 2, m, 0, m]), ([n, n, 3, n, n], [0, 5, m, 5, m]),
+                      ([0, n // 2, 0, n // 3, n], [0, m, 1, m, 2])]:
+        for causal in (0, 1):
+            print(f"[bad offsets {dtype} {off} {koff} causal={causal}]", flush=True)
+            ctx.attention_packed(q, k, v, i32(off), i32(koff), causal=causal, out=out[32:32 + n],
+                                 workspace=ws[guard:guard + size] if size else None)
+    assert (ws[:guard] == 0xA5).all() and (ws[guard + size:] == 0xA5).all()
+    assert (out[:32] == 7).all() and (out[32 + n:] == 7).all()
+
+
+def test_two_streams_split(ctx):
+    """Split packed calls on two streams at once, of their own workspaces."""
+    gen = torch.Generator().manual_seed(15)
+    sides = []
+    for i in range(2):
+        q, k, v = (normal(gen, (n, h, 64), F16).to(DEV) for n, h in ((20 + i, 4), (3000, 2), (3000, 2)))
+        call = (q, k, v, i32([0, 20 + i]), i32([0, 3000]))
+        assert split(ctx, F16, 64, 4, 2, [20 + i], [3000], 1)
+        sides.append((torch.cuda.Stream(), call, ctx.attention_packed(*call)))
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for i, (stream, call, _alone) in enumerate(sides):
+            with torch.cuda.stream(stream):
+                got[i].append(ctx.attention_packed(*call))
+    torch.cuda.synchronize()
+    for i, side in enumerate(sides):
+        assert all(torch.equal(x, side[2]) for x in got[i])
+
+
 # -------------------------------------------------------------- attention_paged
 
 
