@@ -1228,15 +1228,22 @@ struct PackedPlan {
         // 6000 182, 195, eight of 1374, causal, 58, 66; 32 heads of 128 over 8:
         // 12000 2486, 2236, 4122 362, 345, 2748 160, 171, twenty of 300 68, 81).
         // f32: tiles of 32 queries a wave where they fill the chip's SIMDs and
-        // themselves, else 16 by four waves (us with these and with tiles, 16
-        // heads of 64 and of 128: one sequence of 200 tokens 10, 21 and 13, 42; of
-        // 1000 49, 65 and 106, 143; eight of 200 27, 24 and 51, 46; a hundred of
-        // 50 41, 46 and 78, 87); at head dim 64 tiles split over many keys, too
-        // (one head of 7000 tokens 63, 117 with 16, causal; 94, 159 not).
-        if (half)
+        // themselves, else 16 by four waves, which at head dim 128, on the same
+        // instructions, are but a third behind (us with 16 and with tiles; 16
+        // heads of 64: one sequence of 1000 tokens 49, 65, eight of 200 27, 24, a
+        // hundred of 50 41, 46; 32 heads of 128, causal: one of 1283 168, 199, of
+        // 2000 381, 356, twenty of 300 255, 286); tiles, too, that split many keys
+        // (one head of 7000 causal tokens: of 64 117, 63, of 128 288, 142; 16 of
+        // 128, 1100 over 5000 551, 471; but 4 of 128, 2000 causal tokens 75, 85).
+        if (half) {
             (n_q / 256 + b) * h >= 2 * cus && n_q >= 2048 * b ? cut(kWide, 256) : cut(kFour, 128 >> share);
-        else
-            ((n_q / 32 + b) * h >= 4 * cus || (d == 64 && long_keys)) && n_q >= 128 * b ? cut(kTile, kBM) : cut(kFew, 16);
+        } else {
+            const int64_t blocks = (n_q / 32 + b) * h;
+            const bool tiled = d == 64 ? (blocks >= 4 * cus || long_keys) && n_q >= 128 * b
+                                       : (blocks >= 7 * cus && n_q >= 640 * b) ||
+                                             (long_keys && n_q >= 256 * b && (!causal || n_k >= 4096 * b));
+            tiled ? cut(kTile, kBM) : cut(kFew, 16);
+        }
         pieces = items = pitch = 0;
         // Keys are split where the tiles fill less than half of the chip, or less
         // than all of it under a causal mask, whose last tile would hold the call

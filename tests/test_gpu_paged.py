@@ -265,6 +265,7 @@ def test_packed_split_keys(ctx, dtype, d, causal):
         (2, 2, [1, 1, 1, 1], [0, 2100, 64, 65]),
         (2, 1, [200, 130], [3001, 1500]),
         (1, 1, [2200], [2200]),
+        (1, 1, [300], [4200]),
     ]):
         print(f"[packed split {dtype} d={d} causal={causal} case {i}]", flush=True)
         assert split(ctx, dtype, d, h, h_kv, nq, nk, causal)
@@ -416,16 +417,16 @@ def gpu_reference(q, k, v, seen, scale):
 
 
 @pytest.mark.parametrize("what", ["plain", "inf", "nan", "huge", "huge q", "tiny"])
-@pytest.mark.parametrize("d", [64, 128])
-def test_packed_f32_tiles(ctx, d, what):
+@pytest.mark.parametrize("d,h,h_kv", [(64, 16, 8), (128, 16, 8), (128, 32, 4)])
+def test_packed_f32_tiles(ctx, d, h, h_kv, what):
     """f32 over enough queries for the tiles of 32 a wave, with values that the
     three bf16 parts do not hold among them."""
-    lens, h, h_kv = [1301, 900, 130], 16, 8
+    lens = [1301, 900, 130]
     gen = torch.Generator().manual_seed(d)
     q, k, v = (normal(gen, (sum(lens), x, d), F32) for x in (h, h_kv, h_kv))
     if what in ("inf", "nan"):
         x = math.inf if what == "inf" else math.nan
-        v[700, 3, 7], v[1310, :, 1], v[2331 - 40, 5] = x, -x, x
+        v[700, 3, 7], v[1310, :, 1], v[2331 - 40, min(5, h_kv - 1)] = x, -x, x
     elif what == "huge":
         v[700] *= 2.0 ** 60
         k[1500, 2] *= 2.0 ** 55
