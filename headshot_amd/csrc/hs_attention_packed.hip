@@ -1253,12 +1253,16 @@ struct PackedPlan {
         // tokens 95, 108, 8 of 128 over 2, 6000 134, 146, but 16 over 4, 3000 86,
         // 76). Into as many pieces as the chip holds at once, or twice that where
         // a tile would have but two or three (1374 tokens over 30000, 16 heads of
-        // 64, f32: 1082 us, 1204). The causal mask empties up to half of the
-        // items, beyond those.
+        // 64, f32: 1082 us, 1204), and those only of many keys (4 heads of 128
+        // over 2, f16, five sequences of 4395 keys 46, 68; 16 of 64, one of 1600,
+        // not causal, 38, 29) or in the tiles of f32 (16 of 64, 1600, 85, 101).
+        // The causal mask empties up to half of the items, beyond those.
         const int64_t slots = cus * (kernel == kFew || (half && d == 64) ? 3 : 2);
         const bool uneven = causal && (!half || n_k >= 5120 * b);
+        const bool coarse = 4 * tiles * all > slots;
         if (kernel == kWide || (uneven ? 1 : 2) * tiles * all > slots || !long_keys) return;
-        pieces = (4 * tiles * all > slots && kernel != kFew ? 2 : 1) * slots / all - tiles;
+        if (coarse && kernel != kTile && n_k < 4096) return;
+        pieces = (coarse && kernel != kFew ? 2 : 1) * slots / all - tiles;
         if (pieces < 1) pieces = 1;
         items = (causal ? 2 : 1) * pieces + tiles;
         pitch = n_q < bm ? n_q : bm;
