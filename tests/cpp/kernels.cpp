@@ -498,6 +498,32 @@ void layernorm_prologue_equals_sequence(HipContext& ctx) {
     }
 }
 
+// One token over many keys, whose packed attention splits them, is the paged one.
+void packed_token_over_many_keys(HipContext& ctx) {
+    const size_t h = 4, h_kv = 2, d = 64, page = 64, n = 3000, pages = 47;
+    std::vector<int32_t> ints(pages);
+    for (size_t i = 0; i < pages; i++) ints[i] = static_cast<int32_t>((i * 5 + 3) % pages);
+    ints.insert(ints.end(), {0, 1, 0, static_cast<int32_t>(n)});  // query offsets, key offsets; lens at the end
+    int32_t* dev = nullptr;
+    hs::hip_check(hipMalloc(&dev, ints.size() * sizeof(int32_t)), "hipMalloc");
+    hs::hip_check(hipMemcpy(dev, ints.data(), ints.size() * sizeof(int32_t), hipMemcpyHostToDevice), "hipMemcpy");
+    Rng rng{78};
+    for (Dtype dt : {Dtype::F32, Dtype::F16}) {
+        const auto q = ctx.tensor_from_f32({1, h * d}, rng.vec(h * d), dt);
+        const auto k = ctx.tensor_from_f32({n, h_kv * d}, rng.vec(n * h_kv * d), dt);
+        const auto v = ctx.tensor_from_f32({n, h_kv * d}, rng.vec(n * h_kv * d), dt);
+        hs::PagedKV cache{ctx.empty_typed({pages, h_kv, page, d}, dt), ctx.empty_typed({pages, h_kv, page, d}, dt), dev,
+                          dev + pages + 3, 1, pages};
+        ctx.kv_append(cache, nullptr, k, v, dev + pages + 2);
+        const auto want = ctx.download(ctx.attention_paged(q, cache));
+        const auto got = ctx.download(ctx.attention_packed(q, k, v, d, dev + pages, 1, dev + pages + 2));
+        for (size_t c = 0; c < h * d; c++)
+            // both are off by at most their type's roundings (values below 4)
+            if (!(std::fabs(got[c] - want[c]) <= (dt == Dtype::F32 ? 1e-5f : 1.6e-2f))) throw Failure("packed token differs from the paged one");
+    }
+    hs::hip_check(hipFree(dev), "hipFree");
+}
+
 // A prompt of two sequences and a step of both: the pages hold what was
 // appended, and a step's attention is the packed attention's next row.
 void paged_step_continues_a_prompt(HipContext& ctx) {
@@ -581,6 +607,7 @@ int main(int argc, char** argv) {
         {"qknorm_rope_pair_equals_two_calls", qknorm_rope_pair_equals_two_calls},
         {"layernorm_prologue_equals_sequence", layernorm_prologue_equals_sequence},
         {"paged_step_continues_a_prompt", paged_step_continues_a_prompt},
+        {"packed_token_over_many_keys", packed_token_over_many_keys},
         {"contract_violations_throw", contract_violations_throw},
     };
     HipContext ctx;
