@@ -421,10 +421,10 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
             u32x4 p[2][2];
             // The tile's weights against a reference, rounded to f16 (2^-11 of
             // each, inside the result's own rounding), and the sum of the
-            // rounded ones over the lane's keys: two packed f16 levels (sums
-            // of four), then f32.
+            // rounded ones over the lane's keys, in f32 like the product's.
             auto weights = [&](float mul, float ref) {
-                f16x2 w2[16];
+                const f16x2 one = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -432,17 +432,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
                         const uint32_t w = pk_f16(__builtin_amdgcn_exp2f(fmaf(s[i][r], mul, -ref)),
                                                   __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], mul, -ref)));
                         p[i][r / 8][r % 8 / 2] = w;
-                        w2[8 * i + r / 2] = u2h2(w);
+                        sum[r / 2 % 4] = __builtin_amdgcn_fdot2(u2h2(w), one, sum[r / 2 % 4], false);
                     }
-#pragma unroll
-                for (int i = 0; i < 8; i++) w2[i] = w2[i] + w2[i + 8];
-#pragma unroll
-                for (int i = 0; i < 4; i++) w2[i] = w2[i] + w2[i + 4];
-                const f16x2 one = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_fdot2(w2[i], one, sum, false);
-                return sum;
+                return (sum[0] + sum[1]) + (sum[2] + sum[3]);
             };
             // Past the first tile the weights are taken against the reference
             // as it is; only a query whose sum says that one may not fit f16
