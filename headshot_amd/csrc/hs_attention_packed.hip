@@ -282,16 +282,26 @@ struct FlashF16 {
     };
 };
 
-// A weight's exponent may run this far (log2) above the reference maximum
-// before the reference moves.
-constexpr float kLazyMax = 8.0f;
-// A running maximum before any score. It is finite, so that a masked score
+// A query's reference is set this far (log2) below its largest score, so that its
+// largest weight is 2^12: weights keep f16's 11 bits down to 2^-26 of the largest,
+// and below, where f16 is subnormal, are at most 2^-37 of it off. (With a largest
+// weight of 1 a key 17 nats above the others, of value 0, left them up to 45%
+// off.) A weight may then grow 16 times past the largest before it passes f16 and
+// the reference moves, which scores that spread wide do more often (16 heads of
+// 64, 10992 tokens by frames, scores of standard deviation 1 and 3 nats: 213 and
+// 227 us, 207 and 209 with 1; with 2^13 2% more at 1, with 2^14 12%).
+constexpr float kWeightBits = 12.0f;
+constexpr float kPastF16 = 65520.0f;  // the least that f16 rounds to infinity
+// Tiles for which a wave looks for the scores' maximum ahead of the weights once
+// references have moved: weights that do not fit are computed twice, which is
+// some 190 instructions against 20 (3 nats: 227 us, 249 without; 4 and 16 tiles
+// within 1%). A query's result is the same either way.
+constexpr int kWary = 8;
+// A reference before any score. It is finite, so that a masked score
 // weighs exp2(-inf - kFloor) = 0 against it.
 constexpr float kFloor = -3.0e38f;
 // A maximum (log2) beyond which its rounding, 2^-24 of it, shows in a weight.
 constexpr float kFar = 65536.0f;
-// A lane's row sum over a tile beyond which a weight may not fit f16.
-constexpr float kRowSumMax = 32768.0f;
 
 template <int D, int W, int SUB, bool SPLIT>
 __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed_f16_kernel(PackedArgs a) {
@@ -338,6 +348,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
 #pragma unroll
     for (int i = 0; i < DB; i++) o[i] = f32x16{};
     float m = kFloor, l = 0.0f;
+    int wary = 0;  // tiles to go
 
     // Staging: load i of the thread is row row0 + kRowStep i, piece `piece`. The
     // tile's address is the scalar part of the load's, the thread's the other.
@@ -419,9 +430,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
                         if (key0 + 32 * i + 8 * (r / 4) + 4 * hh + r % 4 >= seen) s[i][r] = -INFINITY;
             }
             u32x4 p[2][2];
-            // The tile's weights against a reference, rounded to f16 (2^-11 of
-            // each, inside the result's own rounding), and the sum of the
-            // rounded ones over the lane's keys, in f32 like the product's.
+            // The tile's weights against a reference, rounded to f16 (see
+            // kWeightBits), and the sum of the rounded ones over the lane's
+            // keys, in f32 like the product's.
             auto weights = [&](float mul, float ref) {
                 const f16x2 one = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -437,12 +448,13 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
                 return (sum[0] + sum[1]) + (sum[2] + sum[3]);
             };
             // Past the first tile the weights are taken against the reference
-            // as it is; only a query whose sum says that one may not fit f16
-            // moves its own.
-            bool own = key0 == (SPLIT ? t.begin : 0) || fabsf(m) > kFar, move = __any(own);
+            // as it is; only a query of which one does not fit f16, so that its
+            // sum is infinite, moves its own. Where the wave's references have
+            // moved lately, the scores' maximum says so ahead of the weights.
+            bool own = key0 == (SPLIT ? t.begin : 0) || fabsf(m) > kFar, move = wary > 0 || __any(own);
             if (!move) {
                 const float sum = weights(c, m);
-                own = !(halves_max(sum) <= kRowSumMax) || !(sum <= kRowSumMax);
+                own = !(halves_sum(sum) < INFINITY);
                 move = __any(own);
                 if (!move) l += sum;
             }
@@ -452,9 +464,17 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
                 for (int i = 0; i < 2; i++)
 #pragma unroll
                     for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[i][r]);
-                const float cand = fmaxf(m, halves_max(mx) * c);
-                const float next = own && cand > m + kLazyMax ? cand : m;
-                const float corr = __builtin_amdgcn_exp2f(m - next);
+                mx = halves_max(mx);
+                own |= __builtin_amdgcn_exp2f(fmaf(mx, c, -m)) >= kPastF16;
+                const float next = own ? fmaxf(m, mx * c - kWeightBits) : m;
+                float corr = 1.0f;
+                wary--;
+                if (__any(next != m)) {
+                    corr = __builtin_amdgcn_exp2f(m - next);
+                    wary = kWary;
+#pragma unroll
+                    for (int i = 0; i < DB; i++) o[i] *= corr;
+                }
                 // The multiply-add leaves the rounding of s c in the exponent:
                 // where that is not small, the product is rounded first, as
                 // the reference's was.
@@ -467,8 +487,6 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
                 }
                 l = fmaf(l, corr, weights(far ? 1.0f : c, far ? 0.0f : next));
                 m = next;
-#pragma unroll
-                for (int i = 0; i < DB; i++) o[i] *= corr;
             }
             // O^T += V^T P^T. The transposing read gives lane i of 16 channel
             // i of 4 keys: two reads make the 8 keys, in the scores' order.
@@ -700,6 +718,10 @@ typedef bf16x8 b8;
 constexpr int kSD = 64, kSKPitch = kSD + 8, kSVPitch = kSD + 32;
 constexpr uint32_t kSplitMaxBits = 0x58800000u;  // 2^50
 constexpr float kSplitScale = 0x1p23f;
+// The reference moves where a lane's row sum over a tile passes this, to a
+// maximum this far (log2) above it.
+constexpr float kRowSumMax = 32768.0f;
+constexpr float kLazyMax = 8.0f;
 
 struct SplitSmem {
     uint16_t k[3][kBN * kSKPitch];
@@ -880,8 +902,8 @@ __global__ __launch_bounds__(kThreads, 2) void packed_split_kernel(PackedArgs a)
                 }
             return ps[0] + ps[1];
         };
-        // as in f16: the reference moves on the first tile and where a weight
-        // might pass 2^15 times the largest at it, for the query's own sums only
+        // the reference moves on the first tile and where a weight might pass
+        // 2^15 times the largest at it, for the query's own sums only
         bool own = key0 == begin, move = own;
         if (!move) {
             const float ps = weights(m);

@@ -54,3 +54,81 @@ def test_packed_constant_values(ctx, d, h, h_kv, nq, nk):
                                        scale=scale)
             got = got[(R.seen_keys(nq, nk, causal) > 0).to(DEV)].float()
             assert (got == 1).all(), f"scale {scale}, causal {causal}: {(got - 1).abs().max()} off"
+
+
+# ---------------------------------------------------- one key with all the weight
+
+
+def sink(d, nq, nk, h, h_kv, at, above, seed):
+    """f16 rows of which key ``at`` scores ``above`` more than the others, whose
+    scores lie within 1/4 of each other; its value is 0, theirs 500 to 1500.
+    (Channel 0 makes that score: the queries' is 4, the key's above sqrt(d) / 4.)"""
+    gen = torch.Generator().manual_seed(seed)
+    q = torch.randn(nq, h, d, generator=gen).clamp(-2, 2) * 0.1
+    k = torch.randn(nk, h_kv, d, generator=gen).clamp(-2, 2) * 0.1
+    v = torch.rand(nk, h_kv, d, generator=gen) * 1000 + 500
+    q[..., 0], k[..., 0] = 4, 0
+    k[at], v[at] = 0, 0
+    k[at, :, 0] = above * math.sqrt(d) / 4
+    return q.half(), k.half(), v.half()
+
+
+def sink_bound(q, k, ref, nk, scale, lost):
+    """No value is negative, so a weight's relative error is the result's, twice
+    (numerator and denominator). Of a weight: the score's (a sum of d products
+    and a multiplication, each partial sum within the largest sum |q k|, and the
+    exponential's four roundings; see attention_bound) and the rounding for the
+    product, 2^-11. The row's sums add n 2^-24 each, and the result is rounded.
+    Below 2^-14 a weight's rounding is no longer relative: 2^-25 of the unit, of
+    which the largest weight is 2^lost at least."""
+    d, group = q.shape[2], q.shape[1] // k.shape[1]
+    size = ((q.double().abs().permute(1, 0, 2) @ k.double().abs().repeat_interleave(group, 1).permute(1, 2, 0)).amax()
+            * scale).item()
+    weight = 2 * (d + 4) * R.U32 * size + (2 * size + 4) * R.U32
+    relative = 2 * weight + 2 * R.HALF[F16] + 2 * nk * R.U32 + R.HALF[F16]
+    return relative * ref.abs() + nk * 2.0 ** -(25 + lost) * 1500 + R.TINY[F16]
+
+
+def sink_reference(q, k, v, seen, scale):
+    """In f64 on the GPU, head by head."""
+    group = q.shape[1] // k.shape[1]
+    q, k, v = (t.to(DEV).double() for t in (q, k, v))
+    out = torch.zeros_like(q)
+    hidden = torch.arange(k.shape[0], device=DEV) >= seen.to(DEV)[:, None]
+    for i in range(q.shape[1]):
+        s = (q[:, i] @ k[:, i // group].T.contiguous() * scale).masked_fill(hidden, -math.inf)
+        out[:, i] = torch.softmax(s, -1) @ v[:, i // group]
+    return out.cpu()
+
+
+# The largest weight: 2^12 in attention_packed, unless a later score raised it.
+@pytest.mark.parametrize("above", [14, 16, 17, 18])
+@pytest.mark.parametrize("d,h,h_kv,nq,nk", [
+    (64, 2, 1, 100, 300), (128, 2, 2, 70, 1100), (128, 4, 1, 5, 700), (64, 1, 1, 1900, 1900), (64, 2, 1, 9, 3000),
+    (64, 64, 8, 2048, 2048), (128, 64, 8, 2048, 2048),
+])
+def test_packed_sink(ctx, d, h, h_kv, nq, nk, above):
+    for at in (0, 63, nk // 2, nk - 1):
+        q, k, v = sink(d, nq, nk, h, h_kv, at, above, d + nk + at)
+        got = ctx.attention_packed(*(t.to(DEV) for t in (q, k, v)), i32([0, nq]), i32([0, nk]), causal=0)
+        ref = sink_reference(q, k, v, torch.full((nq,), nk), 1 / math.sqrt(d))
+        R.assert_within(got.unflatten(1, (h, d)), ref, sink_bound(q, k, ref, nk, 1 / math.sqrt(d), 12),
+                        f"key {at}, {above} above")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_rows_apart(ctx, d):
+    """A row is the same beside rows whose scores rise by steps along the keys,
+    so that their wave's references move, and beside even ones."""
+    gen = torch.Generator().manual_seed(d)
+    q, k, v = (torch.randn(n, 2, d, generator=gen).half() for n in (90, 900, 900))
+    k[..., 0] = (torch.arange(900) // 50)[:, None].half()  # what the first channel of a query adds
+    q[..., 0] = 0
+    args = i32([0, 90]), i32([0, 900])
+    even = ctx.attention_packed(*(t.to(DEV) for t in (q, k, v)), *args, causal=0)
+    for at in (0, 40, 63):
+        steep = q.clone()
+        steep[at, :, 0] = 4 * math.sqrt(d)
+        got = ctx.attention_packed(*(t.to(DEV) for t in (steep, k, v)), *args, causal=0)
+        rest = torch.arange(90) != at
+        assert torch.equal(got[rest.to(DEV)], even[rest.to(DEV)]) and not torch.equal(got[at], even[at])
