@@ -507,23 +507,25 @@ __global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_p
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 sc[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - m);
-                sum += sc[i][j];
+                if constexpr (!P::kHalf) sum += sc[i][j];
             }
-        l = fmaf(l, corr, sum);
-#pragma unroll
-        for (int i = 0; i < DB; i++) o[i] *= corr;
-        // O^T += V^T P^T
+        u32x4 p;  // f16: the weights, rounded (2^-11 of each) for their product and their sum alike
         if constexpr (P::kHalf) {
-            // the weights rounded to f16 (2^-11 of each)
-            u32x4 p;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j += 2) {
                     f16x2 w;
                     w.x = static_cast<f16>(sc[i][j]), w.y = static_cast<f16>(sc[i][j + 1]);
+                    sum = __builtin_amdgcn_fdot2(w, f16x2{static_cast<f16>(1.0f), static_cast<f16>(1.0f)}, sum, false);
                     p[2 * i + j / 2] = h22u(w);
                 }
+        }
+        l = fmaf(l, corr, sum);
+#pragma unroll
+        for (int i = 0; i < DB; i++) o[i] *= corr;
+        // O^T += V^T P^T
+        if constexpr (P::kHalf) {
             const T* va = vs + (4 * g + n / 4) * P::kPitch + 4 * (n % 4);
 #pragma unroll
             for (int i = 0; i < DB; i++) {

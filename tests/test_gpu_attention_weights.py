@@ -25,7 +25,7 @@ def i32(values):
 # (keys that score 0, the others -1; scale). Weights of one, and others of which
 # f16 makes something else: 1 + e^-7.42 = 1 + 0.61 x 2^-10, which rounds up to 1 +
 # 2^-10, and e^-0.69268 = 1/2 + 0.95 x 2^-12, which rounds down to 1/2.
-PATTERNS = [(lambda j: j % 64 < 32, 7.42), (lambda j: j == 0, 0.69268)]
+PATTERNS = [(lambda j: j % 64 < 32, 7.42), (lambda j: j % 16 == 0, 0.69268)]
 
 
 def two_levels(pattern, d, nq, nk, h, h_kv):
@@ -132,3 +132,27 @@ def test_packed_rows_apart(ctx, d):
         got = ctx.attention_packed(*(t.to(DEV) for t in (steep, k, v)), *args, causal=0)
         rest = torch.arange(90) != at
         assert torch.equal(got[rest.to(DEV)], even[rest.to(DEV)]) and not torch.equal(got[at], even[at])
+
+
+# --------------------------------------------------------- the same over the pages
+
+
+def pages_of(k, v, page=16):
+    """A cache of one sequence: its pages, the last filled up with zeros."""
+    n, h_kv, d = k.shape
+    count = -(-n // page)
+    rows = torch.zeros(2, count * page, h_kv, d, dtype=k.dtype)
+    rows[0, :n], rows[1, :n] = k, v
+    rows = rows.unflatten(1, (count, page)).transpose(2, 3).contiguous().to(DEV)
+    return PagedKV(rows[0], rows[1], i32([list(range(count))]), i32([n]))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,h_kv,nk", [(1, 1, 100), (8, 2, 1000), (20, 1, 333), (4, 4, 2000)])
+def test_paged_constant_values(ctx, d, h, h_kv, nk):
+    """As test_packed_constant_values."""
+    for page in (4, 16):
+        for pattern, scale in PATTERNS:
+            q, k, v = two_levels(pattern, d, 1, nk, h, h_kv)
+            got = ctx.attention_paged(q.to(DEV), pages_of(k, v, page), scale=scale).float()
+            assert (got == 1).all(), f"page {page}, scale {scale}: {(got - 1).abs().max()} off"
