@@ -1,6 +1,7 @@
 // A paged key-value cache for gfx950: appending new tokens (with QK-norm and
 // the position rotation) and the attention of one new token per sequence.
 #include <cmath>
+#include <type_traits>
 
 #include "hs_packed.hpp"
 
@@ -219,6 +220,7 @@ void launch_append(hipStream_t st, const AppendArgs<T>& a) {
 typedef f16 h8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 
 __device__ __forceinline__ h8 as_h8(u32x4 v) { return __builtin_bit_cast(h8, v); }
@@ -229,6 +231,15 @@ constexpr int kMostPerCu = 4;  // workgroups of any of the kernels
 constexpr int kPagedWaves = 4;
 constexpr float kNone = -3.0e38f;   // a running maximum that has seen no key
 constexpr float kFloor = -2.9e38f;  // the least of one that has
+// f16: a weight goes to the product with V as two f16 values, its 11 leading bits
+// and the next 11, which makes the product as good as one of f32 weights (errors
+// against 64 bits 2.5e-4 with the leading bits alone, 2.0e-4 so, which is the
+// result's rounding) for 1-2% of the time. The largest weight of a step is this
+// unit, so that the others, f16 being subnormal below 2^-14, are 2^-40 of it off at
+// most (of a unit of 1, 45% at a score 17 nats below). The second part times an
+// infinity is NaN or the other infinity: a step that has one among its values
+// leaves the second parts out.
+constexpr float kHalfUnit = 32768.0f;
 
 template <typename T, int D>
 struct Paged {
@@ -437,6 +448,16 @@ __global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_p
                 if (WHOLE ? key0 + row >= v_end[P::kVRows * i / 16] : !(v_ok >> i & 1)) vr[i] = u32x4{};
             }
         }
+        bool odd = false;  // f16: an infinity or NaN among the values
+        if constexpr (P::kHalf) {
+            u16x2 most = {0, 0};
+#pragma unroll
+            for (int i = 0; i < P::kVLoads; i++)
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, vr[i][e] & 0x7FFF7FFFu));
+            odd = __any(most.x >= 0x7C00 || most.y >= 0x7C00);
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
         for (int i = 0; i < P::kVLoads; i++)
@@ -507,34 +528,39 @@ __global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_p
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 sc[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - m);
-                if constexpr (!P::kHalf) sum += sc[i][j];
+                if constexpr (P::kHalf) sc[i][j] *= kHalfUnit;
+                sum += sc[i][j];
             }
-        u32x4 p;  // f16: the weights, rounded (2^-11 of each) for their product and their sum alike
-        if constexpr (P::kHalf) {
-#pragma unroll
-            for (int i = 0; i < 2; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {
-                    f16x2 w;
-                    w.x = static_cast<f16>(sc[i][j]), w.y = static_cast<f16>(sc[i][j + 1]);
-                    sum = __builtin_amdgcn_fdot2(w, f16x2{static_cast<f16>(1.0f), static_cast<f16>(1.0f)}, sum, false);
-                    p[2 * i + j / 2] = h22u(w);
-                }
-        }
         l = fmaf(l, corr, sum);
 #pragma unroll
         for (int i = 0; i < DB; i++) o[i] *= corr;
         // O^T += V^T P^T
         if constexpr (P::kHalf) {
-            const T* va = vs + (4 * g + n / 4) * P::kPitch + 4 * (n % 4);
+            u32x4 p, rest;
 #pragma unroll
-            for (int i = 0; i < DB; i++) {
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    f16x2 w, r;
+                    w.x = static_cast<f16>(sc[i][j]), w.y = static_cast<f16>(sc[i][j + 1]);
+                    r.x = static_cast<f16>(sc[i][j] - static_cast<float>(w.x));
+                    r.y = static_cast<f16>(sc[i][j + 1] - static_cast<float>(w.y));
+                    p[2 * i + j / 2] = h22u(w), rest[2 * i + j / 2] = h22u(r);
+                }
+            const T* va = vs + (4 * g + n / 4) * P::kPitch + 4 * (n % 4);
+            auto read_v = [&](int i) {
                 const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + 16 * i)));
                 const u32x2 hi =
                     __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + 16 * P::kPitch + 16 * i)));
                 u32x4 w;
                 w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), as_h8(p), o[i], 0, 0, 0);
+                return as_h8(w);
+            };
+#pragma unroll
+            for (int i = 0; i < DB; i++) {
+                const h8 w = read_v(i);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, as_h8(p), o[i], 0, 0, 0);
+                if (!odd) o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(w, as_h8(rest), o[i], 0, 0, 0);
             }
         } else {
 #pragma unroll

@@ -441,13 +441,15 @@ int64_t hs_attention_paged_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t
 
 /* Attention of one new token per sequence over its paged keys: q (b, Hq*D),
  * rows q_stride apart -> out (b, Hq*D): out[s] = softmax(scale q[s] K_s^T) V_s
- * over the lens[s] keys of sequence s, zeros where there are none. Long
- * sequences are split over their keys and joined; the split, and with it the
- * order of the sums, follows all lengths of the call. workspace (16-byte
- * aligned, hs_attention_paged_workspace bytes) holds nothing between calls:
- * calls that may run at the same time need one each. Nothing is read on the
- * host, so a captured call follows lens and page_table. out overlaps
- * nothing else. */
+ * over the lens[s] keys of sequence s, zeros where there are none. Softmax
+ * statistics and sums are f32; in f16 each weight is rounded to 22 bits (11 beside
+ * an infinity or NaN), or to 2^-40 of the largest if that is more; an infinity
+ * among the values whose weight that makes 0 gives NaN. Long sequences are split
+ * over their keys and joined; the split, and with it the order of the sums, follows
+ * all lengths of the call. workspace (16-byte aligned, hs_attention_paged_workspace
+ * bytes) holds nothing between calls: calls that may run at the same time need one
+ * each. Nothing is read on the host, so a captured call follows lens and
+ * page_table. out overlaps nothing else. */
 hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                              const void* k_cache, const void* v_cache, const void* page_table,
                              const void* lens, void* out, void* workspace,

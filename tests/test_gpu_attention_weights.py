@@ -150,9 +150,58 @@ def pages_of(k, v, page=16):
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("h,h_kv,nk", [(1, 1, 100), (8, 2, 1000), (20, 1, 333), (4, 4, 2000)])
 def test_paged_constant_values(ctx, d, h, h_kv, nk):
-    """As test_packed_constant_values."""
+    """As test_packed_constant_values, the weights the same to 2^-22."""
     for page in (4, 16):
         for pattern, scale in PATTERNS:
             q, k, v = two_levels(pattern, d, 1, nk, h, h_kv)
             got = ctx.attention_paged(q.to(DEV), pages_of(k, v, page), scale=scale).float()
             assert (got == 1).all(), f"page {page}, scale {scale}: {(got - 1).abs().max()} off"
+
+
+# The largest weight: 2^15 in attention_paged.
+@pytest.mark.parametrize("above", [14, 16, 17, 18])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,h_kv,nk", [(1, 1, 100), (1, 1, 32), (8, 2, 700), (20, 1, 128), (2, 2, 3000)])
+def test_paged_sink(ctx, d, h, h_kv, nk, above):
+    for at in (0, nk // 2, nk - 1):
+        q, k, v = sink(d, 1, nk, h, h_kv, at, above, d + nk + at)
+        got = ctx.attention_paged(q.to(DEV), pages_of(k, v))
+        ref = sink_reference(q, k, v, torch.full((1,), nk), 1 / math.sqrt(d))
+        R.assert_within(got.unflatten(1, (h, d)), ref, sink_bound(q, k, ref, nk, 1 / math.sqrt(d), 15),
+                        f"key {at}, {above} above")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,h_kv,nk", [(8, 8, 2), (8, 2, 20), (20, 1, 333), (4, 4, 3000)])
+def test_paged_f16_weights(ctx, d, h, h_kv, nk):
+    """f16 results are off by their own rounding and what f32 weights would be
+    off: scores as in attention_bound, small ones here; 2^-22 of a weight, twice;
+    and sums of chains of up to 128 keys a wave, its pieces and waves behind."""
+    gen = torch.Generator().manual_seed(d + nk)
+    q = (torch.randn(1, h, d, generator=gen) * 0.05).half()
+    k, v = (torch.randn(nk, h_kv, d, generator=gen).half() for _ in range(2))
+    scale = 1 / math.sqrt(d)
+    ref, mag = R.attention(q.double(), k.double(), v.double(), [nk], scale)
+    size = (q.double().abs().transpose(0, 1) @ k.double().abs().repeat_interleave(h // h_kv, 1).permute(1, 2, 0)).amax()
+    weight = 2 * (d + 4) * R.U32 * size * scale + (2 * size * scale + 4) * R.U32 + 2.0 ** -22
+    bound = (2 * weight + 2 * min(nk, 200) * R.U32) * mag + R.HALF[F16] * ref.abs() + R.TINY[F16]
+    got = ctx.attention_paged(q.to(DEV), pages_of(k, v))
+    R.assert_within(got.unflatten(1, (h, d)), ref, bound, f"{nk} keys")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_paged_infinity_beside(ctx, d):
+    """An infinity among the values is its own channel's alone, whatever bits its
+    key's weight has; the others stay within a weight's leading 11 bits."""
+    gen = torch.Generator().manual_seed(d)
+    q, k, v = (torch.randn(n, 2, d, generator=gen).half() for n in (1, 700, 700))
+    plain = v.clone()
+    for j, x in ((3, math.inf), (40, -math.inf), (699, math.inf)):
+        v[j, :, j % 7] = x
+        plain[j, :, j % 7] = 0
+    ref, mag = R.attention(q.double(), k.double(), plain.double(), [700], 1 / math.sqrt(d))
+    got = ctx.attention_paged(q.to(DEV), pages_of(k, v)).unflatten(1, (2, d)).cpu()
+    assert (got[..., 3] == math.inf).all() and (got[..., 40 % 7] == -math.inf).all() and (got[..., 699 % 7] == math.inf).all()
+    rest = [c for c in range(d) if c not in (3, 40 % 7, 699 % 7)]
+    bound = R.attention_bound(ref, mag, q, k, plain, [700], 1 / math.sqrt(d), F16)
+    R.assert_within(got[..., rest], ref[..., rest], bound[..., rest], "the other channels")
