@@ -357,14 +357,25 @@ def block_forward_reference(ctx: HipContext, wts: BlockWeights, x, s: int, t: in
 
 def block_forward_cached(ctx: HipContext, wts: BlockWeights, x, cache, heads: int = HEADS,
                          offsets=None, rope=None, positions=None, causal: int = 1,
-                         eps: float = 1e-6):
+                         eps: float = 1e-6, check: bool = True):
     """``block_forward`` for sequences that grow, over this block's ``cache``
     (``PagedKV``, its ``lens`` counting x's tokens already). With ``offsets``
     x holds whole prompts, sequence after sequence, that fill empty sequences
     and attend among themselves (``causal`` as ``attention_packed``: 1 by
     token, T by frames of T tokens); without, one new token per sequence, that
     sees every key the cache holds. ``rope`` = (sin, cos) with ``positions`` as
-    ``kv_append``, or None. Returns the block output, x's shape."""
+    ``kv_append``, or None. Returns the block output, x's shape.
+
+    A prompt's keys are not attended over together with ones that its sequence
+    holds already, so such a call is refused: ``check`` reads ``lens`` on the
+    host before anything runs (30-40 us, and it waits for the stream). A model's
+    further blocks, whose caches share ``lens``, can leave it out; a call that is
+    being captured cannot read it and is not checked."""
+    if offsets is not None and check and not (cache.lens.is_cuda and torch.cuda.is_current_stream_capturing()):
+        assert offsets.shape == (cache.lens.numel() + 1,) and offsets.dtype == torch.int32, \
+            "offsets wants (sequences + 1) int32"
+        assert torch.equal(offsets.diff(), cache.lens), \
+            "a prompt fills empty sequences: lens must be the lengths that offsets give"
     p = wts.p
     dim = x.shape[1]
     d = dim // heads
