@@ -158,7 +158,6 @@ fn i32_of(v: usize, what: &str) -> i32 {
     i32::try_from(v).unwrap_or_else(|_| panic!("{what} {v} exceeds i32"))
 }
 
-/// One device's op surface on one HIP stream.
 /// One layer's paged key-value cache: `k`, `v` (n_pages, heads, page, d) and
 /// int32 device arrays (sequences, max_pages) and (sequences) that the caller
 /// owns and layers share. `lens` counts a call's new tokens already.
@@ -182,6 +181,7 @@ impl PagedKv {
     }
 }
 
+/// One device's op surface on one HIP stream.
 pub struct HipContext {
     stream: ffi::HsStream,
 }
