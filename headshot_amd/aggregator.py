@@ -372,8 +372,8 @@ def block_forward_cached(ctx: HipContext, wts: BlockWeights, x, cache, heads: in
     further blocks, whose caches share ``lens``, can leave it out; a call that is
     being captured cannot read it and is not checked."""
     if offsets is not None and check and not (cache.lens.is_cuda and torch.cuda.is_current_stream_capturing()):
-        assert offsets.shape == (cache.lens.numel() + 1,) and offsets.dtype == torch.int32, \
-            "offsets wants (sequences + 1) int32"
+        assert (offsets.shape == (cache.lens.numel() + 1,) and offsets.dtype == torch.int32
+                and offsets.device == cache.lens.device), "offsets wants (sequences + 1) int32 beside the cache"
         assert torch.equal(offsets.diff(), cache.lens), \
             "a prompt fills empty sequences: lens must be the lengths that offsets give"
     p = wts.p

@@ -28,7 +28,7 @@ def test_prompt_into_held_sequences(lens):
 
 
 def test_prompt_offsets():
-    for offsets in (i32([0, 8], "cpu"), i32([0, 5, 8], "cpu").long(), i32([[0, 5, 8]], "cpu")):
+    for offsets in (i32([0, 8], "cpu"), i32([0, 5, 8], "cpu").long(), i32([[0, 5, 8]], "cpu"), i32([0, 5, 8], "meta")):
         with pytest.raises(AssertionError, match="offsets wants"):
             block_forward_cached(None, None, torch.zeros(8, 128), cache([5, 3], "cpu"), 2, offsets=offsets)
 
