@@ -10,11 +10,12 @@
 // some query sees in part are masked. Few queries over many keys are split over
 // the keys, too (PackedPlan).
 //
-// Bounds: matrix and vector issue. f16: by frames, 10992 tokens of 16 heads of
-// 64, 204-214 us (760-795 TFLOP/s, matrix cores busy 45% of the time); prompts of
-// 12926 tokens, 32 heads of 128 over 8, 517-545 us (890-937 TFLOP/s, 45%); a plain
-// product of 8192^3 reaches 1246. f32, head dim 64: 4122 tokens by frames 215-226
-// us (137-144 TFLOP/s; some 360 on the f32 matrix instructions, whose plain
+// Bounds: matrix and vector issue, and the ends of calls of one to two rounds of
+// workgroups. f16: by frames, 10992 tokens of 16 heads of 64, 210-218 us (745-773
+// TFLOP/s; CUs busy 84% of it, their matrix cores 44% of that); prompts of 12926
+// tokens, 32 heads of 128 over 8, 524-560 us (865-925 TFLOP/s; 92%, 44%); a plain
+// product of 8192^3 reaches 1246. f32, head dim 64: 4122 tokens by frames 215-229
+// us (135-144 TFLOP/s; some 360 us on the f32 matrix instructions, whose plain
 // product reaches 154). Short calls are a chain of loads, find a tile, read it,
 // multiply, of 6 us and more: eight f32 sequences of up to 200 tokens, 16 heads
 // of 128, 20 us.
@@ -1236,6 +1237,8 @@ struct PackedPlan {
         if (half && n_q <= 64 * b && group % 2 == 0) share = n_q <= 32 * b && group % 4 == 0 ? 2 : 1;
         const int64_t all = h >> share;
         const auto cut = [&](Kernel k, int rows) { kernel = k, bm = rows, tiles = n_q / rows + (b < n_q ? b : n_q); };
+        // (All figures are of one sequence or of equal ones, and the rules see the
+        // average: a long sequence among many short ones may run as they do.)
         // f16: tiles of 256 queries for long sequences that make enough of them,
         // 128 else: more reuse against more masked keys and longer tails (us with
         // 128 and 256; 16 heads of 64: one sequence of 12000 tokens 694, 630, of

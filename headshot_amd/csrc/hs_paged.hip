@@ -205,8 +205,8 @@ void launch_append(hipStream_t st, const AppendArgs<T>& a) {
 // the scores' registers hold it. Loads run a step ahead. The four waves' (O, m,
 // l) join in LDS, the ranges of a sequence in a second launch.
 //
-// 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 177 us, 5.8
-// TB/s; one token over 130531 keys of 16 heads of 64 89 us, 6.0 TB/s. 19
+// 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 179 us, 5.8
+// TB/s; one token over 130531 keys of 16 heads of 64 91 us, 5.9 TB/s. 19
 // sequences of up to 3001 keys, 28 heads of 64 over 4, 13 us.
 //
 // Ranges: a sequence's keys are cut into pieces of `chunk` units of 4 kStep

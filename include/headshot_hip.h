@@ -418,7 +418,8 @@ hs_status hs_kv_append(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q
  * A query that sees no key gets zeros. Keys and values that a query does not
  * see do not enter its result, whatever they hold. Softmax statistics and sums
  * are f32; in f16 each weight is rounded to 11 bits, or to 2^-37 of the largest if
- * that is more. Few queries over many keys are split over the keys and joined,
+ * that is more; an infinity among the values seen whose weight that makes 0 gives
+ * NaN. Few queries over many keys are split over the keys and joined,
  * by the counts given and all lengths of the call; such calls take
  * hs_attention_packed_workspace bytes (16-byte aligned; NULL serves the others),
  * which hold nothing between calls: calls that may run at the same time need
