@@ -467,7 +467,9 @@ __global__ __launch_bounds__(64 * W, D == 64 ? (W == 8 ? 4 : 3) : 2) void packed
                     for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[i][r]);
                 mx = halves_max(mx);
                 own |= __builtin_amdgcn_exp2f(fmaf(mx, c, -m)) >= kPastF16;
-                const float next = own ? fmaxf(m, mx * c - kWeightBits) : m;
+                // (a maximum of 2^26 and more may round 8 further down, too far)
+                const float top = mx * c, low = top - kWeightBits;
+                const float next = own ? fmaxf(m, top - low > kWeightBits + 2.0f ? top : low) : m;
                 float corr = 1.0f;
                 wary--;
                 if (__any(next != m)) {

@@ -205,3 +205,29 @@ def test_paged_infinity_beside(ctx, d):
     rest = [c for c in range(d) if c not in (3, 40 % 7, 699 % 7)]
     bound = R.attention_bound(ref, mag, q, k, plain, [700], 1 / math.sqrt(d), F16)
     R.assert_within(got[..., rest], ref[..., rest], bound[..., rest], "the other channels")
+
+
+# ------------------------------------------------------------------ enormous scores
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("d,h,h_kv,nk", [(64, 2, 1, 300), (128, 2, 2, 300), (64, 1, 1, 2100), (128, 1, 1, 2100)])
+def test_enormous_scores(ctx, d, h, h_kv, nk, sign):
+    """Scores up to 2^29, at each power of two: keys 3, 100 and nk - 1 share the
+    largest, others lie at half of it and at 0 (sign 1), or at the double and more
+    below (-1), thousands of powers of two away in weight. The result is the mean
+    of three values whatever an exponent's rounding is."""
+    at = [3, 100, nk - 1]
+    for bits in range(12, 30):
+        a, b = bits - bits // 2, bits // 2
+        q, k = torch.zeros(5, h, d), torch.zeros(nk, h_kv, d)
+        q[..., 0] = 2.0 ** a
+        k[..., 0] = (torch.arange(nk) % 2 / 2 if sign > 0 else -2.0 - torch.arange(nk) % 2)[:, None] * 2.0 ** b
+        k[at, :, 0] = sign * 2.0 ** b
+        v = torch.randn(nk, h_kv, d, generator=torch.Generator().manual_seed(bits)).half()
+        ref = v[at].double().mean(0).repeat_interleave(h // h_kv, 0)
+        bound = (R.HALF[F16] + 8 * R.U32) * ref.abs() + 8 * R.U32 * v[at].double().abs().mean(0).max() + R.TINY[F16]
+        got = ctx.attention_packed(*(t.half().to(DEV) for t in (q, k, v)), i32([0, 5]), i32([0, nk]), causal=0, scale=1.0)
+        R.assert_within(got.unflatten(1, (h, d)), ref.expand(5, h, d), bound.expand(5, h, d), f"packed, 2^{bits}")
+        got = ctx.attention_paged(q[:1].half().to(DEV), pages_of(k.half(), v), scale=1.0)
+        R.assert_within(got.unflatten(1, (h, d)), ref[None], bound[None], f"paged, 2^{bits}")
