@@ -168,6 +168,41 @@ extern "C" {
                               workspace: *mut c_void, workspace_bytes: i64, b: i32, h: i32,
                               h_kv: i32, d: i32, page: i32, n_pages: i32, max_pages: i32,
                               scale: f32) -> HsStatus;
+    pub fn hs_kv_append_f8(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
+                           k: *const c_void, k_stride: i64, v: *const c_void, v_stride: i64,
+                           qn_w: *const f32, qn_b: *const f32, kn_w: *const f32,
+                           kn_b: *const f32, sin_tab: *const f32, cos_tab: *const f32,
+                           table_rows: i32, positions: *const c_void, offsets: *const c_void,
+                           page_table: *const c_void, lens: *const c_void, q_out: *mut c_void,
+                           k_out: *mut c_void, k_cache: *mut c_void, v_cache: *mut c_void,
+                           k_scale: *mut c_void, v_scale: *mut c_void, n: i64, b: i32, h: i32,
+                           h_kv: i32, d: i32, page: i32, n_pages: i32, max_pages: i32,
+                           eps: f32) -> HsStatus;
+    pub fn hs_attention_paged_f8_workspace(b: i32, h: i32, h_kv: i32, d: i32) -> i64;
+    pub fn hs_attention_paged_f8(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
+                                 k_cache: *const c_void, v_cache: *const c_void,
+                                 k_scale: *const c_void, v_scale: *const c_void,
+                                 page_table: *const c_void, lens: *const c_void,
+                                 out: *mut c_void, workspace: *mut c_void, workspace_bytes: i64,
+                                 b: i32, h: i32, h_kv: i32, d: i32, page: i32, n_pages: i32,
+                                 max_pages: i32, scale: f32) -> HsStatus;
+    pub fn hs_attention_prompts_f8_workspace(dt: HsDtype, n: i64, b: i32, h: i32, h_kv: i32,
+                                             d: i32, page: i32, max_pages: i32,
+                                             causal: i32) -> i64;
+    pub fn hs_attention_prompts_f8(stream: HsStream, dt: HsDtype, q: *const c_void, q_stride: i64,
+                                   k_cache: *const c_void, v_cache: *const c_void,
+                                   k_scale: *const c_void, v_scale: *const c_void,
+                                   page_table: *const c_void, lens: *const c_void,
+                                   offsets: *const c_void, out: *mut c_void,
+                                   workspace: *mut c_void, workspace_bytes: i64, n: i64, b: i32,
+                                   h: i32, h_kv: i32, d: i32, page: i32, n_pages: i32,
+                                   max_pages: i32, causal: i32, scale: f32) -> HsStatus;
+    pub fn hs_plan_pages_workspace(n: i64, b: i32, max_pages: i32) -> i64;
+    pub fn hs_plan_pages(stream: HsStream, counts: *const c_void, lens: *mut c_void,
+                         page_table: *mut c_void, free: *mut c_void, state: *mut c_void,
+                         offsets: *mut c_void, positions: *mut c_void, slots: *mut c_void,
+                         workspace: *mut c_void, workspace_bytes: i64, n: i64, b: i32, page: i32,
+                         n_pages: i32, max_pages: i32) -> HsStatus;
 
     // host-side RoPE tables
     pub fn hs_rope_periods(out16: *mut f32);

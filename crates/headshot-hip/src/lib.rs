@@ -181,6 +181,39 @@ impl PagedKv {
     }
 }
 
+/// The same held in 8 bits: e4m3 codes `k`, `v` (n_pages, heads, page, d) and
+/// scales (n_pages, heads), one byte each, device memory that the caller owns.
+/// `dtype` is the type of the rows beside it.
+pub struct PagedKv8 {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut c_void,
+    pub v_scale: *mut c_void,
+    pub dtype: Dtype,
+    pub n_pages: usize,
+    pub heads: usize,
+    pub page: usize,
+    pub d: usize,
+    pub page_table: *const i32,
+    pub lens: *const i32,
+    pub sequences: usize,
+    pub max_pages: usize,
+}
+
+/// The pages of caches that share `page_table` (sequences, max_pages) and `lens`
+/// (sequences): free ones in a ring, `free` (n_pages) and `state` (3), int32
+/// device arrays that the caller owns.
+pub struct PagePool {
+    pub page_table: *mut i32,
+    pub lens: *mut i32,
+    pub free: *mut i32,
+    pub state: *mut i32,
+    pub sequences: usize,
+    pub max_pages: usize,
+    pub n_pages: usize,
+    pub page: usize,
+}
+
 /// One device's op surface on one HIP stream.
 pub struct HipContext {
     stream: ffi::HsStream,
@@ -817,6 +850,126 @@ impl HipContext {
                               i32_of(n_pages, "n_pages"), i32_of(cache.max_pages, "max_pages"), eps)
         }, "kv_append");
         (q_out, k_out)
+    }
+
+    /// `kv_append` into a cache held in 8 bits.
+    #[allow(clippy::too_many_arguments)]
+    pub fn kv_append_f8(&self, cache: &PagedKv8, q: Option<&HipTensor>, k: &HipTensor,
+                        v: &HipTensor, offsets: *const i32, qn: Option<(&HipTensor, &HipTensor)>,
+                        kn: Option<(&HipTensor, &HipTensor)>,
+                        rope: Option<(&HipTensor, &HipTensor)>, positions: *const i32, eps: f32,
+                        k_rows: bool) -> (Option<HipTensor>, Option<HipTensor>) {
+        let (dt, d) = (cache.dtype, cache.d);
+        let (n, width) = k.dims();
+        assert_eq!(width, cache.heads * d, "kv_append k width");
+        assert_eq!(v.dims(), (n, width), "kv_append v shape");
+        assert!(k.dtype == dt && v.dtype == dt, "kv_append k/v dtype");
+        let q_width = q.map_or(0, |q| {
+            let (rows, w) = q.dims();
+            assert!(rows == n && w % d == 0 && q.dtype == dt, "kv_append q");
+            w
+        });
+        let norm = |p: Option<(&HipTensor, &HipTensor)>, what: &str| {
+            p.map_or((ptr::null(), ptr::null()),
+                     |(w, b)| (opt_f32(Some(w), d, what), opt_f32(Some(b), d, what)))
+        };
+        let ((qw, qb), (kw, kb)) = (norm(qn, "q-norm"), norm(kn, "k-norm"));
+        let rows = rope.map_or(0, |(sin, _)| sin.len() / d);
+        let (sn, cs) = rope.map_or((ptr::null(), ptr::null()), |(sin, cos)| {
+            (opt_f32(Some(sin), rows * d, "rope sin table"),
+             opt_f32(Some(cos), rows * d, "rope cos table"))
+        });
+        let q_out = q.map(|_| self.empty_typed(&[n, q_width], dt));
+        let k_out = k_rows.then(|| self.empty_typed(&[n, width], dt));
+        let out = |t: &Option<HipTensor>| t.as_ref().map_or(ptr::null_mut(), |t| t.mptr());
+        check(unsafe {
+            ffi::hs_kv_append_f8(self.stream, dt.raw(), q.map_or(ptr::null(), |q| q.cptr()),
+                                 q_width as i64, k.cptr(), width as i64, v.cptr(), width as i64,
+                                 qw, qb, kw, kb, sn, cs, i32_of(rows, "rows"),
+                                 positions as *const c_void, offsets as *const c_void,
+                                 cache.page_table as *const c_void, cache.lens as *const c_void,
+                                 out(&q_out), out(&k_out), cache.k, cache.v, cache.k_scale,
+                                 cache.v_scale, n as i64, i32_of(cache.sequences, "sequences"),
+                                 i32_of(q_width / d, "h"), i32_of(cache.heads, "h_kv"),
+                                 i32_of(d, "d"), i32_of(cache.page, "page"),
+                                 i32_of(cache.n_pages, "n_pages"),
+                                 i32_of(cache.max_pages, "max_pages"), eps)
+        }, "kv_append");
+        (q_out, k_out)
+    }
+
+    /// `attention_paged` over a cache held in 8 bits.
+    pub fn attention_paged_f8(&self, q: &HipTensor, cache: &PagedKv8) -> HipTensor {
+        let (b, width) = q.dims();
+        let d = cache.d;
+        assert_eq!(b, cache.sequences, "attention_paged q rows");
+        assert!(width % d == 0 && q.dtype == cache.dtype, "attention_paged q");
+        let (bi, h, kv, di) = (i32_of(b, "b"), i32_of(width / d, "h"),
+                               i32_of(cache.heads, "h_kv"), i32_of(d, "d"));
+        let bytes = unsafe { ffi::hs_attention_paged_f8_workspace(bi, h, kv, di) };
+        let ws = self.empty_typed(&[(bytes as usize + 3) / 4], Dtype::F32);
+        let out = self.empty_typed(&[b, width], q.dtype);
+        check(unsafe {
+            ffi::hs_attention_paged_f8(self.stream, q.dtype.raw(), q.cptr(), width as i64,
+                                       cache.k, cache.v, cache.k_scale, cache.v_scale,
+                                       cache.page_table as *const c_void,
+                                       cache.lens as *const c_void, out.mptr(), ws.mptr(), bytes,
+                                       bi, h, kv, di, i32_of(cache.page, "page"),
+                                       i32_of(cache.n_pages, "n_pages"),
+                                       i32_of(cache.max_pages, "max_pages"),
+                                       1.0 / (d as f32).sqrt())
+        }, "attention_paged");
+        out
+    }
+
+    /// Attention of several new tokens per sequence over a cache held in 8 bits,
+    /// which has their own keys already: `q` (n, heads * d), `offsets`
+    /// (sequences + 1) int32 on the device; `causal` 0 = every key, c = by groups
+    /// of c tokens.
+    pub fn attention_paged_prompts(&self, q: &HipTensor, cache: &PagedKv8, offsets: *const i32,
+                                   causal: usize) -> HipTensor {
+        let (n, width) = q.dims();
+        let d = cache.d;
+        assert!(width % d == 0 && q.dtype == cache.dtype, "attention_paged_prompts q");
+        let (b, h, kv, di) = (i32_of(cache.sequences, "b"), i32_of(width / d, "h"),
+                              i32_of(cache.heads, "h_kv"), i32_of(d, "d"));
+        let (page, width_pages, c) = (i32_of(cache.page, "page"),
+                                      i32_of(cache.max_pages, "max_pages"),
+                                      i32_of(causal, "causal"));
+        let bytes = unsafe {
+            ffi::hs_attention_prompts_f8_workspace(q.dtype.raw(), n as i64, b, h, kv, di, page,
+                                                   width_pages, c)
+        };
+        let ws = self.empty_typed(&[(bytes as usize + 3) / 4], Dtype::F32);
+        let out = self.empty_typed(&[n, width], q.dtype);
+        check(unsafe {
+            ffi::hs_attention_prompts_f8(self.stream, q.dtype.raw(), q.cptr(), width as i64,
+                                         cache.k, cache.v, cache.k_scale, cache.v_scale,
+                                         cache.page_table as *const c_void,
+                                         cache.lens as *const c_void, offsets as *const c_void,
+                                         out.mptr(), ws.mptr(), bytes, n as i64, b, h, kv, di,
+                                         page, i32_of(cache.n_pages, "n_pages"), width_pages, c,
+                                         1.0 / (d as f32).sqrt())
+        }, "attention_paged_prompts");
+        out
+    }
+
+    /// Hands out the pages of a call's new tokens and takes back dropped ones':
+    /// `counts` (sequences), `offsets` (sequences + 1) and, null or not,
+    /// `positions` (n) int32, `slots` (n) int64, on the device.
+    pub fn plan_pages(&self, pool: &PagePool, counts: *const i32, n: usize, offsets: *mut i32,
+                      positions: *mut i32, slots: *mut i64) {
+        let (b, width) = (i32_of(pool.sequences, "sequences"), i32_of(pool.max_pages, "max_pages"));
+        let bytes = unsafe { ffi::hs_plan_pages_workspace(n as i64, b, width) };
+        let ws = self.empty_typed(&[(bytes as usize + 3) / 4], Dtype::F32);
+        check(unsafe {
+            ffi::hs_plan_pages(self.stream, counts as *const c_void, pool.lens as *mut c_void,
+                               pool.page_table as *mut c_void, pool.free as *mut c_void,
+                               pool.state as *mut c_void, offsets as *mut c_void,
+                               positions as *mut c_void, slots as *mut c_void, ws.mptr(), bytes,
+                               n as i64, b, i32_of(pool.page, "page"),
+                               i32_of(pool.n_pages, "n_pages"), width)
+        }, "plan_pages");
     }
 
     /// Attention of packed sequences: `q` (n, heads * d), `k`, `v` (m, kv_heads

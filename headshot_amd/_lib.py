@@ -74,6 +74,17 @@ SIGNATURES = {
     "hs_attention_paged_workspace": (_I64, [_I32, _I32, _I32, _I32]),
     "hs_attention_paged": (_S, [_P, _I32, _P, _I64, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32,
                                 _I32, _I32, _I32, _I32, _F]),
+    "hs_kv_append_f8": (_S, [_P, _I32, _P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _P, _P, _I32,
+                             _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32,
+                             _I32, _I32, _F]),
+    "hs_attention_paged_f8_workspace": (_I64, [_I32, _I32, _I32, _I32]),
+    "hs_attention_paged_f8": (_S, [_P, _I32, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32,
+                                   _I32, _I32, _I32, _I32, _I32, _F]),
+    "hs_attention_prompts_f8_workspace": (_I64, [_I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I32]),
+    "hs_attention_prompts_f8": (_S, [_P, _I32, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64,
+                                     _I32, _I32, _I32, _I32, _I32, _I32, _I32, _I32, _F]),
+    "hs_plan_pages_workspace": (_I64, [_I64, _I32, _I32]),
+    "hs_plan_pages": (_S, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32]),
     "hs_rope_periods": (None, [_P]),
     "hs_rope_tables": (_S, [_P, _I32, _I32, _P, _P]),
 }

@@ -19,6 +19,7 @@ import torch
 
 from . import rope as _rope
 from .context import HipContext
+from .paged import PagedKV8
 
 DIM, HEADS, HEAD_DIM, HIDDEN = 1024, 16, 64, 4096
 
@@ -359,19 +360,22 @@ def block_forward_cached(ctx: HipContext, wts: BlockWeights, x, cache, heads: in
                          offsets=None, rope=None, positions=None, causal: int = 1,
                          eps: float = 1e-6, check: bool = True):
     """``block_forward`` for sequences that grow, over this block's ``cache``
-    (``PagedKV``, its ``lens`` counting x's tokens already). With ``offsets``
-    x holds whole prompts, sequence after sequence, that fill empty sequences
-    and attend among themselves (``causal`` as ``attention_packed``: 1 by
-    token, T by frames of T tokens); without, one new token per sequence, that
-    sees every key the cache holds. ``rope`` = (sin, cos) with ``positions`` as
+    (``PagedKV`` or ``PagedKV8``, its ``lens`` counting x's tokens already).
+    With ``offsets`` x holds new tokens, sequence after sequence, that attend
+    among themselves (``causal`` as ``attention_packed``: 1 by token, T by
+    frames of T tokens); without, one new token per sequence, that sees every
+    key the cache holds. ``rope`` = (sin, cos) with ``positions`` as
     ``kv_append``, or None. Returns the block output, x's shape.
 
-    A prompt's keys are not attended over together with ones that its sequence
-    holds already, so such a call is refused: ``check`` reads ``lens`` on the
-    host before anything runs (30-40 us, and it waits for the stream). A model's
-    further blocks, whose caches share ``lens``, can leave it out; a call that is
-    being captured cannot read it and is not checked."""
-    if offsets is not None and check and not (cache.lens.is_cuda and torch.cuda.is_current_stream_capturing()):
+    Over a ``PagedKV8`` the new tokens of ``offsets`` also see the keys that
+    their sequences hold already. Over a ``PagedKV`` they are whole prompts of
+    empty sequences, whose unpaged keys are attended over, and others are
+    refused: ``check`` reads ``lens`` on the host before anything runs (30-40 us,
+    and it waits for the stream). A model's further blocks, whose caches share
+    ``lens``, can leave it out; a call that is being captured cannot read it and
+    is not checked."""
+    eight = type(cache) is PagedKV8
+    if offsets is not None and check and not eight and not (cache.lens.is_cuda and torch.cuda.is_current_stream_capturing()):
         assert (offsets.shape == (cache.lens.numel() + 1,) and offsets.dtype == torch.int32
                 and offsets.device == cache.lens.device), "offsets wants (sequences + 1) int32 beside the cache"
         assert torch.equal(offsets.diff(), cache.lens), \
@@ -382,9 +386,11 @@ def block_forward_cached(ctx: HipContext, wts: BlockWeights, x, cache, heads: in
     normed = ctx.layernorm(x, *p.ln1, eps=eps)
     q, k, v = ctx.linear(normed, wts.qkv_w, wts.qkv_b).split(dim, 1)
     q, k = ctx.kv_append(cache, k, v, offsets, q=q, qn=p.qn, kn=p.kn, rope=rope,
-                         positions=positions, eps=eps, k_rows=offsets is not None)
+                         positions=positions, eps=eps, k_rows=offsets is not None and not eight)
     if offsets is None:
         attn = ctx.attention_paged(q, cache)
+    elif eight:
+        attn = ctx.attention_paged_prompts(q, cache, offsets, causal=causal)
     else:
         q, k, v = (t.unflatten(1, (heads, d)) for t in (q, k, v))
         attn = ctx.attention_packed(q, k, v, offsets, causal=causal)

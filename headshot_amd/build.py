@@ -32,6 +32,8 @@ HIP_SOURCES = [
     "hs_attention.hip",
     "hs_attention_packed.hip",
     "hs_paged.hip",
+    "hs_paged_f8.hip",
+    "hs_pages.hip",
     "hs_cache.hip",
     "hs_gemm.hip",
 ]
@@ -56,6 +58,7 @@ HIP_FLAGS = [
 SOURCE_FLAGS = {
     "hs_attention_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "hs_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "hs_paged_f8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "hs_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
 }
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-Wall",

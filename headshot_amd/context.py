@@ -23,6 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .paged import PagedKV8
 
 F32 = torch.float32
 F16 = torch.float16
@@ -617,7 +618,7 @@ class HipContext:
     def kv_append(self, cache, k, v, offsets=None, q=None, qn=None, kn=None, rope=None,
                   positions=None, eps: float = 1e-5, k_rows: bool = False, out_q=None, out_k=None):
         """Appends new tokens' keys and values to their sequences' pages
-        (``PagedKV``), with QK-norm and the position rotation of
+        (``PagedKV``, ``PagedKV8``), with QK-norm and the position rotation of
         ``rope_apply`` on the way.
 
         ``k``, ``v`` (n, heads * d) or (n, heads, d) rows, sequence after
@@ -630,7 +631,13 @@ class HipContext:
         key's number; a row outside the tables is not rotated. A token whose
         page lies outside the table or the pool is not stored, and rows behind
         ``offsets[-1]`` stay as they are. Returns (q, k) as contiguous
-        rows, None for what was not asked (``q``, ``k_rows``)."""
+        rows, None for what was not asked (``q``, ``k_rows``).
+
+        A ``PagedKV8`` takes the new keys and values as codes, those of a page
+        and head over one scale: the least power of two that brings them to
+        448, or the page's own where that is larger and the call goes on with
+        the page; older codes follow a scale that grows. Magnitudes past
+        f16's (61440) are held as that, infinities and NaN as NaN."""
         n_pages, h_kv, page, d, b, max_pages = cache.shape
         dtype, dev = cache.dtype, _device()
         if cache.device_index != dev:
@@ -672,6 +679,15 @@ class HipContext:
         if positions is not None:
             assert rope is not None, "positions without rope"
             pos = _dense(positions, n, torch.int32, dev, "positions")
+        if type(cache) is PagedKV8:
+            self._launch_held("kv_append", self.lib.hs_kv_append_f8,
+                              (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.page_table, cache.lens, k, v,
+                               offsets, q, qn, kn, rope, positions, out_q, out_k), _DT[dtype], qp, qs, kp, ks, vp, vs,
+                              qw, qb, kw, kb, sn, cs, rows, pos, off, cache.page_table.data_ptr(),
+                              cache.lens.data_ptr(), qo, ko, cache.k.data_ptr(), cache.v.data_ptr(),
+                              cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), n, b, h, h_kv, d, page, n_pages,
+                              max_pages, eps)
+            return out_q, out_k
         self._launch_held("kv_append", self.lib.hs_kv_append,
                           (cache.k, cache.v, cache.page_table, cache.lens, k, v, offsets, q, qn, kn, rope, positions,
                            out_q, out_k), _DT[dtype], qp, qs, kp, ks, vp, vs, qw, qb, kw, kb, sn, cs, rows, pos, off,
@@ -726,12 +742,12 @@ class HipContext:
 
     def attention_paged(self, q, cache, scale=None, out=None, workspace=None) -> torch.Tensor:
         """Attention of one new token per sequence over the keys that
-        ``cache`` (``PagedKV``) holds: ``q`` (sequences, heads, d) or
-        (sequences, heads * d) -> (sequences, heads * d), zeros for a sequence
-        without keys. heads is a multiple of the cache's. ``workspace`` (uint8,
-        ``attention_paged_workspace`` bytes) keeps the call from allocating;
-        calls that may run at the same time need one each. ``scale`` None is 1
-        / sqrt(d)."""
+        ``cache`` (``PagedKV``, ``PagedKV8``) holds: ``q`` (sequences, heads, d)
+        or (sequences, heads * d) -> (sequences, heads * d), zeros for a
+        sequence without keys. heads is a multiple of the cache's.
+        ``workspace`` (uint8, ``attention_paged_workspace`` bytes) keeps the
+        call from allocating; calls that may run at the same time need one
+        each. ``scale`` None is 1 / sqrt(d)."""
         n_pages, h_kv, page, d, b, max_pages = cache.shape
         dtype, dev = cache.dtype, _device()
         if cache.device_index != dev:
@@ -744,19 +760,116 @@ class HipContext:
             op = out.data_ptr()
         else:
             op = _dense(out, b * h * d, dtype, dev, "out")
+        eight = type(cache) is PagedKV8
         if workspace is None:
-            size = self.lib.hs_attention_paged_workspace(b, h, h_kv, d)
+            size = (self.lib.hs_attention_paged_f8_workspace if eight else
+                    self.lib.hs_attention_paged_workspace)(b, h, h_kv, d)
             workspace = q.new_empty(size, dtype=torch.uint8)
             wp = workspace.data_ptr()
         else:
             size = workspace.numel()
             wp = _dense(workspace, size, torch.uint8, dev, "workspace")
+        if scale is None:
+            scale = 1.0 / math.sqrt(d)
+        if eight:
+            self._launch_held("attention_paged", self.lib.hs_attention_paged_f8,
+                              (q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.page_table, cache.lens, out,
+                               workspace), _DT[dtype], qp, qs, cache.k.data_ptr(), cache.v.data_ptr(),
+                              cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.page_table.data_ptr(),
+                              cache.lens.data_ptr(), op, wp, size, b, h, h_kv, d, page, n_pages, max_pages, scale)
+            return out
         self._launch_held("attention_paged", self.lib.hs_attention_paged,
                           (q, cache.k, cache.v, cache.page_table, cache.lens, out, workspace), _DT[dtype], qp, qs,
                           cache.k.data_ptr(), cache.v.data_ptr(), cache.page_table.data_ptr(), cache.lens.data_ptr(),
-                          op, wp, size, b, h, h_kv, d, page, n_pages, max_pages,
+                          op, wp, size, b, h, h_kv, d, page, n_pages, max_pages, scale)
+        return out
+
+    def attention_paged_prompts(self, q, cache, offsets, causal: int = 1, scale=None, out=None,
+                                workspace=None) -> torch.Tensor:
+        """Attention of several new tokens per sequence over the keys that
+        ``cache`` (``PagedKV8``) holds, their own among them: ``q`` (n, heads,
+        d) rows at int32 ``offsets`` (sequences + 1) -> (n, heads * d). The
+        last of sequence s's tokens is its key ``lens[s] - 1``; ``causal`` as
+        ``attention_packed`` (0: every key, c: groups of c tokens, counted
+        from key 0). A token that sees nothing gets zeros; rows behind
+        ``offsets[-1]`` are not written. heads is a multiple of the cache's.
+        ``workspace`` (uint8, ``attention_paged_prompts_workspace`` bytes)
+        keeps the call from allocating; calls that may run at the same time
+        need one each. ``scale`` None is 1 / sqrt(d)."""
+        assert type(cache) is PagedKV8, "attention_paged_prompts wants a PagedKV8"
+        n_pages, h_kv, page, d, b, max_pages = cache.shape
+        dtype, dev = cache.dtype, _device()
+        if cache.device_index != dev:
+            raise AssertionError("the cache must live in memory of the current device")
+        assert 0 <= causal < 2 ** 31, f"causal {causal}"
+        h = math.prod(q.shape[1:]) // d
+        qp, n, qs = _rows(q, h, d, dtype, dev, "q")
+        off = _dense(offsets, b + 1, torch.int32, dev, "offsets")
+        if out is None:
+            out = q.new_empty((n, h * d))
+            op = out.data_ptr()
+        else:
+            op = _dense(out, n * h * d, dtype, dev, "out")
+        dt, wp, size = _DT[dtype], None, 0
+        if workspace is not None:
+            size = workspace.numel()
+            wp = _dense(workspace, size, torch.uint8, dev, "workspace")
+        else:
+            size = self.lib.hs_attention_prompts_f8_workspace(dt, n, b, h, h_kv, d, page, max_pages, causal)
+            if size:
+                workspace = q.new_empty(size, dtype=torch.uint8)
+                wp = workspace.data_ptr()
+        self._launch_held("attention_paged_prompts", self.lib.hs_attention_prompts_f8,
+                          (q, cache.k, cache.v, cache.k_scale, cache.v_scale, cache.page_table, cache.lens, offsets,
+                           out, workspace), dt, qp, qs, cache.k.data_ptr(), cache.v.data_ptr(),
+                          cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.page_table.data_ptr(),
+                          cache.lens.data_ptr(), off, op, wp, size, n, b, h, h_kv, d, page, n_pages, max_pages, causal,
                           1.0 / math.sqrt(d) if scale is None else scale)
         return out
+
+    def plan_pages(self, pool, counts, n: int, out=None, workspace=None):
+        """Hands out the pages of a call's new tokens, and takes back those of
+        dropped ones: sequence s of ``pool`` (``PagePool``) grows by
+        ``counts[s]`` (int32) tokens or, below 0, drops as many of its last.
+        ``pool.lens`` and ``pool.page_table`` are brought up to date for
+        ``kv_append`` and what follows it. Pages given back are handed out from
+        the next call on; an entry that there was no page for is -1, its
+        tokens have no place, and ``pool.state[2]`` counts such pages.
+
+        Returns (offsets, positions, slots): int32 rows by sequence
+        (sequences + 1), each new token's key number (int32) and place
+        (int64, page * page size + row, -1 without one) in its row, of at
+        most ``n``; rows behind ``offsets[-1]`` are not written. ``out`` is
+        the three to write into. Nothing is read on the host, so a captured
+        call follows ``counts``. ``workspace`` (uint8,
+        ``plan_pages_workspace`` bytes) keeps a long call from allocating."""
+        b, max_pages, n_pages = pool.shape
+        dev = _device()
+        if pool.device_index != dev:
+            raise AssertionError("the pool must live in memory of the current device")
+        assert 0 <= n < 2 ** 30, f"plan_pages: n {n}"
+        cp = _dense(counts, b, torch.int32, dev, "counts")
+        if out is None:
+            offsets, positions = (counts.new_empty(x) for x in (b + 1, n))
+            slots = counts.new_empty(n, dtype=torch.int64)
+        else:
+            offsets, positions, slots = out
+        size, wp = 0, None
+        if workspace is not None:
+            size = workspace.numel()
+            wp = _dense(workspace, size, torch.uint8, dev, "workspace")
+        else:
+            size = self.lib.hs_plan_pages_workspace(n, b, max_pages)
+            if size:
+                workspace = counts.new_empty(size, dtype=torch.uint8)
+                wp = workspace.data_ptr()
+        self._launch_held("plan_pages", self.lib.hs_plan_pages,
+                          (pool.page_table, pool.lens, pool.free, pool.state, counts, offsets, positions, slots,
+                           workspace), cp, pool.lens.data_ptr(), pool.page_table.data_ptr(), pool.free.data_ptr(),
+                          pool.state.data_ptr(), _dense(offsets, b + 1, torch.int32, dev, "offsets"),
+                          _dense(positions, n, torch.int32, dev, "positions"),
+                          _dense(slots, n, torch.int64, dev, "slots"), wp, size, n, b, pool.page, n_pages, max_pages)
+        return offsets, positions, slots
 
     def attention_packed_workspace(self, dtype, n_q: int, n_k: int, sequences: int, heads: int,
                                    kv_heads: int, d: int, causal: int = 1) -> int:
@@ -764,9 +877,24 @@ class HipContext:
         where the keys are not split."""
         return self.lib.hs_attention_packed_workspace(_DT[dtype], n_q, n_k, sequences, heads, kv_heads, d, causal)
 
-    def attention_paged_workspace(self, sequences: int, heads: int, kv_heads: int, d: int) -> int:
-        """Bytes of workspace of ``attention_paged`` on the current device."""
-        return self.lib.hs_attention_paged_workspace(sequences, heads, kv_heads, d)
+    def attention_paged_workspace(self, sequences: int, heads: int, kv_heads: int, d: int,
+                                  eight: bool = False) -> int:
+        """Bytes of workspace of ``attention_paged`` on the current device;
+        ``eight``: over a ``PagedKV8``."""
+        return (self.lib.hs_attention_paged_f8_workspace if eight else
+                self.lib.hs_attention_paged_workspace)(sequences, heads, kv_heads, d)
+
+    def attention_paged_prompts_workspace(self, cache, n: int, heads: int, causal: int = 1) -> int:
+        """Bytes of workspace of ``attention_paged_prompts`` for ``n`` tokens
+        over ``cache`` on the current device; 0 where the keys are not split."""
+        n_pages, h_kv, page, d, b, max_pages = cache.shape
+        return self.lib.hs_attention_prompts_f8_workspace(_DT[cache.dtype], n, b, heads, h_kv, d, page, max_pages,
+                                                          causal)
+
+    def plan_pages_workspace(self, pool, n: int) -> int:
+        """Bytes of workspace of ``plan_pages``; 0 for calls of one launch."""
+        b, max_pages, _ = pool.shape
+        return self.lib.hs_plan_pages_workspace(n, b, max_pages)
 
     def bias_gelu(self, x, bias=None, out=None) -> torch.Tensor:
         """fc1 bias epilogue + GELU (model/block.rs:173-174)."""

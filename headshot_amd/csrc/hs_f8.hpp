@@ -1,0 +1,75 @@
+// A cache held in 8 bits: e4m3 codes (sign, 4 bits of exponent, 3 of mantissa;
+// no infinities, one NaN a sign) and, for each page and head, one scale 2^(c -
+// 127) of which c is kept (E8M0). A code times a scale has 4 significant bits, so
+// bf16 holds it as it is, whatever the scale, and f16 where f16 reaches.
+#pragma once
+
+#include "hs_paged.hpp"
+
+namespace hs {
+namespace {
+
+constexpr int kScaleBias = 127;
+constexpr int kScaleLeast = kScaleBias - 117;  // 448 2^-117: codes from 2^-126
+constexpr int kScaleMost = kScaleBias + 120;
+
+// The largest magnitude that a cache of T's rows holds, 15/8 2^15 and 15/8 2^127:
+// what would round to the next code is no T. (f16's own largest, 65504, is as far
+// from it as any value may be from its code, 2^-4.)
+template <typename T>
+constexpr float kHeldMost = sizeof(T) == 2 ? 61440.0f : 3.1901471898837979e38f;
+
+__device__ __forceinline__ float scale_value(uint32_t c) { return u2f(c << 23); }
+
+// Kept form of the least scale 2^e with most <= 448 2^e = 7/8 2^(e + 9), most
+// finite: its exponent less 8, or less 9 up to 7/8 of the next power of two.
+__device__ __forceinline__ int scale_for(float most) {
+    const uint32_t b = f2u(most);
+    const int e = static_cast<int>(b >> 23) - 8 + ((b & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return max(e, kScaleLeast);
+}
+
+// 8 codes to 8 halves of T, times a scale.
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ u32x4 f16_of_codes(uint32_t lo, uint32_t hi, float scale) {
+    u32x4 r;
+    r[0] = h22u(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false));
+    r[1] = h22u(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, true));
+    r[2] = h22u(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, false));
+    r[3] = h22u(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, scale, true));
+    return r;
+}
+__device__ __forceinline__ u32x4 bf16_of_codes(uint32_t lo, uint32_t hi, float scale) {
+    u32x4 r;
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
+    return r;
+}
+
+// 4 values to 4 codes, rounded to nearest even. (In range: a finite value past
+// 448 would become NaN.)
+__device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d) {
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true));
+}
+
+// 4 codes times 2^-down, rounded again.
+__device__ __forceinline__ uint32_t codes_down(uint32_t w, int down) {
+    const float f = u2f(static_cast<uint32_t>(127 - min(down, 126)) << 23);
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    return codes_of(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
+}
+
+// The host's checks of such a cache.
+[[maybe_unused]] hs_status check_cache_f8(const char* op, const void* k_cache, const void* v_cache, const void* k_scale,
+                                          const void* v_scale, const void* page_table, const void* lens, int32_t page,
+                                          int32_t n_pages, int32_t max_pages, int32_t h_kv, int32_t d) {
+    if (hs_status rc = check_cache(op, k_cache, v_cache, page_table, lens, page, n_pages, max_pages, h_kv, d)) return rc;
+    if (n_pages > 0 && (!k_scale || !v_scale)) return fail(HS_EINVAL, "%s: null scales", op);
+    return HS_OK;
+}
+
+}  // namespace
+}  // namespace hs

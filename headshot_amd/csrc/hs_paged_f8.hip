@@ -1,0 +1,448 @@
+// A paged key-value cache held in 8 bits for gfx950: appending new tokens and the
+// attention of new tokens over it.
+#include "hs_f8.hpp"
+
+namespace hs {
+namespace {
+
+// ---------------------------------------------------------------------------
+// kv_append
+//
+// A page's new keys of one head take a scale together, so a unit of work is one
+// (page of a sequence, head, k or v): its rows are read, normalised and rotated
+// into registers, their largest magnitude gives the scale, and the codes follow.
+// A page that the call goes on with keeps the larger scale of the two; where that
+// is the new one, the older codes are brought to it, which is exact but for those
+// that become subnormal.
+//
+// A unit's rows are held by one wave where a page has at most 2048 / D, else by
+// four, kRowsHeld rows each; pages past that are read twice.
+template <typename T>
+struct Append8Args {
+    AppendArgs<T> rows;  // q, and k where its rows are asked for
+    const int *offsets, *page_table, *lens;
+    uint8_t *k_cache, *v_cache, *k_scale, *v_scale;
+    int n_pages, row_blocks;
+};
+
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp<kQuadXor1>(v));
+    v = fmaxf(v, dpp<kQuadXor2>(v));
+    v = fmaxf(v, dpp<kRowHalfMirror>(v));
+    v = fmaxf(v, dpp<kRowMirror>(v));
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+
+// A unit's place: tokens [token, token + rows) of the call become rows [first,
+// first + rows) of page `page`.
+struct PageUnit {
+    int token, rows, first, page, pos;
+};
+template <typename T>
+__device__ __forceinline__ bool find_unit(const Append8Args<T>& a, int index, PageUnit& t) {
+    const AppendArgs<T>& r = a.rows;
+    const int shift = r.page_shift, limit = r.max_pages << shift;
+    int s, entry, begin, end, m_end;  // keys [begin, end) of the sequence; its tokens end at row m_end
+    if (!a.offsets) {
+        s = index;
+        if (s >= r.b) return false;
+        const int len = a.lens[s];
+        begin = len - 1, end = len, m_end = s + 1;
+        if (begin < 0 || begin >= limit) return false;
+        entry = begin >> shift;
+    } else {
+        const int lane = lane_id();
+        int before = 0;
+        s = -1;
+        for (int base = 0; base < r.b; base += 64) {
+            int count = 0, b0 = 0, e0 = 0, z0 = 0;
+            if (base + lane < r.b) {
+                const RowRange q = row_range(a.offsets, base + lane, r.n);
+                const int len = max(a.lens[base + lane], 0);
+                b0 = max(len - (q.end - q.begin), 0), e0 = min(len, limit), z0 = q.end;
+                // (the last token of the rows is key len - 1, whether it has a place or not)
+                if (q.end > q.begin && e0 > b0) count = ((e0 - 1) >> shift) - (b0 >> shift) + 1;
+                z0 -= len;  // token of key p: p + z0
+            }
+            const int sum = wave_prefix_sum(count);
+            const uint64_t hit = __ballot(before + sum > index);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                s = base + l;
+                begin = lane_value(b0, l), end = lane_value(e0, l), m_end = lane_value(z0, l);
+                entry = (begin >> shift) + index - before - (lane_value(sum, l) - lane_value(count, l));
+                break;
+            }
+            before += lane_value(sum, 63);
+        }
+        if (s < 0) return false;
+        m_end += end;  // as if the sequence ended at `end`
+    }
+    t.page = a.page_table[static_cast<int64_t>(s) * r.max_pages + entry];
+    if (t.page < 0 || t.page >= a.n_pages) return false;
+    const int lo = max(begin, entry << shift), hi = min(end, (entry + 1) << shift);
+    t.pos = lo, t.first = lo & ((1 << shift) - 1), t.rows = hi - lo;
+    t.token = m_end - (end - lo);
+    return true;
+}
+
+template <typename T, int D, bool NORM, bool ROPE, int W>
+__device__ void append_page(const Append8Args<T>& a, int index) {
+    const AppendArgs<T>& r = a.rows;
+    constexpr int V = Vec<T>::N, G = D / (2 * V), kRows = 64 / G;  // rows per load
+    constexpr int kHeld = 2048 / D, P = kHeld / kRows;             // rows and loads that a wave holds
+    __shared__ float tops[W];
+    const int lane = lane_id(), wave = W == 1 ? 0 : wave_in_block();
+    const int units = 2 * r.h_kv;
+    const int unit = index / units, which = index - unit * units;
+    const bool is_v = which >= r.h_kv;
+    const int head = is_v ? which - r.h_kv : which;
+    PageUnit t;
+    if (!find_unit(a, unit, t)) return;  // the same for all waves of a unit
+    const T* src = (is_v ? r.v : r.k) + head * D;
+    const int64_t stride = is_v ? r.v_stride : r.k_stride;
+    uint8_t* codes = (is_v ? a.v_cache : a.k_cache) + ((((static_cast<int64_t>(t.page) * r.h_kv + head) << r.page_shift)) * D);
+    uint8_t* scale = (is_v ? a.v_scale : a.k_scale) + static_cast<int64_t>(t.page) * r.h_kv + head;
+    const int old = t.first > 0 ? min(static_cast<int>(*scale), kScaleMost) : 0;
+    const int piece = lane % G, c = piece * V, c2 = D / 2 + c;
+
+    // the transformed row's two chunks, 0 beyond the unit's rows
+    const auto load = [&](int row, float (&x)[V], float (&y)[V]) {
+        if (row >= t.rows) {
+#pragma unroll
+            for (int e = 0; e < V; e++) x[e] = y[e] = 0.0f;
+            return;
+        }
+        const T* p = src + (t.token + row) * stride;
+        unpack(ld_stream(p + c), x, T{});
+        unpack(ld_stream(p + c2), y, T{});
+        if (is_v) return;
+        if (NORM && r.kn_w) {
+            float sum = 0.0f, sq = 0.0f;
+#pragma unroll
+            for (int e = 0; e < V; e++) sum += x[e] + y[e];
+            const float mean = lanes_sum<G>(sum) * (1.0f / D);
+#pragma unroll
+            for (int e = 0; e < V; e++) sq = fmaf(x[e] - mean, x[e] - mean, fmaf(y[e] - mean, y[e] - mean, sq));
+            const float inv = rsqrtf(lanes_sum<G>(sq) * (1.0f / D) + r.eps);
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                x[e] = fmaf((x[e] - mean) * inv, r.kn_w[c + e], r.kn_b[c + e]);
+                y[e] = fmaf((y[e] - mean) * inv, r.kn_w[c2 + e], r.kn_b[c2 + e]);
+            }
+        }
+        if constexpr (ROPE) {
+            const int at = r.positions ? r.positions[t.token + row] : t.pos + row;
+            if (at >= 0 && at < r.table_rows) {
+                const float* cr = r.cos_tab + static_cast<int64_t>(at) * D;
+                const float* sr = r.sin_tab + static_cast<int64_t>(at) * D;
+#pragma unroll
+                for (int e = 0; e < V; e++) {
+                    const float u = x[e], v = y[e];
+                    x[e] = fmaf(u, cr[c + e], -(v * sr[c + e]));
+                    y[e] = fmaf(v, cr[c2 + e], u * sr[c2 + e]);
+                }
+            }
+        }
+    };
+    const auto most_of = [&](float most, const float (&x)[V]) {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const float m = fabsf(x[e]);
+            most = fmaxf(most, m < INFINITY ? m : 0.0f);
+        }
+        return most;
+    };
+    const auto held = [&](float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -kHeldMost<T>), kHeldMost<T>) : x; };
+    const auto put = [&](int row, const float (&x)[V], const float (&y)[V], float inv) {
+        if (row >= t.rows) return;
+        uint8_t* p = codes + static_cast<int64_t>(t.first + row) * D;
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            const float(&z)[V] = half ? y : x;
+            uint32_t w[V / 4];
+#pragma unroll
+            for (int i = 0; i < V / 4; i++)
+                w[i] = codes_of(held(z[4 * i]) * inv, held(z[4 * i + 1]) * inv, held(z[4 * i + 2]) * inv, held(z[4 * i + 3]) * inv);
+            uint32_t* at = reinterpret_cast<uint32_t*>(p + (half ? c2 : c));
+            if constexpr (V == 8)
+                *reinterpret_cast<u32x2*>(at) = u32x2{w[0], w[1]};
+            else
+                *at = w[0];
+        }
+    };
+
+    // the first of the wave's rows in round `round`, and of its i-th load's for this lane
+    const auto row_of = [&](int round, int i) { return (round * W + wave) * kHeld + i * kRows + lane / G; };
+    float x[P][V], y[P][V], most = 0.0f;
+    const int rounds = W == 1 ? 1 : (t.rows + kHeld * W - 1) / (kHeld * W);
+    for (int round = rounds - 1; round >= 0; round--)
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            load(row_of(round, i), x[i], y[i]);
+            most = most_of(most_of(most, x[i]), y[i]);
+        }
+    most = wave_max(most);
+    if constexpr (W > 1) {
+        if (lane == 0) tops[wave] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < W; w++) most = fmaxf(most, tops[w]);
+    }
+    const int next = max(old, scale_for(fminf(most, kHeldMost<T>)));
+    const float inv = scale_value(2 * kScaleBias - next);
+    for (int round = 0; round < rounds; round++)
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            if (round > 0) load(row_of(round, i), x[i], y[i]);
+            put(row_of(round, i), x[i], y[i], inv);
+        }
+    if (t.first > 0 && next > old) {
+        for (int i = (wave * 64 + lane) * 16; i < t.first * D; i += W * 1024) {
+            u32x4 w = ld16(codes + i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = codes_down(w[e], next - old);
+            st16(codes + i, w);
+        }
+    }
+    // (each wave has read the old scale: through the barrier above, or it is alone)
+    if (wave == 0 && lane == 0) *scale = static_cast<uint8_t>(next);
+}
+
+template <typename T, int D, bool NORM, bool ROPE, int W>
+__global__ __launch_bounds__(256) void kv_append_f8_kernel(Append8Args<T> a) {
+    const int block = blockIdx.x;
+    if (block < a.row_blocks)
+        append_rows<T, D, NORM, ROPE>(a.rows, block * 4 + wave_in_block());
+    else if constexpr (W == 1)
+        append_page<T, D, NORM, ROPE, 1>(a, (block - a.row_blocks) * 4 + wave_in_block());
+    else
+        append_page<T, D, NORM, ROPE, W>(a, block - a.row_blocks);
+}
+
+template <typename T, int D, int W>
+void launch_append_f8(hipStream_t st, const Append8Args<T>& a, uint32_t blocks) {
+    const dim3 grid(blocks);
+    const bool norm = a.rows.qn_w || a.rows.kn_w, rope = a.rows.sin_tab != nullptr;
+    if (norm && rope)
+        kv_append_f8_kernel<T, D, true, true, W><<<grid, dim3(256), 0, st>>>(a);
+    else if (norm)
+        kv_append_f8_kernel<T, D, true, false, W><<<grid, dim3(256), 0, st>>>(a);
+    else if (rope)
+        kv_append_f8_kernel<T, D, false, true, W><<<grid, dim3(256), 0, st>>>(a);
+    else
+        kv_append_f8_kernel<T, D, false, false, W><<<grid, dim3(256), 0, st>>>(a);
+}
+
+// ---------------------------------------------------------------------------
+// attention over the cache
+
+struct Attend8Args {
+    const void* q;
+    const uint8_t *k, *v, *k_scale, *v_scale;
+    void* out;
+    const int *page_table, *lens, *offsets;  // offsets null: one query a sequence
+    int64_t q_stride;
+    int n, b, h, h_kv, page_shift, n_pages, max_pages, causal;
+    float scale;
+};
+
+// A workgroup takes a query and a head, a wave every fourth key: its score, then
+// the running maximum, sum and weighted values.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attend_f8_kernel(Attend8Args a) {
+    constexpr int E = D / 64;  // channels per lane
+    __shared__ float o[4][D], m[4], l[4];
+    const int row = static_cast<int>(blockIdx.x) / a.h, head = static_cast<int>(blockIdx.x) - row * a.h;
+    const int s = a.offsets ? sequence_of(a.offsets, a.b, row) : row;
+    if (s < 0) return;
+    const int kv = head / (a.h / a.h_kv), lane = lane_id(), wave = wave_in_block();
+    const int len = max(a.lens[s], 0), held = held_length(a.lens, s, a.max_pages, a.page_shift);
+    int seen = held;
+    if (a.offsets && a.causal) {
+        const int at = len - (min(max(a.offsets[s + 1], 0), a.n) - row);
+        const int64_t end = at < 0 ? 0 : (static_cast<int64_t>(at / a.causal) + 1) * a.causal;
+        seen = end < held ? static_cast<int>(end) : held;
+    }
+    float q[E], acc[E] = {}, top = kNone, sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; e++) q[e] = load_elem(static_cast<const T*>(a.q) + row * a.q_stride + head * D + lane * E + e);
+    for (int key = wave; key < seen; key += 4) {
+        const int page = a.page_table[static_cast<int64_t>(s) * a.max_pages + (key >> a.page_shift)];
+        if (page < 0 || page >= a.n_pages) continue;
+        const int64_t block = static_cast<int64_t>(page) * a.h_kv + kv;
+        const int64_t at = ((block << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * D + lane * E;
+        float dot = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) dot = fmaf(q[e], __builtin_amdgcn_cvt_f32_fp8(a.k[at + e], 0) * scale_value(a.k_scale[block]), dot);
+        const float score = as_f32(wave_sum(dot) * (a.scale * 1.4426950408889634f));
+        const float next = fmaxf(fmaxf(top, score), kFloor);
+        const float corr = __builtin_amdgcn_exp2f(top - next), p = __builtin_amdgcn_exp2f(score - next);
+        top = next, sum = fmaf(sum, corr, p);
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] = fmaf(acc[e], corr, p * (__builtin_amdgcn_cvt_f32_fp8(a.v[at + e], 0) * scale_value(a.v_scale[block])));
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) o[wave][lane * E + e] = acc[e];
+    if (lane == 0) m[wave] = top, l[wave] = sum;
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+    float x = 0.0f, w = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float f = __builtin_amdgcn_exp2f(m[i] - top);
+        x = fmaf(o[i][threadIdx.x], f, x), w = fmaf(l[i], f, w);
+    }
+    store_elem(static_cast<T*>(a.out) + (static_cast<int64_t>(row) * a.h + head) * D + threadIdx.x, top == kNone ? 0.0f : x / w);
+}
+
+hs_status check_attend(const char* op, hs_dtype dt, const Attend8Args& a, int d, int page, const void* workspace,
+                       int64_t workspace_bytes, int64_t need) {
+    const int64_t width = static_cast<int64_t>(a.h) * d, e = dtype_size(dt);
+    if (hs_status rc = check_rows(op, "q", a.q, a.n, a.q_stride, width, dt)) return rc;
+    if (!a.out) return fail(HS_EINVAL, "%s: null out", op);
+    if (hs_status rc = check_cache_f8(op, a.k, a.v, a.k_scale, a.v_scale, a.page_table, a.lens, page, a.n_pages, a.max_pages, a.h_kv, d)) return rc;
+    if (!aligned16(a.out) || !aligned16(workspace)) return fail(HS_EUNSUPPORTED, "%s: out and workspace must be 16-byte aligned", op);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(HS_EINVAL, "%s: workspace of %lld bytes, %lld needed", op, static_cast<long long>(workspace_bytes), static_cast<long long>(need));
+    const int64_t cache = static_cast<int64_t>(a.n_pages) * page * a.h_kv * d, scales = static_cast<int64_t>(a.n_pages) * a.h_kv;
+    const struct {
+        const void* p;
+        int64_t bytes;
+    } in[5] = {{a.q, row_bytes(a.n, a.q_stride, width, dt)}, {a.k, cache}, {a.v, cache}, {a.k_scale, scales}, {a.v_scale, scales}};
+    for (const auto& r : in) {
+        if (overlaps(a.out, a.n * width * e, r.p, r.bytes)) return fail(HS_EINVAL, "%s: out overlaps another buffer", op);
+        if (overlaps(workspace, need, r.p, r.bytes)) return fail(HS_EINVAL, "%s: workspace overlaps an input", op);
+    }
+    if (overlaps(a.out, a.n * width * e, workspace, need)) return fail(HS_EINVAL, "%s: out overlaps another buffer", op);
+    if (!std::isfinite(a.scale)) return fail(HS_EINVAL, "%s: scale must be finite", op);
+    return HS_OK;
+}
+
+void launch_attend(hipStream_t st, hs_dtype dt, int d, const Attend8Args& a) {
+    const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.n) * a.h));
+    if (dt == HS_F16)
+        (d == 64 ? attend_f8_kernel<f16, 64> : attend_f8_kernel<f16, 128>)<<<grid, dim3(256), 0, st>>>(a);
+    else
+        (d == 64 ? attend_f8_kernel<float, 64> : attend_f8_kernel<float, 128>)<<<grid, dim3(256), 0, st>>>(a);
+}
+
+}  // namespace
+}  // namespace hs
+
+extern "C" hs_status hs_kv_append_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride, const void* k,
+                                     int64_t k_stride, const void* v, int64_t v_stride, const float* qn_w,
+                                     const float* qn_b, const float* kn_w, const float* kn_b, const float* sin_tab,
+                                     const float* cos_tab, int32_t table_rows, const void* positions,
+                                     const void* offsets, const void* page_table, const void* lens, void* q_out,
+                                     void* k_out, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                                     int64_t n, int32_t b, int32_t h, int32_t h_kv, int32_t d, int32_t page,
+                                     int32_t n_pages, int32_t max_pages, float eps) {
+    using namespace hs;
+    const char* op = "kv_append_f8";
+    AppendCall c{q, k, v, q_stride, k_stride, v_stride, qn_w, qn_b, kn_w, kn_b, sin_tab, cos_tab, table_rows, positions,
+                 offsets, page_table, lens, q_out, k_out, n, b, h, h_kv, d, page, n_pages, max_pages, eps};
+    bool done = false;
+    if (hs_status rc = check_append(op, dt, c, done)) return rc;
+    if (done) return HS_OK;
+    if (hs_status rc = check_cache_f8(op, k_cache, v_cache, k_scale, v_scale, page_table, lens, page, n_pages, max_pages, h_kv, d)) return rc;
+    const int64_t cache = static_cast<int64_t>(n_pages) * page * h_kv * d, scales = static_cast<int64_t>(n_pages) * h_kv;
+    const ByteRange outs[6] = {c.q_rows(dt), c.k_rows(dt), {k_cache, cache}, {v_cache, cache}, {k_scale, scales}, {v_scale, scales}};
+    if (hs_status rc = check_append_overlaps(op, dt, c, outs, 6)) return rc;
+    // rows of q, and of k where they are asked for: waves as kv_append's
+    const int64_t heads = static_cast<int64_t>(c.h) + (k_out ? h_kv : 0);
+    const int parts = static_cast<int>(ceil_div(heads, dt == HS_F16 ? 1024 / d : 512 / d));
+    const int64_t row_blocks = ceil_div(n * parts, 4);
+    // pages that the tokens can lie in, at most
+    const bool wide = offsets && page > 2048 / d;
+    const int64_t pages = (offsets ? n / page + 2 * std::min<int64_t>(b, n) : b) * 2 * h_kv;
+    const int64_t page_blocks = wide ? pages : ceil_div(pages, 4);
+    if (row_blocks + page_blocks >= (int64_t{1} << 24)) return fail(HS_EINVAL, "%s: too many tokens", op);
+    const auto run = [&](auto zero) {
+        using T = decltype(zero);
+        Append8Args<T> a;
+        c.fill(a.rows);
+        a.rows.parts = parts, a.rows.heads = static_cast<int>(heads);
+        a.rows.k_cache = a.rows.v_cache = nullptr, a.rows.n_pages = 0;  // rows only
+        a.offsets = static_cast<const int*>(offsets), a.page_table = static_cast<const int*>(page_table);
+        a.lens = static_cast<const int*>(lens);
+        a.k_cache = static_cast<uint8_t*>(k_cache), a.v_cache = static_cast<uint8_t*>(v_cache);
+        a.k_scale = static_cast<uint8_t*>(k_scale), a.v_scale = static_cast<uint8_t*>(v_scale);
+        a.n_pages = n_pages, a.row_blocks = static_cast<int>(row_blocks);
+        const auto st = static_cast<hipStream_t>(stream);
+        const uint32_t blocks = static_cast<uint32_t>(row_blocks + page_blocks);
+        if (d == 64)
+            wide ? launch_append_f8<T, 64, 4>(st, a, blocks) : launch_append_f8<T, 64, 1>(st, a, blocks);
+        else
+            wide ? launch_append_f8<T, 128, 4>(st, a, blocks) : launch_append_f8<T, 128, 1>(st, a, blocks);
+    };
+    if (dt == HS_F16)
+        run(f16{});
+    else
+        run(float{});
+    return check_launch(op);
+}
+
+extern "C" int64_t hs_attention_paged_f8_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d) {
+    return hs_attention_paged_workspace(b, h, h_kv, d);
+}
+
+extern "C" hs_status hs_attention_paged_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                                           const void* k_cache, const void* v_cache, const void* k_scale,
+                                           const void* v_scale, const void* page_table, const void* lens, void* out,
+                                           void* workspace, int64_t workspace_bytes, int32_t b, int32_t h,
+                                           int32_t h_kv, int32_t d, int32_t page, int32_t n_pages, int32_t max_pages,
+                                           float scale) {
+    using namespace hs;
+    const char* op = "attention_paged_f8";
+    if (hs_status rc = check_heads(op, dt, h, h_kv, d)) return rc;
+    if (b < 0) return fail(HS_EINVAL, "%s: negative count", op);
+    if (b == 0 || h == 0) return HS_OK;
+    if (static_cast<int64_t>(b) * h >= (int64_t{1} << 23)) return fail(HS_EINVAL, "%s: b * Hq must be below 2^23", op);
+    Attend8Args a;
+    a.q = q, a.q_stride = q_stride, a.out = out;
+    a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
+    a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
+    a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens), a.offsets = nullptr;
+    a.n = b, a.b = b, a.h = h, a.h_kv = h_kv, a.n_pages = n_pages, a.max_pages = max_pages, a.causal = 0, a.scale = scale;
+    if (hs_status rc = check_attend(op, dt, a, d, page, workspace, workspace_bytes, hs_attention_paged_f8_workspace(b, h, h_kv, d))) return rc;
+    a.page_shift = exact_log2(page);
+    if (n_pages == 0) a.max_pages = 0;  // no page to read: no sequence has keys
+    launch_attend(static_cast<hipStream_t>(stream), dt, d, a);
+    return check_launch(op);
+}
+
+extern "C" int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int32_t b, int32_t h, int32_t h_kv,
+                                                     int32_t d, int32_t page, int32_t max_pages, int32_t causal) {
+    return 0;
+}
+
+extern "C" hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                                             const void* k_cache, const void* v_cache, const void* k_scale,
+                                             const void* v_scale, const void* page_table, const void* lens,
+                                             const void* offsets, void* out, void* workspace, int64_t workspace_bytes,
+                                             int64_t n, int32_t b, int32_t h, int32_t h_kv, int32_t d, int32_t page,
+                                             int32_t n_pages, int32_t max_pages, int32_t causal, float scale) {
+    using namespace hs;
+    const char* op = "attention_prompts_f8";
+    if (hs_status rc = check_heads(op, dt, h, h_kv, d)) return rc;
+    if (n < 0 || b < 0) return fail(HS_EINVAL, "%s: negative count", op);
+    if (causal < 0) return fail(HS_EINVAL, "%s: causal %d", op, causal);
+    if (n == 0 || b == 0 || h == 0) return HS_OK;
+    if (n >= (int64_t{1} << 30) / h) return fail(HS_EINVAL, "%s: n * Hq must be below 2^30", op);
+    if (!offsets) return fail(HS_EINVAL, "%s: null offsets", op);
+    Attend8Args a;
+    a.q = q, a.q_stride = q_stride, a.out = out;
+    a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
+    a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
+    a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens), a.offsets = static_cast<const int*>(offsets);
+    a.n = static_cast<int>(n), a.b = b, a.h = h, a.h_kv = h_kv, a.n_pages = n_pages, a.max_pages = max_pages, a.causal = causal, a.scale = scale;
+    if (hs_status rc = check_attend(op, dt, a, d, page, workspace, workspace_bytes,
+                                    hs_attention_prompts_f8_workspace(dt, n, b, h, h_kv, d, page, max_pages, causal))) return rc;
+    a.page_shift = exact_log2(page);
+    if (n_pages == 0) a.max_pages = 0;
+    launch_attend(static_cast<hipStream_t>(stream), dt, d, a);
+    return check_launch(op);
+}

@@ -458,6 +458,93 @@ hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int
                              int32_t d, int32_t page, int32_t n_pages, int32_t max_pages,
                              float scale);
 
+/* The same cache held in 8 bits: k_cache and v_cache (n_pages, Hkv, page, D)
+ * of e4m3 codes (1, 4 and 3 bits; no infinities), k_scale and v_scale (n_pages,
+ * Hkv) of one byte each, c standing for 2^(c - 127) (E8M0, c from 10 to 247): a
+ * value is its code's times its page's and head's scale. dt is the type of the
+ * rows beside it. The rules for lengths, offsets and pages are those above. */
+
+/* hs_kv_append into such a cache; q_out and k_out are as there. The new keys (and
+ * values) of a page and head share a scale: the least 2^e, e >= -117, that brings
+ * the largest finite magnitude among them to 448 or less; where the call goes on
+ * with a page, the larger of that and the page's own, to which the codes of the
+ * page's rows before them are brought (times a power of two, rounded again where
+ * that leaves fewer bits). A code is the f32 value over the scale rounded to
+ * nearest even. Magnitudes past 61440 (HS_F16) or 15/8 2^127 (HS_F32) are held as
+ * that; infinities and NaN as NaN. Whoever begins a page sets its scale, so the
+ * pages of a new sequence need no values. No page takes new tokens of two
+ * sequences in one call. */
+hs_status hs_kv_append_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                          const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          const float* qn_w, const float* qn_b, const float* kn_w,
+                          const float* kn_b, const float* sin_tab, const float* cos_tab,
+                          int32_t table_rows, const void* positions, const void* offsets,
+                          const void* page_table, const void* lens, void* q_out, void* k_out,
+                          void* k_cache, void* v_cache, void* k_scale, void* v_scale, int64_t n,
+                          int32_t b, int32_t h, int32_t h_kv, int32_t d, int32_t page,
+                          int32_t n_pages, int32_t max_pages, float eps);
+
+/* Bytes of workspace that hs_attention_paged_f8 takes for b sequences on the
+ * current device; 0 for shapes that it refuses. */
+int64_t hs_attention_paged_f8_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d);
+
+/* hs_attention_paged over such a cache. */
+hs_status hs_attention_paged_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                                const void* k_cache, const void* v_cache, const void* k_scale,
+                                const void* v_scale, const void* page_table, const void* lens,
+                                void* out, void* workspace, int64_t workspace_bytes, int32_t b,
+                                int32_t h, int32_t h_kv, int32_t d, int32_t page, int32_t n_pages,
+                                int32_t max_pages, float scale);
+
+/* Bytes of workspace that hs_attention_prompts_f8 takes on the current device; 0
+ * for shapes that it refuses, and for those whose keys are not split. */
+int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int32_t b, int32_t h, int32_t h_kv,
+                                          int32_t d, int32_t page, int32_t max_pages,
+                                          int32_t causal);
+
+/* Attention of several new tokens per sequence over such a cache, which holds
+ * their own keys already: q (n, Hq*D) at offsets (b + 1) -> out (n, Hq*D). The
+ * last of sequence s's tokens is key lens[s] - 1; causal is as for
+ * hs_attention_packed, groups counted from key 0. A token that sees no key gets
+ * zeros, rows of no sequence are not written. Keys and values that a token does
+ * not see do not enter its result, whatever they hold. workspace is as for
+ * hs_attention_paged. */
+hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                                  const void* k_cache, const void* v_cache, const void* k_scale,
+                                  const void* v_scale, const void* page_table, const void* lens,
+                                  const void* offsets, void* out, void* workspace,
+                                  int64_t workspace_bytes, int64_t n, int32_t b, int32_t h,
+                                  int32_t h_kv, int32_t d, int32_t page, int32_t n_pages,
+                                  int32_t max_pages, int32_t causal, float scale);
+
+/* Bytes of workspace that hs_plan_pages takes; 0 for calls of one launch. */
+int64_t hs_plan_pages_workspace(int64_t n, int32_t b, int32_t max_pages);
+
+/* Hands pages out and takes them back: sequence s grows by counts[s] tokens, or
+ * drops -counts[s] of its last (at most all it has). lens (b) and page_table (b,
+ * max_pages) are brought up to date: entries for the pages that a sequence now
+ * needs are filled, those that it no longer needs become -1. Free pages lie in a
+ * ring, free (n_pages), state[1] of them from place state[0] on: the call takes
+ * them from its front, in the order of the sequences and their entries, and gives
+ * dropped ones back behind its end, in the same order, to be taken from the next
+ * call on. state[2] becomes the pages that were needed and not there (none free,
+ * or past the table's width): such entries are -1, tokens there have no place, and
+ * a sequence gets no pages behind one until it has dropped it. Every entry below a
+ * sequence's length is a page of its own, up to the first that was not there. A
+ * length is held to 2^30.
+ *
+ * offsets (b + 1) become the new tokens' rows by sequence, 0 for those that drop;
+ * positions (n) int32 and slots (n) int64, either NULL, each new token's key
+ * number, and page * page size + row, -1 without a place. Rows past n or behind the
+ * last sequence are not written. Arrays are int32 but for slots and overlap nothing
+ * else; workspace (16-byte aligned) holds nothing between calls. Two calls on the
+ * same state must not run at the same time. HS_EINVAL at 2^30 for n, b, n_pages and
+ * max_pages * page, 2^31 for b * max_pages. */
+hs_status hs_plan_pages(hs_stream_t stream, const void* counts, void* lens, void* page_table,
+                        void* free, void* state, void* offsets, void* positions, void* slots,
+                        void* workspace, int64_t workspace_bytes, int64_t n, int32_t b,
+                        int32_t page, int32_t n_pages, int32_t max_pages);
+
 /* ---------------------------------------------------------------------- */
 /* Host-side RoPE tables (computed once per session, as the reference does) */
 

@@ -158,6 +158,26 @@ struct PagedKV {
     size_t sequences, max_pages;
 };
 
+// The same held in 8 bits (headshot_hip.h): e4m3 codes k and v (n_pages, heads,
+// page, d) and scales (n_pages, heads), one byte each, all the caller's; dtype is
+// the type of the rows beside it.
+struct PagedKV8 {
+    void *k, *v, *k_scale, *v_scale;
+    Dtype dtype;
+    size_t n_pages, heads, page, d;
+    const int32_t* page_table;
+    const int32_t* lens;
+    size_t sequences, max_pages;
+};
+
+// The pages of caches that share page_table (sequences, max_pages) and lens
+// (sequences): free pages in a ring, free (n_pages) and state (3), int32 device
+// arrays that the caller owns (headshot_hip.h, hs_plan_pages).
+struct PagePool {
+    int32_t *page_table, *lens, *free, *state;
+    size_t sequences, max_pages, n_pages, page;
+};
+
 // RoPE tables + unrotated prefix for one attention call (model/block.rs:42-47).
 struct Rope {
     const HipTensor* sin;
@@ -471,6 +491,43 @@ class HipContext {
         return {std::move(q_out), std::move(k_out)};
     }
 
+    // The same into a cache held in 8 bits (hs_kv_append_f8).
+    std::pair<HipTensor, HipTensor> kv_append(const PagedKV8& cache, const HipTensor* q, const HipTensor& k,
+                                              const HipTensor& v, const int32_t* offsets,
+                                              const Norm* qn = nullptr, const Norm* kn = nullptr,
+                                              const HipTensor* sin = nullptr, const HipTensor* cos = nullptr,
+                                              const int32_t* positions = nullptr, float eps = 1e-5f,
+                                              bool k_rows = false) const {
+        const size_t d = cache.d, width = cache.heads * d;
+        const Dtype dt = cache.dtype;
+        HS_REQUIRE(width > 0 && k.dtype() == dt && v.dtype() == dt && k.last() == width && v.len() == k.len(),
+                   "kv_append: k and v must be (n, heads * d) in the cache's dtype");
+        const size_t n = k.len() / width;
+        size_t qw = 0;
+        if (q) {
+            qw = q->last();
+            HS_REQUIRE(q->dtype() == dt && qw % d == 0 && q->len() == n * qw, "kv_append: q must be (n, heads * d)");
+        }
+        for (const Norm* norm : {qn, kn})
+            if (norm) ln_params(*norm, d);
+        HS_REQUIRE(!sin == !cos, "kv_append: sin and cos go together");
+        if (sin)
+            HS_REQUIRE(sin->dtype() == Dtype::F32 && cos->dtype() == Dtype::F32 && sin->last() == d &&
+                           cos->len() == sin->len(), "kv_append: tables must be f32 (rows, d)");
+        HipTensor q_out = empty_typed({q ? n : 0, qw}, dt), k_out = empty_typed({k_rows ? n : 0, width}, dt);
+        check(hs_kv_append_f8(stream_, hs_dtype(dt), q ? q->data() : nullptr, static_cast<int64_t>(qw), k.data(),
+                              static_cast<int64_t>(width), v.data(), static_cast<int64_t>(width),
+                              qn ? qn->weight->f32() : nullptr, qn ? qn->bias->f32() : nullptr,
+                              kn ? kn->weight->f32() : nullptr, kn ? kn->bias->f32() : nullptr,
+                              sin ? sin->f32() : nullptr, cos ? cos->f32() : nullptr,
+                              sin ? i32(sin->len() / d) : 0, positions, offsets, cache.page_table, cache.lens,
+                              q_out.data(), k_out.data(), cache.k, cache.v, cache.k_scale, cache.v_scale,
+                              static_cast<int64_t>(n), i32(cache.sequences), i32(qw / d), i32(cache.heads), i32(d),
+                              i32(cache.page), i32(cache.n_pages), i32(cache.max_pages), eps),
+              "kv_append");
+        return {std::move(q_out), std::move(k_out)};
+    }
+
     // Attention of packed sequences (hs_attention_packed): q (n, heads * d), k,
     // v (m, kv_heads * d), offsets (sequences + 1) int32 on the device.
     HipTensor attention_packed(const HipTensor& q, const HipTensor& k, const HipTensor& v, size_t d,
@@ -514,6 +571,60 @@ class HipContext {
                                  1.0f / std::sqrt(static_cast<float>(d))),
               "attention_paged");
         return out;
+    }
+
+    // The same over a cache held in 8 bits (hs_attention_paged_f8).
+    HipTensor attention_paged(const HipTensor& q, const PagedKV8& cache) const {
+        const size_t d = cache.d;
+        HS_REQUIRE(q.dtype() == cache.dtype, "attention_paged: dtype");
+        HS_REQUIRE(d > 0 && q.last() % d == 0 && q.len() == cache.sequences * q.last(),
+                   "attention_paged: q must be (sequences, heads * d)");
+        const int32_t b = i32(cache.sequences), h = i32(q.last() / d), h_kv = i32(cache.heads);
+        const int64_t bytes = hs_attention_paged_f8_workspace(b, h, h_kv, i32(d));
+        HipTensor out = empty_typed({cache.sequences, q.last()}, q.dtype());
+        HipTensor ws = empty_typed({static_cast<size_t>(bytes + 3) / 4}, Dtype::F32);
+        check(hs_attention_paged_f8(stream_, hs_dtype(q.dtype()), q.data(), static_cast<int64_t>(q.last()), cache.k,
+                                    cache.v, cache.k_scale, cache.v_scale, cache.page_table, cache.lens, out.data(),
+                                    ws.data(), bytes, b, h, h_kv, i32(d), i32(cache.page), i32(cache.n_pages),
+                                    i32(cache.max_pages), 1.0f / std::sqrt(static_cast<float>(d))),
+              "attention_paged");
+        return out;
+    }
+
+    // Attention of several new tokens per sequence over a cache held in 8 bits
+    // (hs_attention_prompts_f8): q (n, heads * d), offsets (sequences + 1) int32 on
+    // the device.
+    HipTensor attention_paged_prompts(const HipTensor& q, const PagedKV8& cache, const int32_t* offsets,
+                                      int32_t causal = 1) const {
+        const size_t d = cache.d;
+        HS_REQUIRE(q.dtype() == cache.dtype, "attention_paged_prompts: dtype");
+        HS_REQUIRE(d > 0 && q.last() > 0 && q.last() % d == 0, "attention_paged_prompts: q must be (n, heads * d)");
+        const size_t n = q.len() / q.last();
+        const int32_t b = i32(cache.sequences), h = i32(q.last() / d), h_kv = i32(cache.heads);
+        const int64_t bytes = hs_attention_prompts_f8_workspace(hs_dtype(q.dtype()), static_cast<int64_t>(n), b, h, h_kv,
+                                                                i32(d), i32(cache.page), i32(cache.max_pages), causal);
+        HipTensor out = empty_typed({n, q.last()}, q.dtype());
+        HipTensor ws = empty_typed({static_cast<size_t>(bytes + 3) / 4}, Dtype::F32);
+        check(hs_attention_prompts_f8(stream_, hs_dtype(q.dtype()), q.data(), static_cast<int64_t>(q.last()), cache.k,
+                                      cache.v, cache.k_scale, cache.v_scale, cache.page_table, cache.lens, offsets,
+                                      out.data(), ws.data(), bytes, static_cast<int64_t>(n), b, h, h_kv, i32(d),
+                                      i32(cache.page), i32(cache.n_pages), i32(cache.max_pages), causal,
+                                      1.0f / std::sqrt(static_cast<float>(d))),
+              "attention_paged_prompts");
+        return out;
+    }
+
+    // Hands out the pages of a call's new tokens and takes back dropped ones'
+    // (hs_plan_pages): counts (sequences), offsets (sequences + 1) and, null or
+    // not, positions (n) int32, slots (n) int64, on the device.
+    void plan_pages(const PagePool& pool, const int32_t* counts, size_t n, int32_t* offsets, int32_t* positions,
+                    int64_t* slots) const {
+        const int32_t b = i32(pool.sequences), width = i32(pool.max_pages);
+        const int64_t bytes = hs_plan_pages_workspace(static_cast<int64_t>(n), b, width);
+        HipTensor ws = empty_typed({static_cast<size_t>(bytes + 3) / 4}, Dtype::F32);
+        check(hs_plan_pages(stream_, counts, pool.lens, pool.page_table, pool.free, pool.state, offsets, positions, slots,
+                            ws.data(), bytes, static_cast<int64_t>(n), b, i32(pool.page), i32(pool.n_pages), width),
+              "plan_pages");
     }
 
     // engine/ops.rs:336-348

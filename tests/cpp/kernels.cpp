@@ -568,6 +568,58 @@ void paged_step_continues_a_prompt(HipContext& ctx) {
     hs::hip_check(hipFree(dev), "hipFree");
 }
 
+// Pages handed out, a prompt and a step over a cache in 8 bits: the step's
+// attention is the prompts' attention of the same token.
+void eight_bit_cache_step_is_a_prompt_row(HipContext& ctx) {
+    const size_t h = 4, h_kv = 2, d = 64, page = 16, pages = 8, b = 2, width = 4, n = 27;
+    const size_t codes = pages * h_kv * page * d, scales = pages * h_kv;
+    const size_t ints = b * width + b + pages + 3 + 2 * b + (b + 1) + n;
+    int32_t* dev = nullptr;
+    int64_t* slots = nullptr;
+    uint8_t* bytes = nullptr;
+    hs::hip_check(hipMalloc(&dev, ints * sizeof(int32_t)), "hipMalloc");
+    hs::hip_check(hipMalloc(&slots, n * sizeof(int64_t)), "hipMalloc");
+    hs::hip_check(hipMalloc(&bytes, 2 * (codes + scales)), "hipMalloc");
+    int32_t* table = dev;
+    int32_t* lens = table + b * width;
+    int32_t* free_pages = lens + b;
+    int32_t* state = free_pages + pages;
+    int32_t* counts = state + 3;
+    int32_t* offsets = counts + 2 * b;
+    int32_t* positions = offsets + b + 1;
+    Rng rng{79};
+    for (Dtype dt : {Dtype::F32, Dtype::F16}) {
+        std::vector<int32_t> init(ints, -1);
+        for (size_t s = 0; s < b; s++) init[b * width + s] = 0;
+        for (size_t i = 0; i < pages; i++) init[b * width + b + i] = static_cast<int32_t>((i * 3 + 1) % pages);
+        const size_t at = b * width + b + pages;
+        init[at] = 0, init[at + 1] = pages, init[at + 2] = 0;
+        init[at + 3] = 20, init[at + 4] = 7, init[at + 5] = 1, init[at + 6] = 1;
+        hs::hip_check(hipMemcpy(dev, init.data(), ints * sizeof(int32_t), hipMemcpyHostToDevice), "hipMemcpy");
+        const hs::PagePool pool{table, lens, free_pages, state, b, width, pages, page};
+        const hs::PagedKV8 cache{bytes, bytes + codes, bytes + 2 * codes, bytes + 2 * codes + scales, dt, pages, h_kv,
+                                 page, d, table, lens, b, width};
+        const auto rows = [&](size_t count, size_t heads) { return ctx.tensor_from_f32({count, heads * d}, rng.vec(count * heads * d), dt); };
+        const auto k = rows(n, h_kv), v = rows(n, h_kv), k1 = rows(b, h_kv), v1 = rows(b, h_kv), q1 = rows(b, h);
+        ctx.plan_pages(pool, counts, n, offsets, positions, slots);
+        ctx.kv_append(cache, nullptr, k, v, offsets);
+        ctx.plan_pages(pool, counts + b, b, offsets, positions, slots);
+        ctx.kv_append(cache, nullptr, k1, v1, nullptr);
+        const auto step = ctx.download(ctx.attention_paged(q1, cache));
+        const auto prompt = ctx.download(ctx.attention_paged_prompts(q1, cache, offsets));
+        for (size_t i = 0; i < b * h * d; i++)
+            // both are off by at most their type's roundings (values below 4)
+            if (!(std::fabs(step[i] - prompt[i]) <= (dt == Dtype::F32 ? 1e-5f : 1.6e-2f))) throw Failure("step differs from the prompt's row");
+        std::vector<int32_t> after(ints);
+        hs::hip_check(hipMemcpy(after.data(), dev, ints * sizeof(int32_t), hipMemcpyDeviceToHost), "hipMemcpy");
+        if (after[b * width] != 21 || after[b * width + 1] != 8 || after[at + 1] != static_cast<int32_t>(pages) - 3)
+            throw Failure("plan_pages: lengths or free pages");
+    }
+    hs::hip_check(hipFree(dev), "hipFree");
+    hs::hip_check(hipFree(slots), "hipFree");
+    hs::hip_check(hipFree(bytes), "hipFree");
+}
+
 void contract_violations_throw(HipContext& ctx) {
     auto x = ctx.tensor_from_slice({4, 8}, std::vector<float>(32, 1.0f));
     auto w = ctx.tensor_from_slice({7}, std::vector<float>(7, 1.0f));
@@ -608,6 +660,7 @@ int main(int argc, char** argv) {
         {"layernorm_prologue_equals_sequence", layernorm_prologue_equals_sequence},
         {"paged_step_continues_a_prompt", paged_step_continues_a_prompt},
         {"packed_token_over_many_keys", packed_token_over_many_keys},
+        {"eight_bit_cache_step_is_a_prompt_row", eight_bit_cache_step_is_a_prompt_row},
         {"contract_violations_throw", contract_violations_throw},
     };
     HipContext ctx;
