@@ -51,16 +51,6 @@ void launch_append(hipStream_t st, const AppendArgs<T>& a) {
 // out. Lengths are device data: each workgroup computes chunk and finds its
 // piece from all of them (64 a step).
 
-// f16: a weight goes to the product with V as two f16 values, its 11 leading bits
-// and the next 11, which makes the product as good as one of f32 weights (errors
-// against 64 bits 2.5e-4 with the leading bits alone, 2.0e-4 so, which is the
-// result's rounding) for 1-2% of the time. The largest weight of a step is this
-// unit, so that the others, f16 being subnormal below 2^-14, are 2^-40 of it off at
-// most (of a unit of 1, 45% at a score 17 nats below). The second part times an
-// infinity is NaN or the other infinity: a step that has one among its values
-// leaves the second parts out.
-constexpr float kHalfUnit = 32768.0f;
-
 template <typename T, int D>
 struct Paged {
     static constexpr bool kHalf = sizeof(T) == 2;
@@ -317,37 +307,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_p
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    // join the waves
-    __syncthreads();
-    if (n < live_heads) {
-#pragma unroll
-        for (int i = 0; i < DB; i++) *reinterpret_cast<f32x4*>(&sm.o[wave][n * P::kOPitch + 16 * i + 4 * g]) = o[i];
-        if (g == 0) sm.m[wave][n] = m, sm.l[wave][n] = l;
-    }
-    __syncthreads();
-    for (int x = threadIdx.x; x < live_heads * (D / 4); x += 64 * kPagedWaves) {
-        const int head = x / (D / 4), d0 = x % (D / 4) * 4;
-        float top = sm.m[0][head];
-#pragma unroll
-        for (int w = 1; w < kPagedWaves; w++) top = fmaxf(top, sm.m[w][head]);
-        f32x4 sum = {};
-        float weight = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kPagedWaves; w++) {
-            const float f = __builtin_amdgcn_exp2f(sm.m[w][head] - top);
-            sum += *reinterpret_cast<const f32x4*>(&sm.o[w][head * P::kOPitch + d0]) * f;
-            weight = fmaf(sm.l[w][head], f, weight);
-        }
-        if (count == 1) {
-            T* orow = static_cast<T*>(a.out) + (static_cast<int64_t>(s) * a.h + head0 + head) * D + d0;
-#pragma unroll
-            for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(top == kNone ? 0.0f : sum[e] / weight);
-        } else {
-            const int64_t row = static_cast<int64_t>(blockIdx.x) * a.width + head;
-            *reinterpret_cast<f32x4*>(a.ws_o + row * D + d0) = sum;
-            if (d0 == 0) a.ws_ml[2 * row] = top, a.ws_ml[2 * row + 1] = weight;
-        }
-    }
+    join_waves<T, D>(a, sm, s, count, head0, live_heads, o, m, l);
 }
 
 // f32, a key head of one query head (no sharing): the matrix instructions would
@@ -517,31 +477,6 @@ __global__ __launch_bounds__(64 * kPagedWaves, 4) void paged_single_kernel(Paged
         *reinterpret_cast<f32x4*>(a.ws_o + row * D + d0) = sum;
         if (d0 == 0) a.ws_ml[2 * row] = top, a.ws_ml[2 * row + 1] = weight;
     }
-}
-
-template <typename T, int D, typename K>
-hs_status launch_pieces(const char* op, hipStream_t st, PagedArgs a, K whole, K rows, int unit, int per_cu) {
-    const PagedPlan plan(a.b, a.h, a.h_kv, per_cu);
-    a.ws_ml = a.ws_o + plan.rows * D;
-    a.ws_cut = reinterpret_cast<int*>(a.ws_ml + 2 * plan.rows);
-    a.group = plan.group, a.passes = plan.passes, a.width = plan.width;
-    // (rounded up by twice the error of the kernels' sum over the lengths)
-    a.per_round = static_cast<float>((1.0 + (a.b / 64 + 64) * 0x1p-23) / static_cast<double>(plan.ranges));
-    // no more pieces than a table's width of keys has, either
-    const int64_t most = ceil_div(static_cast<int64_t>(a.max_pages) << a.page_shift, int64_t{unit});
-    const int64_t items = a.b * plan.heads * (most > 1 ? most : 1);
-    const dim3 grid(static_cast<uint32_t>(items < plan.items ? items : plan.items));
-    (a.page_shift >= 4 ? whole : rows)<<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
-    if (hs_status rc = check_launch(op)) return rc;
-    if (most <= 1) return HS_OK;  // no sequence has two pieces
-    const int64_t joined = static_cast<int64_t>(a.b) * a.h;
-    const dim3 joins(static_cast<uint32_t>(joined));
-    // few rows may have a thousand pieces each
-    if (joined <= 64)
-        paged_join_kernel<T, D, 1024><<<joins, dim3(1024), 0, st>>>(a);
-    else
-        paged_join_kernel<T, D, 256><<<joins, dim3(256), 0, st>>>(a);
-    return check_launch(op);
 }
 
 template <typename T, int D>

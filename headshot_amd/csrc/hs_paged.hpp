@@ -199,6 +199,16 @@ constexpr int kPagedWaves = 4;
 constexpr float kNone = -3.0e38f;   // a running maximum that has seen no key
 constexpr float kFloor = -2.9e38f;  // the least of one that has
 
+// f16: a weight goes to the product with V as two f16 values, its 11 leading bits
+// and the next 11, which makes the product as good as one of f32 weights (errors
+// against 64 bits 2.5e-4 with the leading bits alone, 2.0e-4 so, which is the
+// result's rounding) for 1-2% of the time. The largest weight of a step is this
+// unit, so that the others, f16 being subnormal below 2^-14, are 2^-40 of it off at
+// most (of a unit of 1, 45% at a score 17 nats below). The second part times an
+// infinity is NaN or the other infinity: a step that has one among its values
+// leaves the second parts out.
+constexpr float kHalfUnit = 32768.0f;
+
 struct PagedArgs {
     const void *q, *k, *v;
     void* out;
@@ -275,6 +285,46 @@ __device__ __forceinline__ Tile16 tile_of(const PagedArgs& a, int page, int kv, 
     return {((static_cast<int64_t>(there ? page : 0) * a.h_kv + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1)), there};
 }
 
+// A workgroup's waves' sums of up to kGroup query heads joined in LDS: the result,
+// or the piece's in the workspace. Lane (n, g) holds channels 16 i + 4 g + .. of
+// head n; l is a head's whole sum of the wave.
+template <typename T, int D, typename S>
+__device__ __forceinline__ void join_waves(const PagedArgs& a, S& sm, int s, int count, int head0, int live_heads,
+                                           const f32x4 (&o)[D / 16], float m, float l) {
+    constexpr int kOPitch = D + 4;
+    const int lane = lane_id(), wave = wave_in_block(), n = lane & 15, g = lane >> 4;
+    __syncthreads();
+    if (n < live_heads) {
+#pragma unroll
+        for (int i = 0; i < D / 16; i++) *reinterpret_cast<f32x4*>(&sm.o[wave][n * kOPitch + 16 * i + 4 * g]) = o[i];
+        if (g == 0) sm.m[wave][n] = m, sm.l[wave][n] = l;
+    }
+    __syncthreads();
+    for (int x = threadIdx.x; x < live_heads * (D / 4); x += 64 * kPagedWaves) {
+        const int head = x / (D / 4), d0 = x % (D / 4) * 4;
+        float top = sm.m[0][head];
+#pragma unroll
+        for (int w = 1; w < kPagedWaves; w++) top = fmaxf(top, sm.m[w][head]);
+        f32x4 sum = {};
+        float weight = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(sm.m[w][head] - top);
+            sum += *reinterpret_cast<const f32x4*>(&sm.o[w][head * kOPitch + d0]) * f;
+            weight = fmaf(sm.l[w][head], f, weight);
+        }
+        if (count == 1) {
+            T* orow = static_cast<T*>(a.out) + (static_cast<int64_t>(s) * a.h + head0 + head) * D + d0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(top == kNone ? 0.0f : sum[e] / weight);
+        } else {
+            const int64_t row = static_cast<int64_t>(blockIdx.x) * a.width + head;
+            *reinterpret_cast<f32x4*>(a.ws_o + row * D + d0) = sum;
+            if (d0 == 0) a.ws_ml[2 * row] = top, a.ws_ml[2 * row + 1] = weight;
+        }
+    }
+}
+
 // The pieces of one (sequence, query head) joined, THREADS / (D / 4) at a time.
 template <typename T, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
@@ -333,6 +383,32 @@ struct PagedPlan {
         rows = items * width;
     }
 };
+
+// The pieces' kernel (of whole 16 keys in a page, or by rows) and their join.
+template <typename T, int D, typename A, typename K>
+hs_status launch_pieces(const char* op, hipStream_t st, A a, K whole, K rows, int unit, int per_cu) {
+    const PagedPlan plan(a.b, a.h, a.h_kv, per_cu);
+    a.ws_ml = a.ws_o + plan.rows * D;
+    a.ws_cut = reinterpret_cast<int*>(a.ws_ml + 2 * plan.rows);
+    a.group = plan.group, a.passes = plan.passes, a.width = plan.width;
+    // (rounded up by twice the error of the kernels' sum over the lengths)
+    a.per_round = static_cast<float>((1.0 + (a.b / 64 + 64) * 0x1p-23) / static_cast<double>(plan.ranges));
+    // no more pieces than a table's width of keys has, either
+    const int64_t most = ceil_div(static_cast<int64_t>(a.max_pages) << a.page_shift, int64_t{unit});
+    const int64_t items = a.b * plan.heads * (most > 1 ? most : 1);
+    const dim3 grid(static_cast<uint32_t>(items < plan.items ? items : plan.items));
+    (a.page_shift >= 4 ? whole : rows)<<<grid, dim3(64 * kPagedWaves), 0, st>>>(a);
+    if (hs_status rc = check_launch(op)) return rc;
+    if (most <= 1) return HS_OK;  // no sequence has two pieces
+    const int64_t joined = static_cast<int64_t>(a.b) * a.h;
+    const dim3 joins(static_cast<uint32_t>(joined));
+    // few rows may have a thousand pieces each
+    if (joined <= 64)
+        paged_join_kernel<T, D, 1024><<<joins, dim3(1024), 0, st>>>(a);
+    else
+        paged_join_kernel<T, D, 256><<<joins, dim3(256), 0, st>>>(a);
+    return check_launch(op);
+}
 
 [[maybe_unused]] hs_status check_cache(const char* op, const void* k_cache, const void* v_cache, const void* page_table,
                       const void* lens, int32_t page, int32_t n_pages, int32_t max_pages, int32_t h_kv, int32_t d) {
