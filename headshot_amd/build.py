@@ -33,6 +33,7 @@ HIP_SOURCES = [
     "hs_attention_packed.hip",
     "hs_paged.hip",
     "hs_paged_f8.hip",
+    "hs_prompts_f8.hip",
     "hs_pages.hip",
     "hs_cache.hip",
     "hs_gemm.hip",
@@ -59,6 +60,7 @@ SOURCE_FLAGS = {
     "hs_attention_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "hs_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "hs_paged_f8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "hs_prompts_f8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "hs_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans"],
 }
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-Wall",

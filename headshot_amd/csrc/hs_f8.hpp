@@ -62,12 +62,60 @@ __device__ __forceinline__ uint32_t codes_down(uint32_t w, int down) {
     return codes_of(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
 }
 
+// 8 f32 values in parts whose sum they are, 8 leading bits each (cut, not rounded:
+// what is left is exact, and a value near f32's largest stays one).
+__device__ __forceinline__ void cut3(const float (&x)[8], u32x4 (&part)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t a = f2u(x[2 * i]), b = f2u(x[2 * i + 1]);
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+            part[p][i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            if (p < 2) {
+                a = f2u(u2f(a) - u2f(a & 0xFFFF0000u));
+                b = f2u(u2f(b) - u2f(b & 0xFFFF0000u));
+            }
+        }
+    }
+}
+
 // The host's checks of such a cache.
 [[maybe_unused]] hs_status check_cache_f8(const char* op, const void* k_cache, const void* v_cache, const void* k_scale,
                                           const void* v_scale, const void* page_table, const void* lens, int32_t page,
                                           int32_t n_pages, int32_t max_pages, int32_t h_kv, int32_t d) {
     if (hs_status rc = check_cache(op, k_cache, v_cache, page_table, lens, page, n_pages, max_pages, h_kv, d)) return rc;
     if (n_pages > 0 && (!k_scale || !v_scale)) return fail(HS_EINVAL, "%s: null scales", op);
+    return HS_OK;
+}
+
+// A call that attends over such a cache, n rows of q.
+struct AttendCall {
+    const void* q;
+    int64_t q_stride;
+    const void *k_cache, *v_cache, *k_scale, *v_scale, *page_table, *lens;
+    void *out, *workspace;
+    int64_t workspace_bytes, n;
+    int32_t h, h_kv, d, page, n_pages, max_pages;
+    float scale;
+};
+
+[[maybe_unused]] hs_status check_attend_f8(const char* op, hs_dtype dt, const AttendCall& c, int64_t need) {
+    const int64_t width = static_cast<int64_t>(c.h) * c.d;
+    if (hs_status rc = check_rows(op, "q", c.q, c.n, c.q_stride, width, dt)) return rc;
+    if (!c.out) return fail(HS_EINVAL, "%s: null out", op);
+    if (hs_status rc = check_cache_f8(op, c.k_cache, c.v_cache, c.k_scale, c.v_scale, c.page_table, c.lens, c.page, c.n_pages, c.max_pages, c.h_kv, c.d))
+        return rc;
+    if (!aligned16(c.out) || !aligned16(c.workspace)) return fail(HS_EUNSUPPORTED, "%s: out and workspace must be 16-byte aligned", op);
+    if (need > 0 && (!c.workspace || c.workspace_bytes < need))
+        return fail(HS_EINVAL, "%s: workspace of %lld bytes, %lld needed", op, static_cast<long long>(c.workspace_bytes), static_cast<long long>(need));
+    const int64_t scales = static_cast<int64_t>(c.n_pages) * c.h_kv, codes = scales * c.page * c.d, bytes = c.n * width * dtype_size(dt);
+    const ByteRange in[5] = {{c.q, row_bytes(c.n, c.q_stride, width, dt)}, {c.k_cache, codes}, {c.v_cache, codes}, {c.k_scale, scales}, {c.v_scale, scales}};
+    for (const ByteRange& r : in) {
+        if (overlaps(c.out, bytes, r.p, r.bytes)) return fail(HS_EINVAL, "%s: out overlaps another buffer", op);
+        if (overlaps(c.workspace, need, r.p, r.bytes)) return fail(HS_EINVAL, "%s: workspace overlaps an input", op);
+    }
+    if (overlaps(c.out, bytes, c.workspace, need)) return fail(HS_EINVAL, "%s: out overlaps another buffer", op);
+    if (!std::isfinite(c.scale)) return fail(HS_EINVAL, "%s: scale must be finite", op);
     return HS_OK;
 }
 

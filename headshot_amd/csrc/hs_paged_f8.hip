@@ -1,5 +1,5 @@
 // A paged key-value cache held in 8 bits for gfx950: appending new tokens and the
-// attention of new tokens over it.
+// attention of one new token per sequence.
 #include "hs_f8.hpp"
 
 namespace hs {
@@ -236,8 +236,8 @@ void launch_append_f8(hipStream_t st, const Append8Args<T>& a, uint32_t blocks) 
 }
 
 // ---------------------------------------------------------------------------
-// attention over the cache
-
+// attention_paged
+//
 // Single tokens: as attention_paged (hs_paged.hip), of half its bytes or a
 // quarter. A wave takes kStep keys at a time on its own; codes become f16 (f16
 // caches) or bf16 (f32) values with their page's scale on the way, exactly: K's in
@@ -278,23 +278,6 @@ struct Paged8 {
 struct Paged8Args : PagedArgs {
     const uint8_t *k_scale, *v_scale;
 };
-
-// 8 f32 values in parts whose sum they are, 8 leading bits each (cut, not rounded:
-// what is left is exact, and a value near f32's largest stays one).
-__device__ __forceinline__ void cut3(const float (&x)[8], u32x4 (&part)[3]) {
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        uint32_t a = f2u(x[2 * i]), b = f2u(x[2 * i + 1]);
-#pragma unroll
-        for (int p = 0; p < 3; p++) {
-            part[p][i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-            if (p < 2) {
-                a = f2u(u2f(a) - u2f(a & 0xFFFF0000u));
-                b = f2u(u2f(b) - u2f(b & 0xFFFF0000u));
-            }
-        }
-    }
-}
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -552,97 +535,6 @@ hs_status launch_paged_f8(const char* op, hipStream_t st, const Paged8Args& a) {
     return launch_pieces<T, D>(op, st, a, attention_paged_f8_kernel<T, D, true>, attention_paged_f8_kernel<T, D, false>, P::kUnit, P::kPerCu);
 }
 
-struct Attend8Args {
-    const void* q;
-    const uint8_t *k, *v, *k_scale, *v_scale;
-    void* out;
-    const int *page_table, *lens, *offsets;  // offsets null: one query a sequence
-    int64_t q_stride;
-    int n, b, h, h_kv, page_shift, n_pages, max_pages, causal;
-    float scale;
-};
-
-// A workgroup takes a query and a head, a wave every fourth key: its score, then
-// the running maximum, sum and weighted values.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void attend_f8_kernel(Attend8Args a) {
-    constexpr int E = D / 64;  // channels per lane
-    __shared__ float o[4][D], m[4], l[4];
-    const int row = static_cast<int>(blockIdx.x) / a.h, head = static_cast<int>(blockIdx.x) - row * a.h;
-    const int s = a.offsets ? sequence_of(a.offsets, a.b, row) : row;
-    if (s < 0) return;
-    const int kv = head / (a.h / a.h_kv), lane = lane_id(), wave = wave_in_block();
-    const int len = max(a.lens[s], 0), held = held_length(a.lens, s, a.max_pages, a.page_shift);
-    int seen = held;
-    if (a.offsets && a.causal) {
-        const int at = len - (min(max(a.offsets[s + 1], 0), a.n) - row);
-        const int64_t end = at < 0 ? 0 : (static_cast<int64_t>(at / a.causal) + 1) * a.causal;
-        seen = end < held ? static_cast<int>(end) : held;
-    }
-    float q[E], acc[E] = {}, top = kNone, sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) q[e] = load_elem(static_cast<const T*>(a.q) + row * a.q_stride + head * D + lane * E + e);
-    for (int key = wave; key < seen; key += 4) {
-        const int page = a.page_table[static_cast<int64_t>(s) * a.max_pages + (key >> a.page_shift)];
-        if (page < 0 || page >= a.n_pages) continue;
-        const int64_t block = static_cast<int64_t>(page) * a.h_kv + kv;
-        const int64_t at = ((block << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * D + lane * E;
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) dot = fmaf(q[e], __builtin_amdgcn_cvt_f32_fp8(a.k[at + e], 0) * scale_value(a.k_scale[block]), dot);
-        const float score = as_f32(wave_sum(dot) * (a.scale * 1.4426950408889634f));
-        const float next = fmaxf(fmaxf(top, score), kFloor);
-        const float corr = __builtin_amdgcn_exp2f(top - next), p = __builtin_amdgcn_exp2f(score - next);
-        top = next, sum = fmaf(sum, corr, p);
-#pragma unroll
-        for (int e = 0; e < E; e++) acc[e] = fmaf(acc[e], corr, p * (__builtin_amdgcn_cvt_f32_fp8(a.v[at + e], 0) * scale_value(a.v_scale[block])));
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) o[wave][lane * E + e] = acc[e];
-    if (lane == 0) m[wave] = top, l[wave] = sum;
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-    float x = 0.0f, w = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float f = __builtin_amdgcn_exp2f(m[i] - top);
-        x = fmaf(o[i][threadIdx.x], f, x), w = fmaf(l[i], f, w);
-    }
-    store_elem(static_cast<T*>(a.out) + (static_cast<int64_t>(row) * a.h + head) * D + threadIdx.x, top == kNone ? 0.0f : x / w);
-}
-
-hs_status check_attend(const char* op, hs_dtype dt, const Attend8Args& a, int d, int page, const void* workspace,
-                       int64_t workspace_bytes, int64_t need) {
-    const int64_t width = static_cast<int64_t>(a.h) * d, e = dtype_size(dt);
-    if (hs_status rc = check_rows(op, "q", a.q, a.n, a.q_stride, width, dt)) return rc;
-    if (!a.out) return fail(HS_EINVAL, "%s: null out", op);
-    if (hs_status rc = check_cache_f8(op, a.k, a.v, a.k_scale, a.v_scale, a.page_table, a.lens, page, a.n_pages, a.max_pages, a.h_kv, d)) return rc;
-    if (!aligned16(a.out) || !aligned16(workspace)) return fail(HS_EUNSUPPORTED, "%s: out and workspace must be 16-byte aligned", op);
-    if (need > 0 && (!workspace || workspace_bytes < need))
-        return fail(HS_EINVAL, "%s: workspace of %lld bytes, %lld needed", op, static_cast<long long>(workspace_bytes), static_cast<long long>(need));
-    const int64_t cache = static_cast<int64_t>(a.n_pages) * page * a.h_kv * d, scales = static_cast<int64_t>(a.n_pages) * a.h_kv;
-    const struct {
-        const void* p;
-        int64_t bytes;
-    } in[5] = {{a.q, row_bytes(a.n, a.q_stride, width, dt)}, {a.k, cache}, {a.v, cache}, {a.k_scale, scales}, {a.v_scale, scales}};
-    for (const auto& r : in) {
-        if (overlaps(a.out, a.n * width * e, r.p, r.bytes)) return fail(HS_EINVAL, "%s: out overlaps another buffer", op);
-        if (overlaps(workspace, need, r.p, r.bytes)) return fail(HS_EINVAL, "%s: workspace overlaps an input", op);
-    }
-    if (overlaps(a.out, a.n * width * e, workspace, need)) return fail(HS_EINVAL, "%s: out overlaps another buffer", op);
-    if (!std::isfinite(a.scale)) return fail(HS_EINVAL, "%s: scale must be finite", op);
-    return HS_OK;
-}
-
-void launch_attend(hipStream_t st, hs_dtype dt, int d, const Attend8Args& a) {
-    const dim3 grid(static_cast<uint32_t>(static_cast<int64_t>(a.n) * a.h));
-    if (dt == HS_F16)
-        (d == 64 ? attend_f8_kernel<f16, 64> : attend_f8_kernel<f16, 128>)<<<grid, dim3(256), 0, st>>>(a);
-    else
-        (d == 64 ? attend_f8_kernel<float, 64> : attend_f8_kernel<float, 128>)<<<grid, dim3(256), 0, st>>>(a);
-}
-
 }  // namespace
 }  // namespace hs
 
@@ -715,54 +607,19 @@ extern "C" hs_status hs_attention_paged_f8(hs_stream_t stream, hs_dtype dt, cons
     if (b < 0) return fail(HS_EINVAL, "%s: negative count", op);
     if (b == 0 || h == 0) return HS_OK;
     if (static_cast<int64_t>(b) * h >= (int64_t{1} << 23)) return fail(HS_EINVAL, "%s: b * Hq must be below 2^23", op);
-    Attend8Args a;
-    a.q = q, a.q_stride = q_stride, a.out = out;
-    a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
-    a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
-    a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens), a.offsets = nullptr;
-    a.n = b, a.b = b, a.h = h, a.h_kv = h_kv, a.n_pages = n_pages, a.max_pages = max_pages, a.causal = 0, a.scale = scale;
-    if (hs_status rc = check_attend(op, dt, a, d, page, workspace, workspace_bytes, hs_attention_paged_f8_workspace(b, h, h_kv, d))) return rc;
+    const int64_t need = hs_attention_paged_f8_workspace(b, h, h_kv, d);
+    if (hs_status rc = check_attend_f8(op, dt, {q, q_stride, k_cache, v_cache, k_scale, v_scale, page_table, lens, out, workspace,
+                                                workspace_bytes, b, h, h_kv, d, page, n_pages, max_pages, scale}, need))
+        return rc;
     Paged8Args p;
     p.q = q, p.k = k_cache, p.v = v_cache, p.out = out, p.q_stride = q_stride;
     p.ws_o = static_cast<float*>(workspace);
-    p.page_table = a.page_table, p.lens = a.lens, p.k_scale = a.k_scale, p.v_scale = a.v_scale;
+    p.page_table = static_cast<const int*>(page_table), p.lens = static_cast<const int*>(lens);
+    p.k_scale = static_cast<const uint8_t*>(k_scale), p.v_scale = static_cast<const uint8_t*>(v_scale);
     p.b = b, p.h = h, p.h_kv = h_kv, p.page_shift = exact_log2(page), p.n_pages = n_pages;
     p.max_pages = n_pages > 0 ? max_pages : 0;  // no page to read: no sequence has keys
     p.scale = scale;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (dt == HS_F16) return d == 64 ? launch_paged_f8<f16, 64>(op, st, p) : launch_paged_f8<f16, 128>(op, st, p);
     return d == 64 ? launch_paged_f8<float, 64>(op, st, p) : launch_paged_f8<float, 128>(op, st, p);
-}
-
-extern "C" int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int32_t b, int32_t h, int32_t h_kv,
-                                                     int32_t d, int32_t page, int32_t max_pages, int32_t causal) {
-    return 0;
-}
-
-extern "C" hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
-                                             const void* k_cache, const void* v_cache, const void* k_scale,
-                                             const void* v_scale, const void* page_table, const void* lens,
-                                             const void* offsets, void* out, void* workspace, int64_t workspace_bytes,
-                                             int64_t n, int32_t b, int32_t h, int32_t h_kv, int32_t d, int32_t page,
-                                             int32_t n_pages, int32_t max_pages, int32_t causal, float scale) {
-    using namespace hs;
-    const char* op = "attention_prompts_f8";
-    if (hs_status rc = check_heads(op, dt, h, h_kv, d)) return rc;
-    if (n < 0 || b < 0) return fail(HS_EINVAL, "%s: negative count", op);
-    if (causal < 0) return fail(HS_EINVAL, "%s: causal %d", op, causal);
-    if (n == 0 || b == 0 || h == 0) return HS_OK;
-    if (n >= (int64_t{1} << 30) / h) return fail(HS_EINVAL, "%s: n * Hq must be below 2^30", op);
-    if (!offsets) return fail(HS_EINVAL, "%s: null offsets", op);
-    Attend8Args a;
-    a.q = q, a.q_stride = q_stride, a.out = out;
-    a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
-    a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
-    a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens), a.offsets = static_cast<const int*>(offsets);
-    a.n = static_cast<int>(n), a.b = b, a.h = h, a.h_kv = h_kv, a.n_pages = n_pages, a.max_pages = max_pages, a.causal = causal, a.scale = scale;
-    if (hs_status rc = check_attend(op, dt, a, d, page, workspace, workspace_bytes,
-                                    hs_attention_prompts_f8_workspace(dt, n, b, h, h_kv, d, page, max_pages, causal))) return rc;
-    a.page_shift = exact_log2(page);
-    if (n_pages == 0) a.max_pages = 0;
-    launch_attend(static_cast<hipStream_t>(stream), dt, d, a);
-    return check_launch(op);
 }

@@ -1,0 +1,677 @@
+// Attention of several new tokens per sequence over a paged cache held in 8 bits,
+// for gfx950: O_i = sum_j w_ij v_j / sum_j w_ij, w_ij = exp(scale q_i k_j - m_i) over
+// the keys j of its sequence that query i sees, in one pass over the keys with a
+// running m_i.
+//
+// A workgroup takes a tile of one sequence and key head: kRows rows, a row being a
+// token and one of the query heads that share the key head, tokens first. So few
+// tokens of shared heads fill a tile, and a key is read and turned from its code
+// once for all heads that see it. Keys go through LDS 64 at a time, double
+// buffered: codes of the next ones lie in registers while these compute, and become
+// f16 (f16 caches) or bf16 (f32) values with their page's scale on the way into LDS,
+// exactly. Scores are transposed, S^T = K Q^T: lanes n and n + 32 hold row n's, so
+// its statistics are the lane's own, and V^T takes P^T from the registers that the
+// scores were in.
+//
+// Lengths are device data: the launch has a workgroup for every item that there
+// can be, and each finds its own. Where tiles are few the keys are cut into pieces,
+// of which an item is one, and a second launch joins them.
+#include <cmath>
+
+#include "hs_f8.hpp"
+
+namespace hs {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kXcds = 8;
+constexpr int kBN = 64;  // keys per tile
+
+__device__ __forceinline__ uint32_t pk_f16(float a, float b) {
+    f16x2 h;
+    h.x = static_cast<f16>(a), h.y = static_cast<f16>(b);
+    return h22u(h);
+}
+// v of this lane and of lane ^ 32, in the same order in both.
+__device__ __forceinline__ f32x2 both_halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(f2u(v), f2u(v), false, false);
+    return f32x2{u2f(static_cast<uint32_t>(r[0])), u2f(static_cast<uint32_t>(r[1]))};
+}
+__device__ __forceinline__ float halves_max(float v) {
+    const f32x2 r = both_halves(v);
+    return fmaxf(r.x, r.y);
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const f32x2 r = both_halves(v);
+    return r.x + r.y;
+}
+
+struct PromptArgs {
+    const void* q;
+    const uint8_t *k, *v, *k_scale, *v_scale;
+    void* out;
+    int64_t q_stride;
+    const int *page_table, *lens, *offsets;
+    int n, b, h, h_kv, group, page_shift, n_pages, max_pages, causal;
+    float scale;
+    // keys cut into pieces
+    float *ws_o, *ws_ml;  // per (item, key head, row of the tile): D sums; maximum and weight sum
+    float per_piece;      // 1 / pieces wanted of a key head; 0: whole keys
+    int items, pitch;     // items of a key head that the launch has, rows of each
+};
+
+// One sequence: its queries' rows, its length and the keys it holds.
+struct PromptSeq {
+    int q0, nq, len, nk;
+};
+__device__ __forceinline__ PromptSeq sequence_at(const PromptArgs& a, int s) {
+    const RowRange r = row_range(a.offsets, s, a.n);
+    return {r.begin, r.end - r.begin, max(a.lens[s], 0), held_length(a.lens, s, a.max_pages, a.page_shift)};
+}
+// Keys that the sequence's query i sees.
+__device__ __forceinline__ int keys_seen(const PromptSeq& t, int i, int causal) {
+    if (causal == 0) return t.nk;
+    const int at = i + t.len - t.nq;
+    if (at < 0) return 0;
+    const int64_t end = causal == 1 ? static_cast<int64_t>(at) + 1 : (static_cast<int64_t>(at / causal) + 1) * causal;
+    return end < t.nk ? static_cast<int>(end) : t.nk;
+}
+
+// An item: piece `piece` of the pieces of a tile. chunk units of 64 keys are a
+// piece, the same for all sequences of the call, as many as make the pieces wanted of
+// all tiles (half of a causal mask's own keys count); every workgroup computes it from
+// all lengths, 64 a step. The total is summed in f32, whose error per_piece covers;
+// chunk is at least half of the exact total over the pieces wanted, so that a call's
+// items pass neither twice those and its tiles nor, as offsets that do not ascend
+// may have it, what the launch has: such items are left out.
+constexpr int kLeastUnits = 4;
+
+struct PromptItem {
+    int s, tiles, local;  // sequence, its tiles, the one
+    int piece, pieces, chunk, item;  // item: piece 0's
+};
+__device__ __forceinline__ int tiles_of(const PromptArgs& a, int nq, int rows) {
+    return static_cast<int>((static_cast<int64_t>(nq) * a.group + rows - 1) / rows);
+}
+template <bool BY_TILE>
+__device__ __forceinline__ bool find_item(const PromptArgs& a, int rows, int index, PromptItem& t) {
+    const int lane = lane_id();
+    const bool split = a.per_piece > 0.0f;
+    t.chunk = 1 << 24;
+    if (split) {
+        float total = 0.0f;
+        for (int base = 0; base < a.b; base += 64)
+            if (base + lane < a.b) {
+                const PromptSeq s = sequence_at(a, base + lane);
+                const int masked = a.causal ? min(s.nq, s.nk) : 0;
+                total += static_cast<float>(tiles_of(a, s.nq, rows)) *
+                         (static_cast<float>((s.nk + kBN - 1) / kBN) - static_cast<float>(masked) * (0.5f / kBN));
+            }
+        t.chunk = static_cast<int>(fminf(fmaxf(ceilf(wave_sum(total) * a.per_piece), static_cast<float>(kLeastUnits)), 16777216.0f));
+    }
+    int tiles_before = 0, items_before = 0;
+    for (int base = 0; base < a.b; base += 64) {
+        int tiles = 0, pieces = 1;
+        if (base + lane < a.b) {
+            const PromptSeq s = sequence_at(a, base + lane);
+            tiles = tiles_of(a, s.nq, rows);
+            pieces = max(((s.nk + kBN - 1) / kBN + t.chunk - 1) / t.chunk, 1);
+        }
+        const int tile_sum = wave_prefix_sum(tiles), item_sum = wave_prefix_sum(tiles * pieces);
+        const uint64_t hit = __ballot((BY_TILE ? tiles_before + tile_sum : items_before + item_sum) > index);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            t.s = base + l;
+            t.tiles = lane_value(tiles, l), t.pieces = lane_value(pieces, l);
+            const int before = items_before + lane_value(item_sum, l) - t.tiles * t.pieces;
+            t.local = BY_TILE ? index - tiles_before - (lane_value(tile_sum, l) - t.tiles) : (index - before) / t.pieces;
+            t.item = before + t.local * t.pieces;
+            // in another order from tile to tile: the last pieces, which an early
+            // tile's queries do not see, are not one XCD's
+            t.piece = BY_TILE ? 0 : (index - t.item + t.local) % t.pieces;
+            return t.item + t.pieces <= a.items;
+        }
+        tiles_before += lane_value(tile_sum, 63), items_before += lane_value(item_sum, 63);
+    }
+    return false;
+}
+// Pieces of a tile whose last query sees `most` keys: the ones that see any.
+__device__ __forceinline__ int pieces_seen(int most, int chunk) {
+    return max(static_cast<int>((most + static_cast<int64_t>(kBN) * chunk - 1) / (static_cast<int64_t>(kBN) * chunk)), 1);
+}
+
+// What a workgroup works on.
+struct PromptTile {
+    PromptSeq seq;
+    int s, kv;
+    int first, rows;              // its rows of the sequence's: from `first` on, and how many the sequence has
+    int begin, end, count, item;  // keys of the piece, of how many the tile has, its place
+};
+// Workgroup b runs on XCD b % 8: where the key heads divide by it, an XCD takes h_kv
+// / 8 of them in a row, so that a head's tiles read their keys through one L2. A
+// sequence's last queries see the most keys and go first.
+__device__ __forceinline__ bool prompt_tile(const PromptArgs& a, int rows, PromptTile& t) {
+    const int b = blockIdx.x;
+    int index;
+    if (a.h_kv % kXcds == 0) {
+        const int slot = b / kXcds, heads = a.h_kv / kXcds;
+        index = slot / heads;
+        t.kv = b % kXcds * heads + slot % heads;
+    } else {
+        index = b / a.h_kv;
+        t.kv = b % a.h_kv;
+    }
+    PromptItem c;
+    if (!find_item<false>(a, rows, index, c)) return false;
+    t.s = c.s, t.seq = sequence_at(a, c.s);
+    t.rows = t.seq.nq * a.group;
+    t.first = (c.tiles - 1 - c.local) * rows;
+    const int most = keys_seen(t.seq, (min(t.first + rows, t.rows) - 1) / a.group, a.causal);
+    t.count = pieces_seen(most, c.chunk), t.item = c.item + c.piece;
+    if (c.piece >= t.count) return false;
+    const int64_t begin = static_cast<int64_t>(c.piece) * c.chunk * kBN;
+    t.begin = static_cast<int>(begin);
+    t.end = c.piece + 1 < t.count ? static_cast<int>(begin + static_cast<int64_t>(c.chunk) * kBN) : most;
+    return true;
+}
+__device__ __forceinline__ int64_t partial_row(const PromptArgs& a, int item, int kv, int row) {
+    return (static_cast<int64_t>(item) * a.h_kv + kv) * a.pitch + row;
+}
+__device__ __forceinline__ int64_t row_out(const PromptArgs& a, const PromptSeq& s, int kv, int row) {
+    const int token = row / a.group;
+    return static_cast<int64_t>(s.q0 + token) * a.h + kv * a.group + (row - token * a.group);
+}
+
+// The reference of a row's weights is set this far (log2) below its largest score,
+// so that its largest weight is 2^12: f16 weights keep 11 bits down to 2^-26 of the
+// largest. It moves when one would pass f16.
+constexpr float kWeightBits = 12.0f;
+constexpr float kPastF16 = 65520.0f;  // the least that f16 rounds to infinity
+// Tiles for which a wave looks for the scores' maximum ahead of the weights once
+// references have moved.
+constexpr int kWary = 8;
+// A reference before any score: finite, so that a masked score weighs nothing.
+constexpr float kStart = -3.0e38f;
+// A maximum (log2) beyond which its rounding, 2^-24 of it, shows in a weight.
+constexpr float kFar = 65536.0f;
+
+template <typename T, int D, int W>
+struct Prompt8 {
+    static constexpr bool kHalf = sizeof(T) == 2;
+    static constexpr int kThr = 64 * W, kRows = 32 * W;
+    static constexpr int kParts = kHalf ? 1 : 3;   // of a query value and of a weight
+    static constexpr int KS = D / 16, DB = D / 32;
+    static constexpr int kPieces = D / 16;         // 16-byte pieces of a row of codes
+    static constexpr int kRowStep = kThr / kPieces;
+    static constexpr int kPer = kBN / kRowStep;    // loads of a thread
+    // 16-bit values per row: K's 16 rows at one column, and the transposing read's 4
+    // rows of 64 bytes, touch every bank once
+    static constexpr int kKPitch = D + 8, kVPitch = D + 32;
+    static constexpr int kPerCu = D == 64 ? (kHalf ? 3 : 2) : (kHalf ? 2 : 1);
+    struct Smem {
+        uint16_t k[2][kBN * kKPitch];
+        uint16_t v[2][kBN * kVPitch];
+        uint8_t there[2][kBN];
+        int gap[2];  // the tile of each buffer if some of its keys are not there
+        int odd;     // a tile whose values not every row sees holds NaN
+    };
+};
+
+template <typename T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+    if constexpr (sizeof(T) == 2)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(a), as_h8(b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+template <typename T, int D, int W>
+__global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void prompts_f8_kernel(PromptArgs a) {
+    using F = Prompt8<T, D, W>;
+    constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
+    __shared__ __align__(16) typename F::Smem sm;
+    PromptTile t;
+    if (!prompt_tile(a, F::kRows, t)) return;  // workgroup-uniform, before any barrier
+    const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
+    const int n = lane & 31, hh = lane >> 5;
+
+    // The keys seen grow with the token: the tile's last live row has the most
+    const int row = t.first + 32 * wave + n;
+    const bool live = t.first + 32 * wave < t.rows;  // wave-uniform
+    const auto seen_by = [&](int r) { return keys_seen(t.seq, min(r, t.rows - 1) / a.group, a.causal); };
+    const int seen = seen_by(row);
+    const int wave_least = seen_by(t.first + 32 * wave);
+    const int wave_most = live ? seen_by(t.first + 32 * wave + 31) : 0;
+    const int tile_least = seen_by(t.first);
+    const int tile0 = t.begin / kBN, ntiles = (t.end + kBN - 1) / kBN;
+
+    // Q^T as the B operand: lane (n, hh) holds dims 16 ks + 8 hh .. + 8. A
+    // negative scale is taken as one of -q.
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
+    u32x4 qa[KS][F::kParts];
+    {
+        const int r = min(row, t.rows - 1), token = r / a.group;
+        const T* qr = static_cast<const T*>(a.q) + (t.seq.q0 + token) * a.q_stride + (t.kv * a.group + (r - token * a.group)) * D + 8 * hh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            if constexpr (F::kHalf) {
+                u32x4 x = ld16(qr + 16 * ks);
+                qa[ks][0] = a.scale < 0.0f ? x ^ 0x80008000u : x;
+            } else {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[e] = a.scale < 0.0f ? -qr[16 * ks + e] : qr[16 * ks + e];
+                cut3(x, qa[ks]);
+            }
+        }
+        // arrived before the loop, whose prefetches it would wait for otherwise
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) asm volatile("" ::"v"(qa[ks][0]));
+    }
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int i = 0; i < DB; i++) o[i] = f32x16{};
+    float m = kStart, l = 0.0f;
+    int wary = 0;  // tiles to go
+
+    // Staging: load i of the thread is row row0 + kRowStep i of the tile, 16 codes
+    // at `piece`. Pages are looked up a tile ahead of the codes.
+    const int row0 = tid / F::kPieces, piece = tid % F::kPieces;
+    const int* pages = a.page_table + static_cast<int64_t>(t.s) * a.max_pages;
+    int page[kPer];
+    u32x4 pk[kPer], pv[kPer];
+    uint32_t pks[kPer], pvs[kPer];
+    uint32_t ok = 0;  // by load: a key of the piece that there is
+    auto find_pages = [&](int key0) {
+#pragma unroll
+        for (int i = 0; i < kPer; i++) page[i] = pages[min(key0 + row0 + i * F::kRowStep, t.end - 1) >> a.page_shift];
+    };
+    auto load = [&](int key0) {
+        ok = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int key = key0 + row0 + i * F::kRowStep;
+            const bool there = page[i] >= 0 && page[i] < a.n_pages && key < t.end;
+            const int64_t block = static_cast<int64_t>(there ? page[i] : 0) * a.h_kv + t.kv;
+            const int64_t at = ((block << a.page_shift) + (there ? key & ((1 << a.page_shift) - 1) : 0)) * D + piece * 16;
+            pk[i] = ld16(a.k + at), pv[i] = ld16(a.v + at);
+            pks[i] = a.k_scale[block], pvs[i] = a.v_scale[block];
+            ok |= there ? 1u << i : 0u;
+        }
+    };
+    auto store = [&](int buf, int j) {
+        const bool masked = j * kBN + kBN > tile_least;  // some row does not see all of these values
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int r = row0 + i * F::kRowStep;
+            const bool there = ok >> i & 1;
+            if (piece == 0) sm.there[buf][r] = there;
+            if (!there && j * kBN + r < t.end) sm.gap[buf] = j;
+            const float ks = scale_value(pks[i]), vs = there ? scale_value(pvs[i]) : 1.0f;
+            const u32x4 codes = there ? pv[i] : u32x4{};
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                uint16_t* kp = &sm.k[buf][r * F::kKPitch + piece * 16 + 8 * half];
+                uint16_t* vp = &sm.v[buf][r * F::kVPitch + piece * 16 + 8 * half];
+                u32x4 x;
+                if constexpr (F::kHalf) {
+                    st16(kp, f16_of_codes(pk[i][2 * half], pk[i][2 * half + 1], ks));
+                    x = f16_of_codes(codes[2 * half], codes[2 * half + 1], vs);
+                } else {
+                    st16(kp, bf16_of_codes(pk[i][2 * half], pk[i][2 * half + 1], ks));
+                    x = bf16_of_codes(codes[2 * half], codes[2 * half + 1], vs);
+                }
+                if (masked) {
+                    constexpr uint32_t kExp = F::kHalf ? 0x7C00u : 0x7F80u;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t keep = ((x[w] & kExp) == kExp ? 0u : 0xFFFFu) | ((x[w] & kExp << 16) == kExp << 16 ? 0u : 0xFFFF0000u);
+                        odd |= keep != 0xFFFFFFFFu;
+                        x[w] &= keep;
+                    }
+                }
+                st16(vp, x);
+            }
+        }
+        if (odd) sm.odd = 1;
+    };
+    if (tid == 0) sm.odd = 0, sm.gap[0] = sm.gap[1] = -1;
+    __syncthreads();
+    if (tile0 < ntiles) {
+        find_pages(tile0 * kBN);
+        load(tile0 * kBN);
+        if (tile0 + 1 < ntiles) find_pages((tile0 + 1) * kBN);
+        store(tile0 & 1, tile0);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int j = tile0; j < ntiles; j++) {
+        const int cur = j & 1, key0 = j * kBN;
+        if (j + 1 < ntiles) {
+            load(key0 + kBN);
+            if (j + 2 < ntiles) find_pages(key0 + 2 * kBN);
+        }
+        if (key0 < wave_most) {
+            // S^T: s[i] holds keys 32 i .. + 32 of the tile, register r of lane
+            // (n, hh) key 8 (r / 4) + 4 hh + r % 4, row n
+            f32x16 s[2];
+            const f32x16 z = {};
+            const uint16_t* ka = sm.k[cur] + n * F::kKPitch + 8 * hh;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const u32x4 k = ld16(ka + 32 * i * F::kKPitch + 16 * ks);
+#pragma unroll
+                    for (int p = F::kParts - 1; p >= 0; p--)
+                        s[i] = mfma32<T>(k, qa[ks][p], ks || p + 1 < F::kParts ? s[i] : z);
+                }
+            if (key0 + kBN > wave_least) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (key0 + 32 * i + 8 * (r / 4) + 4 * hh + r % 4 >= seen) s[i][r] = -INFINITY;
+            }
+            if (sm.gap[cur] == j) {
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++)
+                        if (!sm.there[cur][32 * i + 8 * (r / 4) + 4 * hh + r % 4]) s[i][r] = -INFINITY;
+            }
+            // O^T += V^T P^T. The transposing read gives lane i of 16 channel i of 4
+            // keys: two reads make the 8 keys, in the scores' order.
+            const uint16_t* va = sm.v[cur] + (4 * hh + (n & 15) / 4) * F::kVPitch + (n & 16) + 4 * (n & 3);
+            auto read_v = [&](int g, int db) {
+                const uint16_t* r0 = va + 16 * g * F::kVPitch + 32 * db;
+                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)r0));
+                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(r0 + 8 * F::kVPitch)));
+                u32x4 w;
+                w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
+                return w;
+            };
+            if constexpr (F::kHalf) {
+                u32x4 p[2][2];
+                // The tile's weights against a reference, rounded to f16, and the
+                // sum of the rounded ones over the lane's keys, in f32 like the
+                // product's.
+                auto weights = [&](float mul, float ref) {
+                    const f16x2 one = {static_cast<f16>(1.0f), static_cast<f16>(1.0f)};
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r += 2) {
+                            const uint32_t w = pk_f16(__builtin_amdgcn_exp2f(fmaf(s[i][r], mul, -ref)),
+                                                      __builtin_amdgcn_exp2f(fmaf(s[i][r + 1], mul, -ref)));
+                            p[i][r / 8][r % 8 / 2] = w;
+                            sum[r / 2 % 4] = __builtin_amdgcn_fdot2(u2h2(w), one, sum[r / 2 % 4], false);
+                        }
+                    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                };
+                // Past the first tile the weights are taken against the reference
+                // as it is; only a row of which one does not fit f16, so that its
+                // sum is infinite, moves its own. Where the wave's references have
+                // moved lately, the scores' maximum says so ahead of the weights.
+                bool own = j == tile0 || fabsf(m) > kFar, move = wary > 0 || __any(own);
+                if (!move) {
+                    const float sum = weights(c, m);
+                    own = !(halves_sum(sum) < INFINITY);
+                    move = __any(own);
+                    if (!move) l += sum;
+                }
+                if (move) {
+                    float mx = s[0][0];
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int r = 0; r < 16; r++) mx = fmaxf(mx, s[i][r]);
+                    mx = halves_max(mx);
+                    // (a row that has seen no key takes its reference from the first)
+                    own |= m == kStart || __builtin_amdgcn_exp2f(fmaf(mx, c, -m)) >= kPastF16;
+                    // (a maximum of 2^26 and more may round 8 further down, too far)
+                    const float top = mx * c, low = top - kWeightBits;
+                    const float next = own ? fmaxf(m, top - low > kWeightBits + 2.0f ? top : low) : m;
+                    float corr = 1.0f;
+                    wary--;
+                    if (__any(next != m)) {
+                        corr = __builtin_amdgcn_exp2f(m - next);
+                        wary = kWary;
+#pragma unroll
+                        for (int i = 0; i < DB; i++) o[i] *= corr;
+                    }
+                    // The multiply-add leaves the rounding of s c in the exponent:
+                    // where that is not small, the product is rounded first, as
+                    // the reference's was.
+                    const bool far = __any(fabsf(next) > kFar);
+                    if (far) {
+#pragma unroll
+                        for (int i = 0; i < 2; i++)
+#pragma unroll
+                            for (int r = 0; r < 16; r++) s[i][r] = as_f32(s[i][r] * c) - next;
+                    }
+                    l = fmaf(l, corr, weights(far ? 1.0f : c, far ? 0.0f : next));
+                    m = next;
+                }
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+#pragma unroll
+                    for (int db = 0; db < DB; db++) o[db] = mfma32<T>(read_v(g, db), p[g / 2][g % 2], o[db]);
+            } else {
+                // rounded before the maximum is taken off: that one then weighs 1
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        s[i][r] = as_f32(s[i][r] * c);
+                        mx = fmaxf(mx, s[i][r]);
+                    }
+                const float next = fmaxf(m, halves_max(mx));
+                const float corr = __builtin_amdgcn_exp2f(m - next);
+                m = next;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < DB; i++) o[i] *= corr;
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        x[e] = __builtin_amdgcn_exp2f(s[g / 2][8 * (g % 2) + e] - m);
+                        sum += x[e];
+                    }
+                    u32x4 p[3];
+                    cut3(x, p);
+#pragma unroll
+                    for (int db = 0; db < DB; db++) {
+                        const u32x4 v = read_v(g, db);
+#pragma unroll
+                        for (int i = 2; i >= 0; i--) o[db] = mfma32<T>(v, p[i], o[db]);
+                    }
+                }
+                l = fmaf(l, corr, sum);
+            }
+        }
+        if (j + 1 < ntiles) store(cur ^ 1, j + 1);
+        __syncthreads();
+    }
+    if (row >= t.rows) return;
+    if (tile0 < ntiles && sm.odd) {
+        // NaN among values that some rows of the tile see and others do not went
+        // into LDS as zeros; here they reach the rows that do see them
+        for (int key = max(tile_least / kBN * kBN, t.begin); key < min(seen, t.end); key++) {
+            const int p = pages[key >> a.page_shift];
+            if (p < 0 || p >= a.n_pages) continue;
+            const int64_t block = static_cast<int64_t>(p) * a.h_kv + t.kv;
+            const uint8_t* r = a.v + ((block << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * D + 4 * hh;
+            const float scale = scale_value(a.v_scale[block]);
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) {
+                    const uint32_t code = r[32 * db + 8 * (x / 4) + x % 4];
+                    const uint32_t half = F::kHalf ? h22u(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, scale, false))
+                                                   : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code, scale, false));
+                    const float v = F::kHalf ? static_cast<float>(u2h2(half).x) : u2f(half << 16);
+                    if ((f2u(v) & 0x7F800000u) == 0x7F800000u) o[db][x] += v;
+                }
+        }
+    }
+    const float lsum = halves_sum(l);
+    if (t.count > 1) {
+        const int64_t at = partial_row(a, t.item, t.kv, row - t.first);
+        float* p = a.ws_o + at * D + 4 * hh;
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; r4++) {
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = f2u(o[db][4 * r4 + e]);
+                st16(p + 32 * db + 8 * r4, w);
+            }
+        if (hh == 0) a.ws_ml[2 * at] = m, a.ws_ml[2 * at + 1] = lsum;
+        return;
+    }
+    const float inv = 1.0f / lsum;
+    T* orow = static_cast<T*>(a.out) + row_out(a, t.seq, t.kv, row) * D + 4 * hh;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; r4++) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if constexpr (F::kHalf)
+                    x[e] = lsum == 0.0f ? 0.0f : o[db][4 * r4 + e] * inv;
+                else
+                    x[e] = lsum == 0.0f ? 0.0f : o[db][4 * r4 + e] / lsum;
+            }
+            if constexpr (F::kHalf)
+                *reinterpret_cast<u32x2*>(orow + 32 * db + 8 * r4) = u32x2{pk_f16(x[0], x[1]), pk_f16(x[2], x[3])};
+            else
+                *reinterpret_cast<f32x4*>(orow + 32 * db + 8 * r4) = f32x4{x[0], x[1], x[2], x[3]};
+        }
+}
+
+// The pieces of one tile's rows joined, 256 / (D / 4) rows to a workgroup.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prompts_join_kernel(PromptArgs a, int rows) {
+    constexpr int kLanes = D / 4, kGroupRows = 256 / kLanes;
+    const int per_tile = (a.pitch + kGroupRows - 1) / kGroupRows;
+    const int tile_head = static_cast<int>(blockIdx.x) / per_tile;
+    const int tile = tile_head / a.h_kv, kv = tile_head - tile * a.h_kv;
+    PromptItem c;
+    if (!find_item<true>(a, rows, tile, c)) return;
+    const PromptSeq s = sequence_at(a, c.s);
+    const int all = s.nq * a.group, first = (c.tiles - 1 - c.local) * rows, mine = min(rows, all - first);
+    const int count = pieces_seen(keys_seen(s, (first + mine - 1) / a.group, a.causal), c.chunk);
+    if (count == 1) return;  // written by its only piece
+    const int row = (static_cast<int>(blockIdx.x) - tile_head * per_tile) * kGroupRows + static_cast<int>(threadIdx.x) / kLanes;
+    const int col = threadIdx.x % kLanes;
+    if (row >= mine) return;
+    float top = kStart, weight = 0.0f;
+    f32x4 sum = {};
+    for (int i = 0; i < count; i++) {
+        const int64_t at = partial_row(a, c.item + i, kv, row);
+        const float m = a.ws_ml[2 * at], l = a.ws_ml[2 * at + 1];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + at * D + 4 * col);
+        const float next = fmaxf(top, m);
+        const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
+        sum = sum * old + v * f;
+        weight = fmaf(weight, old, l * f);
+        top = next;
+    }
+    T* orow = static_cast<T*>(a.out) + row_out(a, s, kv, first + row) * D + 4 * col;
+#pragma unroll
+    for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(weight == 0.0f ? 0.0f : sum[e] / weight);
+}
+
+// How a call is cut into tiles, and whether its keys are.
+struct PromptPlan {
+    int64_t tiles;          // of a key head, as many as sequences of these rows can have
+    int64_t pieces, items;  // of a key head: wanted (0: whole keys), and what they can come to
+    int64_t pitch;
+    int rows;
+    PromptPlan(hs_dtype dt, int64_t n, int64_t b, int64_t h, int64_t h_kv, int d, int64_t keys) {
+        const int64_t group = h / h_kv, slots = num_cus() * (d == 64 ? (dt == HS_F16 ? 3 : 2) : (dt == HS_F16 ? 2 : 1));
+        rows = 128;
+        tiles = n * group / rows + (b < n ? b : n);
+        pieces = 0, items = tiles, pitch = 0;
+        if (keys <= kLeastUnits * kBN || n * group / rows * h_kv >= 4 * slots) return;
+        pieces = ceil_div(2 * slots, h_kv);
+        items = 2 * pieces + tiles;
+        pitch = n * group < rows ? n * group : rows;
+    }
+    int64_t workspace(int64_t h_kv, int d) const { return pieces ? items * h_kv * pitch * (d + 2) * 4 : 0; }
+};
+
+}  // namespace
+}  // namespace hs
+
+extern "C" int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int32_t b, int32_t h, int32_t h_kv,
+                                                     int32_t d, int32_t page, int32_t max_pages, int32_t causal) {
+    using namespace hs;
+    if (n <= 0 || b <= 0 || h <= 0 || causal < 0 || n >= (int64_t{1} << 30) / h || exact_log2(page) < 0 || max_pages < 0) return 0;
+    if (static_cast<int64_t>(max_pages) * page >= (int64_t{1} << 30)) return 0;
+    if (check_heads("attention_prompts_f8_workspace", dt, h, h_kv, d)) return 0;
+    return PromptPlan(dt, n, b, h, h_kv, d, static_cast<int64_t>(max_pages) * page).workspace(h_kv, d);
+}
+
+extern "C" hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
+                                             const void* k_cache, const void* v_cache, const void* k_scale,
+                                             const void* v_scale, const void* page_table, const void* lens,
+                                             const void* offsets, void* out, void* workspace, int64_t workspace_bytes,
+                                             int64_t n, int32_t b, int32_t h, int32_t h_kv, int32_t d, int32_t page,
+                                             int32_t n_pages, int32_t max_pages, int32_t causal, float scale) {
+    using namespace hs;
+    const char* op = "attention_prompts_f8";
+    if (hs_status rc = check_heads(op, dt, h, h_kv, d)) return rc;
+    if (n < 0 || b < 0) return fail(HS_EINVAL, "%s: negative count", op);
+    if (causal < 0) return fail(HS_EINVAL, "%s: causal %d", op, causal);
+    if (n == 0 || b == 0 || h == 0) return HS_OK;
+    if (n >= (int64_t{1} << 30) / h) return fail(HS_EINVAL, "%s: n * Hq must be below 2^30", op);
+    if (!offsets) return fail(HS_EINVAL, "%s: null offsets", op);
+    const int64_t need = hs_attention_prompts_f8_workspace(dt, n, b, h, h_kv, d, page, max_pages, causal);
+    if (hs_status rc = check_attend_f8(op, dt, {q, q_stride, k_cache, v_cache, k_scale, v_scale, page_table, lens, out, workspace,
+                                                workspace_bytes, n, h, h_kv, d, page, n_pages, max_pages, scale}, need))
+        return rc;
+    PromptArgs a;
+    a.q = q, a.q_stride = q_stride, a.out = out;
+    a.k = static_cast<const uint8_t*>(k_cache), a.v = static_cast<const uint8_t*>(v_cache);
+    a.k_scale = static_cast<const uint8_t*>(k_scale), a.v_scale = static_cast<const uint8_t*>(v_scale);
+    a.page_table = static_cast<const int*>(page_table), a.lens = static_cast<const int*>(lens);
+    a.offsets = static_cast<const int*>(offsets);
+    a.n = static_cast<int>(n), a.b = b, a.h = h, a.h_kv = h_kv, a.group = h / h_kv, a.page_shift = exact_log2(page);
+    a.n_pages = n_pages, a.max_pages = n_pages > 0 ? max_pages : 0;  // no page to read: no sequence has keys
+    a.causal = causal, a.scale = scale;
+    const PromptPlan plan(dt, n, b, h, h_kv, d, static_cast<int64_t>(max_pages) * page);
+    const int threads = 256;
+    const int64_t groups = plan.items * h_kv;
+    if (groups >= (int64_t{1} << 31) / threads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
+    a.ws_o = static_cast<float*>(workspace);
+    a.ws_ml = a.ws_o + (plan.pieces ? plan.items * h_kv * plan.pitch * d : 0);
+    // (rounded up by twice the error of the kernels' sum over the sequences)
+    a.per_piece = plan.pieces ? static_cast<float>((1.0 + (b / 64 + 64) * 0x1p-23) / static_cast<double>(plan.pieces)) : 0.0f;
+    a.items = static_cast<int>(plan.items), a.pitch = static_cast<int>(plan.pitch);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    const auto go = [&](auto kernel, auto join) {
+        kernel<<<dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, st>>>(a);
+        if (hs_status rc = check_launch(op)) return rc;
+        if (!plan.pieces) return HS_OK;
+        const int64_t blocks = plan.tiles * h_kv * ceil_div(plan.pitch, 256 / (d / 4));
+        join<<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, st>>>(a, plan.rows);
+        return check_launch(op);
+    };
+    if (dt == HS_F16) {
+        if (d == 64) return go(prompts_f8_kernel<f16, 64, 4>, prompts_join_kernel<f16, 64>);
+        return go(prompts_f8_kernel<f16, 128, 4>, prompts_join_kernel<f16, 128>);
+    }
+    if (d == 64) return go(prompts_f8_kernel<float, 64, 4>, prompts_join_kernel<float, 64>);
+    return go(prompts_f8_kernel<float, 128, 4>, prompts_join_kernel<float, 128>);
+}
