@@ -30,7 +30,6 @@ __device__ __forceinline__ int scale_for(float most) {
 }
 
 // 8 codes to 8 halves of T, times a scale.
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ u32x4 f16_of_codes(uint32_t lo, uint32_t hi, float scale) {
     u32x4 r;
     r[0] = h22u(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, scale, false));
@@ -46,6 +45,12 @@ __device__ __forceinline__ u32x4 bf16_of_codes(uint32_t lo, uint32_t hi, float s
     r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false));
     r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true));
     return r;
+}
+
+// As a cache of T's rows takes them to the matrix cores.
+template <typename T>
+__device__ __forceinline__ u32x4 values_of(uint32_t lo, uint32_t hi, float scale) {
+    return sizeof(T) == 2 ? f16_of_codes(lo, hi, scale) : bf16_of_codes(lo, hi, scale);
 }
 
 // 4 values to 4 codes, rounded to nearest even. (In range: a finite value past

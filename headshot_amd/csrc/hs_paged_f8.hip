@@ -286,10 +286,6 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-template <typename T>
-__device__ __forceinline__ u32x4 values_of(uint32_t lo, uint32_t hi, float scale) {
-    return sizeof(T) == 2 ? f16_of_codes(lo, hi, scale) : bf16_of_codes(lo, hi, scale);
-}
 
 // WHOLE: pages of at least 16 keys, so that 16 keys from a multiple of 16 lie in
 // one page; else each row looks its own up.

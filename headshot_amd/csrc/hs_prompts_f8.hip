@@ -16,6 +16,7 @@
 // Lengths are device data: the launch has a workgroup for every item that there
 // can be, and each finds its own. Where tiles are few the keys are cut into pieces,
 // of which an item is one, and a second launch joins them.
+#include <algorithm>
 #include <cmath>
 
 #include "hs_f8.hpp"
@@ -56,9 +57,12 @@ struct PromptArgs {
     int n, b, h, h_kv, group, page_shift, n_pages, max_pages, causal;
     float scale;
     // keys cut into pieces
+    int4* cut;            // per tile: its first item, its pieces, its first row of all, its rows; behind them the tiles' number
     float *ws_o, *ws_ml;  // per (item, key head, row of the tile): D sums; maximum and weight sum
-    float per_piece;      // 1 / pieces wanted of a key head; 0: whole keys
-    int items, pitch;     // items of a key head that the launch has, rows of each
+    int tiles;            // of a key head at most
+    int places;           // workgroups of a key head that the chip holds at once; 0: whole keys
+    bool one_round;       // fewer tiles than those
+    int items, blocks;    // items of a key head that the launch has, blocks of 32 rows of each
 };
 
 // One sequence: its queries' rows, its length and the keys it holds.
@@ -78,61 +82,89 @@ __device__ __forceinline__ int keys_seen(const PromptSeq& t, int i, int causal) 
     return end < t.nk ? static_cast<int>(end) : t.nk;
 }
 
-// An item: piece `piece` of the pieces of a tile. chunk units of 64 keys are a
-// piece, the same for all sequences of the call, as many as make the pieces wanted of
-// all tiles (half of a causal mask's own keys count); every workgroup computes it from
-// all lengths, 64 a step. The total is summed in f32, whose error per_piece covers;
-// chunk is at least half of the exact total over the pieces wanted, so that a call's
-// items pass neither twice those and its tiles nor, as offsets that do not ascend
-// may have it, what the launch has: such items are left out.
+// An item: piece `piece` of the pieces of a tile. `fair` units of 64 keys are what each
+// of the key head's places on the chip gets of all tiles' work (half of a causal
+// mask's own keys count). Where tiles are fewer than places, a sequence's tiles are cut
+// into as many whole fair parts as they have, so that the call is one round; else
+// only tiles that would outlast the others are, into pieces of 3/4 of a fair part. A
+// sequence's pieces are of one size, `chunk`. Every workgroup computes this from all
+// lengths, 64 a step. The total is at least half of the exact one, so a call's items
+// do not pass 8/3 of the places and its tiles; what else offsets that do not ascend
+// may come to is left out.
 constexpr int kLeastUnits = 4;
+constexpr float kLonger = 16.0f;  // units that a tile's writing and joining of pieces cost, and more
 
 struct PromptItem {
     int s, tiles, local;  // sequence, its tiles, the one
     int piece, pieces, chunk, item;  // item: piece 0's
+    int tile;                        // of the call's
 };
 __device__ __forceinline__ int tiles_of(const PromptArgs& a, int nq, int rows) {
     return static_cast<int>((static_cast<int64_t>(nq) * a.group + rows - 1) / rows);
 }
-template <bool BY_TILE>
+__device__ __forceinline__ int wave_most(int v) {
+    v = max(v, dpp_zero<kQuadXor1>(v));
+    v = max(v, dpp_zero<kQuadXor2>(v));
+    v = max(v, dpp_zero<kRowHalfMirror>(v));
+    v = max(v, dpp_zero<kRowMirror>(v));
+    return max(max(lane_value(v, 0), lane_value(v, 16)), max(lane_value(v, 32), lane_value(v, 48)));
+}
 __device__ __forceinline__ bool find_item(const PromptArgs& a, int rows, int index, PromptItem& t) {
     const int lane = lane_id();
-    const bool split = a.per_piece > 0.0f;
-    t.chunk = 1 << 24;
-    if (split) {
+    float fair = 16777216.0f;
+    if (a.places > 0) {
         float total = 0.0f;
         for (int base = 0; base < a.b; base += 64)
             if (base + lane < a.b) {
                 const PromptSeq s = sequence_at(a, base + lane);
-                const int masked = a.causal ? min(s.nq, s.nk) : 0;
+                const int masked = a.causal ? max(min(s.nq, s.nk) - a.causal, 0) : 0;
                 total += static_cast<float>(tiles_of(a, s.nq, rows)) *
                          (static_cast<float>((s.nk + kBN - 1) / kBN) - static_cast<float>(masked) * (0.5f / kBN));
             }
-        t.chunk = static_cast<int>(fminf(fmaxf(ceilf(wave_sum(total) * a.per_piece), static_cast<float>(kLeastUnits)), 16777216.0f));
+        fair = fmaxf(wave_sum(total) / static_cast<float>(a.places), static_cast<float>(kLeastUnits));
     }
     int tiles_before = 0, items_before = 0;
     for (int base = 0; base < a.b; base += 64) {
-        int tiles = 0, pieces = 1;
+        int tiles = 0, pieces = 1, chunk = 1;
         if (base + lane < a.b) {
             const PromptSeq s = sequence_at(a, base + lane);
+            const int units = (s.nk + kBN - 1) / kBN;
             tiles = tiles_of(a, s.nq, rows);
-            pieces = max(((s.nk + kBN - 1) / kBN + t.chunk - 1) / t.chunk, 1);
+            if (a.one_round)
+                pieces = max(static_cast<int>(static_cast<float>(units) / fair), 1);
+            else if (static_cast<float>(units) > fair + kLonger)
+                pieces = static_cast<int>(ceilf(static_cast<float>(units) / (0.75f * fair)));
+            chunk = max((units + pieces - 1) / pieces, 1);
         }
-        const int tile_sum = wave_prefix_sum(tiles), item_sum = wave_prefix_sum(tiles * pieces);
-        const uint64_t hit = __ballot((BY_TILE ? tiles_before + tile_sum : items_before + item_sum) > index);
+        // the sequences of long pieces first, by quarters of the longest, so that a
+        // call does not end on them
+        int tile_sum = 0, item_sum = 0, tile_end = 0, item_end = 0;
+        const int longest = a.b > 1 ? wave_most(chunk) : chunk;
+        const int quarter = min((longest - chunk) * 4 / longest, 3);
+        for (int k = 0; k < (a.b > 1 ? 4 : 1); k++) {
+            const int tile_add = wave_prefix_sum(quarter == k ? tiles : 0);
+            const int item_add = wave_prefix_sum(quarter == k ? tiles * pieces : 0);
+            if (quarter == k) tile_sum = tile_end + tile_add, item_sum = item_end + item_add;
+            tile_end += lane_value(tile_add, 63), item_end += lane_value(item_add, 63);
+        }
+        const uint64_t hit = __ballot(items_before + item_sum > index && items_before + item_sum - tiles * pieces <= index);
         if (hit) {
             const int l = __builtin_ctzll(hit);
             t.s = base + l;
-            t.tiles = lane_value(tiles, l), t.pieces = lane_value(pieces, l);
+            t.tiles = lane_value(tiles, l), t.pieces = lane_value(pieces, l), t.chunk = lane_value(chunk, l);
             const int before = items_before + lane_value(item_sum, l) - t.tiles * t.pieces;
-            t.local = BY_TILE ? index - tiles_before - (lane_value(tile_sum, l) - t.tiles) : (index - before) / t.pieces;
+            // all tiles' first pieces, then their second ones, ..: sizes fall slowly
+            // with the number. (Workgroups go to an XCD's four engines in turn and wait
+            // for theirs: with a tile's long and short pieces beside each other two
+            // engines had all the long ones, 2048 tokens over 4096 took 188 us for 179.)
+            const int rest = index - before;
+            t.piece = rest / t.tiles;
+            t.local = rest - t.piece * t.tiles;
             t.item = before + t.local * t.pieces;
-            // in another order from tile to tile: the last pieces, which an early
-            // tile's queries do not see, are not one XCD's
-            t.piece = BY_TILE ? 0 : (index - t.item + t.local) % t.pieces;
+            t.tile = tiles_before + lane_value(tile_sum, l) - t.tiles + t.local;
             return t.item + t.pieces <= a.items;
         }
-        tiles_before += lane_value(tile_sum, 63), items_before += lane_value(item_sum, 63);
+        tiles_before += tile_end, items_before += item_end;
     }
     return false;
 }
@@ -163,20 +195,33 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs& a, int rows, Promp
         t.kv = b % a.h_kv;
     }
     PromptItem c;
-    if (!find_item<false>(a, rows, index, c)) return false;
+    if (a.places > 0 && b == 0) {
+        int tiles = 0;
+        for (int base = 0; base < a.b && tiles < a.tiles; base += 64) {
+            const int s = base + lane_id();
+            tiles += lane_value(wave_prefix_sum(s < a.b ? tiles_of(a, sequence_at(a, s).nq, rows) : 0), 63);
+        }
+        if (threadIdx.x == 0) a.cut[a.tiles] = {min(tiles, a.tiles), 0, 0, 0};
+    }
+    if (!find_item(a, rows, index, c)) return false;
     t.s = c.s, t.seq = sequence_at(a, c.s);
     t.rows = t.seq.nq * a.group;
     t.first = (c.tiles - 1 - c.local) * rows;
     const int most = keys_seen(t.seq, (min(t.first + rows, t.rows) - 1) / a.group, a.causal);
     t.count = pieces_seen(most, c.chunk), t.item = c.item + c.piece;
+    if (a.places > 0 && c.piece == 0 && t.kv == 0 && threadIdx.x == 0 && c.tile < a.tiles)
+        a.cut[c.tile] = {c.item, t.count, t.seq.q0 * a.group + t.first, min(t.rows - t.first, rows)};
     if (c.piece >= t.count) return false;
     const int64_t begin = static_cast<int64_t>(c.piece) * c.chunk * kBN;
     t.begin = static_cast<int>(begin);
     t.end = c.piece + 1 < t.count ? static_cast<int>(begin + static_cast<int64_t>(c.chunk) * kBN) : most;
     return true;
 }
-__device__ __forceinline__ int64_t partial_row(const PromptArgs& a, int item, int kv, int row) {
-    return (static_cast<int64_t>(item) * a.h_kv + kv) * a.pitch + row;
+// A piece's 32 rows of a wave in the workspace: D sums each as the lanes hold them,
+// registers 4 i .. + 4 of all lanes after one another, so that a store is 1 KiB in a
+// row (by rows, it is 32 bytes of each).
+__device__ __forceinline__ int64_t partial_block(const PromptArgs& a, int item, int kv, int wave) {
+    return (static_cast<int64_t>(item) * a.h_kv + kv) * a.blocks + wave;
 }
 __device__ __forceinline__ int64_t row_out(const PromptArgs& a, const PromptSeq& s, int kv, int row) {
     const int token = row / a.group;
@@ -202,13 +247,16 @@ struct Prompt8 {
     static constexpr int kThr = 64 * W, kRows = 32 * W;
     static constexpr int kParts = kHalf ? 1 : 3;   // of a query value and of a weight
     static constexpr int KS = D / 16, DB = D / 32;
-    static constexpr int kPieces = D / 16;         // 16-byte pieces of a row of codes
-    static constexpr int kRowStep = kThr / kPieces;
+    static constexpr int kLoad = kBN * D / kThr < 16 ? kBN * D / kThr : 16;  // codes of a load
+    static constexpr int kPieces = D / kLoad;      // loads of a row
+    static constexpr int kRowStep = kThr / kPieces, kWaveRows = 64 / kPieces;
     static constexpr int kPer = kBN / kRowStep;    // loads of a thread
     // 16-bit values per row: K's 16 rows at one column, and the transposing read's 4
     // rows of 64 bytes, touch every bank once
     static constexpr int kKPitch = D + 8, kVPitch = D + 32;
-    static constexpr int kPerCu = D == 64 ? (kHalf ? 3 : 2) : (kHalf ? 2 : 1);
+    // waves of a SIMD, by the registers and LDS; workgroups of a CU
+    static constexpr int kPerCu = D == 64 ? (kHalf ? (W == 8 ? 4 : 3) : 3) : 2;
+    static constexpr int kGroups = kPerCu * 4 / W;
     struct Smem {
         uint16_t k[2][kBN * kKPitch];
         uint16_t v[2][kBN * kVPitch];
@@ -226,8 +274,10 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-template <typename T, int D, int W>
-__global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void prompts_f8_kernel(PromptArgs a) {
+// WHOLE: pages of at least 16 keys, so that a wave's load, 8 or 16 rows, lies in one
+// page and is 1 KiB or half of that in a row.
+template <typename T, int D, int W, bool WHOLE>
+__global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8_kernel(PromptArgs a) {
     using F = Prompt8<T, D, W>;
     constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
     __shared__ __align__(16) typename F::Smem sm;
@@ -276,54 +326,63 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void pr
     float m = kStart, l = 0.0f;
     int wary = 0;  // tiles to go
 
-    // Staging: load i of the thread is row row0 + kRowStep i of the tile, 16 codes
-    // at `piece`. Pages are looked up a tile ahead of the codes.
+    // Staging: load i of the thread is row row0 + kRowStep i of the tile, kLoad
+    // codes at `piece`. Pages are looked up a tile ahead of the codes.
+    constexpr int kWords = F::kLoad / 4;
+    typedef uint32_t codes_t __attribute__((ext_vector_type(kWords)));
     const int row0 = tid / F::kPieces, piece = tid % F::kPieces;
     const int* pages = a.page_table + static_cast<int64_t>(t.s) * a.max_pages;
     int page[kPer];
-    u32x4 pk[kPer], pv[kPer];
+    codes_t pk[kPer], pv[kPer];
     uint32_t pks[kPer], pvs[kPer];
-    uint32_t ok = 0;  // by load: a key of the piece that there is
+    uint32_t ok = 0;  // by load: a key of the piece that there is (WHOLE: its page is)
     auto find_pages = [&](int key0) {
 #pragma unroll
-        for (int i = 0; i < kPer; i++) page[i] = pages[min(key0 + row0 + i * F::kRowStep, t.end - 1) >> a.page_shift];
+        for (int i = 0; i < kPer; i++) {
+            const int r = WHOLE ? wave * F::kWaveRows : row0;
+            page[i] = pages[min(key0 + r + i * F::kRowStep, t.end - 1) >> a.page_shift];
+        }
     };
     auto load = [&](int key0) {
         ok = 0;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
-            const int key = key0 + row0 + i * F::kRowStep;
-            const bool there = page[i] >= 0 && page[i] < a.n_pages && key < t.end;
+            const int key = key0 + (WHOLE ? wave * F::kWaveRows : row0) + i * F::kRowStep;
+            const bool there = page[i] >= 0 && page[i] < a.n_pages && (WHOLE || key < t.end);
             const int64_t block = static_cast<int64_t>(there ? page[i] : 0) * a.h_kv + t.kv;
-            const int64_t at = ((block << a.page_shift) + (there ? key & ((1 << a.page_shift) - 1) : 0)) * D + piece * 16;
-            pk[i] = ld16(a.k + at), pv[i] = ld16(a.v + at);
+            const int64_t at = ((block << a.page_shift) + (WHOLE || there ? key & ((1 << a.page_shift) - 1) : 0)) * D;
+            const uint32_t lane_at = WHOLE ? lane * F::kLoad : piece * F::kLoad;
+            pk[i] = *reinterpret_cast<const codes_t*>(a.k + at + lane_at);
+            pv[i] = *reinterpret_cast<const codes_t*>(a.v + at + lane_at);
             pks[i] = a.k_scale[block], pvs[i] = a.v_scale[block];
             ok |= there ? 1u << i : 0u;
         }
     };
     auto store = [&](int buf, int j) {
         const bool masked = j * kBN + kBN > tile_least;  // some row does not see all of these values
+        const bool last = j * kBN + kBN > t.end;
         bool odd = false;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
             const int r = row0 + i * F::kRowStep;
-            const bool there = ok >> i & 1;
-            if (piece == 0) sm.there[buf][r] = there;
-            if (!there && j * kBN + r < t.end) sm.gap[buf] = j;
-            const float ks = scale_value(pks[i]), vs = there ? scale_value(pvs[i]) : 1.0f;
-            const u32x4 codes = there ? pv[i] : u32x4{};
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                uint16_t* kp = &sm.k[buf][r * F::kKPitch + piece * 16 + 8 * half];
-                uint16_t* vp = &sm.v[buf][r * F::kVPitch + piece * 16 + 8 * half];
-                u32x4 x;
-                if constexpr (F::kHalf) {
-                    st16(kp, f16_of_codes(pk[i][2 * half], pk[i][2 * half + 1], ks));
-                    x = f16_of_codes(codes[2 * half], codes[2 * half + 1], vs);
-                } else {
-                    st16(kp, bf16_of_codes(pk[i][2 * half], pk[i][2 * half + 1], ks));
-                    x = bf16_of_codes(codes[2 * half], codes[2 * half + 1], vs);
+            float vs = scale_value(pvs[i]);
+            const float ks = scale_value(pks[i]);
+            if (WHOLE ? last || !(ok >> i & 1) : true) {
+                const bool there = (ok >> i & 1) && j * kBN + r < t.end;
+                if (piece == 0) sm.there[buf][r] = there;
+                if (!there) {
+                    if (j * kBN + r < t.end) sm.gap[buf] = j;
+                    pv[i] = codes_t{}, vs = 1.0f;
                 }
+            } else if (piece == 0) {
+                sm.there[buf][r] = 1;
+            }
+#pragma unroll
+            for (int half = 0; half < F::kLoad / 8; half++) {
+                uint16_t* kp = &sm.k[buf][r * F::kKPitch + piece * F::kLoad + 8 * half];
+                uint16_t* vp = &sm.v[buf][r * F::kVPitch + piece * F::kLoad + 8 * half];
+                st16(kp, values_of<T>(pk[i][2 * half], pk[i][2 * half + 1], ks));
+                u32x4 x = values_of<T>(pv[i][2 * half], pv[i][2 * half + 1], vs);
                 if (masked) {
                     constexpr uint32_t kExp = F::kHalf ? 0x7C00u : 0x7F80u;
 #pragma unroll
@@ -357,6 +416,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void pr
         if (key0 < wave_most) {
             // S^T: s[i] holds keys 32 i .. + 32 of the tile, register r of lane
             // (n, hh) key 8 (r / 4) + 4 hh + r % 4, row n
+            const bool gap = sm.gap[cur] == j;
             f32x16 s[2];
             const f32x16 z = {};
             const uint16_t* ka = sm.k[cur] + n * F::kKPitch + 8 * hh;
@@ -376,7 +436,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void pr
                     for (int r = 0; r < 16; r++)
                         if (key0 + 32 * i + 8 * (r / 4) + 4 * hh + r % 4 >= seen) s[i][r] = -INFINITY;
             }
-            if (sm.gap[cur] == j) {
+            if (gap) {
 #pragma unroll
                 for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -524,8 +584,8 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void pr
     }
     const float lsum = halves_sum(l);
     if (t.count > 1) {
-        const int64_t at = partial_row(a, t.item, t.kv, row - t.first);
-        float* p = a.ws_o + at * D + 4 * hh;
+        const int64_t block = partial_block(a, t.item, t.kv, wave);
+        float* p = a.ws_o + block * 32 * D + lane * 4;
 #pragma unroll
         for (int db = 0; db < DB; db++)
 #pragma unroll
@@ -533,8 +593,9 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void pr
                 u32x4 w;
 #pragma unroll
                 for (int e = 0; e < 4; e++) w[e] = f2u(o[db][4 * r4 + e]);
-                st16(p + 32 * db + 8 * r4, w);
+                st16_nt(p + (4 * db + r4) * 256, w);
             }
+        const int64_t at = block * 32 + n;
         if (hh == 0) a.ws_ml[2 * at] = m, a.ws_ml[2 * at + 1] = lsum;
         return;
     }
@@ -559,56 +620,103 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu * W / 4)) void pr
         }
 }
 
-// The pieces of one tile's rows joined, 256 / (D / 4) rows to a workgroup.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void prompts_join_kernel(PromptArgs a, int rows) {
-    constexpr int kLanes = D / 4, kGroupRows = 256 / kLanes;
-    const int per_tile = (a.pitch + kGroupRows - 1) / kGroupRows;
-    const int tile_head = static_cast<int>(blockIdx.x) / per_tile;
-    const int tile = tile_head / a.h_kv, kv = tile_head - tile * a.h_kv;
-    PromptItem c;
-    if (!find_item<true>(a, rows, tile, c)) return;
-    const PromptSeq s = sequence_at(a, c.s);
-    const int all = s.nq * a.group, first = (c.tiles - 1 - c.local) * rows, mine = min(rows, all - first);
-    const int count = pieces_seen(keys_seen(s, (first + mine - 1) / a.group, a.causal), c.chunk);
-    if (count == 1) return;  // written by its only piece
-    const int row = (static_cast<int>(blockIdx.x) - tile_head * per_tile) * kGroupRows + static_cast<int>(threadIdx.x) / kLanes;
-    const int col = threadIdx.x % kLanes;
-    if (row >= mine) return;
-    float top = kStart, weight = 0.0f;
-    f32x4 sum = {};
-    for (int i = 0; i < count; i++) {
-        const int64_t at = partial_row(a, c.item + i, kv, row);
-        const float m = a.ws_ml[2 * at], l = a.ws_ml[2 * at + 1];
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + at * D + 4 * col);
+// The pieces of one tile's rows joined, four channels of a row to a thread, as the
+// workspace has them; `share` workgroups to a tile. SPREAD: few tiles, a wave takes
+// every fourth piece of 64 threads' channels.
+struct Joined {
+    f32x4 sum;
+    float top, weight;
+    __device__ __forceinline__ void add(f32x4 v, float m, float l) {
         const float next = fmaxf(top, m);
         const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
         sum = sum * old + v * f;
         weight = fmaf(weight, old, l * f);
         top = next;
     }
-    T* orow = static_cast<T*>(a.out) + row_out(a, s, kv, first + row) * D + 4 * col;
+};
+template <typename T, int D, bool SPREAD>
+__global__ __launch_bounds__(256) void prompts_join_kernel(PromptArgs a, int share) {
+    constexpr int kParts = D / 32 * (SPREAD ? 4 : 1);  // of a block of 32 rows
+    __shared__ Joined others[3][SPREAD ? 64 : 1];
+    const int tile_head = static_cast<int>(blockIdx.x) / share;
+    const int tile = tile_head / a.h_kv, kv = tile_head - tile * a.h_kv;
+    const int4 c = a.cut[tile];
+    const int item = c.x, count = c.y, rows = c.w;
+    if (tile >= a.cut[a.tiles].x || count <= 1) return;  // written by its only piece
+    // (what offsets that do not ascend leave of a cut)
+    if (item < 0 || item + count > a.items || rows > 32 * a.blocks || c.z < 0 || c.z + rows > a.n * a.group) return;
+    const int lane = threadIdx.x % 64, wave = wave_in_block();
+    const int64_t step = static_cast<int64_t>(a.h_kv) * a.blocks;
+    for (int x = static_cast<int>(blockIdx.x) - tile_head * share; x < (rows + 31) / 32 * kParts; x += share) {
+        const int block = x / kParts, part = x - block * kParts, row = 32 * block + lane % 32;
+        const int at = SPREAD ? part : 4 * part + wave;  // 32 rows of 8 channels
+        const int64_t from = partial_block(a, item, kv, block);
+        const float* o = a.ws_o + from * 32 * D + (at * 64 + lane) * 4;
+        const float* ml = a.ws_ml + (from * 32 + lane % 32) * 2;
+        constexpr int kAhead = 4, kStep = SPREAD ? 4 : 1;  // pieces whose loads are under way at once
+        Joined j = {f32x4{}, kStart, 0.0f};
+        for (int i0 = SPREAD ? wave : 0; i0 < count; i0 += kAhead * kStep) {
+            f32x2 stat[kAhead];
+            f32x4 v[kAhead];
 #pragma unroll
-    for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(weight == 0.0f ? 0.0f : sum[e] / weight);
+            for (int i = 0; i < kAhead; i++) {
+                const int64_t piece = min(i0 + i * kStep, count - 1) * step;
+                stat[i] = *reinterpret_cast<const f32x2*>(ml + piece * 64);
+                v[i] = __builtin_bit_cast(f32x4, ld16_nt(o + piece * 32 * D));
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (i0 + i * kStep < count) j.add(v[i], stat[i].x, stat[i].y);
+        }
+        if constexpr (SPREAD) {
+            __syncthreads();  // the last round's have been read
+            if (wave > 0) others[wave - 1][lane] = j;
+            __syncthreads();
+            if (wave > 0) continue;
+#pragma unroll
+            for (int w = 0; w < 3; w++) j.add(others[w][lane].sum, others[w][lane].top, others[w][lane].weight);
+        }
+        if (row >= rows) continue;
+        const int all = c.z + row, token = all / a.group;
+        const int64_t to = static_cast<int64_t>(token) * a.h + kv * a.group + (all - token * a.group);
+        T* orow = static_cast<T*>(a.out) + to * D + 8 * at + 4 * (lane / 32);
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = j.weight == 0.0f ? 0.0f : j.sum[e] / j.weight;
+        if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<u32x2*>(orow) = u32x2{pk_f16(y[0], y[1]), pk_f16(y[2], y[3])};
+        else
+            *reinterpret_cast<f32x4*>(orow) = f32x4{y[0], y[1], y[2], y[3]};
+    }
 }
 
 // How a call is cut into tiles, and whether its keys are.
 struct PromptPlan {
     int64_t tiles;          // of a key head, as many as sequences of these rows can have
-    int64_t pieces, items;  // of a key head: wanted (0: whole keys), and what they can come to
-    int64_t pitch;
+    int64_t places, items;  // of a key head: on the chip at once (0: whole keys), and in the call at most
+    bool one_round;         // fewer tiles than places
+    int64_t blocks;  // of 32 rows of a tile
     int rows;
-    PromptPlan(hs_dtype dt, int64_t n, int64_t b, int64_t h, int64_t h_kv, int d, int64_t keys) {
-        const int64_t group = h / h_kv, slots = num_cus() * (d == 64 ? (dt == HS_F16 ? 3 : 2) : (dt == HS_F16 ? 2 : 1));
-        rows = 128;
+    PromptPlan(hs_dtype dt, int64_t n, int64_t b, int64_t h, int64_t h_kv, int d, int64_t keys, bool whole) {
+        const int64_t group = h / h_kv;
+        rows = whole && dt == HS_F16 && n * group / 256 * h_kv >= 2 * num_cus() && n >= 512 * b ? 256 : 128;
+        const int64_t slots = num_cus() * per_cu(dt, d, rows);
         tiles = n * group / rows + (b < n ? b : n);
-        pieces = 0, items = tiles, pitch = 0;
-        if (keys <= kLeastUnits * kBN || n * group / rows * h_kv >= 4 * slots) return;
-        pieces = ceil_div(2 * slots, h_kv);
-        items = 2 * pieces + tiles;
-        pitch = n * group < rows ? n * group : rows;
+        items = tiles, blocks = 0;
+        places = std::max<int64_t>(slots / h_kv, 1);
+        one_round = tiles < places;
+        if (keys <= kLeastUnits * kBN || tiles >= 8 * places) places = 0;
+        if (!places) return;
+        items = 3 * places + tiles;
+        blocks = ceil_div(std::min<int64_t>(n * group, rows), 32);
     }
-    int64_t workspace(int64_t h_kv, int d) const { return pieces ? items * h_kv * pitch * (d + 2) * 4 : 0; }
+    static int per_cu(hs_dtype dt, int d, int rows) {
+        const bool half = dt == HS_F16;
+        if (rows == 256) return d == 64 ? Prompt8<f16, 64, 8>::kGroups : Prompt8<f16, 128, 8>::kGroups;
+        return d == 64 ? (half ? Prompt8<f16, 64, 4>::kGroups : Prompt8<float, 64, 4>::kGroups)
+                       : (half ? Prompt8<f16, 128, 4>::kGroups : Prompt8<float, 128, 4>::kGroups);
+    }
+    int64_t workspace(int64_t h_kv, int d) const { return places ? (tiles + 1) * 16 + items * h_kv * blocks * 32 * (d + 2) * 4 : 0; }
 };
 
 }  // namespace
@@ -620,7 +728,7 @@ extern "C" int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int
     if (n <= 0 || b <= 0 || h <= 0 || causal < 0 || n >= (int64_t{1} << 30) / h || exact_log2(page) < 0 || max_pages < 0) return 0;
     if (static_cast<int64_t>(max_pages) * page >= (int64_t{1} << 30)) return 0;
     if (check_heads("attention_prompts_f8_workspace", dt, h, h_kv, d)) return 0;
-    return PromptPlan(dt, n, b, h, h_kv, d, static_cast<int64_t>(max_pages) * page).workspace(h_kv, d);
+    return PromptPlan(dt, n, b, h, h_kv, d, static_cast<int64_t>(max_pages) * page, page >= 16).workspace(h_kv, d);
 }
 
 extern "C" hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
@@ -650,28 +758,34 @@ extern "C" hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, co
     a.n = static_cast<int>(n), a.b = b, a.h = h, a.h_kv = h_kv, a.group = h / h_kv, a.page_shift = exact_log2(page);
     a.n_pages = n_pages, a.max_pages = n_pages > 0 ? max_pages : 0;  // no page to read: no sequence has keys
     a.causal = causal, a.scale = scale;
-    const PromptPlan plan(dt, n, b, h, h_kv, d, static_cast<int64_t>(max_pages) * page);
-    const int threads = 256;
+    const PromptPlan plan(dt, n, b, h, h_kv, d, static_cast<int64_t>(max_pages) * page, page >= 16);
+    const int threads = 2 * plan.rows;
     const int64_t groups = plan.items * h_kv;
     if (groups >= (int64_t{1} << 31) / threads) return fail(HS_EINVAL, "%s: too many sequences and heads", op);
-    a.ws_o = static_cast<float*>(workspace);
-    a.ws_ml = a.ws_o + (plan.pieces ? plan.items * h_kv * plan.pitch * d : 0);
-    // (rounded up by twice the error of the kernels' sum over the sequences)
-    a.per_piece = plan.pieces ? static_cast<float>((1.0 + (b / 64 + 64) * 0x1p-23) / static_cast<double>(plan.pieces)) : 0.0f;
-    a.items = static_cast<int>(plan.items), a.pitch = static_cast<int>(plan.pitch);
+    a.cut = static_cast<int4*>(workspace), a.tiles = static_cast<int>(plan.tiles);
+    a.ws_o = static_cast<float*>(workspace) + (plan.tiles + 1) * 4;
+    a.ws_ml = a.ws_o + (plan.places ? plan.items * h_kv * plan.blocks * 32 * d : 0);
+    a.places = static_cast<int>(plan.places), a.one_round = plan.one_round;
+    a.items = static_cast<int>(plan.items), a.blocks = static_cast<int>(plan.blocks);
     hipStream_t st = static_cast<hipStream_t>(stream);
-    const auto go = [&](auto kernel, auto join) {
+    const auto go = [&](auto kernel, auto join, auto spread) {
         kernel<<<dim3(static_cast<uint32_t>(groups)), dim3(threads), 0, st>>>(a);
         if (hs_status rc = check_launch(op)) return rc;
-        if (!plan.pieces) return HS_OK;
-        const int64_t blocks = plan.tiles * h_kv * ceil_div(plan.pitch, 256 / (d / 4));
-        join<<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, st>>>(a, plan.rows);
+        if (!plan.places) return HS_OK;
+        const int64_t heads = plan.tiles * h_kv, whole = plan.blocks * (d / 32);
+        const bool few = heads * whole < 4 * num_cus();
+        const int64_t share = few ? 4 * whole : heads < 4 * num_cus() ? whole : 1;
+        (few ? spread : join)<<<dim3(static_cast<uint32_t>(heads * share)), dim3(256), 0, st>>>(a, static_cast<int>(share));
         return check_launch(op);
     };
-    if (dt == HS_F16) {
-        if (d == 64) return go(prompts_f8_kernel<f16, 64, 4>, prompts_join_kernel<f16, 64>);
-        return go(prompts_f8_kernel<f16, 128, 4>, prompts_join_kernel<f16, 128>);
-    }
-    if (d == 64) return go(prompts_f8_kernel<float, 64, 4>, prompts_join_kernel<float, 64>);
-    return go(prompts_f8_kernel<float, 128, 4>, prompts_join_kernel<float, 128>);
+    const bool whole = page >= 16, wide = plan.rows == 256;
+    const auto pick = [&](auto zero) {
+        using T = decltype(zero);
+        if (d == 64)
+            return go(wide ? prompts_f8_kernel<f16, 64, 8, true> : whole ? prompts_f8_kernel<T, 64, 4, true> : prompts_f8_kernel<T, 64, 4, false>,
+                      prompts_join_kernel<T, 64, false>, prompts_join_kernel<T, 64, true>);
+        return go(wide ? prompts_f8_kernel<f16, 128, 8, true> : whole ? prompts_f8_kernel<T, 128, 4, true> : prompts_f8_kernel<T, 128, 4, false>,
+                  prompts_join_kernel<T, 128, false>, prompts_join_kernel<T, 128, true>);
+    };
+    return dt == HS_F16 ? pick(f16{}) : pick(float{});
 }
