@@ -35,6 +35,16 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// V floats by 16-byte loads.
+template <int V>
+__device__ __forceinline__ void ld_values(const float* p, float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V / 4; i++) {
+        const float4 x = ld_f32x4(p + 4 * i);
+        f[4 * i] = x.x, f[4 * i + 1] = x.y, f[4 * i + 2] = x.z, f[4 * i + 3] = x.w;
+    }
+}
+
 template <typename T>
 struct AppendArgs {
     const T *q, *k, *v;
@@ -80,12 +90,10 @@ __device__ __forceinline__ void append_rows(const AppendArgs<T>& a, int unit) {
             const float* cr = a.cos_tab + static_cast<int64_t>(row) * D;
             const float* sr = a.sin_tab + static_cast<int64_t>(row) * D;
             const float sign = kLine && piece < G / 2 ? -1.0f : 1.0f;
+            ld_values(cr + c, cl), ld_values(sr + c, sl);
 #pragma unroll
-            for (int e = 0; e < V; e++) cl[e] = cr[c + e], sl[e] = sign * sr[c + e];
-            if constexpr (!kLine) {
-#pragma unroll
-                for (int e = 0; e < V; e++) ch[e] = cr[c2 + e], sh[e] = sr[c2 + e];
-            }
+            for (int e = 0; e < V; e++) sl[e] *= sign;
+            if constexpr (!kLine) ld_values(cr + c2, ch), ld_values(sr + c2, sh);
         }
     }
     const int part = unit - token * a.parts;

@@ -1,5 +1,8 @@
 // A paged key-value cache held in 8 bits for gfx950: appending new tokens and the
 // attention of one new token per sequence.
+#include <algorithm>
+#include <type_traits>
+
 #include "hs_f8.hpp"
 
 namespace hs {
@@ -9,20 +12,25 @@ namespace {
 // kv_append
 //
 // A page's new keys of one head take a scale together, so a unit of work is one
-// (page of a sequence, head, k or v): its rows are read, normalised and rotated
-// into registers, their largest magnitude gives the scale, and the codes follow.
-// A page that the call goes on with keeps the larger scale of the two; where that
-// is the new one, the older codes are brought to it, which is exact but for those
-// that become subnormal.
+// page of a sequence, and its rows are read, normalised and rotated into registers,
+// their largest magnitude gives the scale, and the codes follow. A page that the
+// call goes on with keeps the larger scale of the two; where that is the new one, the
+// older codes are brought to it, which is exact but for those that become subnormal.
 //
-// A unit's rows are held by one wave where a page has at most 2048 / D, else by
-// four, kRowsHeld rows each; pages past that are read twice.
+// A page's rows are held by one wave where it has at most 2048 / D, else by two or
+// four; pages of more than four times that are read twice. A wave goes through several
+// heads' keys, or values, with the next head's rows under way, so that the place and
+// the rotation of its rows are looked up once.
+//
+// Prompts make two launches, of the queries' rows as kv_append's and of the pages,
+// which want different registers; a step is one.
 template <typename T>
 struct Append8Args {
     AppendArgs<T> rows;  // q, and k where its rows are asked for
     const int *offsets, *page_table, *lens;
     uint8_t *k_cache, *v_cache, *k_scale, *v_scale;
     int n_pages, row_blocks;
+    int split;  // waves (W of them: workgroups) that share a page's heads
 };
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -88,37 +96,54 @@ __device__ __forceinline__ bool find_unit(const Append8Args<T>& a, int index, Pa
 }
 
 template <typename T, int D, bool NORM, bool ROPE, int W>
-__device__ void append_page(const Append8Args<T>& a, int index) {
+__device__ __forceinline__ void append_page(const Append8Args<T>& a, int index) {
     const AppendArgs<T>& r = a.rows;
     constexpr int V = Vec<T>::N, G = D / (2 * V), kRows = 64 / G;  // rows per load
     constexpr int kHeld = 2048 / D, P = kHeld / kRows;             // rows and loads that a wave holds
-    __shared__ float tops[W];
+    __shared__ float tops[2][W];
     const int lane = lane_id(), wave = W == 1 ? 0 : wave_in_block();
-    const int units = 2 * r.h_kv;
-    const int unit = index / units, which = index - unit * units;
-    const bool is_v = which >= r.h_kv;
-    const int head = is_v ? which - r.h_kv : which;
+    const int unit = index / (2 * a.split), which = index - unit * 2 * a.split;
+    const bool is_v = which >= a.split;
     PageUnit t;
     if (!find_unit(a, unit, t)) return;  // the same for all waves of a unit
-    const T* src = (is_v ? r.v : r.k) + head * D;
     const int64_t stride = is_v ? r.v_stride : r.k_stride;
-    uint8_t* codes = (is_v ? a.v_cache : a.k_cache) + ((((static_cast<int64_t>(t.page) * r.h_kv + head) << r.page_shift)) * D);
-    uint8_t* scale = (is_v ? a.v_scale : a.k_scale) + static_cast<int64_t>(t.page) * r.h_kv + head;
-    const int old = t.first > 0 ? min(static_cast<int>(*scale), kScaleMost) : 0;
+    const T* rows = (is_v ? r.v : r.k) + t.token * stride;
+    const int64_t block0 = static_cast<int64_t>(t.page) * r.h_kv;
+    uint8_t* scales = (is_v ? a.v_scale : a.k_scale) + block0;
     const int piece = lane % G, c = piece * V, c2 = D / 2 + c;
+    const bool norm = NORM && !is_v && r.kn_w, rope = ROPE && !is_v;
+    const int rounds = W == 1 ? 1 : (t.rows + kHeld * W - 1) / (kHeld * W);
+    const auto row_of = [&](int round, int i) { return (round * W + wave) * kHeld + i * kRows + lane / G; };
 
-    // the transformed row's two chunks, 0 beyond the unit's rows
-    const auto load = [&](int row, float (&x)[V], float (&y)[V]) {
-        if (row >= t.rows) {
+    // a row's place in the tables, or none; kept for the rows of the only round
+    float cl[P][V], ch[P][V], sl[P][V], sh[P][V];
+    bool turns[P];
+    const auto find_turn = [&](int row, int i) {
+        turns[i] = false;
+        if (!rope || row >= t.rows) return;
+        const int at = r.positions ? r.positions[t.token + row] : t.pos + row;
+        turns[i] = at >= 0 && at < r.table_rows;
+        if (!turns[i]) return;
+        const float* cr = r.cos_tab + static_cast<int64_t>(at) * D;
+        const float* sr = r.sin_tab + static_cast<int64_t>(at) * D;
+        ld_values(cr + c, cl[i]), ld_values(cr + c2, ch[i]), ld_values(sr + c, sl[i]), ld_values(sr + c2, sh[i]);
+    };
+    u32x4 lo[P], hi[P];
+    const auto load = [&](int round, int head) {
 #pragma unroll
-            for (int e = 0; e < V; e++) x[e] = y[e] = 0.0f;
-            return;
+        for (int i = 0; i < P; i++) {
+            const int row = row_of(round, i);
+            lo[i] = hi[i] = u32x4{};
+            if (row >= t.rows) continue;
+            const T* p = rows + row * stride + head * D;
+            lo[i] = ld_stream(p + c), hi[i] = ld_stream(p + c2);
         }
-        const T* p = src + (t.token + row) * stride;
-        unpack(ld_stream(p + c), x, T{});
-        unpack(ld_stream(p + c2), y, T{});
-        if (is_v) return;
-        if (NORM && r.kn_w) {
+    };
+    // load i's two chunks as the cache is to take them
+    const auto turned = [&](int i, float (&x)[V], float (&y)[V]) {
+        unpack(lo[i], x, T{});
+        unpack(hi[i], y, T{});
+        if (norm) {
             float sum = 0.0f, sq = 0.0f;
 #pragma unroll
             for (int e = 0; e < V; e++) sum += x[e] + y[e];
@@ -126,113 +151,141 @@ __device__ void append_page(const Append8Args<T>& a, int index) {
 #pragma unroll
             for (int e = 0; e < V; e++) sq = fmaf(x[e] - mean, x[e] - mean, fmaf(y[e] - mean, y[e] - mean, sq));
             const float inv = rsqrtf(lanes_sum<G>(sq) * (1.0f / D) + r.eps);
+            float wl[V], wh[V], bl[V], bh[V];
+            ld_values(r.kn_w + c, wl), ld_values(r.kn_w + c2, wh), ld_values(r.kn_b + c, bl), ld_values(r.kn_b + c2, bh);
 #pragma unroll
             for (int e = 0; e < V; e++) {
-                x[e] = fmaf((x[e] - mean) * inv, r.kn_w[c + e], r.kn_b[c + e]);
-                y[e] = fmaf((y[e] - mean) * inv, r.kn_w[c2 + e], r.kn_b[c2 + e]);
+                x[e] = fmaf((x[e] - mean) * inv, wl[e], bl[e]);
+                y[e] = fmaf((y[e] - mean) * inv, wh[e], bh[e]);
             }
         }
-        if constexpr (ROPE) {
-            const int at = r.positions ? r.positions[t.token + row] : t.pos + row;
-            if (at >= 0 && at < r.table_rows) {
-                const float* cr = r.cos_tab + static_cast<int64_t>(at) * D;
-                const float* sr = r.sin_tab + static_cast<int64_t>(at) * D;
+        if (rope && turns[i]) {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+                const float u = x[e], v = y[e];
+                x[e] = fmaf(u, cl[i][e], -(v * sl[i][e]));
+                y[e] = fmaf(v, ch[i][e], u * sh[i][e]);
+            }
+        }
+    };
+    const auto held = [&](float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -kHeldMost<T>), kHeldMost<T>) : x; };
+
+    const int head0 = is_v ? which - a.split : which;
+    load(rounds - 1, head0);
+    if (rounds == 1) {
+#pragma unroll
+        for (int i = 0; i < P; i++) find_turn(row_of(0, i), i);
+    }
+    int turn = 0;
+    for (int head = head0; head < r.h_kv; head += a.split, turn ^= 1) {
+        uint8_t* codes = (is_v ? a.v_cache : a.k_cache) + ((block0 + head) << r.page_shift) * D;
+        const int old = t.first > 0 ? min(static_cast<int>(scales[head]), kScaleMost) : 0;
+        float x[P][V], y[P][V], most = 0.0f;
+        for (int round = rounds - 1; round >= 0; round--) {
+            if (round < rounds - 1) load(round, head);
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+                if (rounds > 1) find_turn(row_of(round, i), i);
+                turned(i, x[i], y[i]);
+                if (row_of(round, i) >= t.rows) continue;
 #pragma unroll
                 for (int e = 0; e < V; e++) {
-                    const float u = x[e], v = y[e];
-                    x[e] = fmaf(u, cr[c + e], -(v * sr[c + e]));
-                    y[e] = fmaf(v, cr[c2 + e], u * sr[c2 + e]);
+                    const float m = fabsf(x[i][e]), n = fabsf(y[i][e]);
+                    most = fmaxf(most, fmaxf(m < INFINITY ? m : 0.0f, n < INFINITY ? n : 0.0f));
                 }
             }
         }
-    };
-    const auto most_of = [&](float most, const float (&x)[V]) {
+        if (rounds == 1 && head + a.split < r.h_kv) load(0, head + a.split);
+        most = wave_max(most);
+        if constexpr (W > 1) {
+            if (lane == 0) tops[turn][wave] = most;
+            __syncthreads();  // (every wave has read the old scale, too)
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float m = fabsf(x[e]);
-            most = fmaxf(most, m < INFINITY ? m : 0.0f);
+            for (int w = 0; w < W; w++) most = fmaxf(most, tops[turn][w]);
         }
-        return most;
-    };
-    const auto held = [&](float x) { return fabsf(x) < INFINITY ? fminf(fmaxf(x, -kHeldMost<T>), kHeldMost<T>) : x; };
-    const auto put = [&](int row, const float (&x)[V], const float (&y)[V], float inv) {
-        if (row >= t.rows) return;
-        uint8_t* p = codes + static_cast<int64_t>(t.first + row) * D;
+        const int next = max(old, scale_for(fminf(most, kHeldMost<T>)));
+        const float inv = scale_value(2 * kScaleBias - next);
+        for (int round = 0; round < rounds; round++) {
+            if (round > 0) load(round, head);
 #pragma unroll
-        for (int half = 0; half < 2; half++) {
-            const float(&z)[V] = half ? y : x;
-            uint32_t w[V / 4];
+            for (int i = 0; i < P; i++) {
+                const int row = row_of(round, i);
+                if (round > 0) {
+                    find_turn(row, i);
+                    turned(i, x[i], y[i]);
+                }
+                if (row >= t.rows) continue;
+                uint8_t* p = codes + (t.first + row) * D;
 #pragma unroll
-            for (int i = 0; i < V / 4; i++)
-                w[i] = codes_of(held(z[4 * i]) * inv, held(z[4 * i + 1]) * inv, held(z[4 * i + 2]) * inv, held(z[4 * i + 3]) * inv);
-            uint32_t* at = reinterpret_cast<uint32_t*>(p + (half ? c2 : c));
-            if constexpr (V == 8)
-                *reinterpret_cast<u32x2*>(at) = u32x2{w[0], w[1]};
-            else
-                *at = w[0];
+                for (int half = 0; half < 2; half++) {
+                    const float(&z)[V] = half ? y[i] : x[i];
+                    uint32_t w[V / 4];
+#pragma unroll
+                    for (int e = 0; e < V / 4; e++)
+                        w[e] = codes_of(held(z[4 * e]) * inv, held(z[4 * e + 1]) * inv, held(z[4 * e + 2]) * inv, held(z[4 * e + 3]) * inv);
+                    uint32_t* at = reinterpret_cast<uint32_t*>(p + (half ? c2 : c));
+                    if constexpr (V == 8)
+                        *reinterpret_cast<u32x2*>(at) = u32x2{w[0], w[1]};
+                    else
+                        *at = w[0];
+                }
+            }
         }
-    };
-
-    // the first of the wave's rows in round `round`, and of its i-th load's for this lane
-    const auto row_of = [&](int round, int i) { return (round * W + wave) * kHeld + i * kRows + lane / G; };
-    float x[P][V], y[P][V], most = 0.0f;
-    const int rounds = W == 1 ? 1 : (t.rows + kHeld * W - 1) / (kHeld * W);
-    for (int round = rounds - 1; round >= 0; round--)
+        if (next > old && t.first > 0) {
+            for (int i = (wave * 64 + lane) * 16; i < t.first * D; i += W * 1024) {
+                u32x4 w = ld16(codes + i);
 #pragma unroll
-        for (int i = 0; i < P; i++) {
-            load(row_of(round, i), x[i], y[i]);
-            most = most_of(most_of(most, x[i]), y[i]);
+                for (int e = 0; e < 4; e++) w[e] = codes_down(w[e], next - old);
+                st16(codes + i, w);
+            }
         }
-    most = wave_max(most);
-    if constexpr (W > 1) {
-        if (lane == 0) tops[wave] = most;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < W; w++) most = fmaxf(most, tops[w]);
+        if (wave == 0 && lane == 0) scales[head] = static_cast<uint8_t>(next);
+        if (rounds > 1 && head + a.split < r.h_kv) load(rounds - 1, head + a.split);
     }
-    const int next = max(old, scale_for(fminf(most, kHeldMost<T>)));
-    const float inv = scale_value(2 * kScaleBias - next);
-    for (int round = 0; round < rounds; round++)
-#pragma unroll
-        for (int i = 0; i < P; i++) {
-            if (round > 0) load(row_of(round, i), x[i], y[i]);
-            put(row_of(round, i), x[i], y[i], inv);
-        }
-    if (t.first > 0 && next > old) {
-        for (int i = (wave * 64 + lane) * 16; i < t.first * D; i += W * 1024) {
-            u32x4 w = ld16(codes + i);
-#pragma unroll
-            for (int e = 0; e < 4; e++) w[e] = codes_down(w[e], next - old);
-            st16(codes + i, w);
-        }
-    }
-    // (each wave has read the old scale: through the barrier above, or it is alone)
-    if (wave == 0 && lane == 0) *scale = static_cast<uint8_t>(next);
 }
 
-template <typename T, int D, bool NORM, bool ROPE, int W>
+// A call's rows, then its pages.
+template <typename T, int D, bool NORM, bool ROPE>
 __global__ __launch_bounds__(256) void kv_append_f8_kernel(Append8Args<T> a) {
     const int block = blockIdx.x;
     if (block < a.row_blocks)
         append_rows<T, D, NORM, ROPE>(a.rows, block * 4 + wave_in_block());
-    else if constexpr (W == 1)
-        append_page<T, D, NORM, ROPE, 1>(a, (block - a.row_blocks) * 4 + wave_in_block());
     else
-        append_page<T, D, NORM, ROPE, W>(a, block - a.row_blocks);
+        append_page<T, D, NORM, ROPE, 1>(a, (block - a.row_blocks) * 4 + wave_in_block());
+}
+template <typename T, int D, bool NORM, bool ROPE>
+__global__ __launch_bounds__(256) void append_rows_kernel(Append8Args<T> a) {
+    append_rows<T, D, NORM, ROPE>(a.rows, static_cast<int>(blockIdx.x) * 4 + wave_in_block());
+}
+template <typename T, int D, bool NORM, bool ROPE, int W>
+__global__ __launch_bounds__(W == 2 ? 128 : 256) void append_pages_kernel(Append8Args<T> a) {
+    append_page<T, D, NORM, ROPE, W>(a, W == 1 ? static_cast<int>(blockIdx.x) * 4 + wave_in_block() : static_cast<int>(blockIdx.x));
 }
 
-template <typename T, int D, int W>
-void launch_append_f8(hipStream_t st, const Append8Args<T>& a, uint32_t blocks) {
-    const dim3 grid(blocks);
-    const bool norm = a.rows.qn_w || a.rows.kn_w, rope = a.rows.sin_tab != nullptr;
-    if (norm && rope)
-        kv_append_f8_kernel<T, D, true, true, W><<<grid, dim3(256), 0, st>>>(a);
-    else if (norm)
-        kv_append_f8_kernel<T, D, true, false, W><<<grid, dim3(256), 0, st>>>(a);
-    else if (rope)
-        kv_append_f8_kernel<T, D, false, true, W><<<grid, dim3(256), 0, st>>>(a);
+template <typename T, int D, bool NORM, bool ROPE>
+hs_status launch_append_f8(const char* op, hipStream_t st, Append8Args<T> a, int64_t row_blocks, int64_t pages) {
+    const int h_kv = a.rows.h_kv, page = 1 << a.rows.page_shift;
+    a.row_blocks = static_cast<int>(row_blocks);
+    if (!a.offsets) {
+        a.split = h_kv;
+        const int64_t blocks = row_blocks + ceil_div(pages * 2 * h_kv, 4);
+        kv_append_f8_kernel<T, D, NORM, ROPE><<<dim3(static_cast<uint32_t>(blocks)), dim3(256), 0, st>>>(a);
+        return check_launch(op);
+    }
+    const int waves = page <= 2048 / D ? 1 : page <= 4096 / D ? 2 : 4;
+    // a page's heads by so many waves that the chip has 16 waves a CU
+    a.split = static_cast<int>(std::clamp<int64_t>(ceil_div(int64_t{16} * num_cus(), 2 * pages * waves), 1, h_kv));
+    const int64_t units = pages * 2 * a.split;
+    const auto go = [&](auto kernel, int64_t blocks, int threads) { kernel<<<dim3(static_cast<uint32_t>(blocks)), dim3(threads), 0, st>>>(a); };
+    if (waves == 1)
+        go(append_pages_kernel<T, D, NORM, ROPE, 1>, ceil_div(units, 4), 256);
+    else if (waves == 2)
+        go(append_pages_kernel<T, D, NORM, ROPE, 2>, units, 128);
     else
-        kv_append_f8_kernel<T, D, false, false, W><<<grid, dim3(256), 0, st>>>(a);
+        go(append_pages_kernel<T, D, NORM, ROPE, 4>, units, 256);
+    if (hs_status rc = check_launch(op)) return rc;
+    if (row_blocks) append_rows_kernel<T, D, NORM, ROPE><<<dim3(static_cast<uint32_t>(row_blocks)), dim3(256), 0, st>>>(a);
+    return check_launch(op);
 }
 
 // ---------------------------------------------------------------------------
@@ -558,10 +611,8 @@ extern "C" hs_status hs_kv_append_f8(hs_stream_t stream, hs_dtype dt, const void
     const int parts = static_cast<int>(ceil_div(heads, dt == HS_F16 ? 1024 / d : 512 / d));
     const int64_t row_blocks = ceil_div(n * parts, 4);
     // pages that the tokens can lie in, at most
-    const bool wide = offsets && page > 2048 / d;
-    const int64_t pages = (offsets ? n / page + 2 * std::min<int64_t>(b, n) : b) * 2 * h_kv;
-    const int64_t page_blocks = wide ? pages : ceil_div(pages, 4);
-    if (row_blocks + page_blocks >= (int64_t{1} << 24)) return fail(HS_EINVAL, "%s: too many tokens", op);
+    const int64_t pages = offsets ? n / page + 2 * std::min<int64_t>(b, n) : b;
+    if (row_blocks + pages * 2 * h_kv >= (int64_t{1} << 23)) return fail(HS_EINVAL, "%s: too many tokens", op);
     const auto run = [&](auto zero) {
         using T = decltype(zero);
         Append8Args<T> a;
@@ -572,19 +623,17 @@ extern "C" hs_status hs_kv_append_f8(hs_stream_t stream, hs_dtype dt, const void
         a.lens = static_cast<const int*>(lens);
         a.k_cache = static_cast<uint8_t*>(k_cache), a.v_cache = static_cast<uint8_t*>(v_cache);
         a.k_scale = static_cast<uint8_t*>(k_scale), a.v_scale = static_cast<uint8_t*>(v_scale);
-        a.n_pages = n_pages, a.row_blocks = static_cast<int>(row_blocks);
+        a.n_pages = n_pages;
         const auto st = static_cast<hipStream_t>(stream);
-        const uint32_t blocks = static_cast<uint32_t>(row_blocks + page_blocks);
-        if (d == 64)
-            wide ? launch_append_f8<T, 64, 4>(st, a, blocks) : launch_append_f8<T, 64, 1>(st, a, blocks);
-        else
-            wide ? launch_append_f8<T, 128, 4>(st, a, blocks) : launch_append_f8<T, 128, 1>(st, a, blocks);
+        const bool norm = qn_w || kn_w, rope = sin_tab;
+        const auto go = [&](auto dim) {
+            constexpr int D = decltype(dim)::value;
+            if (norm) return rope ? launch_append_f8<T, D, true, true>(op, st, a, row_blocks, pages) : launch_append_f8<T, D, true, false>(op, st, a, row_blocks, pages);
+            return rope ? launch_append_f8<T, D, false, true>(op, st, a, row_blocks, pages) : launch_append_f8<T, D, false, false>(op, st, a, row_blocks, pages);
+        };
+        return d == 64 ? go(std::integral_constant<int, 64>{}) : go(std::integral_constant<int, 128>{});
     };
-    if (dt == HS_F16)
-        run(f16{});
-    else
-        run(float{});
-    return check_launch(op);
+    return dt == HS_F16 ? run(f16{}) : run(float{});
 }
 
 extern "C" int64_t hs_attention_paged_f8_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d) {
