@@ -298,17 +298,23 @@ hs_status launch_append_f8(const char* op, hipStream_t st, Append8Args<T> a, int
 // their way to the wave's slice of LDS, from which V^T takes P^T. What the codes
 // leave to round is the query and the weights: in f16 weights go as two f16 values
 // of 11 bits each (the queries are f16), in f32 both go as three bf16 ones, which
-// hold all 24 bits. 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 107
-// us, 4.8 TB/s; one token over 130531 keys of 16 heads of 64 58 us, 4.6 TB/s; eight
-// f32 sequences of up to 800, 16 heads of 128, 13 us.
+// hold all 24 bits.
+//
+// 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 104 us, 5.0 TB/s, of
+// which the join is 5 (the same loads with nothing computed: 98); one token over
+// 130531 keys of 16 heads of 64 54 us, 5.0 TB/s (48); eight f32 sequences of up to
+// 800, 16 heads of 128, 13 us. Steps of 64 keys at head dim 64 take 30 us for 34 of 32
+// where pages hold 8 keys, and at 128 spill; pieces of units of 256 keys 29 us for 33
+// of 128 (20 sequences of up to 3001, 16 heads of 128).
 //
 // A lane's 16-byte load of a row of K is 16 dims, two operands of 8: dims 64 i +
 // 16 g + 8 e, which the queries follow.
 template <typename T, int D>
 struct Paged8 {
     static constexpr bool kHalf = sizeof(T) == 2;
-    static constexpr int kStep = 32;
-    static constexpr int kUnit = kPagedWaves * kStep;
+    static constexpr int kStep = D == 64 ? 64 : 32;  // keys per wave and step, 4 KiB of each of K and V
+    static constexpr int kKeys = kPagedWaves * kStep;  // of the workgroup and step
+    static constexpr int kUnit = 256;                  // of which pieces are made
     static constexpr int kParts = kHalf ? 1 : 3;    // of a query value
     static constexpr int kSums = kHalf ? 2 : 3;     // of a weight
     static constexpr int kTiles = kStep / 16;
@@ -318,10 +324,10 @@ struct Paged8 {
     static constexpr int kVLoads = kStep / kVRows;
     static constexpr int kPitch = D + 16;           // (hs_paged.hip)
     static constexpr int kOPitch = D + 4;
-    static constexpr int kPerCu = kHalf || D == 64 ? 4 : 3;  // workgroups, by their registers
+    static constexpr int kPerCu = D == 64 ? 4 : 3;  // workgroups, by their registers
     struct Smem {
         union {
-            uint16_t v[kPagedWaves][kStep * kPitch];
+            uint16_t v[kPagedWaves][32 * kPitch];  // half of a step's keys at a time
             float o[kPagedWaves][kGroup * kOPitch];
         };
         float m[kPagedWaves][kGroup], l[kPagedWaves][kGroup];
@@ -410,12 +416,13 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
             if (!WHOLE && tile.there && key < end) k_ok |= 1u << i;
         }
     };
-    auto load_v = [&](int key0) {
-        v_ok = 0;
+    // of the half-step h, from key key0 + 32 h on
+    constexpr int kHalfLoads = P::kVLoads / (kStep / 32);
+    auto load_v = [&](int key0, int h) {
         if constexpr (WHOLE) {
             constexpr int kPer = P::kVLoads / kTiles;
 #pragma unroll
-            for (int i = 0; i < kTiles; i++) {
+            for (int i = 2 * h; i < 2 * h + 2; i++) {
                 const Tile16 tile = tile_of(a, page[i], kv, key0 + 16 * i);
                 const uint8_t* p = vb + tile.row * D;
 #pragma unroll
@@ -424,8 +431,9 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
                 v_end[i] = tile.there ? end : 0;
             }
         } else {
+            v_ok &= ~(((1u << kHalfLoads) - 1) << h * kHalfLoads);
 #pragma unroll
-            for (int i = 0; i < P::kVLoads; i++) {
+            for (int i = h * kHalfLoads; i < (h + 1) * kHalfLoads; i++) {
                 const int key = key0 + P::kVRows * i + v_row;
                 const Tile16 tile = tile_of(a, page_of(key), kv, key);
                 if (tile.there && key < end) v_ok |= 1u << i;
@@ -444,34 +452,14 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
     const int start = begin + wave * kStep;
     if (start < end) {
         if (WHOLE) find_pages(start);
-        load_v(start);
         load_k(start);
-        if (WHOLE) find_pages(start + P::kUnit);
+#pragma unroll
+        for (int h = 0; h < kStep / 32; h++) load_v(start, h);
+        if (WHOLE) find_pages(start + P::kKeys);
     }
 #pragma unroll 1
-    for (int key0 = start; key0 < end; key0 += P::kUnit) {
-        const bool more = key0 + P::kUnit < end;
-        // rows that are not there count as zeros: their weight is 0, and 0
-        // times what they hold may not be
-        bool gaps = !WHOLE && __any(v_ok != (1u << P::kVLoads) - 1);
-#pragma unroll
-        for (int i = 0; i < kTiles; i++) gaps |= WHOLE && key0 + 16 * i + 16 > v_end[i];
-        if (gaps) {
-#pragma unroll
-            for (int i = 0; i < P::kVLoads; i++)
-                if (WHOLE ? key0 + P::kVRows * i + v_row >= v_end[P::kVRows * i / 16] : !(v_ok >> i & 1)) vr[i] = u32x4{};
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-        for (int i = 0; i < P::kVLoads; i++) {
-            const float scale = scale_value(vx[WHOLE ? P::kVRows * i / 16 : i]);
-            uint16_t* p = vs + (P::kVRows * i + v_row) * P::kPitch + v_col;
-            st16(p, values_of<T>(vr[i][0], vr[i][1], scale));
-            st16(p + 8, values_of<T>(vr[i][2], vr[i][3], scale));
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (more) load_v(key0 + P::kUnit);
-
+    for (int key0 = start; key0 < end; key0 += P::kKeys) {
+        const bool more = key0 + P::kKeys < end;
         // S^T: register j of lane (n, g) is key 16 i + 4 g + j, query head n
         f32x4 sc[kTiles];
 #pragma unroll
@@ -508,10 +496,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
                 some |= there != 0;
             }
         }
-        if (more) {
-            load_k(key0 + P::kUnit);
-            if (WHOLE) find_pages(key0 + 2 * P::kUnit);
-        }
+        if (more) load_k(key0 + P::kKeys);
 
         // rounded before the maximum is taken off: that one then weighs 1
         float mx = -INFINITY;
@@ -539,9 +524,29 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
         l = fmaf(l, corr, sum);
 #pragma unroll
         for (int i = 0; i < DB; i++) o[i] *= corr;
-        // O^T += V^T P^T
+        // O^T += V^T P^T, 32 keys at a time
 #pragma unroll
-        for (int h = 0; h < kTiles / 2; h++) {
+        for (int h = 0; h < kStep / 32; h++) {
+            // rows that are not there count as zeros: their weight is 0, and 0
+            // times what they hold may not be
+            bool gaps = !WHOLE && __any((v_ok >> h * kHalfLoads & ((1u << kHalfLoads) - 1)) != (1u << kHalfLoads) - 1);
+#pragma unroll
+            for (int i = 2 * h; i < 2 * h + 2; i++) gaps |= WHOLE && key0 + 16 * i + 16 > v_end[i];
+            if (gaps) {
+#pragma unroll
+                for (int i = h * kHalfLoads; i < (h + 1) * kHalfLoads; i++)
+                    if (WHOLE ? key0 + P::kVRows * i + v_row >= v_end[P::kVRows * i / 16] : !(v_ok >> i & 1)) vr[i] = u32x4{};
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+            for (int i = h * kHalfLoads; i < (h + 1) * kHalfLoads; i++) {
+                const float scale = scale_value(vx[WHOLE ? P::kVRows * i / 16 : i]);
+                uint16_t* p = vs + (P::kVRows * (i - h * kHalfLoads) + v_row) * P::kPitch + v_col;
+                st16(p, values_of<T>(vr[i][0], vr[i][1], scale));
+                st16(p + 8, values_of<T>(vr[i][2], vr[i][3], scale));
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (more) load_v(key0 + P::kKeys, h);
             u32x4 p[P::kSums];
             if constexpr (P::kHalf) {
 #pragma unroll
@@ -561,7 +566,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
                 for (int e = 0; e < 8; e++) x[e] = sc[2 * h + e / 4][e % 4];
                 cut3(x, p);
             }
-            const uint16_t* va = vs + (32 * h + 4 * g + n / 4) * P::kPitch + 4 * (n % 4);
+            const uint16_t* va = vs + (4 * g + n / 4) * P::kPitch + 4 * (n % 4);
 #pragma unroll
             for (int i = 0; i < DB; i++) {
                 const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + 16 * i)));
@@ -572,6 +577,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
                 for (int x = P::kSums - 1; x >= 0; x--) o[i] = mfma16<T>(w, p[x], o[i]);
             }
         }
+        if (WHOLE && more) find_pages(key0 + 2 * P::kKeys);
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
