@@ -16,7 +16,6 @@ namespace hs {
 namespace {
 
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / 64;
 constexpr int kLongest = 1 << 30;  // tokens of a sequence
 
 struct PlanArgs {
@@ -50,32 +49,32 @@ __device__ __forceinline__ int page_taken(const PlanArgs& a, const Ring& r, cons
     return s.taken >= 0 && at < r.count ? *ring_at(a, r, at) : -1;
 }
 
-template <typename V>
-__device__ __forceinline__ V wave_scan(V v) {
-    const int lane = lane_id();
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const V u = __shfl_up(v, d, 64);
-        if (lane >= d) v += u;
-    }
-    return v;
+// Sums over this lane and the ones before it. 64 bits in two parts: 64 times 16 bits
+// and 64 times 31 - 16 stay whole.
+__device__ __forceinline__ int64_t wave_sums(int64_t v) {
+    const int lo = wave_prefix_sum(static_cast<int>(v & 0xFFFF)), hi = wave_prefix_sum(static_cast<int>(v >> 16));
+    return (static_cast<int64_t>(hi) << 16) + lo;
+}
+__device__ __forceinline__ int64_t lane_value64(int64_t v, int lane) {
+    const uint32_t lo = lane_value(static_cast<int>(v), lane);
+    return (static_cast<int64_t>(lane_value(static_cast<int>(v >> 32), lane)) << 32) | lo;
 }
 
-// The sequences' shares, `keep` taking each; lens, offsets and the ring's state as
-// the call leaves them. All threads of the workgroup call it and get the ring as it
-// was.
-template <typename K>
+// The sequences' shares, `keep` taking each and its first row; lens, offsets and the
+// ring's state as the call leaves them. All threads of the workgroup (W waves) call
+// it and get the ring as it was.
+template <int W, typename K>
 __device__ __forceinline__ Ring make_shares(const PlanArgs& a, K keep) {
-    __shared__ int64_t sums[kPlanWaves][4];
+    __shared__ int64_t sums[W][4];
     const int lane = lane_id(), wave = wave_in_block();
     Ring ring = {a.state[0], a.state[1]};
     ring.count = min(max(ring.count, 0), a.n_pages);
     ring.head = a.n_pages > 0 && ring.head >= 0 ? ring.head % a.n_pages : 0;
-    int64_t asked = 0, back = 0, rows = 0, wanted = 0;  // by the sequences before
-    for (int base = 0; base < a.b; base += kPlanThreads) {
+    int64_t before[4] = {0, 0, 0, 0};  // by the sequences before: pages asked for, given back, new tokens, pages wanted
+    for (int base = 0; base < a.b; base += 64 * W) {
         const int s = base + static_cast<int>(threadIdx.x);
         Share t = {0, 0, 0, -1, 0};
-        int64_t v[4] = {0, 0, 0, 0};  // pages asked for, given back, new tokens, pages wanted
+        int64_t v[4] = {0, 0, 0, 0};
         int after = 0;
         if (s < a.b) {
             const int change = a.counts[s];
@@ -85,64 +84,71 @@ __device__ __forceinline__ Ring make_shares(const PlanArgs& a, K keep) {
             const int all_have = entries_of(t.old, a.page_shift), all_want = entries_of(after, a.page_shift);
             t.have = min(all_have, a.max_pages), t.want = min(all_want, a.max_pages);
             const int* entries = a.page_table + static_cast<int64_t>(s) * a.max_pages;
-            t.end = t.want;
-            if (t.want > t.have && (t.have == 0 || is_page(a, entries[t.have - 1]))) v[0] = t.want - t.have;
+            // Entries are pages up to the first that was not there, so the last says
+            // whether all are.
+            const bool whole = t.have == 0 || is_page(a, entries[t.have - 1]);
+            t.end = t.have;
+            if (t.want > t.have && whole) v[0] = t.want - t.have;
             if (t.want < t.have) {
-                int lo = t.want, hi = t.have;  // the first entry that is no page
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (is_page(a, entries[mid]))
-                        lo = mid + 1;
-                    else
-                        hi = mid;
+                if (!whole) {
+                    int lo = t.want, hi = t.have - 1;
+                    while (lo < hi) {
+                        const int mid = (lo + hi) >> 1;
+                        if (is_page(a, entries[mid]))
+                            lo = mid + 1;
+                        else
+                            hi = mid;
+                    }
+                    t.end = lo;
                 }
-                t.end = lo, v[1] = lo - t.want;
+                v[1] = t.end - t.want;
             }
             v[2] = max(change, 0);
             v[3] = max(all_want - all_have, 0);
         }
         int64_t mine[4];
+        mine[0] = wave_prefix_sum(static_cast<int>(v[0])), mine[1] = wave_prefix_sum(static_cast<int>(v[1]));  // below 2^31: the table's entries
+        mine[2] = wave_sums(v[2]), mine[3] = wave_sums(v[3]);
+        if (lane == 63) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            mine[i] = wave_scan(v[i]);
-            if (lane == 63) sums[wave][i] = mine[i];
+            for (int i = 0; i < 4; i++) sums[wave][i] = mine[i];
         }
         __syncthreads();
-        int64_t before[4] = {asked, back, rows, wanted}, total[4] = {asked, back, rows, wanted};
-        for (int w = 0; w < kPlanWaves; w++)
+        int64_t first[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (w < wave) before[i] += sums[w][i];
-                total[i] += sums[w][i];
-            }
-        __syncthreads();  // sums are written again
-        if (s < a.b) {
-            const int64_t first = v[0] > 0 ? before[0] + mine[0] - v[0] : v[1] > 0 ? before[1] + mine[1] - v[1] : -1;
-            t.taken = static_cast<int>(first);
-            keep(s, t);
-            a.lens[s] = after;
-            a.offsets[s + 1] = static_cast<int>(min(before[2] + mine[2], int64_t{INT_MAX}));
+        for (int i = 0; i < 4; i++) {
+            const int64_t total = wave_sums(lane < W ? sums[lane][i] : 0);
+            first[i] = before[i] + (wave > 0 ? lane_value64(total, wave - 1) : 0) + mine[i] - v[i];
+            before[i] += lane_value64(total, W - 1);
         }
-        asked = total[0], back = total[1], rows = total[2], wanted = total[3];
+        if (base + 64 * W < a.b) __syncthreads();  // sums are written again
+        if (s < a.b) {
+            t.taken = static_cast<int>(v[0] > 0 ? first[0] : v[1] > 0 ? first[1] : -1);
+            const int row = static_cast<int>(min(first[2], int64_t{INT_MAX})), next = static_cast<int>(min(first[2] + v[2], int64_t{INT_MAX}));
+            keep(s, t, next);
+            if (s == 0) a.offsets[0] = row;
+            a.lens[s] = after;
+            a.offsets[s + 1] = next;
+        }
     }
     if (threadIdx.x == 0) {
-        const int taken = static_cast<int>(min(asked, static_cast<int64_t>(ring.count)));
-        const int given = static_cast<int>(min(back, static_cast<int64_t>(a.n_pages - ring.count)));
-        a.offsets[0] = 0;
+        const int taken = static_cast<int>(min(before[0], static_cast<int64_t>(ring.count)));
+        const int given = static_cast<int>(min(before[1], static_cast<int64_t>(a.n_pages - ring.count)));
+        if (a.b == 0) a.offsets[0] = 0;
         a.state[0] = a.n_pages > 0 ? (ring.head + taken) % a.n_pages : 0;
         a.state[1] = ring.count - taken + given;
-        a.state[2] = static_cast<int>(min(wanted - taken, int64_t{INT_MAX}));
+        a.state[2] = static_cast<int>(min(before[3] - taken, int64_t{INT_MAX}));
     }
     return ring;
 }
 
-// A sequence's entries, by one wave.
-__device__ __forceinline__ void fill_entries(const PlanArgs& a, const Ring& r, int s, const Share& t) {
+// A sequence's entries, `step` lanes of them at a time, this one the lane-th.
+__device__ __forceinline__ void fill_entries(const PlanArgs& a, const Ring& r, int s, const Share& t, int lane, int step) {
     int* entries = a.page_table + static_cast<int64_t>(s) * a.max_pages;
-    for (int e = t.have + lane_id(); e < t.want; e += 64) entries[e] = page_taken(a, r, t, e);
-    for (int e = t.want + lane_id(); e < t.have; e += 64) {
-        const int at = r.count + t.taken + e - t.want;
-        if (e < t.end && at < a.n_pages) *ring_at(a, r, at) = entries[e];
+    for (int e = t.have + lane; e < t.want; e += step) entries[e] = page_taken(a, r, t, e);
+    for (int e = t.want + lane; e < t.have; e += step) {
+        const int64_t at = static_cast<int64_t>(r.count) + t.taken + e - t.want;
+        if (e < t.end && at < a.n_pages) *ring_at(a, r, static_cast<int>(at)) = entries[e];
         entries[e] = -1;
     }
 }
@@ -158,16 +164,36 @@ __device__ __forceinline__ void place_token(const PlanArgs& a, const Ring& r, in
     a.slots[row] = is_page(a, page) ? (static_cast<int64_t>(page) << a.page_shift) + (pos & ((1 << a.page_shift) - 1)) : -1;
 }
 
-// Short calls: at most kPlanThreads sequences.
-__global__ __launch_bounds__(kPlanThreads) void plan_short_kernel(PlanArgs a) {
-    __shared__ Share shares[kPlanThreads];
-    const Ring ring = make_shares(a, [&](int s, const Share& t) { shares[s] = t; });
-    __syncthreads();  // shares and offsets
-    for (int s = wave_in_block(); s < a.b; s += kPlanWaves) fill_entries(a, ring, s, shares[s]);
-    const int rows = min(a.offsets[a.b], a.n);
-    for (int row = threadIdx.x; row < rows; row += kPlanThreads) {
-        const int s = sequence_of(a.offsets, a.b, row);
-        if (s >= 0) place_token(a, ring, s, shares[s], row, row - a.offsets[s]);
+// Short calls, of as many sequences as the workgroup has threads. A sequence that
+// moves a few pages is its thread's, one of more a wave's.
+constexpr int kFewPages = 4;
+
+template <int W>
+__global__ __launch_bounds__(64 * W) void plan_short_kernel(PlanArgs a) {
+    __shared__ Share shares[64 * W];
+    __shared__ int offsets[64 * W + 1];
+    const Ring ring = make_shares<W>(a, [&](int s, const Share& t, int next) { shares[s] = t, offsets[s + 1] = next; });
+    if (threadIdx.x == 0) offsets[0] = 0;
+    __syncthreads();
+    const auto moved = [](const Share& t) { return abs(t.want - t.have); };
+    const int mine = threadIdx.x;
+    const bool many = mine < a.b && moved(shares[mine]) > kFewPages;
+    if (mine < a.b && !many) fill_entries(a, ring, mine, shares[mine], 0, 1);
+    for (uint64_t left = __ballot(many); left; left &= left - 1) {  // each wave its own threads' sequences
+        const int s = wave_in_block() * 64 + __builtin_ctzll(left);
+        fill_entries(a, ring, s, shares[s], lane_id(), 64);
+    }
+    const int rows = min(offsets[a.b], a.n);
+    for (int row = threadIdx.x; row < rows; row += 64 * W) {
+        int lo = 0, hi = a.b;  // the first sequence that ends behind the row
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (offsets[mid + 1] <= row)
+                lo = mid + 1;
+            else
+                hi = mid;
+        }
+        place_token(a, ring, lo, shares[lo], row, row - offsets[lo]);
     }
 }
 
@@ -175,7 +201,7 @@ __device__ __forceinline__ int4 packed_share(const Share& t) { return {t.old, t.
 
 __global__ __launch_bounds__(kPlanThreads) void plan_shares_kernel(PlanArgs a) {
     int* ends = reinterpret_cast<int*>(a.plan + a.b + 1);
-    const Ring ring = make_shares(a, [&](int s, const Share& t) { a.plan[s] = packed_share(t), ends[s] = t.end; });
+    const Ring ring = make_shares<kPlanThreads / 64>(a, [&](int s, const Share& t, int) { a.plan[s] = packed_share(t), ends[s] = t.end; });
     if (threadIdx.x == 0) a.plan[a.b] = {ring.head, ring.count, 0, 0};
 }
 
@@ -190,7 +216,7 @@ __global__ __launch_bounds__(256) void plan_rest_kernel(PlanArgs a, int entry_bl
     const int block = blockIdx.x;
     if (block < entry_blocks) {
         const int s = block * 4 + wave_in_block();
-        if (s < a.b) fill_entries(a, ring, s, share(s));
+        if (s < a.b) fill_entries(a, ring, s, share(s), lane_id(), 64);
         return;
     }
     const int64_t row = static_cast<int64_t>(block - entry_blocks) * 256 + threadIdx.x;
@@ -251,7 +277,10 @@ extern "C" hs_status hs_plan_pages(hs_stream_t stream, const void* counts, void*
     a.n = static_cast<int>(n), a.b = b, a.page_shift = exact_log2(page), a.n_pages = n_pages, a.max_pages = max_pages;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (need == 0) {
-        plan_short_kernel<<<dim3(1), dim3(kPlanThreads), 0, st>>>(a);
+        if (b <= 256 && n <= 1024)
+            plan_short_kernel<4><<<dim3(1), dim3(256), 0, st>>>(a);
+        else
+            plan_short_kernel<kPlanThreads / 64><<<dim3(1), dim3(kPlanThreads), 0, st>>>(a);
         return check_launch(op);
     }
     plan_shares_kernel<<<dim3(1), dim3(kPlanThreads), 0, st>>>(a);
