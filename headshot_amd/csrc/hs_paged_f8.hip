@@ -215,7 +215,7 @@ __device__ __forceinline__ void append_page(const Append8Args<T>& a, int index) 
                     turned(i, x[i], y[i]);
                 }
                 if (row >= t.rows) continue;
-                uint8_t* p = codes + (t.first + row) * D;
+                uint8_t* p = codes + static_cast<int64_t>(t.first + row) * D;
 #pragma unroll
                 for (int half = 0; half < 2; half++) {
                     const float(&z)[V] = half ? y[i] : x[i];
@@ -232,7 +232,7 @@ __device__ __forceinline__ void append_page(const Append8Args<T>& a, int index) 
             }
         }
         if (next > old && t.first > 0) {
-            for (int i = (wave * 64 + lane) * 16; i < t.first * D; i += W * 1024) {
+            for (int64_t i = (wave * 64 + lane) * 16; i < static_cast<int64_t>(t.first) * D; i += W * 1024) {
                 u32x4 w = ld16(codes + i);
 #pragma unroll
                 for (int e = 0; e < 4; e++) w[e] = codes_down(w[e], next - old);
@@ -618,7 +618,7 @@ extern "C" hs_status hs_kv_append_f8(hs_stream_t stream, hs_dtype dt, const void
     const int64_t row_blocks = ceil_div(n * parts, 4);
     // pages that the tokens can lie in, at most
     const int64_t pages = offsets ? n / page + 2 * std::min<int64_t>(b, n) : b;
-    if (row_blocks + pages * 2 * h_kv >= (int64_t{1} << 23)) return fail(HS_EINVAL, "%s: too many tokens", op);
+    if (row_blocks + ceil_div(pages * 2 * h_kv, page <= 2048 / d || !offsets ? 4 : 1) >= (int64_t{1} << 23)) return fail(HS_EINVAL, "%s: too many tokens", op);
     const auto run = [&](auto zero) {
         using T = decltype(zero);
         Append8Args<T> a;

@@ -76,7 +76,7 @@ __device__ __forceinline__ PromptSeq sequence_at(const PromptArgs& a, int s) {
 // Keys that the sequence's query i sees.
 __device__ __forceinline__ int keys_seen(const PromptSeq& t, int i, int causal) {
     if (causal == 0) return t.nk;
-    const int at = i + t.len - t.nq;
+    const int at = t.len - (t.nq - i);
     if (at < 0) return 0;
     const int64_t end = causal == 1 ? static_cast<int64_t>(at) + 1 : (static_cast<int64_t>(at / causal) + 1) * causal;
     return end < t.nk ? static_cast<int>(end) : t.nk;

@@ -473,7 +473,10 @@ hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int
  * nearest even. Magnitudes past 61440 (HS_F16) or 15/8 2^127 (HS_F32) are held as
  * that; infinities and NaN as NaN. Whoever begins a page sets its scale, so the
  * pages of a new sequence need no values. No page takes new tokens of two
- * sequences in one call. */
+ * sequences in one call. HS_EINVAL at 2^23 workgroups: four tokens' q (k) rows of
+ * 1024 (HS_F16) or 512 elements each, and of the n / page + 2 b pages that the
+ * tokens can lie in (b without offsets) times 2 Hkv four each, or one each where a
+ * page has more than 2048 / D rows. */
 hs_status hs_kv_append_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                           const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                           const float* qn_w, const float* qn_b, const float* kn_w,

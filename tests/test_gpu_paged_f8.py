@@ -441,6 +441,71 @@ def test_prompts_longer(ctx, dtype, d, h, h_kv, page, new, past, causal):
     gpu_check(got, q, c, offsets_of(new), new, lens, causal, dtype, "prompts")
 
 
+@pytest.mark.parametrize("d,h,h_kv,page,new,past,causal", [
+    (64, 16, 16, 16, [8300], [0], 1),           # eight waves, head dim 64
+    (128, 32, 8, 16, [4200], [3000], 1),        # and 128
+    (128, 32, 8, 64, [4100], [100], 700),
+    (128, 32, 8, 32, [2100, 40, 1], [0, 9000, 5], 1),  # many tiles, one sequence's much longer
+])
+def test_prompts_that_fill_the_chip(ctx, d, h, h_kv, page, new, past, causal):
+    gen = torch.Generator().manual_seed(d + page)
+    lens = [a + b for a, b in zip(new, past)]
+    _, c = make_cache(gen, lens, h_kv, page, d, F16)
+    q = torch.randn((sum(new), h, d), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).half()
+    off = offsets_of(new)
+    got = ctx.attention_paged_prompts(q, c, i32(off), causal=causal).unflatten(1, (h, d))
+    # each head's first, last and some middle rows against 64 bits; the rest against the same tokens asked for in
+    # pieces, whose tiles are other ones (both are off by at most their bounds)
+    for s, (m, length) in enumerate(zip(new, lens)):
+        pick = sorted({0, m - 1, *range(0, m, max(1, m // 60))})
+        k, v = (gpu_values(c, x, s, length) for x in "kv")
+        seen = R.seen_keys(m, length, causal)[pick]
+        qs = q[off[s]:off[s + 1]][pick]
+        ref, mag = (torch.empty(len(pick), h, d, dtype=torch.float64) for _ in range(2))
+        hidden = torch.arange(length, device=DEV) >= seen.to(DEV)[:, None]
+        for i in range(h):
+            j = i // (h // h_kv)
+            p = torch.softmax((qs[:, i].double() @ k[:, j].T / math.sqrt(d)).masked_fill(hidden, -math.inf), 1)
+            ref[:, i], mag[:, i] = (p @ v[:, j]).cpu(), (p @ v[:, j].abs()).cpu()
+        bound = R.attention_bound(ref, mag, qs.cpu(), k.cpu(), v.cpu(), seen, 1 / math.sqrt(d), F16)
+        R.assert_within(got[off[s]:off[s + 1]][pick], ref, bound, f"sequence {s}")
+    # the last 300 tokens of the first sequence alone
+    tail = min(300, new[0])
+    alone = PagedKV8(*parts_of(c)[:4], c.page_table[:1].contiguous(), i32([lens[0]]), F16)
+    a, b = off[1] - tail, off[1]
+    other = ctx.attention_paged_prompts(q[a:b], alone, i32([0, tail]), causal=causal).unflatten(1, (h, d))
+    assert ((got[a:b].double() - other.double()).abs().amax() <= 2 * bound.amax().item())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_wide_tiles_leave_masked_values_alone(ctx, dtype):
+    """Calls of eight-wave tiles: NaN in keys and values that later tokens see, and pages that are not there."""
+    gen = torch.Generator().manual_seed(5)
+    h, d, n, page = 16, 64, 8192 + 300, 32
+    cpu, c = make_cache(gen, [n], h, page, d, dtype)
+    q = torch.randn((n, h, d), generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).to(dtype)
+    off = i32([0, n])
+    clean = ctx.attention_paged_prompts(q, c, off, causal=1)
+    at = int(cpu.page_table[0, 5000 // page])
+    bits(c.v)[at, :, 5000 % page, 7] = 0x7F
+    bits(c.k)[int(cpu.page_table[0, 8000 // page]), :, 8000 % page] = 0xFF
+    got = ctx.attention_paged_prompts(q, c, off, causal=1)
+    assert torch.equal(got[:5000], clean[:5000])
+    rows = got.unflatten(1, (h, d))
+    assert rows[5000:8000, :, 7].isnan().all() and rows[8000:].isnan().all()
+    keep = [x for x in range(d) if x != 7]
+    assert torch.equal(rows[5000:8000, :, keep], clean.unflatten(1, (h, d))[5000:8000, :, keep])
+    # the pages of keys [0, 64) and [7000, 8192 + 300) not there: as if the sequence had none of them
+    c.page_table[0, :2] = -1
+    c.page_table[0, 7008 // page:] = -1
+    got = ctx.attention_paged_prompts(q[:1000], PagedKV8(*parts_of(c)[:4], c.page_table, i32([1000]), dtype), i32([0, 1000]), causal=1)
+    short = PagedKV8(*parts_of(c)[:4], c.page_table[:, 2:].contiguous(), i32([1000 - 64]), dtype)
+    want = ctx.attention_paged_prompts(q[64:1000], short, i32([0, 1000 - 64]), causal=1)
+    assert (got[:64] == 0).all()
+    eps = torch.finfo(dtype).eps  # another order of sums, values below 448 2^-5 = 14
+    assert ((got[64:].double() - want.double()).abs() <= 32 * eps * 14).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_longer(ctx, dtype):
     gen = torch.Generator().manual_seed(3)
