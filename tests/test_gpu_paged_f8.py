@@ -504,6 +504,9 @@ def test_wide_tiles_leave_masked_values_alone(ctx, dtype):
     assert (got[:64] == 0).all()
     eps = torch.finfo(dtype).eps  # another order of sums, values below 448 2^-5 = 14
     assert ((got[64:].double() - want.double()).abs() <= 32 * eps * 14).all()
+    whole = ctx.attention_paged_prompts(q, c, off, causal=1)
+    assert (whole[:64] == 0).all()
+    assert ((whole[64:1000].double() - want.double()).abs() <= 32 * eps * 14).all()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
