@@ -721,7 +721,8 @@ struct PromptPlan {
         items = tiles, blocks = 0;
         places = std::max<int64_t>(slots / h_kv, 1);
         one_round = tiles < places;
-        if (keys <= kLeastUnits * kBN || tiles >= 8 * places) places = 0;
+        // (a workspace for every item that there can be, some 200 MB at the most)
+        if (keys <= kLeastUnits * kBN || tiles >= 4 * places) places = 0;
         if (!places) return;
         items = 3 * places + tiles;
         blocks = ceil_div(std::min<int64_t>(n * group, rows), 32);
