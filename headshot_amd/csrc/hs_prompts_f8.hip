@@ -122,31 +122,49 @@ __device__ __forceinline__ int wave_most(int v) {
 }
 __device__ __forceinline__ bool find_item(const PromptArgs& a, int rows, int index, PromptItem& t) {
     const int lane = lane_id();
-    float fair = 16777216.0f;
+    // of the sequence base + lane: its tiles, and its keys in units
+    const auto sizes = [&](int base) {
+        if (base + lane >= a.b) return int2{0, 0};
+        const PromptSeq s = sequence_at(a, base + lane);
+        return int2{tiles_of(a, s.nq, rows), (s.nk + kBN - 1) / kBN};
+    };
+    const int2 first = sizes(0);  // read once: few calls have more than 64
+    float fair = 16777216.0f, most = fair;
     if (a.places > 0) {
-        float total = 0.0f;
-        for (int base = 0; base < a.b; base += 64)
-            if (base + lane < a.b) {
+        float total = 0.0f, tiles = 0.0f;
+        for (int base = 0; base < a.b; base += 64) {
+            const int2 x = base ? sizes(base) : first;
+            int masked = 0;
+            if (a.causal && base + lane < a.b) {
                 const PromptSeq s = sequence_at(a, base + lane);
-                const int masked = a.causal ? max(min(s.nq, s.nk) - a.causal, 0) : 0;
-                total += static_cast<float>(tiles_of(a, s.nq, rows)) *
-                         (static_cast<float>((s.nk + kBN - 1) / kBN) - static_cast<float>(masked) * (0.5f / kBN));
+                masked = max(min(s.nq, s.nk) - a.causal, 0);
             }
-        fair = fmaxf(wave_sum(total) / static_cast<float>(a.places), static_cast<float>(kLeastUnits));
+            total += static_cast<float>(x.x) * (static_cast<float>(x.y) - static_cast<float>(masked) * (0.5f / kBN));
+            tiles += static_cast<float>(x.x);
+        }
+        const float places = static_cast<float>(a.places);
+        fair = fmaxf(wave_sum(total) / places, static_cast<float>(kLeastUnits));
+        most = fair;
+        if (a.one_round && a.b > 1) {
+            most = fair * places / (places - 0.5f * fminf(wave_sum(tiles), places));
+            float items = 0.0f;
+            for (int base = 0; base < a.b; base += 64) {
+                const int2 x = base ? sizes(base) : first;
+                items += static_cast<float>(x.x) * ceilf(static_cast<float>(x.y) / most);
+            }
+            most *= fmaxf(wave_sum(items) / places, 1.0f);
+        }
     }
     int tiles_before = 0, items_before = 0;
     for (int base = 0; base < a.b; base += 64) {
-        int tiles = 0, pieces = 1, chunk = 1;
-        if (base + lane < a.b) {
-            const PromptSeq s = sequence_at(a, base + lane);
-            const int units = (s.nk + kBN - 1) / kBN;
-            tiles = tiles_of(a, s.nq, rows);
-            if (a.one_round)
-                pieces = max(static_cast<int>(static_cast<float>(units) / fair), 1);
-            else if (static_cast<float>(units) > fair + kLonger)
-                pieces = static_cast<int>(ceilf(static_cast<float>(units) / (0.75f * fair)));
-            chunk = max((units + pieces - 1) / pieces, 1);
-        }
+        const int2 x = base ? sizes(base) : first;
+        const int tiles = x.x, units = x.y;
+        int pieces = 1;
+        if (a.one_round)
+            pieces = max(static_cast<int>(a.b > 1 ? ceilf(static_cast<float>(units) / most) : static_cast<float>(units) / fair), 1);
+        else if (static_cast<float>(units) > fair + kLonger)
+            pieces = static_cast<int>(ceilf(static_cast<float>(units) / (0.75f * fair)));
+        const int chunk = max((units + pieces - 1) / pieces, 1);
         // the sequences of long pieces first, by quarters of the longest, so that a
         // call does not end on them
         int tile_sum = 0, item_sum = 0, tile_end = 0, item_end = 0;
