@@ -53,6 +53,20 @@ __device__ __forceinline__ u32x4 values_of(uint32_t lo, uint32_t hi, float scale
     return sizeof(T) == 2 ? f16_of_codes(lo, hi, scale) : bf16_of_codes(lo, hi, scale);
 }
 
+// NaN among 8 values turned into zeros; whether there was any.
+template <typename T>
+__device__ __forceinline__ bool zero_nan(u32x4& x) {
+    constexpr uint32_t kExp = sizeof(T) == 2 ? 0x7C00u : 0x7F80u;
+    bool any = false;
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        const uint32_t keep = ((x[w] & kExp) == kExp ? 0u : 0xFFFFu) | ((x[w] & kExp << 16) == kExp << 16 ? 0u : 0xFFFF0000u);
+        any |= keep != 0xFFFFFFFFu;
+        x[w] &= keep;
+    }
+    return any;
+}
+
 // 4 values to 4 codes, rounded to nearest even. (In range: a finite value past
 // 448 would become NaN.)
 __device__ __forceinline__ uint32_t codes_of(float a, float b, float c, float d) {

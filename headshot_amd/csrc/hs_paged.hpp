@@ -288,7 +288,8 @@ struct Tile16 {
     int64_t row;
     bool there;
 };
-__device__ __forceinline__ Tile16 tile_of(const PagedArgs& a, int page, int kv, int key) {
+template <typename A>
+__device__ __forceinline__ Tile16 tile_of(const A& a, int page, int kv, int key) {
     const bool there = page >= 0 && page < a.n_pages;
     return {((static_cast<int64_t>(there ? page : 0) * a.h_kv + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1)), there};
 }

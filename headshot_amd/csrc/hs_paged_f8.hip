@@ -3,7 +3,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "hs_f8.hpp"
+#include "hs_steps_f8.hpp"
 
 namespace hs {
 namespace {
@@ -307,32 +307,21 @@ hs_status launch_append_f8(const char* op, hipStream_t st, Append8Args<T> a, int
 // 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 104 us, 5.0 TB/s, of
 // which the join is 5 (the same loads with nothing computed: 98); one token over
 // 130531 keys of 16 heads of 64 54 us, 5.0 TB/s (48); eight f32 sequences of up to
-// 800, 16 heads of 128, 13 us. Steps of 64 keys at head dim 64 take 30 us for 34 of 32
-// where pages hold 8 keys, and at 128 spill; pieces of units of 256 keys 29 us for 33
+// 800, 16 heads of 128, 13 us; 32 sequences of up to 4000, 16 heads of 64, 33 (f32 35),
+// over pages of 8 keys 35 (38). Steps of 64 keys at head dim 64 take 30 us for 34 of 32,
+// and at 128 spill; pieces of units of 256 keys 29 us for 33
 // of 128 (20 sequences of up to 3001, 16 heads of 128).
-//
-// A lane's 16-byte load of a row of K is 16 dims, two operands of 8: dims 64 i +
-// 16 g + 8 e, which the queries follow.
 template <typename T, int D>
-struct Paged8 {
-    static constexpr bool kHalf = sizeof(T) == 2;
-    static constexpr int kStep = D == 64 ? 64 : 32;  // keys per wave and step, 4 KiB of each of K and V
-    static constexpr int kKeys = kPagedWaves * kStep;  // of the workgroup and step
-    static constexpr int kUnit = 256;                  // of which pieces are made
-    static constexpr int kParts = kHalf ? 1 : 3;    // of a query value
-    static constexpr int kSums = kHalf ? 2 : 3;     // of a weight
-    static constexpr int kTiles = kStep / 16;
-    static constexpr int KL = D / 64;               // loads of a lane per row of K
-    static constexpr int kRowLanes = D / 16;        // lanes per row of V
-    static constexpr int kVRows = 64 / kRowLanes;   // rows per load of a wave
-    static constexpr int kVLoads = kStep / kVRows;
-    static constexpr int kPitch = D + 16;           // (hs_paged.hip)
-    static constexpr int kOPitch = D + 4;
-    static constexpr int kPerCu = D == 64 ? 4 : 3;  // workgroups, by their registers
+struct Paged8 : Steps8<T, D, 1> {
+    using S = Steps8<T, D, 1>;
+    static constexpr int kUnit = 256;               // keys of which pieces are made
+    // workgroups of a CU, by their registers (with one more, spilled: the f32 figures
+    // above 74 and 106 us)
+    static constexpr int per_cu(bool whole) { return D == 64 ? (S::kHalf && whole ? 4 : 3) : S::kHalf || whole ? 3 : 2; }
     struct Smem {
         union {
-            uint16_t v[kPagedWaves][32 * kPitch];  // half of a step's keys at a time
-            float o[kPagedWaves][kGroup * kOPitch];
+            uint16_t v[kPagedWaves][32 * S::kPitch];  // half of a step's keys at a time
+            float o[kPagedWaves][kGroup * S::kOPitch];
         };
         float m[kPagedWaves][kGroup], l[kPagedWaves][kGroup];
     };
@@ -342,23 +331,10 @@ struct Paged8Args : PagedArgs {
     const uint8_t *k_scale, *v_scale;
 };
 
-template <typename T>
-__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (sizeof(T) == 2)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(a), as_h8(b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// WHOLE: pages of at least 16 keys, so that 16 keys from a multiple of 16 lie in
-// one page; else each row looks its own up.
 template <typename T, int D, bool WHOLE>
-__global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void attention_paged_f8_kernel(Paged8Args a) {
+__global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::per_cu(WHOLE))) void attention_paged_f8_kernel(Paged8Args a) {
     using P = Paged8<T, D>;
-    constexpr int kStep = P::kStep, KL = P::KL, kTiles = P::kTiles;
     __shared__ __align__(16) typename P::Smem sm;
-    const int lane = lane_id(), wave = wave_in_block();
-    const int n = lane & 15, g = lane >> 4;
 
     Piece t;
     if (!find_piece(a, P::kUnit, t)) return;  // workgroup-uniform, before any barrier
@@ -366,232 +342,19 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::kPerCu)) void atte
     const int live_heads = min(a.width, a.group - pass * a.width);
     const int head0 = kv * a.group + pass * a.width;
 
-    // Q^T as the B operand, column n the query head (a copy of the last beyond
-    // them); a negative scale is taken as one of -q
-    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1.4e-45f);
-    u32x4 qa[2 * KL][P::kParts];
-    {
-        const T* qr = static_cast<const T*>(a.q) + s * a.q_stride + (head0 + min(n, live_heads - 1)) * D;
-#pragma unroll
-        for (int i = 0; i < 2 * KL; i++) {
-            const T* p = qr + 64 * (i / 2) + 16 * g + 8 * (i % 2);
-            if constexpr (P::kHalf) {
-                qa[i][0] = ld16(p);
-                if (a.scale < 0.0f) qa[i][0] ^= 0x80008000u;
-            } else {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = a.scale < 0.0f ? -p[e] : p[e];
-                cut3(x, qa[i]);
-            }
-        }
-    }
-
-    const int* pages = a.page_table + static_cast<int64_t>(s) * a.max_pages;
-    const uint8_t* kb = static_cast<const uint8_t*>(a.k);
-    const uint8_t* vb = static_cast<const uint8_t*>(a.v);
-    auto page_of = [&](int key) { return pages[min(key, end - 1) >> a.page_shift]; };
-    auto scale_of = [&](const uint8_t* scales, const Tile16& tile) {
-        return tile.there ? scales[tile.row >> a.page_shift] : static_cast<uint8_t>(kScaleBias);
-    };
-    u32x4 kr[kTiles * KL], vr[P::kVLoads];
-    // WHOLE: of the step's 16-key tiles, their pages, and the keys up to which
-    // those loaded are there; else by row of the lane
-    int page[kTiles], k_end[kTiles], v_end[kTiles];
-    uint32_t ks[kTiles], vx[WHOLE ? kTiles : P::kVLoads];  // scales as kept
-    uint32_t k_ok = 0, v_ok = 0;
-    const int v_row = lane / P::kRowLanes, v_col = lane % P::kRowLanes * 16;
-    const uint32_t k_lane = n * D + 16 * g, v_lane = v_row * D + v_col;
-    auto find_pages = [&](int key0) {
-#pragma unroll
-        for (int i = 0; i < kTiles; i++) page[i] = page_of(key0 + 16 * i);
-    };
-    auto load_k = [&](int key0) {
-        k_ok = 0;
-#pragma unroll
-        for (int i = 0; i < kTiles; i++) {
-            const int key = key0 + 16 * i + (WHOLE ? 0 : n);
-            const Tile16 tile = tile_of(a, WHOLE ? page[i] : page_of(key), kv, key);
-            const uint8_t* p = kb + tile.row * D + (WHOLE ? k_lane : 16 * g);
-#pragma unroll
-            for (int x = 0; x < KL; x++) kr[i * KL + x] = ld16_nt(p + 64 * x);
-            ks[i] = scale_of(a.k_scale, tile);
-            k_end[i] = tile.there ? end : 0;
-            if (!WHOLE && tile.there && key < end) k_ok |= 1u << i;
-        }
-    };
-    // of the half-step h, from key key0 + 32 h on
-    constexpr int kHalfLoads = P::kVLoads / (kStep / 32);
-    auto load_v = [&](int key0, int h) {
-        if constexpr (WHOLE) {
-            constexpr int kPer = P::kVLoads / kTiles;
-#pragma unroll
-            for (int i = 2 * h; i < 2 * h + 2; i++) {
-                const Tile16 tile = tile_of(a, page[i], kv, key0 + 16 * i);
-                const uint8_t* p = vb + tile.row * D;
-#pragma unroll
-                for (int x = 0; x < kPer; x++) vr[i * kPer + x] = ld16_nt(p + v_lane + P::kVRows * x * D);
-                vx[i] = scale_of(a.v_scale, tile);
-                v_end[i] = tile.there ? end : 0;
-            }
-        } else {
-            v_ok &= ~(((1u << kHalfLoads) - 1) << h * kHalfLoads);
-#pragma unroll
-            for (int i = h * kHalfLoads; i < (h + 1) * kHalfLoads; i++) {
-                const int key = key0 + P::kVRows * i + v_row;
-                const Tile16 tile = tile_of(a, page_of(key), kv, key);
-                if (tile.there && key < end) v_ok |= 1u << i;
-                vr[i] = ld16_nt(vb + tile.row * D + v_col);
-                vx[i] = scale_of(a.v_scale, tile);
-            }
-        }
-    };
-
-    constexpr int DB = D / 16;
-    f32x4 o[DB];
-#pragma unroll
-    for (int i = 0; i < DB; i++) o[i] = f32x4{};
-    float m = kNone, l = 0.0f;  // l: this lane's keys only
-    uint16_t* vs = sm.v[wave];
-    const int start = begin + wave * kStep;
-    if (start < end) {
-        if (WHOLE) find_pages(start);
-        load_k(start);
-#pragma unroll
-        for (int h = 0; h < kStep / 32; h++) load_v(start, h);
-        if (WHOLE) find_pages(start + P::kKeys);
-    }
-#pragma unroll 1
-    for (int key0 = start; key0 < end; key0 += P::kKeys) {
-        const bool more = key0 + P::kKeys < end;
-        // S^T: register j of lane (n, g) is key 16 i + 4 g + j, query head n
-        f32x4 sc[kTiles];
-#pragma unroll
-        for (int i = 0; i < kTiles; i++) {
-            const float scale = scale_value(ks[i]);
-            f32x4 acc[2] = {f32x4{}, f32x4{}};
-#pragma unroll
-            for (int x = 0; x < 2 * KL; x++) {
-                const u32x4& codes = kr[i * KL + x / 2];
-                const u32x4 k = values_of<T>(codes[2 * (x % 2)], codes[2 * (x % 2) + 1], scale);
-#pragma unroll
-                for (int p = P::kParts - 1; p >= 0; p--) acc[x % 2] = mfma16<T>(k, qa[x][p], acc[x % 2]);
-            }
-            sc[i] = acc[0] + acc[1];
-        }
-        // scores of keys that are not there; the lane's are rows 4 g + j, which
-        // lanes 4 g + j have looked up
-        bool some = false;
-#pragma unroll
-        for (int i = 0; i < kTiles; i++) {
-            if constexpr (WHOLE) {
-                if (key0 + 16 * i + 16 > k_end[i]) {
-                    const int left = k_end[i] - key0 - 16 * i - 4 * g;
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        if (j >= left) sc[i][j] = -INFINITY;
-                }
-                some |= key0 + 16 * i < k_end[i];
-            } else {
-                const uint64_t there = __ballot(k_ok >> i & 1);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (!(there >> (4 * g + j) & 1)) sc[i][j] = -INFINITY;
-                some |= there != 0;
-            }
-        }
-        if (more) load_k(key0 + P::kKeys);
-
-        // rounded before the maximum is taken off: that one then weighs 1
-        float mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < kTiles; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                sc[i][j] = as_f32(sc[i][j] * c);
-                mx = fmaxf(mx, sc[i][j]);
-            }
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float next = fmaxf(fmaxf(m, mx), some ? kFloor : kNone);
-        const float corr = __builtin_amdgcn_exp2f(m - next);
-        m = next;
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kTiles; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                sc[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - m);
-                if constexpr (P::kHalf) sc[i][j] *= kHalfUnit;
-                sum += sc[i][j];
-            }
-        l = fmaf(l, corr, sum);
-#pragma unroll
-        for (int i = 0; i < DB; i++) o[i] *= corr;
-        // O^T += V^T P^T, 32 keys at a time
-#pragma unroll
-        for (int h = 0; h < kStep / 32; h++) {
-            // rows that are not there count as zeros: their weight is 0, and 0
-            // times what they hold may not be
-            bool gaps = !WHOLE && __any((v_ok >> h * kHalfLoads & ((1u << kHalfLoads) - 1)) != (1u << kHalfLoads) - 1);
-#pragma unroll
-            for (int i = 2 * h; i < 2 * h + 2; i++) gaps |= WHOLE && key0 + 16 * i + 16 > v_end[i];
-            if (gaps) {
-#pragma unroll
-                for (int i = h * kHalfLoads; i < (h + 1) * kHalfLoads; i++)
-                    if (WHOLE ? key0 + P::kVRows * i + v_row >= v_end[P::kVRows * i / 16] : !(v_ok >> i & 1)) vr[i] = u32x4{};
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-            for (int i = h * kHalfLoads; i < (h + 1) * kHalfLoads; i++) {
-                const float scale = scale_value(vx[WHOLE ? P::kVRows * i / 16 : i]);
-                uint16_t* p = vs + (P::kVRows * (i - h * kHalfLoads) + v_row) * P::kPitch + v_col;
-                st16(p, values_of<T>(vr[i][0], vr[i][1], scale));
-                st16(p + 8, values_of<T>(vr[i][2], vr[i][3], scale));
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            if (more) load_v(key0 + P::kKeys, h);
-            u32x4 p[P::kSums];
-            if constexpr (P::kHalf) {
-#pragma unroll
-                for (int i = 0; i < 2; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j += 2) {
-                        const float x = sc[2 * h + i][j], y = sc[2 * h + i][j + 1];
-                        f16x2 w, r;
-                        w.x = static_cast<f16>(x), w.y = static_cast<f16>(y);
-                        r.x = static_cast<f16>(x - static_cast<float>(w.x));
-                        r.y = static_cast<f16>(y - static_cast<float>(w.y));
-                        p[0][2 * i + j / 2] = h22u(w), p[1][2 * i + j / 2] = h22u(r);
-                    }
-            } else {
-                float x[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) x[e] = sc[2 * h + e / 4][e % 4];
-                cut3(x, p);
-            }
-            const uint16_t* va = vs + (4 * g + n / 4) * P::kPitch + 4 * (n % 4);
-#pragma unroll
-            for (int i = 0; i < DB; i++) {
-                const u32x2 lo = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + 16 * i)));
-                const u32x2 hi = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(va + 16 * P::kPitch + 16 * i)));
-                u32x4 w;
-                w[0] = lo[0], w[1] = lo[1], w[2] = hi[0], w[3] = hi[1];
-#pragma unroll
-                for (int x = P::kSums - 1; x >= 0; x--) o[i] = mfma16<T>(w, p[x], o[i]);
-            }
-        }
-        if (WHOLE && more) find_pages(key0 + 2 * P::kKeys);
-    }
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
-    join_waves<T, D>(a, sm, s, count, head0, live_heads, o, m, l);
+    // (a copy of the last query head beyond them)
+    const T* q[1] = {static_cast<const T*>(a.q) + s * a.q_stride + (head0 + min(lane_id() & 15, live_heads - 1)) * D};
+    f32x4 o[1][D / 16];
+    float m[1], l[1];
+    attend_steps<T, D, 1, WHOLE, false>(a, a.page_table + static_cast<int64_t>(s) * a.max_pages, kv, begin, end, q, {0}, 0,
+                                        sm.v[wave_in_block()], o, m, l);
+    join_waves<T, D>(a, sm, s, count, head0, live_heads, o[0], m[0], l[0]);
 }
 
 template <typename T, int D>
 hs_status launch_paged_f8(const char* op, hipStream_t st, const Paged8Args& a) {
     using P = Paged8<T, D>;
-    return launch_pieces<T, D>(op, st, a, attention_paged_f8_kernel<T, D, true>, attention_paged_f8_kernel<T, D, false>, P::kUnit, P::kPerCu);
+    return launch_pieces<T, D>(op, st, a, attention_paged_f8_kernel<T, D, true>, attention_paged_f8_kernel<T, D, false>, P::kUnit, P::per_cu(a.page_shift >= 4));
 }
 
 }  // namespace

@@ -23,14 +23,12 @@
 // heads of 64 0.34 ms, 800 (a plain product of 8192^3 reaches 1090 to 1246). f32, three
 // products for one of f16, of bf16 values: 4096 tokens, 32 heads of 128 over 8, 657
 // us, 418 TFLOP/s, 16 heads of 64 202 us, 340 (the f32 matrix instructions' plain
-// product reaches 154). Few tokens: a chain of some 2 us for 64 keys, of which one or
-// two waves compute: 128 tokens of 32 sequences of up to 4000 keys, 28 heads of 64
-// over 4, 28 us. (Codes asked for two tiles ahead gain 2% at head dim 128 and nothing
-// for few tokens, and spill in f32: 4096 tokens of 32 heads 742 us.)
+// product reaches 154). (Codes asked for two tiles ahead gain 2% at head dim 128 and
+// spill in f32: 4096 tokens of 32 heads 742 us.) Sequences of few tokens: few_rows.
 #include <algorithm>
 #include <cmath>
 
-#include "hs_f8.hpp"
+#include "hs_steps_f8.hpp"
 
 namespace hs {
 namespace {
@@ -95,9 +93,13 @@ __device__ __forceinline__ int keys_seen(const PromptSeq& t, int i, int causal) 
 
 // An item: piece `piece` of the pieces of a tile. `fair` units of 64 keys are what each
 // of the key head's places on the chip gets of all tiles' work (half of a causal
-// mask's own keys count). Where tiles are fewer than places, a sequence's tiles are cut
-// into as many whole fair parts as they have, so that the call is one round; else
-// only tiles that would outlast the others are, into pieces of 3/4 of a fair part. A
+// mask's own keys count). Where tiles are fewer than places, one sequence's tiles are cut
+// into as many whole fair parts as they have, so that the call is one round, and those
+// of several into pieces of up to `most` units: a fair part, larger by what rounding
+// up to whole pieces adds, half a piece a tile as a rule, and then by what it adds
+// (whole fair parts of each are up to two long: 8 tokens each of 32 sequences of up to
+// 4000 keys, 32 heads of 128 over 8, 84 us for 64). Else only tiles that would outlast
+// the others are cut, into pieces of 3/4 of a fair part. A
 // sequence's pieces are of one size, `chunk`. Every workgroup computes this from all
 // lengths, 64 a step. The total is at least half of the exact one, so a call's items
 // do not pass 8/3 of the places and its tiles; what else offsets that do not ascend
@@ -303,6 +305,114 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// One code, as values_of has it.
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t code, float scale) {
+    const u32x4 x = values_of<T>(code, 0, scale);
+    return sizeof(T) == 2 ? static_cast<float>(u2h2(x[0]).x) : u2f(x[0] << 16);
+}
+
+// A sequence of up to 16 R rows: its waves take the keys in turn, each all rows, as
+// single tokens' do, and join in LDS. A tile's scheme has one wave of four compute and
+// one tile of keys under way; this one is bound by memory: 2 tokens each of 32 sequences
+// of up to 4000 keys, 16 heads of 64, 39 us, 3.3 TB/s (65), 32 heads of 128 over 8, 43
+// (62; f32 45, 90), 8 tokens each, R = 2, 50 (65); with a prompt of 512 tokens beside 31
+// single ones 46 (77). 128 tokens, 28 heads of 64 over 4, 28: finding the work, the first
+// codes and the join are 15 of them. (A long prompt's last few rows stay a tile, beside
+// its others: 168 us, 179 as these; f32 at head dim 128 by rows spills with R = 2, 142 us
+// for 95.)
+template <typename T, int D>
+struct FewRows {
+    using S = Steps8<T, D, 2>;
+    union {
+        uint16_t v[kPagedWaves][32 * S::kPitch];
+        float o[kPagedWaves][32 * S::kOPitch];
+    };
+    float m[kPagedWaves][32], l[kPagedWaves][32];
+};
+template <typename T, int D, int R, bool WHOLE>
+__device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& t, FewRows<T, D>& sm) {
+    using S = Steps8<T, D, R>;
+    constexpr int DB = D / 16;
+    const int lane = lane_id(), wave = wave_in_block(), n = lane & 15, g = lane >> 4;
+    const int* pages = a.page_table + static_cast<int64_t>(t.s) * a.max_pages;
+    const T* q[R];
+    int seen[R];
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        const int r = min(t.first + 16 * i + n, t.rows - 1), token = r / a.group;
+        q[i] = static_cast<const T*>(a.q) + (t.seq.q0 + token) * a.q_stride + (t.kv * a.group + (r - token * a.group)) * D;
+        seen[i] = keys_seen(t.seq, token, a.causal);
+    }
+    const int least = keys_seen(t.seq, t.first / a.group, a.causal);
+    f32x4 o[R][DB];
+    float m[R], l[R];
+    if (attend_steps<T, D, R, WHOLE, true>(a, pages, t.kv, t.begin, t.end, q, seen, least, sm.v[wave], o, m, l)) {
+        // NaN that went into the sums as zeros: to the rows that see them
+        for (int key0 = t.begin + wave * S::kStep; key0 < t.end; key0 += S::kKeys) {
+            if (key0 + S::kStep <= least) continue;
+            for (int key = key0; key < min(key0 + S::kStep, t.end); key++) {
+                const Tile16 tile = tile_of(a, pages[key >> a.page_shift], t.kv, key);
+                if (!tile.there) continue;
+                const uint8_t* p = a.v + tile.row * D + 4 * g;
+                const float scale = scale_value(a.v_scale[tile.row >> a.page_shift]);
+#pragma unroll
+                for (int i = 0; i < DB; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const float v = value_of<T>(p[16 * i + j], scale);
+                        if ((f2u(v) & 0x7F800000u) != 0x7F800000u) continue;
+#pragma unroll
+                        for (int r = 0; r < R; r++)
+                            if (key < seen[r]) o[r][i][j] += v;
+                    }
+            }
+        }
+    }
+    const int live = min(t.rows - t.first, 16 * R);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int row = 16 * r + n;
+#pragma unroll
+        for (int i = 0; i < DB; i++) *reinterpret_cast<f32x4*>(&sm.o[wave][row * S::kOPitch + 16 * i + 4 * g]) = o[r][i];
+        if (g == 0) sm.m[wave][row] = m[r], sm.l[wave][row] = l[r];
+    }
+    __syncthreads();
+    const int64_t block = partial_block(a, t.item, t.kv, 0);
+    for (int x = threadIdx.x; x < 8 * D; x += 64 * kPagedWaves) {
+        // pieces as the other tiles' (partial_block), else rows of channels
+        const bool piece = t.count > 1;
+        const int row = piece ? x % 32 : x / (D / 4), d0 = piece ? x / 64 * 8 + x / 32 % 2 * 4 : x % (D / 4) * 4;
+        if (row >= live) continue;
+        float top = sm.m[0][row];
+#pragma unroll
+        for (int w = 1; w < kPagedWaves; w++) top = fmaxf(top, sm.m[w][row]);
+        f32x4 sum = {};
+        float weight = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kPagedWaves; w++) {
+            const float f = __builtin_amdgcn_exp2f(sm.m[w][row] - top);
+            sum += *reinterpret_cast<const f32x4*>(&sm.o[w][row * S::kOPitch + d0]) * f;
+            weight = fmaf(sm.l[w][row], f, weight);
+        }
+        if (piece) {
+            st16_nt(a.ws_o + block * 32 * D + x * 4, __builtin_bit_cast(u32x4, sum));
+            const int64_t at = block * 32 + row;
+            if (d0 == 0) a.ws_ml[2 * at] = top, a.ws_ml[2 * at + 1] = weight;
+        } else {
+            T* orow = static_cast<T*>(a.out) + row_out(a, t.seq, t.kv, t.first + row) * D + d0;
+            float y[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = weight == 0.0f ? 0.0f : sum[e] / weight;
+            if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<u32x2*>(orow) = u32x2{pk_f16(y[0], y[1]), pk_f16(y[2], y[3])};
+            else
+                *reinterpret_cast<f32x4*>(orow) = f32x4{y[0], y[1], y[2], y[3]};
+        }
+    }
+}
+
 // WHOLE: pages of at least 16 keys, so that a wave's load, 8 or 16 rows, lies in one
 // page, is 1 KiB or half of that in a row, and has a scalar address (8192 tokens, 32
 // heads of 128 over 8: 1210 us, 1240 by rows of the lanes).
@@ -310,9 +420,17 @@ template <typename T, int D, int W, bool WHOLE>
 __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8_kernel(PromptArgs a) {
     using F = Prompt8<T, D, W>;
     constexpr int KS = F::KS, DB = F::DB, kPer = F::kPer;
-    __shared__ __align__(16) typename F::Smem sm;
+    __shared__ __align__(16) union {
+        typename F::Smem tile;
+        FewRows<T, D> few;
+    } lds;
+    auto& sm = lds.tile;
     PromptTile t;
     if (!prompt_tile(a, F::kRows, t)) return;  // workgroup-uniform, before any barrier
+    if constexpr (W == kPagedWaves) {
+        if (t.rows <= 16) return few_rows<T, D, 1, WHOLE>(a, t, lds.few);
+        if ((WHOLE || F::kHalf || D == 64) && t.rows <= 32) return few_rows<T, D, 2, WHOLE>(a, t, lds.few);
+    }
     const int tid = threadIdx.x, lane = lane_id(), wave = wave_in_block();
     const int n = lane & 31, hh = lane >> 5;
 
@@ -413,15 +531,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
                 uint16_t* vp = &sm.v[buf][r * F::kVPitch + piece * F::kLoad + 8 * half];
                 st16(kp, values_of<T>(pk[i][2 * half], pk[i][2 * half + 1], ks));
                 u32x4 x = values_of<T>(pv[i][2 * half], pv[i][2 * half + 1], vs);
-                if (masked) {
-                    constexpr uint32_t kExp = F::kHalf ? 0x7C00u : 0x7F80u;
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const uint32_t keep = ((x[w] & kExp) == kExp ? 0u : 0xFFFFu) | ((x[w] & kExp << 16) == kExp << 16 ? 0u : 0xFFFF0000u);
-                        odd |= keep != 0xFFFFFFFFu;
-                        x[w] &= keep;
-                    }
-                }
+                if (masked) odd |= zero_nan<T>(x);
                 st16(vp, x);
             }
         }
@@ -604,10 +714,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
             for (int db = 0; db < DB; db++)
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
-                    const uint32_t code = r[32 * db + 8 * (x / 4) + x % 4];
-                    const uint32_t half = F::kHalf ? h22u(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, scale, false))
-                                                   : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(code, scale, false));
-                    const float v = F::kHalf ? static_cast<float>(u2h2(half).x) : u2f(half << 16);
+                    const float v = value_of<T>(r[32 * db + 8 * (x / 4) + x % 4], scale);
                     if ((f2u(v) & 0x7F800000u) == 0x7F800000u) o[db][x] += v;
                 }
         }

@@ -509,6 +509,56 @@ def test_wide_tiles_leave_masked_values_alone(ctx, dtype):
     assert ((whole[64:1000].double() - want.double()).abs() <= 32 * eps * 14).all()
 
 
+@pytest.mark.parametrize("page", [1, 8, 16, 64])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_tokens(ctx, dtype, d, page):
+    """Sequences whose rows (tokens by heads of a key head) are 1 to 16, 17 to 32 and more, beside each other, over
+    keys of part of a wave's step and of several steps of all waves."""
+    for i, (h, h_kv, new, past, causal) in enumerate([
+        (2, 2, [1, 16, 17, 32, 33, 0], [0, 500, 63, 300, 40, 7], 1),
+        (7, 1, [2, 4, 5], [700, 30, 255], 1),
+        (3, 1, [5, 10, 11], [0, 1, 600], 4),
+        (16, 1, [1, 2], [513, 100], 0),
+        (32, 1, [1, 1, 2], [300, 0, 70], 1),
+        (1, 1, [3, 20, 200], [257, 128, 90], 64),
+    ]):
+        print(f"[few {dtype} d={d} page={page} case {i}]", flush=True)
+        run_attend(ctx, 620 + i, dtype, d, h, h_kv, page, [a + b for a, b in zip(new, past)], new, causal, wide=i == 1,
+                   behind=i % 3)
+
+
+@pytest.mark.parametrize("h", [1, 2])
+@pytest.mark.parametrize("page", [4, 16])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_tokens_odd_values(ctx, dtype, page, h):
+    """NaN at keys that some of a sequence's few tokens see and that all see; pages that are not there among them."""
+    def spoil(c):
+        at = lambda s, p: (int(c.page_table[s, p // page]), p % page)  # noqa: E731
+        for s, key, channel in [(0, 295, 5), (0, 301, 63), (0, 20, 9), (1, 600, 17), (1, 612, 0), (2, 3, 40)]:
+            a, r = at(s, key)
+            bits(c.v)[a, 0, r, channel] = 0x7F
+        a, r = at(0, 299)
+        bits(c.k)[a, 0, r] = 0xFF
+        c.page_table[1, 40 // page] = -1
+        c.page_table[2, 1] = c.k.shape[0]
+
+    run_attend(ctx, 640, dtype, 64, h, 1, page, [302, 615, 2 * page + 3], [8, 15, 6], 1, spoil=spoil)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_tokens_beside_many(ctx, dtype):
+    """A long prompt, single tokens and sequences without any in one call; some of whose keys lie in pieces."""
+    gen = torch.Generator().manual_seed(7)
+    new, past = [300, 1, 0, 1, 6, 1, 2], [2000, 5000, 40, 0, 3100, 1, 800]
+    lens = [a + b for a, b in zip(new, past)]
+    for d, h, h_kv, page in [(64, 8, 4, 32), (128, 8, 2, 8)]:
+        _, c = make_cache(gen, lens, h_kv, page, d, dtype)
+        q = normal(gen, (sum(new), h, d), dtype).to(DEV)
+        got = ctx.attention_paged_prompts(q, c, i32(offsets_of(new)), causal=1).unflatten(1, (h, d))
+        gpu_check(got, q, c, offsets_of(new), new, lens, 1, dtype, f"beside {d}")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_longer(ctx, dtype):
     gen = torch.Generator().manual_seed(3)
