@@ -315,10 +315,10 @@ __device__ __forceinline__ float value_of(uint32_t code, float scale) {
 // A sequence of up to 16 R rows: its waves take the keys in turn, each all rows, as
 // single tokens' do, and join in LDS. A tile's scheme has one wave of four compute and
 // one tile of keys under way; this one is bound by memory: 2 tokens each of 32 sequences
-// of up to 4000 keys, 16 heads of 64, 39 us, 3.3 TB/s (65), 32 heads of 128 over 8, 43
+// of up to 4000 keys, 16 heads of 64, 38 us, 3.3 TB/s (65), 32 heads of 128 over 8, 43
 // (62; f32 45, 90), 8 tokens each, R = 2, 50 (65); with a prompt of 512 tokens beside 31
-// single ones 46 (77). 128 tokens, 28 heads of 64 over 4, 28: finding the work, the first
-// codes and the join are 15 of them. (A long prompt's last few rows stay a tile, beside
+// single ones 46 (77). 128 tokens, 28 heads of 64 over 4, 27: finding the work, the first
+// codes and the join are 14 of them. (A long prompt's last few rows stay a tile, beside
 // its others: 168 us, 179 as these; f32 at head dim 128 by rows spills with R = 2, 142 us
 // for 95.)
 template <typename T, int D>
@@ -397,7 +397,7 @@ __device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& 
             weight = fmaf(sm.l[w][row], f, weight);
         }
         if (piece) {
-            st16_nt(a.ws_o + block * 32 * D + x * 4, __builtin_bit_cast(u32x4, sum));
+            st16(a.ws_o + block * 32 * D + x * 4, __builtin_bit_cast(u32x4, sum));
             const int64_t at = block * 32 + row;
             if (d0 == 0) a.ws_ml[2 * at] = top, a.ws_ml[2 * at + 1] = weight;
         } else {
@@ -792,19 +792,28 @@ __global__ __launch_bounds__(256) void prompts_join_kernel(PromptArgs a, int sha
         const float* ml = a.ws_ml + (from * 32 + lane % 32) * 2;
         constexpr int kAhead = 4, kStep = SPREAD ? 4 : 1;  // pieces whose loads are under way at once
         Joined j = {f32x4{}, kStart, 0.0f};
-        for (int i0 = SPREAD ? wave : 0; i0 < count; i0 += kAhead * kStep) {
-            f32x2 stat[kAhead];
-            f32x4 v[kAhead];
+        // (streamed past the caches where there is much of it: 311 us for 317 of the
+        // prompts; few tokens' 28 for 27)
+        const auto add = [&](auto stream) {
+            for (int i0 = SPREAD ? wave : 0; i0 < count; i0 += kAhead * kStep) {
+                f32x2 stat[kAhead];
+                u32x4 v[kAhead];
 #pragma unroll
-            for (int i = 0; i < kAhead; i++) {
-                const int64_t piece = min(i0 + i * kStep, count - 1) * step;
-                stat[i] = *reinterpret_cast<const f32x2*>(ml + piece * 64);
-                v[i] = __builtin_bit_cast(f32x4, ld16_nt(o + piece * 32 * D));
+                for (int i = 0; i < kAhead; i++) {
+                    if (i0 + i * kStep >= count) break;  // wave-uniform
+                    const int64_t piece = (i0 + i * kStep) * step;
+                    stat[i] = *reinterpret_cast<const f32x2*>(ml + piece * 64);
+                    v[i] = decltype(stream)::value ? ld16_nt(o + piece * 32 * D) : ld16(o + piece * 32 * D);
+                }
+#pragma unroll
+                for (int i = 0; i < kAhead; i++)
+                    if (i0 + i * kStep < count) j.add(__builtin_bit_cast(f32x4, v[i]), stat[i].x, stat[i].y);
             }
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (i0 + i * kStep < count) j.add(v[i], stat[i].x, stat[i].y);
-        }
+        };
+        if (rows > 32)
+            add(std::true_type{});
+        else
+            add(std::false_type{});
         if constexpr (SPREAD) {
             __syncthreads();  // the last round's have been read
             if (wave > 0) others[wave - 1][lane] = j;
@@ -915,8 +924,9 @@ extern "C" hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, co
         if (hs_status rc = check_launch(op)) return rc;
         if (!plan.places) return HS_OK;
         const int64_t heads = plan.tiles * h_kv, whole = plan.blocks * (d / 32);
+        // (a tile's blocks to more workgroups than one: the prompts' join 10 us for 16)
         const bool few = heads * whole < 4 * num_cus();
-        const int64_t share = few ? 4 * whole : heads < 4 * num_cus() ? whole : 1;
+        const int64_t share = few ? 4 * whole : std::max<int64_t>(std::min(whole, 16 * num_cus() / heads), 1);
         (few ? spread : join)<<<dim3(static_cast<uint32_t>(heads * share)), dim3(256), 0, st>>>(a, static_cast<int>(share));
         return check_launch(op);
     };
