@@ -104,7 +104,7 @@ __device__ __forceinline__ int keys_seen(const PromptSeq& t, int i, int causal) 
 // lengths, 64 a step. The total is at least half of the exact one, so a call's items
 // do not pass 8/3 of the places and its tiles; what else offsets that do not ascend
 // may come to is left out.
-constexpr int kLeastUnits = 4;
+constexpr int kLeastUnits = 8;  // (4: one token each of 32 sequences, 28 heads of 64 over 4, 21.5 us for 19.6; 12: 21.7)
 constexpr float kLonger = 16.0f;  // units that a tile's writing and joining of pieces cost, and more
 
 struct PromptItem {
@@ -167,12 +167,14 @@ __device__ __forceinline__ bool find_item(const PromptArgs& a, int rows, int ind
         else if (static_cast<float>(units) > fair + kLonger)
             pieces = static_cast<int>(ceilf(static_cast<float>(units) / (0.75f * fair)));
         const int chunk = max((units + pieces - 1) / pieces, 1);
-        // the sequences of long pieces first, by quarters of the longest, so that a
-        // call does not end on them
+        // in several rounds the sequences of long pieces first, by quarters of the
+        // longest, so that a call does not end on them (309 us for 360 of five prompts;
+        // in one round it is 3 us of finding work)
+        const bool ordered = a.b > 1 && !a.one_round;
         int tile_sum = 0, item_sum = 0, tile_end = 0, item_end = 0;
-        const int longest = a.b > 1 ? wave_most(chunk) : chunk;
-        const int quarter = min((longest - chunk) * 4 / longest, 3);
-        for (int k = 0; k < (a.b > 1 ? 4 : 1); k++) {
+        const int longest = ordered ? wave_most(chunk) : chunk;
+        const int quarter = ordered ? min((longest - chunk) * 4 / longest, 3) : 0;
+        for (int k = 0; k < (ordered ? 4 : 1); k++) {
             const int tile_add = wave_prefix_sum(quarter == k ? tiles : 0);
             const int item_add = wave_prefix_sum(quarter == k ? tiles * pieces : 0);
             if (quarter == k) tile_sum = tile_end + tile_add, item_sum = item_end + item_add;
@@ -317,8 +319,8 @@ __device__ __forceinline__ float value_of(uint32_t code, float scale) {
 // one tile of keys under way; this one is bound by memory: 2 tokens each of 32 sequences
 // of up to 4000 keys, 16 heads of 64, 38 us, 3.3 TB/s (65), 32 heads of 128 over 8, 43
 // (62; f32 45, 90), 8 tokens each, R = 2, 50 (65); with a prompt of 512 tokens beside 31
-// single ones 46 (77). 128 tokens, 28 heads of 64 over 4, 27: finding the work, the first
-// codes and the join are 14 of them. (A long prompt's last few rows stay a tile, beside
+// single ones 46 (77). 128 tokens, 28 heads of 64 over 4, 26: finding the work, the first
+// codes and the join are 13 of them. (A long prompt's last few rows stay a tile, beside
 // its others: 168 us, 179 as these; f32 at head dim 128 by rows spills with R = 2, 142 us
 // for 95.)
 template <typename T, int D>
