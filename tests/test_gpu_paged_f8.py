@@ -559,6 +559,20 @@ def test_few_tokens_beside_many(ctx, dtype):
         gpu_check(got, q, c, offsets_of(new), new, lens, 1, dtype, f"beside {d}")
 
 
+@pytest.mark.parametrize("h,h_kv,d", [(2, 1, 64), (16, 16, 64), (16, 8, 128)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_tokens_of_many_sequences(ctx, dtype, h, h_kv, d):
+    """More sequences than a wave's lanes, one much longer than the others, in one round of pieces and in several."""
+    gen = torch.Generator().manual_seed(8)
+    new = [i % 4 for i in range(131)]
+    past = [9000 if i == 66 else 37 * i % 700 for i in range(131)]
+    lens = [a + b for a, b in zip(new, past)]
+    _, c = make_cache(gen, lens, h_kv, 16, d, dtype)
+    q = normal(gen, (sum(new), h, d), dtype).to(DEV)
+    got = ctx.attention_paged_prompts(q, c, i32(offsets_of(new)), causal=1).unflatten(1, (h, d))
+    gpu_check(got, q, c, offsets_of(new), new, lens, 1, dtype, "many")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_paged_longer(ctx, dtype):
     gen = torch.Generator().manual_seed(3)
