@@ -926,7 +926,7 @@ extern "C" hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, co
         if (hs_status rc = check_launch(op)) return rc;
         if (!plan.places) return HS_OK;
         const int64_t heads = plan.tiles * h_kv, whole = plan.blocks * (d / 32);
-        // (a tile's blocks to more workgroups than one: the prompts' join 10 us for 16)
+        // (a tile's blocks to several workgroups: the join of five prompts 14.6 us for 15.9)
         const bool few = heads * whole < 4 * num_cus();
         const int64_t share = few ? 4 * whole : std::max<int64_t>(std::min(whole, 16 * num_cus() / heads), 1);
         (few ? spread : join)<<<dim3(static_cast<uint32_t>(heads * share)), dim3(256), 0, st>>>(a, static_cast<int>(share));
