@@ -19,7 +19,7 @@ import torch
 
 from . import rope as _rope
 from .context import HipContext
-from .paged import PagedKV8
+from .paged import in_eight_bits
 
 DIM, HEADS, HEAD_DIM, HIDDEN = 1024, 16, 64, 4096
 
@@ -374,7 +374,7 @@ def block_forward_cached(ctx: HipContext, wts: BlockWeights, x, cache, heads: in
     and it waits for the stream). A model's further blocks, whose caches share
     ``lens``, can leave it out; a call that is being captured cannot read it and
     is not checked."""
-    eight = type(cache) is PagedKV8
+    eight = in_eight_bits(cache)
     if offsets is not None and check and not eight and not (cache.lens.is_cuda and torch.cuda.is_current_stream_capturing()):
         assert (offsets.shape == (cache.lens.numel() + 1,) and offsets.dtype == torch.int32
                 and offsets.device == cache.lens.device), "offsets wants (sequences + 1) int32 beside the cache"

@@ -23,7 +23,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .paged import PagedKV8
+from .paged import PagedKV8, in_eight_bits
 
 F32 = torch.float32
 F16 = torch.float16
@@ -638,6 +638,7 @@ class HipContext:
         448, or the page's own where that is larger and the call goes on with
         the page; older codes follow a scale that grows. Magnitudes past
         f16's (61440) are held as that, infinities and NaN as NaN."""
+        eight = in_eight_bits(cache)
         n_pages, h_kv, page, d, b, max_pages = cache.shape
         dtype, dev = cache.dtype, _device()
         if cache.device_index != dev:
@@ -679,7 +680,7 @@ class HipContext:
         if positions is not None:
             assert rope is not None, "positions without rope"
             pos = _dense(positions, n, torch.int32, dev, "positions")
-        if type(cache) is PagedKV8:
+        if eight:
             self._launch_held("kv_append", self.lib.hs_kv_append_f8,
                               (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.page_table, cache.lens, k, v,
                                offsets, q, qn, kn, rope, positions, out_q, out_k), _DT[dtype], qp, qs, kp, ks, vp, vs,
@@ -748,6 +749,7 @@ class HipContext:
         ``workspace`` (uint8, ``attention_paged_workspace`` bytes) keeps the
         call from allocating; calls that may run at the same time need one
         each. ``scale`` None is 1 / sqrt(d)."""
+        eight = in_eight_bits(cache)
         n_pages, h_kv, page, d, b, max_pages = cache.shape
         dtype, dev = cache.dtype, _device()
         if cache.device_index != dev:
@@ -760,7 +762,6 @@ class HipContext:
             op = out.data_ptr()
         else:
             op = _dense(out, b * h * d, dtype, dev, "out")
-        eight = type(cache) is PagedKV8
         if workspace is None:
             size = (self.lib.hs_attention_paged_f8_workspace if eight else
                     self.lib.hs_attention_paged_workspace)(b, h, h_kv, d)
@@ -796,7 +797,7 @@ class HipContext:
         ``workspace`` (uint8, ``attention_paged_prompts_workspace`` bytes)
         keeps the call from allocating; calls that may run at the same time
         need one each. ``scale`` None is 1 / sqrt(d)."""
-        assert type(cache) is PagedKV8, "attention_paged_prompts wants a PagedKV8"
+        assert isinstance(cache, PagedKV8), "attention_paged_prompts wants a PagedKV8"
         n_pages, h_kv, page, d, b, max_pages = cache.shape
         dtype, dev = cache.dtype, _device()
         if cache.device_index != dev:

@@ -115,6 +115,15 @@ class PagedKV8:
                         page_table, lens, dtype)
 
 
+def in_eight_bits(cache) -> bool:
+    """Whether ``cache`` is a ``PagedKV8``, a class made from it included; what is neither that nor a ``PagedKV``
+    is refused, since the pools' bytes alone do not say what they hold."""
+    if isinstance(cache, PagedKV8):
+        return True
+    assert isinstance(cache, PagedKV), f"cache wants a PagedKV or a PagedKV8, not {type(cache).__name__}"
+    return False
+
+
 class PagePool:
     """The pages of caches that share ``page_table`` (sequences, max_pages) and
     ``lens`` (sequences,): entry i of a sequence is its page of keys [i page,
