@@ -630,7 +630,8 @@ class HipContext:
         (sin, cos) f32 (rows, d), by row ``positions[token]`` (int32) or the
         key's number; a row outside the tables is not rotated. A token whose
         page lies outside the table or the pool is not stored, and rows behind
-        ``offsets[-1]`` stay as they are. Returns (q, k) as contiguous
+        ``offsets[-1]`` stay as they are. Where ``offsets`` name more than the
+        n rows, these are the first of them. Returns (q, k) as contiguous
         rows, None for what was not asked (``q``, ``k_rows``).
 
         A ``PagedKV8`` takes the new keys and values as codes, those of a page
@@ -793,7 +794,8 @@ class HipContext:
         last of sequence s's tokens is its key ``lens[s] - 1``; ``causal`` as
         ``attention_packed`` (0: every key, c: groups of c tokens, counted
         from key 0). A token that sees nothing gets zeros; rows behind
-        ``offsets[-1]`` are not written. heads is a multiple of the cache's.
+        ``offsets[-1]`` are not written; where they name more than the n rows,
+        these are the first of them. heads is a multiple of the cache's.
         ``workspace`` (uint8, ``attention_paged_prompts_workspace`` bytes)
         keeps the call from allocating; calls that may run at the same time
         need one each. ``scale`` None is 1 / sqrt(d)."""

@@ -71,11 +71,13 @@ __device__ __forceinline__ bool find_unit(const Append8Args<T>& a, int index, Pa
             int count = 0, b0 = 0, e0 = 0, z0 = 0;
             if (base + lane < r.b) {
                 const RowRange q = row_range(a.offsets, base + lane, r.n);
-                const int len = max(a.lens[base + lane], 0);
-                b0 = max(len - (q.end - q.begin), 0), e0 = min(len, limit), z0 = q.end;
-                // (the last token of the rows is key len - 1, whether it has a place or not)
-                if (q.end > q.begin && e0 > b0) count = ((e0 - 1) >> shift) - (b0 >> shift) + 1;
-                z0 -= len;  // token of key p: p + z0
+                // Token of key p: p + z0. The sequence's last one is key len - 1, also where
+                // its rows end past the ones given, which are then the first of them.
+                if (q.end > q.begin) {
+                    z0 = a.offsets[base + lane + 1] - max(a.lens[base + lane], 0);
+                    b0 = max(q.begin - z0, 0), e0 = min(q.end - z0, limit);
+                    if (e0 > b0) count = ((e0 - 1) >> shift) - (b0 >> shift) + 1;
+                }
             }
             const int sum = wave_prefix_sum(count);
             const uint64_t hit = __ballot(before + sum > index);

@@ -74,18 +74,20 @@ struct PromptArgs {
     int items, blocks;    // items of a key head that the launch has, blocks of 32 rows of each
 };
 
-// One sequence: its queries' rows, its length and the keys it holds.
+// One sequence: its queries' rows, the first one's key number and the keys it holds.
+// (Its last query is its last key, also where its rows end past the ones given.)
 struct PromptSeq {
-    int q0, nq, len, nk;
+    int q0, nq, key0, nk;
 };
 __device__ __forceinline__ PromptSeq sequence_at(const PromptArgs& a, int s) {
     const RowRange r = row_range(a.offsets, s, a.n);
-    return {r.begin, r.end - r.begin, max(a.lens[s], 0), held_length(a.lens, s, a.max_pages, a.page_shift)};
+    const int nq = r.end - r.begin;
+    return {r.begin, nq, nq > 0 ? max(a.lens[s], 0) - (a.offsets[s + 1] - r.begin) : 0, held_length(a.lens, s, a.max_pages, a.page_shift)};
 }
 // Keys that the sequence's query i sees.
 __device__ __forceinline__ int keys_seen(const PromptSeq& t, int i, int causal) {
     if (causal == 0) return t.nk;
-    const int at = t.len - (t.nq - i);
+    const int at = t.key0 + i;
     if (at < 0) return 0;
     const int64_t end = causal == 1 ? static_cast<int64_t>(at) + 1 : (static_cast<int64_t>(at / causal) + 1) * causal;
     return end < t.nk ? static_cast<int>(end) : t.nk;

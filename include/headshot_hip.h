@@ -474,7 +474,9 @@ hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int
  * nearest even. Magnitudes past 61440 (HS_F16) or 15/8 2^127 (HS_F32) are held as
  * that; infinities and NaN as NaN. Whoever begins a page sets its scale, so the
  * pages of a new sequence need no values. No page takes new tokens of two
- * sequences in one call. HS_EINVAL at 2^23 workgroups: four tokens' q (k) rows of
+ * sequences in one call. Where offsets name rows past n (a step of fixed n after
+ * hs_plan_pages), the tokens there are not appended; the ones before them keep
+ * the key numbers that they have beside those. HS_EINVAL at 2^23 workgroups: four tokens' q (k) rows of
  * 1024 (HS_F16) or 512 elements each, and of the n / page + 2 b pages that the
  * tokens can lie in (b without offsets) times 2 Hkv four each, or one each where a
  * page has more than 2048 / D rows. */
@@ -508,8 +510,8 @@ int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int32_t b, int
 
 /* Attention of several new tokens per sequence over such a cache, which holds
  * their own keys already: q (n, Hq*D) at offsets (b + 1) -> out (n, Hq*D). The
- * last of sequence s's tokens is key lens[s] - 1; causal is as for
- * hs_attention_packed, groups counted from key 0. A token that sees no key gets
+ * last of sequence s's tokens is key lens[s] - 1, also where it is a row past n;
+ * causal is as for hs_attention_packed, groups counted from key 0. A token that sees no key gets
  * zeros, rows of no sequence are not written. Keys and values that a token does
  * not see do not enter its result, whatever they hold. workspace is as for
  * hs_attention_paged. */
