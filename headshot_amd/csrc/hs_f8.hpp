@@ -53,9 +53,16 @@ __device__ __forceinline__ u32x4 values_of(uint32_t lo, uint32_t hi, float scale
     return sizeof(T) == 2 ? f16_of_codes(lo, hi, scale) : bf16_of_codes(lo, hi, scale);
 }
 
-// NaN among 8 values turned into zeros; whether there was any.
+// One code, as values_of has it.
 template <typename T>
-__device__ __forceinline__ bool zero_nan(u32x4& x) {
+__device__ __forceinline__ float value_of(uint32_t code, float scale) {
+    const u32x4 x = values_of<T>(code, 0, scale);
+    return sizeof(T) == 2 ? static_cast<float>(u2h2(x[0]).x) : u2f(x[0] << 16);
+}
+
+// Infinities and NaN among 8 values turned into zeros; whether there were any.
+template <typename T>
+__device__ __forceinline__ bool zero_odd(u32x4& x) {
     constexpr uint32_t kExp = sizeof(T) == 2 ? 0x7C00u : 0x7F80u;
     bool any = false;
 #pragma unroll
@@ -65,6 +72,14 @@ __device__ __forceinline__ bool zero_nan(u32x4& x) {
         x[w] &= keep;
     }
     return any;
+}
+
+// An infinity or NaN among a sum's values: the first takes the sum's place, the
+// others add up. `found`: bit by sum.
+__device__ __forceinline__ float with_odd(float sum, float v, uint64_t& found, int bit) {
+    const bool first = !(found >> bit & 1);
+    found |= uint64_t{1} << bit;
+    return first ? v : sum + v;
 }
 
 // 4 values to 4 codes, rounded to nearest even. (In range: a finite value past

@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_p
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    join_waves<T, D>(a, sm, s, count, head0, live_heads, o, m, l);
+    join_waves<T, D, false>(a, sm, s, count, head0, live_heads, o, m, l);
 }
 
 // f32, a key head of one query head (no sharing): the matrix instructions would
@@ -484,11 +484,11 @@ hs_status launch_paged(const char* op, hipStream_t st, const PagedArgs& a) {
     if constexpr (sizeof(T) == 4) {
         if (a.h == a.h_kv) {
             using P = PagedSingle<D>;
-            return launch_pieces<T, D>(op, st, a, paged_single_kernel<D, true>, paged_single_kernel<D, false>, P::kUnit, P::kPerCu);
+            return launch_pieces<T, D, false>(op, st, a, paged_single_kernel<D, true>, paged_single_kernel<D, false>, P::kUnit, P::kPerCu);
         }
     }
     using P = Paged<T, D>;
-    return launch_pieces<T, D>(op, st, a, attention_paged_kernel<T, D, true>, attention_paged_kernel<T, D, false>, P::kUnit, P::kPerCu);
+    return launch_pieces<T, D, false>(op, st, a, attention_paged_kernel<T, D, true>, attention_paged_kernel<T, D, false>, P::kUnit, P::kPerCu);
 }
 
 }  // namespace

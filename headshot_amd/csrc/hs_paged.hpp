@@ -5,6 +5,7 @@
 #pragma once
 
 #include <cmath>
+#include <type_traits>
 
 #include "hs_packed.hpp"
 
@@ -213,8 +214,8 @@ constexpr float kFloor = -2.9e38f;  // the least of one that has
 // result's rounding) for 1-2% of the time. The largest weight of a step is this
 // unit, so that the others, f16 being subnormal below 2^-14, are 2^-40 of it off at
 // most (of a unit of 1, 45% at a score 17 nats below). The second part times an
-// infinity is NaN or the other infinity: a step that has one among its values
-// leaves the second parts out.
+// infinity is NaN or the other infinity: over full caches a step that has one among
+// its values leaves the second parts out; over 8 bits see odd_values.
 constexpr float kHalfUnit = 32768.0f;
 
 struct PagedArgs {
@@ -294,10 +295,35 @@ __device__ __forceinline__ Tile16 tile_of(const A& a, int page, int kv, int key)
     return {((static_cast<int64_t>(there ? page : 0) * a.h_kv + kv) << a.page_shift) + (key & ((1 << a.page_shift) - 1)), there};
 }
 
+// Sums times a factor; `keep`: an infinite one stays where the factor is 0.
+template <typename K>
+__device__ __forceinline__ f32x4 times(f32x4 x, float f, K keep) {
+    f32x4 y = x * f;
+    if constexpr (decltype(keep)::value) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] = y[e] != y[e] ? x[e] : y[e];
+    }
+    return y;
+}
+// Sums that f(keep) joins. KEEP: where one is NaN, it is done again with what is
+// infinite kept (kept at once, one token over 130531 keys takes 55 us for 53).
+template <bool KEEP = true, typename F>
+__device__ __forceinline__ f32x4 joined(F f) {
+    f32x4 x = f(std::false_type{});
+    if constexpr (KEEP) {
+        if (x[0] != x[0] || x[1] != x[1] || x[2] != x[2] || x[3] != x[3]) {
+            const f32x4 y = f(std::true_type{});
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = x[e] != x[e] ? y[e] : x[e];
+        }
+    }
+    return x;
+}
+
 // A workgroup's waves' sums of up to kGroup query heads joined in LDS: the result,
 // or the piece's in the workspace. Lane (n, g) holds channels 16 i + 4 g + .. of
-// head n; l is a head's whole sum of the wave.
-template <typename T, int D, typename S>
+// head n; l is a head's whole sum of the wave. KEEP: as there.
+template <typename T, int D, bool KEEP, typename S>
 __device__ __forceinline__ void join_waves(const PagedArgs& a, S& sm, int s, int count, int head0, int live_heads,
                                            const f32x4 (&o)[D / 16], float m, float l) {
     constexpr int kOPitch = D + 4;
@@ -314,14 +340,18 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, S& sm, int s, int
         float top = sm.m[0][head];
 #pragma unroll
         for (int w = 1; w < kPagedWaves; w++) top = fmaxf(top, sm.m[w][head]);
-        f32x4 sum = {};
         float weight = 0.0f;
+        const f32x4 sum = joined<KEEP>([&](auto keep) {
+            f32x4 all = {};
+            weight = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPagedWaves; w++) {
-            const float f = __builtin_amdgcn_exp2f(sm.m[w][head] - top);
-            sum += *reinterpret_cast<const f32x4*>(&sm.o[w][head * kOPitch + d0]) * f;
-            weight = fmaf(sm.l[w][head], f, weight);
-        }
+            for (int w = 0; w < kPagedWaves; w++) {
+                const float f = __builtin_amdgcn_exp2f(sm.m[w][head] - top);
+                all += times(*reinterpret_cast<const f32x4*>(&sm.o[w][head * kOPitch + d0]), f, keep);
+                weight = fmaf(sm.l[w][head], f, weight);
+            }
+            return all;
+        });
         if (count == 1) {
             T* orow = static_cast<T*>(a.out) + (static_cast<int64_t>(s) * a.h + head0 + head) * D + d0;
 #pragma unroll
@@ -335,7 +365,7 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, S& sm, int s, int
 }
 
 // The pieces of one (sequence, query head) joined, THREADS / (D / 4) at a time.
-template <typename T, int D, int THREADS>
+template <typename T, int D, int THREADS, bool KEEP>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
     constexpr int kLanes = D / 4, kRows = THREADS / kLanes;
     __shared__ __align__(16) f32x4 part[kRows][kLanes];
@@ -348,30 +378,37 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs a) {
     const int pass = in_group / a.width, x = in_group - pass * a.width;
     const auto row_of = [&](int i) { return (((before + i) * a.h_kv + kv) * a.passes + pass) * a.width + x; };
     const int row = threadIdx.x / kLanes, col = threadIdx.x % kLanes;
-    float top = kNone, weight = 0.0f;
-    f32x4 sum = {};
-    for (int i = row; i < count; i += kRows) {
-        const int64_t r = row_of(i);
-        const float m = a.ws_ml[2 * r], l = a.ws_ml[2 * r + 1];
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + r * D + 4 * col);
-        const float next = fmaxf(top, m);
-        const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
-        sum = sum * old + v * f;
-        weight = fmaf(weight, old, l * f);
-        top = next;
-    }
-    part[row][col] = sum;
+    float top, weight;
+    part[row][col] = joined<KEEP>([&](auto keep) {
+        f32x4 sum = {};
+        top = kNone, weight = 0.0f;
+        for (int i = row; i < count; i += kRows) {
+            const int64_t r = row_of(i);
+            const float m = a.ws_ml[2 * r], l = a.ws_ml[2 * r + 1];
+            const f32x4 v = *reinterpret_cast<const f32x4*>(a.ws_o + r * D + 4 * col);
+            const float next = fmaxf(top, m);
+            const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
+            sum = times(sum, old, keep) + times(v, f, keep);
+            weight = fmaf(weight, old, l * f);
+            top = next;
+        }
+        return sum;
+    });
     if (col == 0) tops[row] = top, weights[row] = weight;
     __syncthreads();
     if (row != 0) return;
     const int rows = min(kRows, count);
     for (int i = 0; i < rows; i++) top = fmaxf(top, tops[i]);
-    sum = f32x4{}, weight = 0.0f;
-    for (int i = 0; i < rows; i++) {
-        const float f = __builtin_amdgcn_exp2f(tops[i] - top);
-        sum += part[i][col] * f;
-        weight = fmaf(weights[i], f, weight);
-    }
+    const f32x4 sum = joined<KEEP>([&](auto keep) {
+        f32x4 all = {};
+        weight = 0.0f;
+        for (int i = 0; i < rows; i++) {
+            const float f = __builtin_amdgcn_exp2f(tops[i] - top);
+            all += times(part[i][col], f, keep);
+            weight = fmaf(weights[i], f, weight);
+        }
+        return all;
+    });
     T* orow = static_cast<T*>(a.out) + (static_cast<int64_t>(s) * a.h + head) * D + 4 * col;
 #pragma unroll
     for (int e = 0; e < 4; e++) orow[e] = static_cast<T>(top == kNone ? 0.0f : sum[e] / weight);
@@ -394,7 +431,7 @@ struct PagedPlan {
 };
 
 // The pieces' kernel (of whole 16 keys in a page, or by rows) and their join.
-template <typename T, int D, typename A, typename K>
+template <typename T, int D, bool KEEP, typename A, typename K>
 hs_status launch_pieces(const char* op, hipStream_t st, A a, K whole, K rows, int unit, int per_cu) {
     const PagedPlan plan(a.b, a.h, a.h_kv, per_cu);
     a.ws_ml = a.ws_o + plan.rows * D;
@@ -413,9 +450,9 @@ hs_status launch_pieces(const char* op, hipStream_t st, A a, K whole, K rows, in
     const dim3 joins(static_cast<uint32_t>(joined));
     // few rows may have a thousand pieces each
     if (joined <= 64)
-        paged_join_kernel<T, D, 1024><<<joins, dim3(1024), 0, st>>>(a);
+        paged_join_kernel<T, D, 1024, KEEP><<<joins, dim3(1024), 0, st>>>(a);
     else
-        paged_join_kernel<T, D, 256><<<joins, dim3(256), 0, st>>>(a);
+        paged_join_kernel<T, D, 256, KEEP><<<joins, dim3(256), 0, st>>>(a);
     return check_launch(op);
 }
 

@@ -350,13 +350,13 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::per_cu(WHOLE))) vo
     float m[1], l[1];
     attend_steps<T, D, 1, WHOLE, false>(a, a.page_table + static_cast<int64_t>(s) * a.max_pages, kv, begin, end, q, {0}, 0,
                                         sm.v[wave_in_block()], o, m, l);
-    join_waves<T, D>(a, sm, s, count, head0, live_heads, o[0], m[0], l[0]);
+    join_waves<T, D, true>(a, sm, s, count, head0, live_heads, o[0], m[0], l[0]);
 }
 
 template <typename T, int D>
 hs_status launch_paged_f8(const char* op, hipStream_t st, const Paged8Args& a) {
     using P = Paged8<T, D>;
-    return launch_pieces<T, D>(op, st, a, attention_paged_f8_kernel<T, D, true>, attention_paged_f8_kernel<T, D, false>, P::kUnit, P::per_cu(a.page_shift >= 4));
+    return launch_pieces<T, D, true>(op, st, a, attention_paged_f8_kernel<T, D, true>, attention_paged_f8_kernel<T, D, false>, P::kUnit, P::per_cu(a.page_shift >= 4));
 }
 
 }  // namespace

@@ -297,7 +297,7 @@ struct Prompt8 {
         uint16_t v[2][kBN * kVPitch];
         uint8_t there[2][kBN];
         int gap[2];  // the tile of each buffer if some of its keys are not there
-        int odd;     // a tile whose values not every row sees holds NaN
+        int odd;     // a tile whose values not every row sees holds infinities or NaN, left out
     };
 };
 
@@ -307,13 +307,6 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(a), as_h8(b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-
-// One code, as values_of has it.
-template <typename T>
-__device__ __forceinline__ float value_of(uint32_t code, float scale) {
-    const u32x4 x = values_of<T>(code, 0, scale);
-    return sizeof(T) == 2 ? static_cast<float>(u2h2(x[0]).x) : u2f(x[0] << 16);
 }
 
 // A sequence of up to 16 R rows: its waves take the keys in turn, each all rows, as
@@ -351,28 +344,7 @@ __device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& 
     const int least = keys_seen(t.seq, t.first / a.group, a.causal);
     f32x4 o[R][DB];
     float m[R], l[R];
-    if (attend_steps<T, D, R, WHOLE, true>(a, pages, t.kv, t.begin, t.end, q, seen, least, sm.v[wave], o, m, l)) {
-        // NaN that went into the sums as zeros: to the rows that see them
-        for (int key0 = t.begin + wave * S::kStep; key0 < t.end; key0 += S::kKeys) {
-            if (key0 + S::kStep <= least) continue;
-            for (int key = key0; key < min(key0 + S::kStep, t.end); key++) {
-                const Tile16 tile = tile_of(a, pages[key >> a.page_shift], t.kv, key);
-                if (!tile.there) continue;
-                const uint8_t* p = a.v + tile.row * D + 4 * g;
-                const float scale = scale_value(a.v_scale[tile.row >> a.page_shift]);
-#pragma unroll
-                for (int i = 0; i < DB; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float v = value_of<T>(p[16 * i + j], scale);
-                        if ((f2u(v) & 0x7F800000u) != 0x7F800000u) continue;
-#pragma unroll
-                        for (int r = 0; r < R; r++)
-                            if (key < seen[r]) o[r][i][j] += v;
-                    }
-            }
-        }
-    }
+    attend_steps<T, D, R, WHOLE, true>(a, pages, t.kv, t.begin, t.end, q, seen, least, sm.v[wave], o, m, l);
     const int live = min(t.rows - t.first, 16 * R);
     __syncthreads();
 #pragma unroll
@@ -392,14 +364,16 @@ __device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& 
         float top = sm.m[0][row];
 #pragma unroll
         for (int w = 1; w < kPagedWaves; w++) top = fmaxf(top, sm.m[w][row]);
-        f32x4 sum = {};
         float weight = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kPagedWaves; w++) {
-            const float f = __builtin_amdgcn_exp2f(sm.m[w][row] - top);
-            sum += *reinterpret_cast<const f32x4*>(&sm.o[w][row * S::kOPitch + d0]) * f;
-            weight = fmaf(sm.l[w][row], f, weight);
-        }
+        for (int w = 0; w < kPagedWaves; w++) weight = fmaf(sm.l[w][row], __builtin_amdgcn_exp2f(sm.m[w][row] - top), weight);
+        const f32x4 sum = joined([&](auto keep) {
+            f32x4 s = {};
+#pragma unroll
+            for (int w = 0; w < kPagedWaves; w++)
+                s += times(*reinterpret_cast<const f32x4*>(&sm.o[w][row * S::kOPitch + d0]), __builtin_amdgcn_exp2f(sm.m[w][row] - top), keep);
+            return s;
+        });
         if (piece) {
             st16(a.ws_o + block * 32 * D + x * 4, __builtin_bit_cast(u32x4, sum));
             const int64_t at = block * 32 + row;
@@ -482,6 +456,8 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
     // codes at `piece`. Pages are looked up a tile ahead of the codes.
     constexpr int kWords = F::kLoad / 4;
     typedef uint32_t codes_t __attribute__((ext_vector_type(kWords)));
+    typedef const __attribute__((address_space(1))) codes_t* global_codes;
+    typedef const __attribute__((address_space(1))) uint8_t* global_bytes;
     const int row0 = tid / F::kPieces, piece = tid % F::kPieces;
     const int* pages = a.page_table + static_cast<int64_t>(t.s) * a.max_pages;
     int page[kPer];
@@ -504,8 +480,12 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
             const int64_t block = static_cast<int64_t>(there ? page[i] : 0) * a.h_kv + t.kv;
             const int64_t at = ((block << a.page_shift) + (WHOLE || there ? key & ((1 << a.page_shift) - 1) : 0)) * D;
             const uint32_t lane_at = WHOLE ? lane * F::kLoad : piece * F::kLoad;
-            pk[i] = *reinterpret_cast<const codes_t*>(a.k + at + lane_at);
-            pv[i] = *reinterpret_cast<const codes_t*>(a.v + at + lane_at);
+            global_bytes kp = (global_bytes)(a.k + at), vp = (global_bytes)(a.v + at);
+            // a scalar address with a lane's offset, where its sum with that is too many
+            // registers (8192 tokens, 16 heads of 64, 361 us for 342; the others lose 1%)
+            if constexpr (W == 8 && D == 64) asm("" : "+s"(kp), "+s"(vp));
+            pk[i] = *reinterpret_cast<global_codes>(kp + lane_at);
+            pv[i] = *reinterpret_cast<global_codes>(vp + lane_at);
             pks[i] = a.k_scale[block], pvs[i] = a.v_scale[block];
             ok |= there ? 1u << i : 0u;
         }
@@ -535,7 +515,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
                 uint16_t* vp = &sm.v[buf][r * F::kVPitch + piece * F::kLoad + 8 * half];
                 st16(kp, values_of<T>(pk[i][2 * half], pk[i][2 * half + 1], ks));
                 u32x4 x = values_of<T>(pv[i][2 * half], pv[i][2 * half + 1], vs);
-                if (masked) odd |= zero_nan<T>(x);
+                if (masked) odd |= zero_odd<T>(x);
                 st16(vp, x);
             }
         }
@@ -705,10 +685,16 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
         __syncthreads();
     }
     if (row >= t.rows) return;
-    if (tile0 < ntiles && sm.odd) {
-        // NaN among values that some rows of the tile see and others do not went
-        // into LDS as zeros; here they reach the rows that do see them
-        for (int key = max(tile_least / kBN * kBN, t.begin); key < min(seen, t.end); key++) {
+    // Infinities and NaN among the values (odd_values)
+    bool all = false;
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int x = 0; x < 16; x++) all |= !(fabsf(o[db][x]) < INFINITY);
+    if (__builtin_expect(tile0 < ntiles && (all || sm.odd), 0)) {
+        uint64_t found = 0;
+#pragma unroll 1
+        for (int key = all ? t.begin : max(tile_least / kBN * kBN, t.begin); key < min(seen, t.end); key++) {
             const int p = pages[key >> a.page_shift];
             if (p < 0 || p >= a.n_pages) continue;
             const int64_t block = static_cast<int64_t>(p) * a.h_kv + t.kv;
@@ -719,7 +705,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
 #pragma unroll
                 for (int x = 0; x < 16; x++) {
                     const float v = value_of<T>(r[32 * db + 8 * (x / 4) + x % 4], scale);
-                    if ((f2u(v) & 0x7F800000u) == 0x7F800000u) o[db][x] += v;
+                    if (!(fabsf(v) < INFINITY)) o[db][x] = with_odd(o[db][x], v, found, 16 * db + x);
                 }
         }
     }
@@ -767,10 +753,11 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
 struct Joined {
     f32x4 sum;
     float top, weight;
-    __device__ __forceinline__ void add(f32x4 v, float m, float l) {
+    template <typename K>
+    __device__ __forceinline__ void add(f32x4 v, float m, float l, K keep) {
         const float next = fmaxf(top, m);
         const float old = __builtin_amdgcn_exp2f(top - next), f = __builtin_amdgcn_exp2f(m - next);
-        sum = sum * old + v * f;
+        sum = times(sum, old, keep) + times(v, f, keep);
         weight = fmaf(weight, old, l * f);
         top = next;
     }
@@ -795,10 +782,11 @@ __global__ __launch_bounds__(256) void prompts_join_kernel(PromptArgs a, int sha
         const float* o = a.ws_o + from * 32 * D + (at * 64 + lane) * 4;
         const float* ml = a.ws_ml + (from * 32 + lane % 32) * 2;
         constexpr int kAhead = 4, kStep = SPREAD ? 4 : 1;  // pieces whose loads are under way at once
-        Joined j = {f32x4{}, kStart, 0.0f};
+        Joined j;
         // (streamed past the caches where there is much of it: 311 us for 317 of the
         // prompts; few tokens' 28 for 27)
-        const auto add = [&](auto stream) {
+        const auto add = [&](auto stream, auto keep) {
+            j = {f32x4{}, kStart, 0.0f};
             for (int i0 = SPREAD ? wave : 0; i0 < count; i0 += kAhead * kStep) {
                 f32x2 stat[kAhead];
                 u32x4 v[kAhead];
@@ -811,20 +799,28 @@ __global__ __launch_bounds__(256) void prompts_join_kernel(PromptArgs a, int sha
                 }
 #pragma unroll
                 for (int i = 0; i < kAhead; i++)
-                    if (i0 + i * kStep < count) j.add(__builtin_bit_cast(f32x4, v[i]), stat[i].x, stat[i].y);
+                    if (i0 + i * kStep < count) j.add(__builtin_bit_cast(f32x4, v[i]), stat[i].x, stat[i].y, keep);
             }
         };
-        if (rows > 32)
-            add(std::true_type{});
-        else
-            add(std::false_type{});
+        j.sum = joined([&](auto keep) {
+            if (rows > 32 && !decltype(keep)::value)
+                add(std::true_type{}, keep);
+            else
+                add(std::false_type{}, keep);
+            return j.sum;
+        });
         if constexpr (SPREAD) {
             __syncthreads();  // the last round's have been read
             if (wave > 0) others[wave - 1][lane] = j;
             __syncthreads();
             if (wave > 0) continue;
+            const Joined own = j;
+            j.sum = joined([&](auto keep) {
+                j = own;
 #pragma unroll
-            for (int w = 0; w < 3; w++) j.add(others[w][lane].sum, others[w][lane].top, others[w][lane].weight);
+                for (int w = 0; w < 3; w++) j.add(others[w][lane].sum, others[w][lane].top, others[w][lane].weight, keep);
+                return j.sum;
+            });
         }
         if (row >= rows) continue;
         const int all = c.z + row, token = all / a.group;

@@ -32,11 +32,55 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// Infinities and NaN among the values: a channel's are its sum, in the rows that see
+// any. A channel of which all rows see them has a sum that is no number already, but
+// maybe another one, since an infinity times a weight of 0, or the parts of one, is
+// NaN; so they are added by themselves, over all keys where there is such a sum, else
+// over the steps that left them out.
+template <typename T, int D, int R, bool MASKED, typename A>
+__device__ __forceinline__ void odd_values(const A& a, const int* pages, int kv, int begin, int end, const int (&seen)[R], int least,
+                                           bool left_out, f32x4 (&o)[R][D / 16]) {
+    using P = Steps8<T, D, R>;
+    const int g = lane_id() >> 4;
+    bool odd = false;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < D / 16; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) odd |= !(fabsf(o[r][i][j]) < INFINITY);
+    const bool all = __any(odd);
+    if (__builtin_expect(!all && !left_out, 1)) return;
+    uint64_t found = 0;  // by sum
+#pragma unroll 1
+    for (int key0 = begin + wave_in_block() * P::kStep; key0 < end; key0 += P::kKeys) {
+        if (!all && key0 + P::kStep <= least) continue;
+#pragma unroll 1
+        for (int key = key0; key < min(key0 + P::kStep, end); key++) {
+            const Tile16 tile = tile_of(a, pages[key >> a.page_shift], kv, key);
+            if (!tile.there) continue;
+            const uint8_t* p = static_cast<const uint8_t*>(a.v) + tile.row * D + 4 * g;
+            const float scale = scale_value(a.v_scale[tile.row >> a.page_shift]);
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float v = value_of<T>(p[16 * i + j], scale);
+                    if (fabsf(v) < INFINITY) continue;
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+                        if (!MASKED || key < seen[r]) o[r][i][j] = with_odd(o[r][i][j], v, found, (r * (D / 16) + i) * 4 + j);
+                }
+        }
+    }
+}
+
 // The wave's steps of keys [begin, end): R sets of 16 rows, lane (n, g) with row n
 // of each, whose query lies at qr; its sums of channels 16 i + 4 g + .., its largest
 // score (log2) and its sum of weights. `vs` is the wave's slice of LDS. MASKED: a row
-// sees keys below `seen`, all of them those below `least`; returns whether values
-// that not every row sees hold NaN, which went into the sums as zeros.
+// sees keys below `seen`, all of them those below `least`, else all see all; in a step
+// that some row does not see whole, infinities and NaN go into the sums as zeros, and
+// to the rows that see them at the end (odd_values).
 // WHOLE: pages of at least 16 keys, so that 16 keys from a multiple of 16 lie in
 // one page; else a lane looks one key's up, a step ahead, and rows take it from there
 // (by each row, when its codes are asked for: 42 us for 33 of 32 sequences of up to 4000
@@ -45,7 +89,7 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 // A lane's 16-byte load of a row of K is 16 dims, two operands of 8: dims 64 i +
 // 16 g + 8 e, which the queries follow.
 template <typename T, int D, int R, bool WHOLE, bool MASKED, typename A>
-__device__ __forceinline__ bool attend_steps(const A& a, const int* pages, int kv, int begin, int end, const T* const (&qr)[R],
+__device__ __forceinline__ void attend_steps(const A& a, const int* pages, int kv, int begin, int end, const T* const (&qr)[R],
                                              const int (&seen)[R], int least, uint16_t* vs, f32x4 (&o)[R][D / 16],
                                              float (&m)[R], float (&l)[R]) {
     using P = Steps8<T, D, R>;
@@ -253,7 +297,7 @@ __device__ __forceinline__ bool attend_steps(const A& a, const int* pages, int k
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     u32x4 v = values_of<T>(vr[i][2 * x], vr[i][2 * x + 1], scale);
-                    if (masked) odd |= zero_nan<T>(v);
+                    if (masked) odd |= zero_odd<T>(v);
                     st16(p + 8 * x, v);
                 }
             }
@@ -301,7 +345,7 @@ __device__ __forceinline__ bool attend_steps(const A& a, const int* pages, int k
         l[r] += __shfl_xor(l[r], 16, 64);
         l[r] += __shfl_xor(l[r], 32, 64);
     }
-    return MASKED && __any(odd);
+    odd_values<T, D, R, MASKED>(a, pages, kv, begin, end, seen, least, MASKED && __any(odd), o);
 }
 
 }  // namespace
