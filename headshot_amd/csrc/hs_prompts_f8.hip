@@ -853,10 +853,12 @@ struct PromptPlan {
         const int64_t slots = num_cus() * per_cu(dt, d, rows);
         tiles = n * group / rows + (b < n ? b : n);
         items = tiles, blocks = 0;
-        places = std::max<int64_t>(slots / h_kv, 1);
+        places = slots / h_kv;
         one_round = tiles < places;
-        // (a workspace for every item that there can be, some 200 MB at the most)
-        if (keys <= kLeastUnits * kBN || tiles >= 4 * places) places = 0;
+        // (a workspace for every item that there can be: fewer than seven times the places
+        // of all key heads, 243 MB on 256 CUs. Where key heads fill the chip by themselves,
+        // it would be that of each of them, and nothing is gained)
+        if (keys <= kLeastUnits * kBN || places < 2 || tiles >= 4 * places) places = 0;
         if (!places) return;
         items = 3 * places + tiles;
         blocks = ceil_div(std::min<int64_t>(n * group, rows), 32);
