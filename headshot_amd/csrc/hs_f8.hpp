@@ -1,7 +1,8 @@
 // A cache held in 8 bits: e4m3 codes (sign, 4 bits of exponent, 3 of mantissa;
 // no infinities, one NaN a sign) and, for each page and head, one scale 2^(c -
 // 127) of which c is kept (E8M0). A code times a scale has 4 significant bits, so
-// bf16 holds it as it is, whatever the scale, and f16 where f16 reaches.
+// bf16 holds it as it is, whatever the scale, and f16 from 2^-14 to its largest; below,
+// f16 rounds it to a multiple of 2^-24, as it would have rounded the row.
 #pragma once
 
 #include "hs_paged.hpp"

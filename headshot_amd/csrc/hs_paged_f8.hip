@@ -299,7 +299,7 @@ hs_status launch_append_f8(const char* op, hipStream_t st, Append8Args<T> a, int
 //
 // Single tokens: as attention_paged (hs_paged.hip), of half its bytes or a
 // quarter. A wave takes kStep keys at a time on its own; codes become f16 (f16
-// caches) or bf16 (f32) values with their page's scale on the way, exactly: K's in
+// caches) or bf16 (f32) values with their page's scale on the way (hs_f8.hpp): K's in
 // the registers that the load filled, as the A operand of S^T = K Q^T, V's on
 // their way to the wave's slice of LDS, from which V^T takes P^T. What the codes
 // leave to round is the query and the weights: in f16 weights go as two f16 values

@@ -9,7 +9,7 @@
 // once for all heads that see it. Keys go through LDS 64 at a time, double
 // buffered: codes of the next ones lie in registers while these compute, and become
 // f16 (f16 caches) or bf16 (f32) values with their page's scale on the way into LDS,
-// exactly. Scores are transposed, S^T = K Q^T: lanes n and n + 32 hold row n's, so
+// (hs_f8.hpp). Scores are transposed, S^T = K Q^T: lanes n and n + 32 hold row n's, so
 // its statistics are the lane's own, and V^T takes P^T from the registers that the
 // scores were in.
 //

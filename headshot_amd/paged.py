@@ -68,7 +68,8 @@ class PagedKV8:
     """``PagedKV`` held in 8 bits: ``k``, ``v`` (n_pages, heads, page, head_dim)
     of ``torch.float8_e4m3fn`` codes, ``k_scale``, ``v_scale`` (n_pages, heads) of
     ``torch.float8_e8m0fnu``, powers of two. A value is its code times its
-    page's and head's scale. ``dtype`` is the type of the rows beside it, f32
+    page's and head's scale, as ``dtype`` holds that (f16: multiples of 2^-24 below
+    2^-14, infinite past its range). ``dtype`` is the type of the rows beside it, f32
     or f16. ``page_table`` and ``lens`` are as there."""
     __slots__ = ("k", "v", "k_scale", "v_scale", "page_table", "lens", "dtype", "shape", "device_index")
 

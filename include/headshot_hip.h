@@ -461,9 +461,10 @@ hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int
 /* The same cache held in 8 bits: k_cache and v_cache (n_pages, Hkv, page, D)
  * of e4m3 codes (1, 4 and 3 bits; no infinities), k_scale and v_scale (n_pages,
  * Hkv) of one byte each, c standing for 2^(c - 127) (E8M0, c from 10 to 247): a
- * value is its code's times its page's and head's scale (one past the range of dt's
- * type counts as infinite; keys beside HS_F32 rows lie within it). hs_kv_append_f8
- * makes no infinite ones. Infinite values and NaN come through to the tokens that see
+ * value is its code's times its page's and head's scale, as dt's type holds that: exact
+ * in f32, and in f16 from 2^-14 on; below, f16's multiples of 2^-24, as a full f16 cache
+ * holds them. One past the type's range counts as infinite (keys beside HS_F32 rows
+ * lie within it); hs_kv_append_f8 makes none. Infinite values and NaN come through to the tokens that see
  * them, however little they weigh. dt is the type of the rows beside the cache. The
  * rules for lengths, offsets and pages are those above. */
 
