@@ -8,7 +8,7 @@
 // tokens of shared heads fill a tile, and a key is read and turned from its code
 // once for all heads that see it. Keys go through LDS 64 at a time, double
 // buffered: codes of the next ones lie in registers while these compute, and become
-// f16 (f16 caches) or bf16 (f32) values with their page's scale on the way into LDS,
+// f16 (f16 caches) or bf16 (f32) values with their page's scale on the way into LDS
 // (hs_f8.hpp). Scores are transposed, S^T = K Q^T: lanes n and n + 32 hold row n's, so
 // its statistics are the lane's own, and V^T takes P^T from the registers that the
 // scores were in.
@@ -252,6 +252,20 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs& a, int rows, Promp
     t.end = c.piece + 1 < t.count ? static_cast<int>(begin + static_cast<int64_t>(c.chunk) * kBN) : most;
     return true;
 }
+// A reference before any score: finite, so that a masked score weighs nothing.
+constexpr float kStart = -3.0e38f;
+// Whether there are any of the keys [begin, end). (Asked of a row whose weights come to
+// 0: of one that sees no key the result is 0, of one whose scores are all -infinity
+// NaN. A piece's row of the latter kind has a maximum above kStart.)
+__device__ __forceinline__ bool any_keys(const PromptArgs& a, const int* pages, int begin, int end) {
+    for (int i = begin >> a.page_shift; begin < end && i <= (end - 1) >> a.page_shift; i++)
+        if (pages[i] >= 0 && pages[i] < a.n_pages) return true;
+    return false;
+}
+// A result of sums over their weight, which are none's where `none`.
+__device__ __forceinline__ float over_weight(float sum, float weight, bool none) {
+    return weight != 0.0f ? sum / weight : none ? 0.0f : u2f(0x7FC00000u);
+}
 // A piece's 32 rows of a wave in the workspace: D sums each as the lanes hold them,
 // registers 4 i .. + 4 of all lanes after one another, so that a store is 1 KiB in a
 // row (by rows, it is 32 bytes of each).
@@ -271,8 +285,6 @@ constexpr float kPastF16 = 65520.0f;  // the least that f16 rounds to infinity
 // Tiles for which a wave looks for the scores' maximum ahead of the weights once
 // references have moved.
 constexpr int kWary = 8;
-// A reference before any score: finite, so that a masked score weighs nothing.
-constexpr float kStart = -3.0e38f;
 // A maximum (log2) beyond which its rounding, 2^-24 of it, shows in a weight.
 constexpr float kFar = 65536.0f;
 
@@ -374,6 +386,10 @@ __device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& 
                 s += times(*reinterpret_cast<const f32x4*>(&sm.o[w][row * S::kOPitch + d0]), __builtin_amdgcn_exp2f(sm.m[w][row] - top), keep);
             return s;
         });
+        if (weight == 0.0f) {
+            const bool sees = any_keys(a, pages, t.begin, min(keys_seen(t.seq, (t.first + row) / a.group, a.causal), t.end));
+            top = sees ? kFloor : kStart;
+        }
         if (piece) {
             st16(a.ws_o + block * 32 * D + x * 4, __builtin_bit_cast(u32x4, sum));
             const int64_t at = block * 32 + row;
@@ -382,7 +398,7 @@ __device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& 
             T* orow = static_cast<T*>(a.out) + row_out(a, t.seq, t.kv, t.first + row) * D + d0;
             float y[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = weight == 0.0f ? 0.0f : sum[e] / weight;
+            for (int e = 0; e < 4; e++) y[e] = over_weight(sum[e], weight, top == kStart);
             if constexpr (sizeof(T) == 2)
                 *reinterpret_cast<u32x2*>(orow) = u32x2{pk_f16(y[0], y[1]), pk_f16(y[2], y[3])};
             else
@@ -710,6 +726,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
         }
     }
     const float lsum = halves_sum(l);
+    if (lsum == 0.0f) m = any_keys(a, pages, t.begin, min(seen, t.end)) ? kFloor : kStart;
     if (t.count > 1) {
         const int64_t block = partial_block(a, t.item, t.kv, wave);
         float* p = a.ws_o + block * 32 * D + lane * 4;
@@ -726,7 +743,7 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
         if (hh == 0) a.ws_ml[2 * at] = m, a.ws_ml[2 * at + 1] = lsum;
         return;
     }
-    const float inv = 1.0f / lsum;
+    const float inv = 1.0f / lsum, empty = over_weight(0.0f, 0.0f, m == kStart);
     T* orow = static_cast<T*>(a.out) + row_out(a, t.seq, t.kv, row) * D + 4 * hh;
 #pragma unroll
     for (int db = 0; db < DB; db++)
@@ -736,9 +753,9 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 if constexpr (F::kHalf)
-                    x[e] = lsum == 0.0f ? 0.0f : o[db][4 * r4 + e] * inv;
+                    x[e] = lsum == 0.0f ? empty : o[db][4 * r4 + e] * inv;
                 else
-                    x[e] = lsum == 0.0f ? 0.0f : o[db][4 * r4 + e] / lsum;
+                    x[e] = lsum == 0.0f ? empty : o[db][4 * r4 + e] / lsum;
             }
             if constexpr (F::kHalf)
                 *reinterpret_cast<u32x2*>(orow + 32 * db + 8 * r4) = u32x2{pk_f16(x[0], x[1]), pk_f16(x[2], x[3])};
@@ -828,7 +845,7 @@ __global__ __launch_bounds__(256) void prompts_join_kernel(PromptArgs a, int sha
         T* orow = static_cast<T*>(a.out) + to * D + 8 * at + 4 * (lane / 32);
         float y[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = j.weight == 0.0f ? 0.0f : j.sum[e] / j.weight;
+        for (int e = 0; e < 4; e++) y[e] = over_weight(j.sum[e], j.weight, j.top == kStart);
         if constexpr (sizeof(T) == 2)
             *reinterpret_cast<u32x2*>(orow) = u32x2{pk_f16(y[0], y[1]), pk_f16(y[2], y[3])};
         else
