@@ -75,12 +75,34 @@ __device__ __forceinline__ bool zero_odd(u32x4& x) {
     return any;
 }
 
-// An infinity or NaN among a sum's values: the first takes the sum's place, the
-// others add up. `found`: bit by sum.
-__device__ __forceinline__ float with_odd(float sum, float v, uint64_t& found, int bit) {
-    const bool first = !(found >> bit & 1);
-    found |= uint64_t{1} << bit;
-    return first ? v : sum + v;
+// The least scale, as kept, with which a code passes f16 (448 2^8) or bf16 (448
+// 2^120), which makes it infinite.
+template <typename T>
+constexpr uint32_t kScaleWide = kScaleBias + (sizeof(T) == 2 ? 8 : 120);
+
+// Whether there can be infinite ones among the values of keys [begin, end). All lanes
+// of the wave call it.
+template <typename T, typename A>
+__device__ __forceinline__ bool any_infinite(const A& a, const int* pages, int kv, int begin, int end) {
+    bool any = false;
+    for (int i = (begin >> a.page_shift) + lane_id(); begin < end && i <= (end - 1) >> a.page_shift; i += 64) {
+        const int p = pages[i];
+        if (p >= 0 && p < a.n_pages) any |= a.v_scale[static_cast<int64_t>(p) * a.h_kv + kv] >= kScaleWide<T>;
+    }
+    return __any(any);
+}
+
+// A sum that is no number is put aside as a NaN that nothing else makes, which the
+// first infinity or NaN among its values replaces; the others add up. What is left of
+// those is what the sum was.
+constexpr uint32_t kAside = 0x7FC0DE00u;
+__device__ __forceinline__ float put_aside(float x) { return fabsf(x) < INFINITY ? x : u2f(kAside | (x != x ? 0u : x > 0.0f ? 1u : 2u)); }
+__device__ __forceinline__ float with_odd(float sum, float v) {
+    return fabsf(v) < INFINITY ? sum : (f2u(sum) & ~3u) == kAside ? v : sum + v;
+}
+__device__ __forceinline__ float taken_back(float x) {
+    const uint32_t was = f2u(x) & 3u;
+    return (f2u(x) & ~3u) != kAside ? x : was == 0 ? u2f(0x7FC00000u) : was == 1 ? INFINITY : -INFINITY;
 }
 
 // 4 values to 4 codes, rounded to nearest even. (In range: a finite value past

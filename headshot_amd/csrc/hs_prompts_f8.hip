@@ -27,6 +27,7 @@
 // spill in f32: 4096 tokens of 32 heads 742 us.) Sequences of few tokens: few_rows.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "hs_steps_f8.hpp"
 
@@ -700,16 +701,22 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
         if (j + 1 < ntiles) store(cur ^ 1, j + 1);
         __syncthreads();
     }
-    if (row >= t.rows) return;
     // Infinities and NaN among the values (odd_values)
     bool all = false;
 #pragma unroll
     for (int db = 0; db < DB; db++)
 #pragma unroll
         for (int x = 0; x < 16; x++) all |= !(fabsf(o[db][x]) < INFINITY);
+    all = __any(all) && any_infinite<T>(a, pages, t.kv, t.begin, t.end);
+    if (row >= t.rows) return;
     if (__builtin_expect(tile0 < ntiles && (all || sm.odd), 0)) {
-        uint64_t found = 0;
-#pragma unroll 1
+        const auto each = [&](auto f) {
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int x = 0; x < 16; x++) o[db][x] = f(o[db][x]);
+        };
+        if (all) each(put_aside);
         for (int key = all ? t.begin : max(tile_least / kBN * kBN, t.begin); key < min(seen, t.end); key++) {
             const int p = pages[key >> a.page_shift];
             if (p < 0 || p >= a.n_pages) continue;
@@ -719,11 +726,9 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
 #pragma unroll
             for (int db = 0; db < DB; db++)
 #pragma unroll
-                for (int x = 0; x < 16; x++) {
-                    const float v = value_of<T>(r[32 * db + 8 * (x / 4) + x % 4], scale);
-                    if (!(fabsf(v) < INFINITY)) o[db][x] = with_odd(o[db][x], v, found, 16 * db + x);
-                }
+                for (int x = 0; x < 16; x++) o[db][x] = with_odd(o[db][x], value_of<T>(r[32 * db + 8 * (x / 4) + x % 4], scale));
         }
+        if (all) each(taken_back);
     }
     const float lsum = halves_sum(l);
     if (lsum == 0.0f) m = any_keys(a, pages, t.begin, min(seen, t.end)) ? kFloor : kStart;

@@ -35,8 +35,8 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 // Infinities and NaN among the values: a channel's are its sum, in the rows that see
 // any. A channel of which all rows see them has a sum that is no number already, but
 // maybe another one, since an infinity times a weight of 0, or the parts of one, is
-// NaN; so they are added by themselves, over all keys where there is such a sum, else
-// over the steps that left them out.
+// NaN; so where there are infinities, too, they are added by themselves over all keys,
+// else over the steps that left them out.
 template <typename T, int D, int R, bool MASKED, typename A>
 __device__ __forceinline__ void odd_values(const A& a, const int* pages, int kv, int begin, int end, const int (&seen)[R], int least,
                                            bool left_out, f32x4 (&o)[R][D / 16]) {
@@ -49,13 +49,19 @@ __device__ __forceinline__ void odd_values(const A& a, const int* pages, int kv,
         for (int i = 0; i < D / 16; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) odd |= !(fabsf(o[r][i][j]) < INFINITY);
-    const bool all = __any(odd);
+    const bool all = __any(odd) && any_infinite<T>(a, pages, kv, begin, end);
     if (__builtin_expect(!all && !left_out, 1)) return;
-    uint64_t found = 0;  // by sum
-#pragma unroll 1
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int i = 0; i < D / 16; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[r][i][j] = f(o[r][i][j]);
+    };
+    if (all) each(put_aside);
     for (int key0 = begin + wave_in_block() * P::kStep; key0 < end; key0 += P::kKeys) {
         if (!all && key0 + P::kStep <= least) continue;
-#pragma unroll 1
         for (int key = key0; key < min(key0 + P::kStep, end); key++) {
             const Tile16 tile = tile_of(a, pages[key >> a.page_shift], kv, key);
             if (!tile.there) continue;
@@ -66,13 +72,13 @@ __device__ __forceinline__ void odd_values(const A& a, const int* pages, int kv,
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const float v = value_of<T>(p[16 * i + j], scale);
-                    if (fabsf(v) < INFINITY) continue;
 #pragma unroll
                     for (int r = 0; r < R; r++)
-                        if (!MASKED || key < seen[r]) o[r][i][j] = with_odd(o[r][i][j], v, found, (r * (D / 16) + i) * 4 + j);
+                        if (!MASKED || key < seen[r]) o[r][i][j] = with_odd(o[r][i][j], v);
                 }
         }
     }
+    if (all) each(taken_back);
 }
 
 // The wave's steps of keys [begin, end): R sets of 16 rows, lane (n, g) with row n

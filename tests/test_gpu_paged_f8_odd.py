@@ -183,3 +183,28 @@ def test_infinite_values_of_wide_tiles(ctx):
         kept[-9:, heads, 8] = False
         kept[:-9, heads, 8] = True
         assert torch.equal(odd[kept], plain[kept])
+
+
+@pytest.mark.parametrize("new", NEW, ids=str)
+@pytest.mark.parametrize("page", [4, 32])
+@pytest.mark.parametrize("dtype", [F16, F32])
+def test_nan_of_other_pages_beside_infinities(ctx, dtype, page, new):
+    """A channel with an infinity on one page and NaN on an ordinary one, in either order, is NaN; channels with one
+    of them are that; queries of NaN have no finite channel."""
+    gen = torch.Generator().manual_seed(8)
+    c = make_cache(gen, [40, 150, 90], 2, page, 64, dtype)
+    for s, length in enumerate((40, 150, 90)):
+        for first, second, channel in ((3, length // 2, 20), (length // 2 + 1, 4, 21)):
+            bits(c.v)[int(c.page_table[s, first // page]), 0, first % page, channel] = NAN
+            widen(c, s, second + page, [(0, channel, INF)], gen)
+        widen(c, s, 2 * page + 1, [(1, 30, LOW)], gen)
+        bits(c.v)[int(c.page_table[s, 0]), 1, 1, 31] = NAN
+    ref = check(ctx, c, new, 1, 1.0, 0.125, gen, 4)
+    assert ref[-1, 0, 20].isnan() and (ref[:, 2, 30] == -math.inf).any() and ref[:, 2, 31].isnan().any()
+    n = ref.shape[0]
+    q = torch.randn((n, 4, 64), generator=gen).to(dtype)
+    q[n - 1, 3, 9] = math.nan
+    gpu = PagedKV8(*(t.to(DEV) for t in (c.k, c.v, c.k_scale, c.v_scale, c.page_table, c.lens)), dtype)
+    off = None if new is None else [sum(new[:i]) for i in range(4)]
+    got = ctx.attention_paged(q.to(DEV), gpu) if new is None else ctx.attention_paged_prompts(q.to(DEV), gpu, i32(off))
+    assert got.unflatten(1, (4, 64))[n - 1, 3].isnan().all()
