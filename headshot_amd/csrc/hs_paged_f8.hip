@@ -306,13 +306,13 @@ hs_status launch_append_f8(const char* op, hipStream_t st, Append8Args<T> a, int
 // of 11 bits each (the queries are f16), in f32 both go as three bf16 ones, which
 // hold all 24 bits.
 //
-// 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 104 us, 5.0 TB/s, of
+// 64 sequences of up to 8192 keys, 32 heads of 128 over 8, f16: 103 us, 5.0 TB/s, of
 // which the join is 5 (the same loads with nothing computed: 98); one token over
-// 130531 keys of 16 heads of 64 54 us, 5.0 TB/s (48); eight f32 sequences of up to
+// 130531 keys of 16 heads of 64 53 us, 5.0 TB/s (48); eight f32 sequences of up to
 // 800, 16 heads of 128, 13 us; 32 sequences of up to 4000, 16 heads of 64, 33 (f32 35),
-// over pages of 8 keys 35 (38). Steps of 64 keys at head dim 64 take 30 us for 34 of 32,
-// and at 128 spill; pieces of units of 256 keys 29 us for 33
-// of 128 (20 sequences of up to 3001, 16 heads of 128).
+// over pages of 8 keys 35 (38). At head dim 64 a wave's step is 64 keys: 30 us, and 34
+// with steps of 32; at 128 it is 32, as steps of 64 spill. Pieces are made of 256 keys:
+// 29 us, and 33 made of 128 (20 sequences of up to 3001, 16 heads of 128).
 template <typename T, int D>
 struct Paged8 : Steps8<T, D, 1> {
     using S = Steps8<T, D, 1>;

@@ -281,6 +281,12 @@ __device__ __forceinline__ int64_t row_out(const PromptArgs& a, const PromptSeq&
 // The reference of a row's weights is set this far (log2) below its largest score,
 // so that its largest weight is 2^12: f16 weights keep 11 bits down to 2^-26 of the
 // largest. It moves when one would pass f16.
+//
+// A weight is one f16 value here, and two in few_rows and attention_paged, whose time is
+// the keys' bytes. Two would bring the results' distance from 64 bits from 2.8e-4 to the
+// 2.07e-4 that their own rounding makes (1374 tokens over 30228, 16 heads of 64), for
+// half as many products again: 378 us for 260, five prompts of 32 heads of 128 over 8
+// 396 for 311, 8192 tokens over themselves 870 for 640 and, 16 heads of 64, 600 for 342.
 constexpr float kWeightBits = 12.0f;
 constexpr float kPastF16 = 65520.0f;  // the least that f16 rounds to infinity
 // Tiles for which a wave looks for the scores' maximum ahead of the weights once

@@ -497,7 +497,8 @@ hs_status hs_kv_append_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_
  * current device; 0 for shapes that it refuses. */
 int64_t hs_attention_paged_f8_workspace(int32_t b, int32_t h, int32_t h_kv, int32_t d);
 
-/* hs_attention_paged over such a cache. */
+/* hs_attention_paged over such a cache; f16 weights have 22 bits beside infinities and
+ * NaN, too. */
 hs_status hs_attention_paged_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                                 const void* k_cache, const void* v_cache, const void* k_scale,
                                 const void* v_scale, const void* page_table, const void* lens,
@@ -516,8 +517,11 @@ int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int32_t b, int
  * last of sequence s's tokens is key lens[s] - 1, also where it is a row past n;
  * causal is as for hs_attention_packed, groups counted from key 0. A token that sees no key gets
  * zeros, rows of no sequence are not written. Keys and values that a token does
- * not see do not enter its result, whatever they hold. workspace is as for
- * hs_attention_paged. */
+ * not see do not enter its result, whatever they hold; a token that sees some, all
+ * of whose scores are -infinity, gets NaN. Softmax statistics and sums are f32; in f16
+ * each weight is rounded to 11 bits, or to 22 in sequences of up to 32 rows (tokens
+ * times query heads of a key head) of calls that are not all long ones, or to 2^-37 of
+ * the largest if that is more. workspace is as for hs_attention_paged. */
 hs_status hs_attention_prompts_f8(hs_stream_t stream, hs_dtype dt, const void* q, int64_t q_stride,
                                   const void* k_cache, const void* v_cache, const void* k_scale,
                                   const void* v_scale, const void* page_table, const void* lens,
