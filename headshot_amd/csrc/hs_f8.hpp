@@ -54,6 +54,14 @@ __device__ __forceinline__ u32x4 values_of(uint32_t lo, uint32_t hi, float scale
     return sizeof(T) == 2 ? f16_of_codes(lo, hi, scale) : bf16_of_codes(lo, hi, scale);
 }
 
+// A scalar address that stays one beside a lane's offset: the compiler keeps their sum,
+// two registers of every lane's, where it can.
+__device__ __forceinline__ const uint8_t* scalar_address(const uint8_t* p) {
+    auto global = (const __attribute__((address_space(1))) uint8_t*)p;
+    asm("" : "+s"(global));
+    return (const uint8_t*)global;
+}
+
 // One code, as values_of has it.
 template <typename T>
 __device__ __forceinline__ float value_of(uint32_t code, float scale) {

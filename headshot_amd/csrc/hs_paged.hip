@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * kPagedWaves, D == 64 ? 4 : 3) void attention_p
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
-    join_waves<T, D, false>(a, sm, s, count, head0, live_heads, o, m, l);
+    join_waves<T, D, false>(a, sm, s, count, head0, live_heads, o, m, l, [](float*) {});
 }
 
 // f32, a key head of one query head (no sharing): the matrix instructions would

@@ -322,10 +322,11 @@ __device__ __forceinline__ f32x4 joined(F f) {
 
 // A workgroup's waves' sums of up to kGroup query heads joined in LDS: the result,
 // or the piece's in the workspace. Lane (n, g) holds channels 16 i + 4 g + .. of
-// head n; l is a head's whole sum of the wave. KEEP: as there.
-template <typename T, int D, bool KEEP, typename S>
+// head n; l is a head's whole sum of the wave. KEEP: as there. `mend`: what the wave
+// does to its sums in LDS.
+template <typename T, int D, bool KEEP, typename S, typename F>
 __device__ __forceinline__ void join_waves(const PagedArgs& a, S& sm, int s, int count, int head0, int live_heads,
-                                           const f32x4 (&o)[D / 16], float m, float l) {
+                                           const f32x4 (&o)[D / 16], float m, float l, F mend) {
     constexpr int kOPitch = D + 4;
     const int lane = lane_id(), wave = wave_in_block(), n = lane & 15, g = lane >> 4;
     __syncthreads();
@@ -334,6 +335,7 @@ __device__ __forceinline__ void join_waves(const PagedArgs& a, S& sm, int s, int
         for (int i = 0; i < D / 16; i++) *reinterpret_cast<f32x4*>(&sm.o[wave][n * kOPitch + 16 * i + 4 * g]) = o[i];
         if (g == 0) sm.m[wave][n] = m, sm.l[wave][n] = l;
     }
+    mend(sm.o[wave]);
     __syncthreads();
     for (int x = threadIdx.x; x < live_heads * (D / 4); x += 64 * kPagedWaves) {
         const int head = x / (D / 4), d0 = x % (D / 4) * 4;

@@ -348,9 +348,10 @@ __global__ __launch_bounds__(64 * kPagedWaves, (Paged8<T, D>::per_cu(WHOLE))) vo
     const T* q[1] = {static_cast<const T*>(a.q) + s * a.q_stride + (head0 + min(lane_id() & 15, live_heads - 1)) * D};
     f32x4 o[1][D / 16];
     float m[1], l[1];
-    attend_steps<T, D, 1, WHOLE, false>(a, a.page_table + static_cast<int64_t>(s) * a.max_pages, kv, begin, end, q, {0}, 0,
-                                        sm.v[wave_in_block()], o, m, l);
-    join_waves<T, D, true>(a, sm, s, count, head0, live_heads, o[0], m[0], l[0]);
+    const int* pages = a.page_table + static_cast<int64_t>(s) * a.max_pages;
+    const int odd = attend_steps<T, D, 1, WHOLE, false>(a, pages, kv, begin, end, q, {0}, 0, sm.v[wave_in_block()], o, m, l);
+    join_waves<T, D, true>(a, sm, s, count, head0, live_heads, o[0], m[0], l[0],
+                           [&](float* sums) { odd_values<T, D, 1, false>(a, pages, kv, begin, end, {0}, 0, odd, sums); });
 }
 
 template <typename T, int D>

@@ -363,7 +363,7 @@ __device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& 
     const int least = keys_seen(t.seq, t.first / a.group, a.causal);
     f32x4 o[R][DB];
     float m[R], l[R];
-    attend_steps<T, D, R, WHOLE, true>(a, pages, t.kv, t.begin, t.end, q, seen, least, sm.v[wave], o, m, l);
+    const int odd = attend_steps<T, D, R, WHOLE, true>(a, pages, t.kv, t.begin, t.end, q, seen, least, sm.v[wave], o, m, l);
     const int live = min(t.rows - t.first, 16 * R);
     __syncthreads();
 #pragma unroll
@@ -373,6 +373,7 @@ __device__ __forceinline__ void few_rows(const PromptArgs& a, const PromptTile& 
         for (int i = 0; i < DB; i++) *reinterpret_cast<f32x4*>(&sm.o[wave][row * S::kOPitch + 16 * i + 4 * g]) = o[r][i];
         if (g == 0) sm.m[wave][row] = m[r], sm.l[wave][row] = l[r];
     }
+    odd_values<T, D, R, true>(a, pages, t.kv, t.begin, t.end, seen, least, odd, sm.o[wave]);
     __syncthreads();
     const int64_t block = partial_block(a, t.item, t.kv, 0);
     for (int x = threadIdx.x; x < 8 * D; x += 64 * kPagedWaves) {
@@ -479,8 +480,6 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
     // codes at `piece`. Pages are looked up a tile ahead of the codes.
     constexpr int kWords = F::kLoad / 4;
     typedef uint32_t codes_t __attribute__((ext_vector_type(kWords)));
-    typedef const __attribute__((address_space(1))) codes_t* global_codes;
-    typedef const __attribute__((address_space(1))) uint8_t* global_bytes;
     const int row0 = tid / F::kPieces, piece = tid % F::kPieces;
     const int* pages = a.page_table + static_cast<int64_t>(t.s) * a.max_pages;
     int page[kPer];
@@ -503,12 +502,11 @@ __global__ __launch_bounds__(64 * W, (Prompt8<T, D, W>::kPerCu)) void prompts_f8
             const int64_t block = static_cast<int64_t>(there ? page[i] : 0) * a.h_kv + t.kv;
             const int64_t at = ((block << a.page_shift) + (WHOLE || there ? key & ((1 << a.page_shift) - 1) : 0)) * D;
             const uint32_t lane_at = WHOLE ? lane * F::kLoad : piece * F::kLoad;
-            global_bytes kp = (global_bytes)(a.k + at), vp = (global_bytes)(a.v + at);
-            // a scalar address with a lane's offset, where its sum with that is too many
-            // registers (8192 tokens, 16 heads of 64, 361 us for 342; the others lose 1%)
-            if constexpr (W == 8 && D == 64) asm("" : "+s"(kp), "+s"(vp));
-            pk[i] = *reinterpret_cast<global_codes>(kp + lane_at);
-            pv[i] = *reinterpret_cast<global_codes>(vp + lane_at);
+            const uint8_t *kp = a.k + at, *vp = a.v + at;
+            // (without, 8192 tokens, 16 heads of 64, take 361 us for 342; the others lose 1% by it)
+            if constexpr (W == 8 && D == 64) kp = scalar_address(kp), vp = scalar_address(vp);
+            pk[i] = *reinterpret_cast<const codes_t*>(kp + lane_at);
+            pv[i] = *reinterpret_cast<const codes_t*>(vp + lane_at);
             pks[i] = a.k_scale[block], pvs[i] = a.v_scale[block];
             ok |= there ? 1u << i : 0u;
         }

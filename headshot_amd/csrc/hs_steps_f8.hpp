@@ -32,50 +32,60 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// What attend_steps says of its sums.
+constexpr int kLeftOut = 1;  // infinities or NaN went in as zeros
+constexpr int kOdd = 2;      // some are no numbers
+
 // Infinities and NaN among the values: a channel's are its sum, in the rows that see
 // any. A channel of which all rows see them has a sum that is no number already, but
 // maybe another one, since an infinity times a weight of 0, or the parts of one, is
 // NaN; so where there are infinities, too, they are added by themselves over all keys,
-// else over the steps that left them out.
+// else over the steps that left them out. `sums`: the wave's in LDS, rows of kOPitch,
+// each lane with its own. (In registers this takes some from the keys' loop: 8 f32
+// tokens each of 32 sequences, 32 heads of 128 over 8, 83 us for 76.)
 template <typename T, int D, int R, bool MASKED, typename A>
 __device__ __forceinline__ void odd_values(const A& a, const int* pages, int kv, int begin, int end, const int (&seen)[R], int least,
-                                           bool left_out, f32x4 (&o)[R][D / 16]) {
+                                           int what, float* sums) {
     using P = Steps8<T, D, R>;
-    const int g = lane_id() >> 4;
-    bool odd = false;
-#pragma unroll
-    for (int r = 0; r < R; r++)
-#pragma unroll
-        for (int i = 0; i < D / 16; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) odd |= !(fabsf(o[r][i][j]) < INFINITY);
-    const bool all = __any(odd) && any_infinite<T>(a, pages, kv, begin, end);
-    if (__builtin_expect(!all && !left_out, 1)) return;
+    if (__builtin_expect(what == 0, 1)) return;
+    const bool all = what & kOdd && any_infinite<T>(a, pages, kv, begin, end);
+    if (!all && !(what & kLeftOut)) return;
+    const int lane = lane_id(), n = lane & 15, g = lane >> 4;
+    float* mine = sums + n * P::kOPitch + 4 * g;
     const auto each = [&](auto f) {
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int i = 0; i < D / 16; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) o[r][i][j] = f(o[r][i][j]);
+#pragma unroll 1
+        for (int x = 0; x < R * D / 4; x++) {
+            float* p = mine + x / (D / 4) * 16 * P::kOPitch + x % (D / 4) / 4 * 16 + x % 4;
+            *p = f(*p);
+        }
     };
     if (all) each(put_aside);
+#pragma unroll 1
     for (int key0 = begin + wave_in_block() * P::kStep; key0 < end; key0 += P::kKeys) {
         if (!all && key0 + P::kStep <= least) continue;
+#pragma unroll 1
         for (int key = key0; key < min(key0 + P::kStep, end); key++) {
             const Tile16 tile = tile_of(a, pages[key >> a.page_shift], kv, key);
             if (!tile.there) continue;
             const uint8_t* p = static_cast<const uint8_t*>(a.v) + tile.row * D + 4 * g;
             const float scale = scale_value(a.v_scale[tile.row >> a.page_shift]);
+            uint32_t w[D / 16];
 #pragma unroll
-            for (int i = 0; i < D / 16; i++)
+            for (int i = 0; i < D / 16; i++) w[i] = *reinterpret_cast<const uint32_t*>(p + 16 * i);
 #pragma unroll
+            for (int i = 0; i < D / 16; i++) {
+                u32x4 x = values_of<T>(w[i], 0, scale);
+                if (!zero_odd<T>(x)) continue;
+#pragma unroll 1
                 for (int j = 0; j < 4; j++) {
-                    const float v = value_of<T>(p[16 * i + j], scale);
+                    const float v = value_of<T>(w[i] >> 8 * j & 0xFFu, scale);
 #pragma unroll
-                    for (int r = 0; r < R; r++)
-                        if (!MASKED || key < seen[r]) o[r][i][j] = with_odd(o[r][i][j], v);
+                    for (int r = 0; r < R; r++) {
+                        float* at = mine + r * 16 * P::kOPitch + 16 * i + j;
+                        if (!MASKED || key < seen[r]) *at = with_odd(*at, v);
+                    }
                 }
+            }
         }
     }
     if (all) each(taken_back);
@@ -86,7 +96,7 @@ __device__ __forceinline__ void odd_values(const A& a, const int* pages, int kv,
 // score (log2) and its sum of weights. `vs` is the wave's slice of LDS. MASKED: a row
 // sees keys below `seen`, all of them those below `least`, else all see all; in a step
 // that some row does not see whole, infinities and NaN go into the sums as zeros, and
-// to the rows that see them at the end (odd_values).
+// to the rows that see them afterwards (odd_values, which what is returned is for).
 // WHOLE: pages of at least 16 keys, so that 16 keys from a multiple of 16 lie in
 // one page; else a lane looks one key's up, a step ahead, and rows take it from there
 // (by each row, when its codes are asked for: 42 us for 33 of 32 sequences of up to 4000
@@ -95,11 +105,14 @@ __device__ __forceinline__ void odd_values(const A& a, const int* pages, int kv,
 // A lane's 16-byte load of a row of K is 16 dims, two operands of 8: dims 64 i +
 // 16 g + 8 e, which the queries follow.
 template <typename T, int D, int R, bool WHOLE, bool MASKED, typename A>
-__device__ __forceinline__ void attend_steps(const A& a, const int* pages, int kv, int begin, int end, const T* const (&qr)[R],
+__device__ __forceinline__ int attend_steps(const A& a, const int* pages, int kv, int begin, int end, const T* const (&qr)[R],
                                              const int (&seen)[R], int least, uint16_t* vs, f32x4 (&o)[R][D / 16],
                                              float (&m)[R], float (&l)[R]) {
     using P = Steps8<T, D, R>;
     constexpr int kStep = P::kStep, KL = P::KL, kTiles = P::kTiles, DB = D / 16;
+    // registers short of what the loop holds (8 tokens each of 32 sequences of up to 4000
+    // keys, 32 heads of 128 over 8: 67 us, and 76 without)
+    constexpr bool kTight = WHOLE && R == 2 && D == 128 && !P::kHalf;
     const int lane = lane_id(), n = lane & 15, g = lane >> 4;
     bool odd = false;
 
@@ -146,7 +159,9 @@ __device__ __forceinline__ void attend_steps(const A& a, const int* pages, int k
         for (int i = 0; i < kTiles; i++) {
             const int key = key0 + 16 * i + (WHOLE ? 0 : n);
             const Tile16 tile = tile_of(a, WHOLE ? page[i] : __shfl(page[0], 16 * i + n, 64), kv, key);
-            const uint8_t* p = kb + tile.row * D + (WHOLE ? k_lane : 16 * g);
+            const uint8_t* p = kb + tile.row * D;
+            if constexpr (kTight) p = scalar_address(p);
+            p += WHOLE ? k_lane : 16 * g;
 #pragma unroll
             for (int x = 0; x < KL; x++) kr[i * KL + x] = ld16_nt(p + 64 * x);
             ks[i] = scale_of(a.k_scale, tile);
@@ -163,6 +178,7 @@ __device__ __forceinline__ void attend_steps(const A& a, const int* pages, int k
             for (int i = 2 * h; i < 2 * h + 2; i++) {
                 const Tile16 tile = tile_of(a, page[i], kv, key0 + 16 * i);
                 const uint8_t* p = vb + tile.row * D;
+                if constexpr (kTight) p = scalar_address(p);
 #pragma unroll
                 for (int x = 0; x < kPer; x++) vr[i * kPer + x] = ld16_nt(p + v_lane + P::kVRows * x * D);
                 vx[i] = scale_of(a.v_scale, tile);
@@ -351,7 +367,14 @@ __device__ __forceinline__ void attend_steps(const A& a, const int* pages, int k
         l[r] += __shfl_xor(l[r], 16, 64);
         l[r] += __shfl_xor(l[r], 32, 64);
     }
-    odd_values<T, D, R, MASKED>(a, pages, kv, begin, end, seen, least, MASKED && __any(odd), o);
+    bool wild = false;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int i = 0; i < DB; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) wild |= !(fabsf(o[r][i][j]) < INFINITY);
+    return (MASKED && __any(odd) ? kLeftOut : 0) | (__any(wild) ? kOdd : 0);
 }
 
 }  // namespace
