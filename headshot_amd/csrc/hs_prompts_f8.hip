@@ -253,8 +253,10 @@ __device__ __forceinline__ bool prompt_tile(const PromptArgs& a, int rows, Promp
     t.end = c.piece + 1 < t.count ? static_cast<int>(begin + static_cast<int64_t>(c.chunk) * kBN) : most;
     return true;
 }
+
 // A reference before any score: finite, so that a masked score weighs nothing.
 constexpr float kStart = -3.0e38f;
+
 // Whether there are any of the keys [begin, end). (Asked of a row whose weights come to
 // 0: of one that sees no key the result is 0, of one whose scores are all -infinity
 // NaN. A piece's row of the latter kind has a maximum above kStart.)
@@ -267,6 +269,7 @@ __device__ __forceinline__ bool any_keys(const PromptArgs& a, const int* pages, 
 __device__ __forceinline__ float over_weight(float sum, float weight, bool none) {
     return weight != 0.0f ? sum / weight : none ? 0.0f : u2f(0x7FC00000u);
 }
+
 // A piece's 32 rows of a wave in the workspace: D sums each as the lanes hold them,
 // registers 4 i .. + 4 of all lanes after one another, so that a store is 1 KiB in a
 // row (by rows, it is 32 bytes of each).

@@ -464,9 +464,9 @@ hs_status hs_attention_paged(hs_stream_t stream, hs_dtype dt, const void* q, int
  * value is its code's times its page's and head's scale, as dt's type holds that: exact
  * in f32, and in f16 from 2^-14 on; below, f16's multiples of 2^-24, as a full f16 cache
  * holds them. One past the type's range counts as infinite (keys beside HS_F32 rows
- * lie within it); hs_kv_append_f8 makes none. Infinite values and NaN come through to the tokens that see
- * them, however little they weigh. dt is the type of the rows beside the cache. The
- * rules for lengths, offsets and pages are those above. */
+ * lie within it); hs_kv_append_f8 makes none. Infinite values and NaN come through to
+ * the tokens that see them, however little they weigh. dt is the type of the rows
+ * beside the cache. The rules for lengths, offsets and pages are those above. */
 
 /* hs_kv_append into such a cache; q_out and k_out are as there. The new keys (and
  * values) of a page and head share a scale: the least 2^e, e >= -117, that brings
@@ -515,10 +515,10 @@ int64_t hs_attention_prompts_f8_workspace(hs_dtype dt, int64_t n, int32_t b, int
 /* Attention of several new tokens per sequence over such a cache, which holds
  * their own keys already: q (n, Hq*D) at offsets (b + 1) -> out (n, Hq*D). The
  * last of sequence s's tokens is key lens[s] - 1, also where it is a row past n;
- * causal is as for hs_attention_packed, groups counted from key 0. A token that sees no key gets
- * zeros, rows of no sequence are not written. Keys and values that a token does
- * not see do not enter its result, whatever they hold; a token that sees some, all
- * of whose scores are -infinity, gets NaN. Softmax statistics and sums are f32; in f16
+ * causal is as for hs_attention_packed, groups counted from key 0. A token that
+ * sees no key gets zeros, rows of no sequence are not written. Keys and values that
+ * a token does not see do not enter its result, whatever they hold; one that sees
+ * some, all of whose scores are -infinity, gets NaN. Softmax statistics and sums are f32; in f16
  * each weight is rounded to 11 bits, or to 22 in sequences of up to 32 rows (tokens
  * times query heads of a key head) of calls that are not all long ones, or to 2^-37 of
  * the largest if that is more. workspace is as for hs_attention_paged. */
